@@ -111,6 +111,19 @@ DeviceScratch* device_scratch() {
 
 }  // namespace
 
+// The current device's bounds-check word, allocated at its first use.
+int bounds_word(uint32_t** err) {
+    std::lock_guard<std::mutex> lk(g_mu);
+    DeviceScratch* d = device_scratch();
+    if (!d) return set_error(TG_ECUDA, "cudaGetDevice failed");
+    if (!d->err) {
+        int rc = check_cuda(cudaMalloc(&d->err, sizeof(uint32_t)), "cudaMalloc(bounds word)");
+        if (rc != TG_OK) return rc;
+    }
+    *err = d->err;
+    return TG_OK;
+}
+
 // Fills *out from `in` (NULL: the process schedule of tg_set_schedule) with every zero
 // knob replaced by its default, and checks it.  Every tg_* entry point resolves its
 // schedule here.
@@ -169,17 +182,9 @@ int check_csr(const tg_csr* A, const char* op) {
 // Bounds-checked calls validate the CSR structure first and are synchronous on `st`.
 int bounds_check(const tg_csr& A, cudaStream_t st) {
     uint32_t* err = nullptr;
-    {
-        std::lock_guard<std::mutex> lk(g_mu);
-        DeviceScratch* d = device_scratch();
-        if (!d) return set_error(TG_ECUDA, "cudaGetDevice failed");
-        if (!d->err) {
-            int rc = check_cuda(cudaMalloc(&d->err, sizeof(uint32_t)), "cudaMalloc(bounds word)");
-            if (rc != TG_OK) return rc;
-        }
-        err = d->err;
-    }
-    int rc = check_cuda(cudaMemsetAsync(err, 0, sizeof(uint32_t), st), "cudaMemsetAsync");
+    int rc = bounds_word(&err);
+    if (rc != TG_OK) return rc;
+    rc = check_cuda(cudaMemsetAsync(err, 0, sizeof(uint32_t), st), "cudaMemsetAsync");
     if (rc != TG_OK) return rc;
     int64_t blocks = std::min<int64_t>(ceil_div(std::max(A.rows, A.nnz) + 1, 256), 148 * 16);
     csr_check_kernel<<<(unsigned)blocks, 256, 0, st>>>(A.indptr, A.indices, A.rows, A.cols, A.nnz, err);

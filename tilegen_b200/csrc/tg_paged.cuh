@@ -1,0 +1,93 @@
+// Shared pieces of the paged operators (tg_rope.cu, tg_paged_host.cu, tg_prefix_attn*.cu):
+// 16-bit conversions, the CSR page-table lookup and the host-side checks.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include <climits>
+
+#include "../../include/tilegen_b200_paged.h"
+#include "tg_common.cuh"
+
+namespace tg {
+
+constexpr int kSMs = 148;  // B200: two dies of 74
+
+__device__ __forceinline__ float to_f32(float v) { return v; }
+__device__ __forceinline__ float to_f32(__half v) { return __half2float(v); }
+__device__ __forceinline__ float to_f32(__nv_bfloat16 v) { return __bfloat162float(v); }
+template <typename T>
+__device__ __forceinline__ T from_f32(float v);
+template <>
+__device__ __forceinline__ float from_f32<float>(float v) { return v; }
+template <>
+__device__ __forceinline__ __half from_f32<__half>(float v) { return __float2half_rn(v); }
+template <>
+__device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+
+// The sequence that token t belongs to: the last b with q_indptr[b] <= t, clamped to a
+// sequence (token b is sequence b's where there is no q_indptr).
+__device__ __forceinline__ int64_t sequence_of(const int64_t* q_indptr, int64_t rows, int64_t t) {
+    if (!q_indptr) return t;
+    int64_t lo = 0, hi = rows;  // q_indptr[lo] <= t
+    while (hi - lo > 1) {
+        const int64_t mid = (lo + hi) >> 1;
+        if (q_indptr[mid] <= t) lo = mid;
+        else hi = mid;
+    }
+    return lo;
+}
+
+// First token and number of tokens of sequence b, inside [0, tokens] whatever q_indptr holds.
+__device__ __forceinline__ void tokens_of(const int64_t* q_indptr, int64_t tokens, int64_t b, int64_t& first,
+                                          int64_t& n) {
+    if (!q_indptr) {
+        first = b;
+        n = 1;
+        return;
+    }
+    const int64_t a = q_indptr[b], e = q_indptr[b + 1];
+    first = min(max(a, (int64_t)0), tokens);
+    n = min(max(e, first), tokens) - first;
+}
+
+// Pages of row b of the table inside [0, nnz] whatever indptr holds.
+__device__ __forceinline__ void pages_of(const int64_t* indptr, int64_t nnz, int64_t b, int64_t& first, int64_t& n) {
+    const int64_t a = indptr[b], e = indptr[b + 1];
+    first = min(max(a, (int64_t)0), nnz);
+    n = min(max(e, first), nnz) - first;
+}
+
+// host side (tg_paged_host.cu)
+int check_cache(const tg_paged_kv* c, const char* op);
+int check_table(const tg_csr* t, const tg_paged_kv* c, int64_t tokens, const int64_t* q_indptr, const int64_t* seq_len,
+                const char* op);
+int check_rope(const tg_rope* r, int32_t dim, const char* op);
+// Synchronous check of the index arrays on `st` (TG_FLAG_BOUNDS_CHECK).
+int paged_bounds_check(const tg_csr& t, int64_t page_size, const int64_t* seq_len, int64_t max_seq_len, int64_t tokens,
+                       const int64_t* q_indptr, int64_t max_q_len, const int64_t* prefix_pages, int64_t n_prefix,
+                       bool append, const char* op, cudaStream_t st);
+// The device word that bounds checks report into (tg_abi.cu).
+int bounds_word(uint32_t** err);
+
+// Launch with the programmatic-dependency attribute: the kernel may start while the one
+// before it on the stream still runs, and orders itself with pdl_wait().
+template <typename... P, typename... A>
+int launch_pdl(const char* what, void (*kernel)(P...), dim3 grid, int block, size_t smem, cudaStream_t st, A... args) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3((unsigned)block);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, static_cast<P>(args)...);
+    const int rc = check_launch(what);
+    return e != cudaSuccess ? check_cuda(e, what) : rc;
+}
+
+}  // namespace tg

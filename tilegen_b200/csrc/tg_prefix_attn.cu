@@ -1,0 +1,671 @@
+// Attention of a batch that shares a prefix (tg_prefix_attention_*): the kernel for few
+// rows, the join of the parts, planning and the C entry points.
+#include <algorithm>
+
+#include "tg_prefix_attn.cuh"
+
+namespace tg {
+namespace {
+
+// ------------------------------------------------------------------ matrix instructions
+__device__ __forceinline__ void ldmatrix4(uint32_t addr, uint32_t (&r)[4]) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(addr)
+                 : "memory");
+}
+__device__ __forceinline__ void ldmatrix4_trans(uint32_t addr, uint32_t (&r)[4]) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(addr)
+                 : "memory");
+}
+template <typename T>
+__device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    if constexpr (std::is_same<T, __half>::value) {
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                     : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                     : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    } else {
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                     : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                     : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    }
+}
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+    if constexpr (std::is_same<T, __half>::value) {
+        const __half2 h = __floats2half2_rn(lo, hi);
+        return *reinterpret_cast<const uint32_t*>(&h);
+    } else {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+        return *reinterpret_cast<const uint32_t*>(&h);
+    }
+}
+__device__ __forceinline__ float exp2_fast(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+// 16 bytes to shared memory, zeros where !valid (the source is not read then).
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool valid) {
+    const int n = valid ? 16 : 0;
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_async_wait() {
+    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+// Whether one of the eight 16-bit numbers in v is an infinity or NaN.
+template <typename T>
+__device__ __forceinline__ bool any_nonfinite(uint4 v) {
+    constexpr uint32_t kExp = std::is_same<T, __half>::value ? 0x7c00u : 0x7f80u;
+    bool bad = false;
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) bad |= (w[i] & kExp) == kExp || ((w[i] >> 16) & kExp) == kExp;
+    return bad;
+}
+
+// ------------------------------------------------------------------ few rows
+// One CTA: RT*16 rows (of one sequence's tokens x group, or of all tokens over the prefix),
+// one key head, one chunk of keys.  Its four warps take 16 keys in turn, each with its own
+// ring of K and V tiles and its own running maximum and sum, so nothing but the end
+// synchronises the CTA; the four results are joined in shared memory.
+//
+// Bound: HBM (the keys and values of a chunk are read once for 16 RT rows).  The rows are
+// the 16 rows of mma.m16n8k16; S stays in registers and is the A operand of the second
+// product as it lies.  Rows of shared memory are padded by 16 bytes, which makes every
+// ldmatrix free of bank conflicts for any head dim.
+constexpr int kRowWarps = 4;
+constexpr int kStepKeys = 16;
+
+template <int D, int RT>
+struct RowCfg {
+    static constexpr int kPitch = D * 2 + 16;
+    static constexpr int kStage = 2 * kStepKeys * kPitch;  // K then V
+    static constexpr int kStages = D <= 64 ? 6 : D <= 96 ? 4 : 3;
+    static constexpr int kQ = RT * 16 * kPitch;
+    static constexpr int kSmem = kQ + kRowWarps * kStages * kStage;
+    static_assert(kRowWarps * RT * 16 * D * 4 <= kRowWarps * kStages * kStage, "the join reuses the ring");
+    static_assert(RT * 16 * kStepKeys * 4 <= kStepKeys * kPitch, "a step's P fits its K tile");
+};
+
+template <typename T, int D, int RT>
+__global__ void __launch_bounds__(kRowWarps * 32) attn_rows_kernel(const AttnParams p) {
+    using C = RowCfg<D, RT>;
+    constexpr int CH = D / 8;  // 16-byte chunks of a row
+    constexpr int S = C::kStages;
+    extern __shared__ __align__(16) unsigned char smem[];
+    __shared__ float s_m[kRowWarps][RT * 16], s_l[kRowWarps][RT * 16];
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    pdl_trigger();
+    // The grids of a call complete in order: this one (the second) ends after the first.
+    struct AtEnd {
+        __device__ ~AtEnd() {
+            if (blockIdx.x == 0 && blockIdx.y == 0) pdl_wait();
+        }
+    } at_end;
+
+    // ---- which rows, which keys
+    const int h = blockIdx.y;
+    Sequence s;
+    const int64_t* list;
+    int tile, part, nrows, keys, k0, k1;
+    if (p.over_prefix) {
+        part = blockIdx.x % p.prefix_splits;
+        tile = blockIdx.x / p.prefix_splits;
+        s.first = 0;
+        s.n = p.tokens;
+        list = p.prefix_pages;
+        keys = p.prefix_len;
+        k0 = part * p.prefix_chunk;
+        k1 = min(keys, k0 + p.prefix_chunk);
+    } else {
+        const int c = blockIdx.x % p.own_chunks, u = blockIdx.x / p.own_chunks;
+        tile = u % p.tiles;
+        s = sequence(p, u / p.tiles);
+        list = p.indices + s.page0;
+        keys = s.len;
+        k0 = c * p.own_chunk;
+        k1 = min(keys, k0 + p.own_chunk);
+        part = p.prefix_splits + c;
+        if (k0 >= keys && !p.direct) return;  // no such chunk: the join does not ask for it
+    }
+    nrows = s.n * p.group - tile * RT * 16;
+    if (nrows <= 0) return;
+    nrows = min(nrows, RT * 16);
+    const int row0 = tile * RT * 16;
+
+    const char* kbase = static_cast<const char*>(p.k) + h * p.k_head * 2;
+    const char* vbase = static_cast<const char*>(p.v) + h * p.v_head * 2;
+    const uint32_t ring = smem_addr(smem) + C::kQ + warp * S * C::kStage;
+    const int kw = k0 + warp * kStepKeys;  // this warp's first key; its steps are 64 keys apart
+    const int steps = max(0, (k1 - kw + kRowWarps * kStepKeys - 1) / (kRowWarps * kStepKeys));
+
+    // lane & 15: the key of a step whose page this lane looks up
+    auto find = [&](int i, int& page, int& slot) {
+        const int at = kw + i * kRowWarps * kStepKeys + (lane & 15);
+        page = -1;
+        slot = 0;
+        if (at < k1) locate(p, list, at, page, slot);
+    };
+    auto fetch = [&](int stage, int page, int slot) {
+        const uint32_t dst = ring + stage * C::kStage;
+#pragma unroll
+        for (int i = 0; i < kStepKeys * CH / 32; ++i) {
+            const int id = i * 32 + lane, r = id / CH, c = id % CH;
+            const int pg = __shfl_sync(kFull, page, r), sl = __shfl_sync(kFull, slot, r);
+            const bool ok = pg >= 0;
+            const int64_t ko = ok ? pg * p.k_page + sl * p.k_slot : 0, vo = ok ? pg * p.v_page + sl * p.v_slot : 0;
+            cp_async16(dst + r * C::kPitch + c * 16, kbase + ko * 2 + c * 16, ok);
+            cp_async16(dst + (kStepKeys + r) * C::kPitch + c * 16, vbase + vo * 2 + c * 16, ok);
+        }
+    };
+    {
+        int page[S], slot[S];
+#pragma unroll
+        for (int i = 0; i < S; ++i) find(i, page[i], slot[i]);
+#pragma unroll
+        for (int i = 0; i < S; ++i) {
+            if (i < steps) fetch(i, page[i], slot[i]);
+            cp_async_commit();
+        }
+    }
+
+    // ---- queries to shared memory, zeros for rows that are not there
+    for (int i = tid; i < RT * 16 * CH; i += kRowWarps * 32) {
+        const int r = i / CH, c = i % CH;
+        uint4 v = make_uint4(0, 0, 0, 0);
+        if (r < nrows) {
+            const int f = row0 + r, t = s.first + f / p.group, qh = h * p.group + f % p.group;
+            v = *reinterpret_cast<const uint4*>(static_cast<const char*>(p.q) + (t * p.q_tok + qh * p.q_head) * 2 + c * 16);
+        }
+        *reinterpret_cast<uint4*>(smem + r * C::kPitch + c * 16) = v;
+    }
+    // ---- keys that each of the thread's rows sees (none where there is no row)
+    int seen[RT][2];
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            const int r = rt * 16 + (lane >> 2) + 8 * e;
+            seen[rt][e] = 0;
+            if (r < nrows) {
+                const int i = (row0 + r) / p.group;
+                if (!p.over_prefix) {
+                    seen[rt][e] = keys_seen(p, s, i, keys, keys);
+                } else if (!p.causal) {
+                    seen[rt][e] = keys;
+                } else {
+                    const Sequence o = sequence(p, sequence_of(p.q_indptr, p.rows, i));
+                    seen[rt][e] = keys_seen(p, o, i - o.first, (int64_t)keys + o.len, keys);
+                }
+            }
+        }
+    __syncthreads();
+
+    uint32_t qf[RT == 1 ? D / 16 : 1][4];
+    const uint32_t qaddr = smem_addr(smem) + (lane & 15) * C::kPitch + (lane >> 4) * 16;
+    if constexpr (RT == 1) {
+#pragma unroll
+        for (int kk = 0; kk < D / 16; ++kk) ldmatrix4(qaddr + kk * 32, qf[kk]);
+    }
+
+    float o[RT][D / 8][4], m[RT][2], l[RT][2];
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+        m[rt][0] = m[rt][1] = -INFINITY;
+        l[rt][0] = l[rt][1] = 0.f;
+#pragma unroll
+        for (int n = 0; n < D / 8; ++n)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[rt][n][e] = 0.f;
+    }
+
+    int stage = 0;
+    for (int it = 0; it < steps; ++it) {
+        int page, slot;
+        find(it + S, page, slot);
+        cp_async_wait<S - 1>();
+        __syncwarp();
+        const uint32_t kt = ring + stage * C::kStage, vt = kt + kStepKeys * C::kPitch;
+        const int key0 = kw + it * kRowWarps * kStepKeys;
+
+        float sc[RT][2][4];
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+            for (int n = 0; n < 2; ++n)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) sc[rt][n][e] = 0.f;
+        const uint32_t kaddr = kt + ((lane & 7) + ((lane >> 4) << 3)) * C::kPitch + ((lane >> 3) & 1) * 16;
+#pragma unroll
+        for (int kk = 0; kk < D / 16; ++kk) {
+            uint32_t b[4];
+            ldmatrix4(kaddr + kk * 32, b);
+#pragma unroll
+            for (int rt = 0; rt < RT; ++rt) {
+                if constexpr (RT == 1) {
+                    mma16816<T>(sc[rt][0], qf[kk], b[0], b[1]);
+                    mma16816<T>(sc[rt][1], qf[kk], b[2], b[3]);
+                } else {
+                    uint32_t a[4];
+                    ldmatrix4(qaddr + rt * 16 * C::kPitch + kk * 32, a);
+                    mma16816<T>(sc[rt][0], a, b[0], b[1]);
+                    mma16816<T>(sc[rt][1], a, b[2], b[3]);
+                }
+            }
+        }
+
+        uint32_t pf[RT][4];
+        bool part_seen = false;  // a row of this lane sees only some of the step's keys
+        const int step_end = min(key0 + kStepKeys, k1);
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const int r = rt * 16 + (lane >> 2) + 8 * e;
+                part_seen |= r < nrows && seen[rt][e] < step_end;
+                float mx = -INFINITY;
+#pragma unroll
+                for (int n = 0; n < 2; ++n)
+#pragma unroll
+                    for (int x = 0; x < 2; ++x) {
+                        float& v = sc[rt][n][2 * e + x];
+                        v = key0 + n * 8 + 2 * (lane & 3) + x < seen[rt][e] ? v * p.scale_log2 : -INFINITY;
+                        mx = fmaxf(mx, v);
+                    }
+                mx = fmaxf(mx, __shfl_xor_sync(kFull, mx, 1));
+                mx = fmaxf(mx, __shfl_xor_sync(kFull, mx, 2));
+                const float mn = fmaxf(m[rt][e], mx), base = mn == -INFINITY ? 0.f : mn;
+                const float keep = exp2_fast(m[rt][e] - base);
+                m[rt][e] = mn;
+                float sum = 0.f;
+#pragma unroll
+                for (int n = 0; n < 2; ++n)
+#pragma unroll
+                    for (int x = 0; x < 2; ++x) {
+                        float& v = sc[rt][n][2 * e + x];
+                        v = exp2_fast(v - base);
+                        sum += v;
+                    }
+                l[rt][e] = l[rt][e] * keep + sum;
+                if (__any_sync(kFull, keep != 1.f)) {
+#pragma unroll
+                    for (int n = 0; n < D / 8; ++n) {
+                        o[rt][n][2 * e] *= keep;
+                        o[rt][n][2 * e + 1] *= keep;
+                    }
+                }
+                // P is rounded to the values' type for the product, as the output is: relative
+                // errors of half an ulp that average out over the keys.  l sums the unrounded P.
+                pf[rt][e] = pack2<T>(sc[rt][0][2 * e], sc[rt][0][2 * e + 1]);
+                pf[rt][2 + e] = pack2<T>(sc[rt][1][2 * e], sc[rt][1][2 * e + 1]);
+            }
+
+        // A value that only some rows see must not reach the others through 0 * NaN: where a
+        // step is seen in part and holds an infinity or NaN, its product is taken row by row.
+        bool by_rows = false;
+        if (__any_sync(kFull, part_seen)) {
+            bool bad = false;
+            for (int i = lane; i < kStepKeys * CH; i += 32)
+                bad |= any_nonfinite<T>(*reinterpret_cast<const uint4*>(smem + (vt - smem_addr(smem)) + (i / CH) * C::kPitch +
+                                                                      (i % CH) * 16));
+            by_rows = __any_sync(kFull, bad);
+        }
+        if (by_rows) {
+            __syncwarp();
+            float* sp = reinterpret_cast<float*>(smem + (kt - smem_addr(smem)));  // the K tile is done with
+#pragma unroll
+            for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+                for (int n = 0; n < 2; ++n)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        sp[(rt * 16 + (lane >> 2) + 8 * (e >> 1)) * kStepKeys + n * 8 + 2 * (lane & 3) + (e & 1)] = sc[rt][n][e];
+            __syncwarp();
+#pragma unroll 1
+            for (int key = 0; key < kStepKeys; ++key) {
+                const T* vr = reinterpret_cast<const T*>(smem + (vt - smem_addr(smem)) + key * C::kPitch) + 2 * (lane & 3);
+#pragma unroll
+                for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        if (key0 + key >= seen[rt][e]) continue;
+                        const float w = sp[(rt * 16 + (lane >> 2) + 8 * e) * kStepKeys + key];
+#pragma unroll
+                        for (int n = 0; n < D / 8; ++n) {
+                            o[rt][n][2 * e] += w * to_f32(vr[n * 8]);
+                            o[rt][n][2 * e + 1] += w * to_f32(vr[n * 8 + 1]);
+                        }
+                    }
+            }
+        } else {
+            const uint32_t vaddr = vt + (lane & 15) * C::kPitch + (lane >> 4) * 16;
+#pragma unroll
+            for (int dn = 0; dn < D / 16; ++dn) {
+                uint32_t b[4];
+                ldmatrix4_trans(vaddr + dn * 32, b);
+#pragma unroll
+                for (int rt = 0; rt < RT; ++rt) {
+                    mma16816<T>(o[rt][2 * dn], pf[rt], b[0], b[1]);
+                    mma16816<T>(o[rt][2 * dn + 1], pf[rt], b[2], b[3]);
+                }
+            }
+        }
+        __syncwarp();
+        if (it + S < steps) fetch(stage, page, slot);
+        cp_async_commit();
+        stage = stage + 1 == S ? 0 : stage + 1;
+    }
+    cp_async_wait<0>();
+    __syncthreads();  // the rings are free
+
+    // ---- join the four warps
+    float* so = reinterpret_cast<float*>(smem + C::kQ) + warp * RT * 16 * D;
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            float sum = l[rt][e];
+            sum += __shfl_xor_sync(kFull, sum, 1);
+            sum += __shfl_xor_sync(kFull, sum, 2);
+            const int r = rt * 16 + (lane >> 2) + 8 * e;
+            if ((lane & 3) == 0) {
+                s_m[warp][r] = m[rt][e];
+                s_l[warp][r] = sum;
+            }
+#pragma unroll
+            for (int n = 0; n < D / 8; ++n)
+                *reinterpret_cast<float2*>(so + r * D + n * 8 + 2 * (lane & 3)) =
+                    make_float2(o[rt][n][2 * e], o[rt][n][2 * e + 1]);
+        }
+    __syncthreads();
+    const float* all = reinterpret_cast<const float*>(smem + C::kQ);
+    for (int i = tid; i < nrows * (D / 4); i += kRowWarps * 32) {
+        const int r = i / (D / 4), c = i % (D / 4) * 4;
+        float top = s_m[0][r];
+#pragma unroll
+        for (int w = 1; w < kRowWarps; ++w) top = fmaxf(top, s_m[w][r]);
+        const float base = top == -INFINITY ? 0.f : top;
+        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+        float sum = 0.f;
+#pragma unroll
+        for (int w = 0; w < kRowWarps; ++w) {
+            const float f = exp2_fast(s_m[w][r] - base);
+            const float4 x = *reinterpret_cast<const float4*>(all + (w * RT * 16 + r) * D + c);
+            if (s_l[w][r] == 0.f) continue;  // no key of this warp is seen (a NaN score leaves l NaN)
+            acc.x += f * x.x, acc.y += f * x.y, acc.z += f * x.z, acc.w += f * x.w;
+            sum += f * s_l[w][r];
+        }
+        const int f = row0 + r, t = s.first + f / p.group, qh = h * p.group + f % p.group;
+        const int64_t row = (int64_t)t * p.q_heads + qh;
+        if (p.direct) {
+            const float inv = sum == 0.f ? 0.f : 1.f / sum;
+            uint2 y;
+            y.x = pack2<T>(acc.x * inv, acc.y * inv);
+            y.y = pack2<T>(acc.z * inv, acc.w * inv);
+            *reinterpret_cast<uint2*>(static_cast<char*>(p.out) + (t * p.o_tok + qh * p.o_head + c) * 2) = y;
+            if (p.lse && c == 0) p.lse[row] = sum == 0.f ? -INFINITY : (top + log2f(sum)) * 0.69314718055994531f;
+        } else {
+            const int64_t at = (int64_t)part * p.tokens * p.q_heads + row;
+            *reinterpret_cast<float4*>(p.part_o + at * D + c) = acc;
+            if (c == 0) p.part_ml[at] = make_float2(top, sum);
+        }
+    }
+}
+
+// ------------------------------------------------------------------ joining the parts
+// One warp a row.  Bound: L2 (the parts were just written), so loads are 16 bytes a lane and
+// four parts are in flight.
+template <typename T, int D>
+__global__ void __launch_bounds__(128) attn_join_kernel(const AttnParams p) {
+    constexpr int VE = D % 128 == 0 ? 4 : D % 64 == 0 ? 2 : 1, NV = D / (32 * VE);
+    const int lane = threadIdx.x & 31;
+    const int64_t all = (int64_t)p.tokens * p.q_heads, row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
+    pdl_wait();
+    if (row >= all) return;
+    const int t = (int)(row / p.q_heads), qh = (int)(row % p.q_heads);
+    int n = p.prefix_splits;
+    if (p.own_chunks > 0) {
+        const Sequence s = sequence(p, sequence_of(p.q_indptr, p.rows, t));
+        if (t >= s.first && t < s.first + s.n) n += (s.len + p.own_chunk - 1) / p.own_chunk;
+    }
+    float top = -INFINITY;
+    for (int i = lane; i < n; i += 32) top = fmaxf(top, p.part_ml[i * all + row].x);
+#pragma unroll
+    for (int x = 16; x; x >>= 1) top = fmaxf(top, __shfl_xor_sync(kFull, top, x));
+    const float base = top == -INFINITY ? 0.f : top;
+    float acc[NV * VE], sum = 0.f;
+#pragma unroll
+    for (int i = 0; i < NV * VE; ++i) acc[i] = 0.f;
+#pragma unroll 4
+    for (int i = 0; i < n; ++i) {
+        const float2 ml = p.part_ml[i * all + row];
+        const float* x = p.part_o + (i * all + row) * D;
+        const float f = exp2_fast(ml.x - base);
+        if (ml.y == 0.f) continue;  // nothing seen there
+        sum += f * ml.y;
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+            float v[VE];
+            if constexpr (VE == 4) {
+                const float4 y = *reinterpret_cast<const float4*>(x + (j * 32 + lane) * 4);
+                v[0] = y.x, v[1] = y.y, v[2] = y.z, v[3] = y.w;
+            } else if constexpr (VE == 2) {
+                const float2 y = *reinterpret_cast<const float2*>(x + (j * 32 + lane) * 2);
+                v[0] = y.x, v[1] = y.y;
+            } else {
+                v[0] = x[j * 32 + lane];
+            }
+#pragma unroll
+            for (int e = 0; e < VE; ++e) acc[j * VE + e] += f * v[e];
+        }
+    }
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+    T* out = static_cast<T*>(p.out) + t * p.o_tok + qh * p.o_head;
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+        T* y = out + (j * 32 + lane) * VE;
+        if constexpr (VE == 4) {
+            *reinterpret_cast<uint2*>(y) = make_uint2(pack2<T>(acc[j * 4] * inv, acc[j * 4 + 1] * inv),
+                                                      pack2<T>(acc[j * 4 + 2] * inv, acc[j * 4 + 3] * inv));
+        } else if constexpr (VE == 2) {
+            *reinterpret_cast<uint32_t*>(y) = pack2<T>(acc[j * 2] * inv, acc[j * 2 + 1] * inv);
+        } else {
+            *y = from_f32<T>(acc[j] * inv);
+        }
+    }
+    if (p.lse && lane == 0) p.lse[row] = sum == 0.f ? -INFINITY : (top + log2f(sum)) * 0.69314718055994531f;
+}
+
+// ------------------------------------------------------------------ host
+struct Plan {
+    AttnParams p;
+    int rt_own, rt_prefix;  // row tiles of 16 rows of a CTA
+    int64_t own_units, prefix_units;
+    size_t ws_bytes;
+};
+
+int make_plan(const tg_prefix_attention_args* a, Plan* plan, const char* op) {
+    if (!a) return set_error(TG_EINVAL, "%s: null arguments", op);
+    int rc = check_cache(a->cache, op);
+    if (rc == TG_OK && !a->pages) rc = set_error(TG_EINVAL, "%s: null page table", op);
+    if (rc != TG_OK) return rc;
+    const tg_paged_kv& c = *a->cache;
+    const tg_csr& t = *a->pages;
+    if (c.dim != 64 && c.dim != 96 && c.dim != 128 && c.dim != 256)
+        return set_error(TG_EUNSUPPORTED, "%s: head dim must be 64, 96, 128 or 256 (got %d)", op, c.dim);
+    if (a->q_heads < 1 || a->q_heads % c.heads)
+        return set_error(TG_EINVAL, "%s: q_heads (%d) must be a multiple of the cache's heads (%d)", op, a->q_heads,
+                         c.heads);
+    if (a->tokens < 0 || a->tokens > INT32_MAX || t.rows < 0 || t.rows > INT32_MAX || t.nnz < 0)
+        return set_error(TG_EINVAL, "%s: bad size (tokens=%lld sequences=%lld pages=%lld)", op, (long long)a->tokens,
+                         (long long)t.rows, (long long)t.nnz);
+    if (a->prefix_len < 0 || a->n_prefix_pages < 0 || a->prefix_len > INT32_MAX / 2 ||
+        ceil_div(a->prefix_len, c.page_size) > a->n_prefix_pages)
+        return set_error(TG_EINVAL, "%s: prefix_len (%lld) must be in [0, 2^30) and inside its %lld pages of %lld", op,
+                         (long long)a->prefix_len, (long long)a->n_prefix_pages, (long long)c.page_size);
+    if (a->max_seq_len < 0 || a->max_q_len < 0)
+        return set_error(TG_EINVAL, "%s: negative max_seq_len or max_q_len", op);
+    if (!(a->scale > 0.0) || a->scale > 1e30) return set_error(TG_EINVAL, "%s: scale must be positive", op);
+    if (a->flags & ~(TG_FLAG_CAUSAL | TG_FLAG_BOUNDS_CHECK))
+        return set_error(TG_EINVAL, "%s: unknown flags 0x%x", op, a->flags);
+    const int64_t slots = t.nnz > INT32_MAX / c.page_size ? INT32_MAX / 2 : t.nnz * c.page_size;
+    const int64_t max_seq = std::min({a->max_seq_len, slots, (int64_t)INT32_MAX / 2});
+    const int64_t max_q = a->q_indptr ? std::min(a->max_q_len, a->tokens) : 1;
+
+    AttnParams& p = plan->p;
+    p = {};
+    p.q = a->q.data, p.k = c.k, p.v = c.v, p.out = a->out.data, p.lse = a->lse;
+    p.q_tok = a->q.token_stride, p.q_head = a->q.head_stride;
+    p.o_tok = a->out.token_stride, p.o_head = a->out.head_stride;
+    p.k_page = c.k_page_stride, p.k_slot = c.k_slot_stride, p.k_head = c.k_head_stride;
+    p.v_page = c.v_page_stride, p.v_slot = c.v_slot_stride, p.v_head = c.v_head_stride;
+    p.pages = (int)c.pages, p.page_size = (int)c.page_size;
+    p.page_shift = -1;
+    for (int i = 0; i < 31; ++i)
+        if (c.page_size == (1ll << i)) p.page_shift = i;
+    p.q_heads = a->q_heads, p.kv_heads = c.heads, p.group = a->q_heads / c.heads;
+    p.tokens = (int)a->tokens, p.rows = (int)t.rows;
+    p.q_indptr = a->q_indptr, p.indptr = t.indptr, p.indices = t.indices, p.seq_len = a->seq_len;
+    p.prefix_pages = a->prefix_pages, p.nnz = t.nnz;
+    p.max_seq = (int)max_seq, p.max_q = (int)max_q, p.prefix_len = (int)a->prefix_len;
+    p.scale_log2 = (float)(a->scale * 1.4426950408889634);
+    p.causal = (a->flags & TG_FLAG_CAUSAL) != 0;
+
+    // Enough CTAs to fill the GPU several times over, each with at least 64 keys a warp.
+    const int64_t rows_own = max_q * p.group, rows_all = a->tokens * p.group;
+    plan->rt_own = rows_own > 16 && c.dim <= 128 ? 2 : 1;
+    plan->rt_prefix = rows_all > 16 && c.dim <= 128 ? 2 : 1;
+    const int64_t target = kSMs * 8;
+    const int64_t tiles_own = ceil_div(std::max<int64_t>(rows_own, 1), 16 * plan->rt_own);
+    const int64_t tiles_all = ceil_div(std::max<int64_t>(rows_all, 1), 16 * plan->rt_prefix);
+    if (p.prefix_len > 0) {
+        int64_t n = std::max<int64_t>(1, target / (tiles_all * c.heads));
+        p.prefix_chunk = (int)std::max<int64_t>(256, ceil_div(ceil_div(p.prefix_len, n), 64) * 64);
+        p.prefix_splits = (int)ceil_div(p.prefix_len, p.prefix_chunk);
+    }
+    if (max_seq > 0 || p.prefix_len == 0) {
+        int64_t n = std::max<int64_t>(1, target / std::max<int64_t>(1, t.rows * tiles_own * c.heads));
+        p.own_chunk = (int)std::max<int64_t>(256, ceil_div(ceil_div(max_seq, n), 64) * 64);
+        p.own_chunks = (int)std::max<int64_t>(1, ceil_div(max_seq, p.own_chunk));
+    }
+    plan->own_units = t.rows * tiles_own * p.own_chunks;
+    plan->prefix_units = tiles_all * p.prefix_splits;
+    if (plan->own_units > INT32_MAX || plan->prefix_units > INT32_MAX || c.heads > 65535)
+        return set_error(TG_EUNSUPPORTED, "%s: too many rows for one launch", op);
+    p.tiles = (int)tiles_own;
+    const int parts = p.prefix_splits + p.own_chunks;
+    p.direct = parts == 1;
+    const size_t rows = (size_t)a->tokens * a->q_heads;
+    const size_t o_bytes = (parts * rows * c.dim * sizeof(float) + 255) / 256 * 256;
+    plan->ws_bytes = p.direct || rows == 0 ? 0 : o_bytes + (parts * rows * sizeof(float2) + 255) / 256 * 256;
+    return TG_OK;
+}
+
+template <typename T, int D, int RT>
+int rows_launch(const AttnParams& p, int64_t units, bool pdl, cudaStream_t st) {
+    using C = RowCfg<D, RT>;
+    static_assert(C::kSmem <= 227 * 1024 - 1024, "shared memory of a CTA");
+    auto kernel = attn_rows_kernel<T, D, RT>;
+    const int rc = check_cuda(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem),
+                              "cudaFuncSetAttribute");
+    if (rc != TG_OK) return rc;
+    const dim3 grid((unsigned)units, (unsigned)p.kv_heads);
+    if (pdl) return launch_pdl("attn_rows_kernel", kernel, grid, kRowWarps * 32, C::kSmem, st, p);
+    kernel<<<grid, kRowWarps * 32, C::kSmem, st>>>(p);
+    return check_launch("attn_rows_kernel");
+}
+
+template <typename T, int D>
+int attn_run(const Plan& plan, void* ws, cudaStream_t st) {
+    AttnParams p = plan.p;
+    const size_t rows = (size_t)p.tokens * p.q_heads;
+    const size_t parts = p.prefix_splits + p.own_chunks;
+    p.part_o = static_cast<float*>(ws);
+    p.part_ml = reinterpret_cast<float2*>(static_cast<char*>(ws) + (parts * rows * D * sizeof(float) + 255) / 256 * 256);
+    bool first = true;
+    auto launch = [&](const AttnParams& q, int rt, int64_t units) {
+        const bool pdl = !first;
+        first = false;
+        if constexpr (D <= 128) {
+            if (rt == 2) return rows_launch<T, D, 2>(q, units, pdl, st);
+        }
+        return rows_launch<T, D, 1>(q, units, pdl, st);
+    };
+    if (p.prefix_splits > 0) {
+        AttnParams q = p;
+        q.over_prefix = 1;
+        const int rc = launch(q, plan.rt_prefix, plan.prefix_units);
+        if (rc != TG_OK) return rc;
+    }
+    if (p.own_chunks > 0) {
+        const int rc = launch(p, plan.rt_own, plan.own_units);
+        if (rc != TG_OK) return rc;
+    }
+    if (p.direct) return TG_OK;
+    return launch_pdl("attn_join_kernel", attn_join_kernel<T, D>, dim3((unsigned)ceil_div((int64_t)rows, 4)), 128, 0, st,
+                      p);
+}
+
+template <typename T>
+int attention(const tg_prefix_attention_args* a, void* ws, size_t ws_bytes, tg_stream_t stream, const char* op) {
+    Plan plan;
+    int rc = make_plan(a, &plan, op);
+    if (rc == TG_OK) rc = check_table(a->pages, a->cache, a->tokens, a->q_indptr, a->seq_len, op);
+    if (rc != TG_OK) return rc;
+    if (a->tokens == 0) return TG_OK;
+    const tg_paged_kv& c = *a->cache;
+    if (!a->q.data || !a->out.data) return set_error(TG_EINVAL, "%s: null q/out", op);
+    if (a->prefix_len > 0 && !a->prefix_pages) return set_error(TG_EINVAL, "%s: null prefix_pages", op);
+    const uint64_t at = reinterpret_cast<uint64_t>(a->q.data) | reinterpret_cast<uint64_t>(a->out.data) |
+                        reinterpret_cast<uint64_t>(c.k) | reinterpret_cast<uint64_t>(c.v);
+    const uint64_t strides = (uint64_t)(a->q.token_stride | a->q.head_stride | a->out.token_stride | a->out.head_stride |
+                                        c.k_page_stride | c.k_slot_stride | c.k_head_stride | c.v_page_stride |
+                                        c.v_slot_stride | c.v_head_stride);
+    if (at % 16 || strides % 8)
+        return set_error(TG_EINVAL, "%s: rows must be 16-byte aligned (strides multiples of 8 elements)", op);
+    if (ws_bytes < plan.ws_bytes || (plan.ws_bytes && !ws))
+        return set_error(TG_ENOMEM, "%s: workspace of %zu bytes, %zu needed", op, ws ? ws_bytes : (size_t)0,
+                         plan.ws_bytes);
+    if (reinterpret_cast<uint64_t>(ws) % 16)
+        return set_error(TG_EINVAL, "%s: the workspace must be 16-byte aligned", op);
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    if (a->flags & TG_FLAG_BOUNDS_CHECK) {
+        rc = paged_bounds_check(*a->pages, c.page_size, a->seq_len, a->max_seq_len, a->tokens, a->q_indptr,
+                                a->q_indptr ? a->max_q_len : 1, a->prefix_pages, ceil_div(a->prefix_len, c.page_size),
+                                false, op, st);
+        if (rc != TG_OK) return rc;
+    }
+    switch (c.dim) {
+        case 64: return attn_run<T, 64>(plan, ws, st);
+        case 96: return attn_run<T, 96>(plan, ws, st);
+        case 128: return attn_run<T, 128>(plan, ws, st);
+        default: return attn_run<T, 256>(plan, ws, st);
+    }
+}
+
+}  // namespace
+}  // namespace tg
+
+extern "C" {
+
+size_t tg_prefix_attention_workspace_bytes(const tg_prefix_attention_args* a) {
+    tg::Plan plan;
+    return tg::make_plan(a, &plan, "tg_prefix_attention") == TG_OK ? plan.ws_bytes : 0;
+}
+
+int tg_prefix_attention_f16(const tg_prefix_attention_args* a, void* workspace, size_t workspace_bytes,
+                            tg_stream_t stream) {
+    return tg::attention<__half>(a, workspace, workspace_bytes, stream, "tg_prefix_attention_f16");
+}
+
+int tg_prefix_attention_bf16(const tg_prefix_attention_args* a, void* workspace, size_t workspace_bytes,
+                             tg_stream_t stream) {
+    return tg::attention<__nv_bfloat16>(a, workspace, workspace_bytes, stream, "tg_prefix_attention_bf16");
+}
+
+}  // extern "C"

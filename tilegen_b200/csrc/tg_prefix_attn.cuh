@@ -1,0 +1,80 @@
+// Parameters and device pieces shared by the shared-prefix attention kernels.
+//
+// The keys of a sequence are cut into parts: splits of the shared prefix and chunks of the
+// sequence's own pages.  Each part leaves, for each of its rows (token, query head), the
+// maximum m and sum l of exp2(s - m) over its keys (s: the scores times log2 e) and the
+// sum of exp2(s - m) v, all in 32 bits; the parts of a row are joined by
+//   M = max m_i,  out = sum_i exp2(m_i - M) o_i / sum_i exp2(m_i - M) l_i.
+#pragma once
+
+#include "tg_paged.cuh"
+
+namespace tg {
+
+struct AttnParams {
+    const void *q, *k, *v;
+    void* out;
+    float* lse;
+    int64_t q_tok, q_head, o_tok, o_head;
+    int64_t k_page, k_slot, k_head, v_page, v_slot, v_head;
+    int pages, page_size, page_shift;  // page_shift: log2(page_size), -1 where it is no power of two
+    int q_heads, kv_heads, group;
+    int tokens, rows;  // queries, sequences
+    const int64_t *q_indptr, *indptr, *indices, *seq_len, *prefix_pages;
+    int64_t nnz;
+    int max_seq, max_q, prefix_len;
+    float scale_log2;
+    int causal;
+    // parts
+    int prefix_splits, prefix_chunk;  // keys of a split
+    int own_chunks, own_chunk;        // most chunks of a sequence, keys of a chunk
+    int tiles;                        // row tiles of a sequence (own) or of all rows (prefix)
+    int over_prefix;                  // this launch: the prefix, else the sequences' own pages
+    int direct;                       // the only part: rows are finished here
+    float* part_o;                    // [part][token][head][dim]
+    float2* part_ml;                  // [part][token][head]: m, l
+};
+
+// One sequence as the kernels see it: its tokens, its own pages and length.
+struct Sequence {
+    int64_t page0;
+    int first, n, len;
+};
+
+__device__ __forceinline__ Sequence sequence(const AttnParams& p, int64_t b) {
+    Sequence s;
+    int64_t first, n, npages;
+    tokens_of(p.q_indptr, p.tokens, b, first, n);
+    pages_of(p.indptr, p.nnz, b, s.page0, npages);
+    s.first = (int)first;
+    s.n = (int)min(n, (int64_t)p.max_q);
+    const int64_t len = min(min(p.seq_len[b], npages * p.page_size), (int64_t)p.max_seq);
+    s.len = (int)max(len, (int64_t)0);
+    return s;
+}
+
+// Keys that the i-th query of a sequence sees among the first `whole`, of `total` keys.
+__device__ __forceinline__ int keys_seen(const AttnParams& p, const Sequence& s, int i, int64_t total, int whole) {
+    if (!p.causal) return whole;
+    return (int)min(max(total - s.n + i + 1, (int64_t)0), (int64_t)whole);
+}
+
+// Page and slot of token `at` of a page list; page -1 where the list names no page of the cache.
+__device__ __forceinline__ void locate(const AttnParams& p, const int64_t* list, int at, int& page, int& slot) {
+    int j;
+    if (p.page_shift >= 0) {
+        j = at >> p.page_shift;
+        slot = at & (p.page_size - 1);
+    } else {
+        j = at / p.page_size;
+        slot = at - j * p.page_size;
+    }
+    const int64_t id = __ldg(list + j);
+    page = id >= 0 && id < p.pages ? (int)id : -1;
+}
+
+// tg_prefix_attn_tc.cu
+template <typename T>
+int attn_tc_run(const AttnParams& p, int dim, bool pdl, cudaStream_t st);
+
+}  // namespace tg

@@ -15,6 +15,7 @@ from typing import List, Optional
 PKG_DIR = os.path.dirname(os.path.abspath(__file__))
 REPO_DIR = os.path.dirname(PKG_DIR)
 HEADER = os.path.join(REPO_DIR, "include", "tilegen_b200.h")
+HEADER_PAGED = os.path.join(REPO_DIR, "include", "tilegen_b200_paged.h")
 
 TG_OK = 0
 TG_EINVAL = -1
@@ -34,6 +35,11 @@ TG_FLAG_BOUNDS_CHECK = 1
 TG_FLAG_INJECT_BUG = 2
 TG_FLAG_REUSE_PLAN = 4
 TG_FLAG_INDEX32 = 8
+TG_FLAG_CAUSAL = 16
+TG_FLAG_ROPE_INVERSE = 32
+
+TG_ROPE_HALF = 0
+TG_ROPE_INTERLEAVED = 1
 
 STATUS_NAMES = {
     TG_OK: "TG_OK",
@@ -82,6 +88,80 @@ class TgCsr(ctypes.Structure):
         ("indptr", ctypes.c_void_p),
         ("indices", ctypes.c_void_p),
         ("data", ctypes.c_void_p),
+    ]
+
+
+class TgRope(ctypes.Structure):
+    _fields_ = [
+        ("freq", ctypes.c_void_p),
+        ("rot_dim", ctypes.c_int32),
+        ("layout", ctypes.c_int32),
+        ("scale", ctypes.c_double),
+    ]
+
+
+class TgRows(ctypes.Structure):
+    _fields_ = [
+        ("data", ctypes.c_void_p),
+        ("token_stride", ctypes.c_int64),
+        ("head_stride", ctypes.c_int64),
+    ]
+
+
+class TgPagedKV(ctypes.Structure):
+    _fields_ = [
+        ("k", ctypes.c_void_p),
+        ("v", ctypes.c_void_p),
+        ("pages", ctypes.c_int64),
+        ("page_size", ctypes.c_int64),
+        ("heads", ctypes.c_int32),
+        ("dim", ctypes.c_int32),
+        ("k_page_stride", ctypes.c_int64),
+        ("k_slot_stride", ctypes.c_int64),
+        ("k_head_stride", ctypes.c_int64),
+        ("v_page_stride", ctypes.c_int64),
+        ("v_slot_stride", ctypes.c_int64),
+        ("v_head_stride", ctypes.c_int64),
+    ]
+
+
+class TgKvAppendArgs(ctypes.Structure):
+    _fields_ = [
+        ("cache", ctypes.POINTER(TgPagedKV)),
+        ("pages", ctypes.POINTER(TgCsr)),
+        ("seq_len", ctypes.c_void_p),
+        ("tokens", ctypes.c_int64),
+        ("q_indptr", ctypes.c_void_p),
+        ("k", TgRows),
+        ("v", TgRows),
+        ("rope", ctypes.POINTER(TgRope)),
+        ("q", ctypes.POINTER(TgRows)),
+        ("q_out", ctypes.POINTER(TgRows)),
+        ("q_heads", ctypes.c_int32),
+        ("position_base", ctypes.c_int64),
+        ("positions", ctypes.c_void_p),
+        ("flags", ctypes.c_uint32),
+    ]
+
+
+class TgPrefixAttentionArgs(ctypes.Structure):
+    _fields_ = [
+        ("cache", ctypes.POINTER(TgPagedKV)),
+        ("pages", ctypes.POINTER(TgCsr)),
+        ("seq_len", ctypes.c_void_p),
+        ("max_seq_len", ctypes.c_int64),
+        ("prefix_pages", ctypes.c_void_p),
+        ("n_prefix_pages", ctypes.c_int64),
+        ("prefix_len", ctypes.c_int64),
+        ("tokens", ctypes.c_int64),
+        ("q_indptr", ctypes.c_void_p),
+        ("max_q_len", ctypes.c_int64),
+        ("q_heads", ctypes.c_int32),
+        ("q", TgRows),
+        ("out", TgRows),
+        ("lse", ctypes.c_void_p),
+        ("scale", ctypes.c_double),
+        ("flags", ctypes.c_uint32),
     ]
 
 
@@ -152,6 +232,22 @@ SIGNATURES = {
     "launch_axpy": (None, [_P, _P, _P, _F64, _F64, _I64]),
 }
 
+_ROPE = [ctypes.POINTER(TgRope), ctypes.POINTER(TgRows), ctypes.POINTER(TgRows), _I64, ctypes.c_int32,
+         ctypes.c_int32, _P, ctypes.c_uint32, _P]
+
+# every symbol declared in include/tilegen_b200_paged.h
+SIGNATURES_PAGED = {
+    "tg_rope_f32": (ctypes.c_int, _ROPE),
+    "tg_rope_f16": (ctypes.c_int, _ROPE),
+    "tg_rope_bf16": (ctypes.c_int, _ROPE),
+    "tg_kv_append_f32": (ctypes.c_int, [ctypes.POINTER(TgKvAppendArgs), _P]),
+    "tg_kv_append_f16": (ctypes.c_int, [ctypes.POINTER(TgKvAppendArgs), _P]),
+    "tg_kv_append_bf16": (ctypes.c_int, [ctypes.POINTER(TgKvAppendArgs), _P]),
+    "tg_prefix_attention_workspace_bytes": (_SZ, [ctypes.POINTER(TgPrefixAttentionArgs)]),
+    "tg_prefix_attention_f16": (ctypes.c_int, [ctypes.POINTER(TgPrefixAttentionArgs), _P, _SZ, _P]),
+    "tg_prefix_attention_bf16": (ctypes.c_int, [ctypes.POINTER(TgPrefixAttentionArgs), _P, _SZ, _P]),
+}
+
 _lib: Optional[ctypes.CDLL] = None
 
 
@@ -175,7 +271,7 @@ def load() -> ctypes.CDLL:
         L = ctypes.CDLL(path)
     except OSError as exc:
         raise LibraryError("cannot load %s: %s" % (path, exc)) from exc
-    for name, (res, args) in SIGNATURES.items():
+    for name, (res, args) in {**SIGNATURES, **SIGNATURES_PAGED}.items():
         fn = getattr(L, name)
         fn.restype = res
         fn.argtypes = args
