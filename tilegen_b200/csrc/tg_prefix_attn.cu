@@ -32,42 +32,6 @@ __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], 
                      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
     }
 }
-template <typename T>
-__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
-    if constexpr (std::is_same<T, __half>::value) {
-        const __half2 h = __floats2half2_rn(lo, hi);
-        return *reinterpret_cast<const uint32_t*>(&h);
-    } else {
-        const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
-        return *reinterpret_cast<const uint32_t*>(&h);
-    }
-}
-__device__ __forceinline__ float exp2_fast(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-// 16 bytes to shared memory, zeros where !valid (the source is not read then).
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool valid) {
-    const int n = valid ? 16 : 0;
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
-}
-__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void cp_async_wait() {
-    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
-}
-// Whether one of the eight 16-bit numbers in v is an infinity or NaN.
-template <typename T>
-__device__ __forceinline__ bool any_nonfinite(uint4 v) {
-    constexpr uint32_t kExp = std::is_same<T, __half>::value ? 0x7c00u : 0x7f80u;
-    bool bad = false;
-    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) bad |= (w[i] & kExp) == kExp || ((w[i] >> 16) & kExp) == kExp;
-    return bad;
-}
-
 // ------------------------------------------------------------------ few rows
 // One CTA: RT*16 rows (of one sequence's tokens x group, or of all tokens over the prefix),
 // one key head, one chunk of keys.  Its four warps take 16 keys in turn, each with its own
@@ -484,10 +448,30 @@ __global__ void __launch_bounds__(128) attn_join_kernel(const AttnParams p) {
 // ------------------------------------------------------------------ host
 struct Plan {
     AttnParams p;
-    int rt_own, rt_prefix;  // row tiles of 16 rows of a CTA
+    int rt_own, rt_prefix;  // 16-row tiles of a CTA of the kernel for few rows; 0: the tcgen05 kernel
     int64_t own_units, prefix_units;
     size_t ws_bytes;
 };
+
+// Keys of a split of the prefix for the tcgen05 kernel, by the time that the whole call would
+// take: `units` CTAs for each split, one on an SM, 1.2 us for 128 keys and 5 us to begin and end;
+// the SMs that they leave, and their time after them, go to the own parts (own_bytes at 6 TB/s);
+// and each split adds a partial result of every row, written and read.
+int prefix_chunk(int64_t len, int64_t units, int64_t rows, int dim, double own_bytes) {
+    double best = 1e30;
+    int64_t chunk = 0;
+    for (int64_t n = 1; n <= 128; ++n) {
+        const int64_t c = ceil_div(ceil_div(len, n), 128) * 128, ctas = units * ceil_div(len, c);
+        const double cta = 5.0 + 1.2 * (double)(c / 128);
+        const double prefix = cta * (double)ceil_div(ctas, kSMs);
+        const double all = own_bytes / 6e6 + cta * (double)ctas / kSMs;
+        const double join = (double)ceil_div(len, c) * (double)rows * dim * 8 / 6e6;
+        const double t = std::max(prefix, all) + join;
+        if (t < best * 0.999) best = t, chunk = c;
+        if (c == 128) break;
+    }
+    return (int)chunk;
+}
 
 int make_plan(const tg_prefix_attention_args* a, Plan* plan, const char* op) {
     if (!a) return set_error(TG_EINVAL, "%s: null arguments", op);
@@ -536,21 +520,28 @@ int make_plan(const tg_prefix_attention_args* a, Plan* plan, const char* op) {
     p.scale_log2 = (float)(a->scale * 1.4426950408889634);
     p.causal = (a->flags & TG_FLAG_CAUSAL) != 0;
 
-    // Enough CTAs to fill the GPU several times over, each with at least 64 keys a warp.
+    // The kernel for few rows reads the keys once for each 32 rows, the tcgen05 kernel once for
+    // each 256 (it exists for heads of 64 and 128).
     const int64_t rows_own = max_q * p.group, rows_all = a->tokens * p.group;
-    plan->rt_own = rows_own > 16 && c.dim <= 128 ? 2 : 1;
-    plan->rt_prefix = rows_all > 16 && c.dim <= 128 ? 2 : 1;
-    const int64_t target = kSMs * 8;
-    const int64_t tiles_own = ceil_div(std::max<int64_t>(rows_own, 1), 16 * plan->rt_own);
-    const int64_t tiles_all = ceil_div(std::max<int64_t>(rows_all, 1), 16 * plan->rt_prefix);
+    const bool tc = c.dim == 64 || c.dim == 128;
+    plan->rt_own = tc && rows_own > 32 ? 0 : rows_own > 16 && c.dim <= 128 ? 2 : 1;
+    plan->rt_prefix = tc && rows_all > 32 ? 0 : rows_all > 16 && c.dim <= 128 ? 2 : 1;
+    const int64_t step_own = plan->rt_own ? 64 : 128, target_own = plan->rt_own ? kSMs * 8 : kSMs * 2;
+    const int64_t tiles_own = ceil_div(std::max<int64_t>(rows_own, 1), plan->rt_own ? 16 * plan->rt_own : 256);
+    const int64_t tiles_all = ceil_div(std::max<int64_t>(rows_all, 1), plan->rt_prefix ? 16 * plan->rt_prefix : 256);
     if (p.prefix_len > 0) {
-        int64_t n = std::max<int64_t>(1, target / (tiles_all * c.heads));
-        p.prefix_chunk = (int)std::max<int64_t>(256, ceil_div(ceil_div(p.prefix_len, n), 64) * 64);
+        if (plan->rt_prefix) {
+            const int64_t n = std::max<int64_t>(1, kSMs * 8 / (tiles_all * c.heads));
+            p.prefix_chunk = (int)std::max<int64_t>(256, ceil_div(ceil_div(p.prefix_len, n), 64) * 64);
+        } else {
+            p.prefix_chunk = prefix_chunk(p.prefix_len, tiles_all * c.heads, rows_all * c.heads, c.dim,
+                                          (double)t.nnz * c.page_size * c.heads * c.dim * 4);
+        }
         p.prefix_splits = (int)ceil_div(p.prefix_len, p.prefix_chunk);
     }
     if (max_seq > 0 || p.prefix_len == 0) {
-        int64_t n = std::max<int64_t>(1, target / std::max<int64_t>(1, t.rows * tiles_own * c.heads));
-        p.own_chunk = (int)std::max<int64_t>(256, ceil_div(ceil_div(max_seq, n), 64) * 64);
+        const int64_t n = std::max<int64_t>(1, target_own / std::max<int64_t>(1, t.rows * tiles_own * c.heads));
+        p.own_chunk = (int)std::max<int64_t>(256, ceil_div(ceil_div(max_seq, n), step_own) * step_own);
         p.own_chunks = (int)std::max<int64_t>(1, ceil_div(max_seq, p.own_chunk));
     }
     plan->own_units = t.rows * tiles_own * p.own_chunks;
@@ -591,6 +582,9 @@ int attn_run(const Plan& plan, void* ws, cudaStream_t st) {
     auto launch = [&](const AttnParams& q, int rt, int64_t units) {
         const bool pdl = !first;
         first = false;
+        if constexpr (D == 64 || D == 128) {
+            if (rt == 0) return attn_tc_run<T>(q, D, units, pdl, st);
+        }
         if constexpr (D <= 128) {
             if (rt == 2) return rows_launch<T, D, 2>(q, units, pdl, st);
         }

@@ -73,8 +73,44 @@ __device__ __forceinline__ void locate(const AttnParams& p, const int64_t* list,
     page = id >= 0 && id < p.pages ? (int)id : -1;
 }
 
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+    if constexpr (std::is_same<T, __half>::value) {
+        const __half2 h = __floats2half2_rn(lo, hi);
+        return *reinterpret_cast<const uint32_t*>(&h);
+    } else {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+        return *reinterpret_cast<const uint32_t*>(&h);
+    }
+}
+__device__ __forceinline__ float exp2_fast(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+// 16 bytes to shared memory, zeros where !valid (the source is not read then).
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool valid) {
+    const int n = valid ? 16 : 0;
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_async_wait() {
+    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+// Whether one of the eight 16-bit numbers in v is an infinity or NaN.
+template <typename T>
+__device__ __forceinline__ bool any_nonfinite(uint4 v) {
+    constexpr uint32_t kExp = std::is_same<T, __half>::value ? 0x7c00u : 0x7f80u;
+    bool bad = false;
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) bad |= (w[i] & kExp) == kExp || ((w[i] >> 16) & kExp) == kExp;
+    return bad;
+}
+
 // tg_prefix_attn_tc.cu
 template <typename T>
-int attn_tc_run(const AttnParams& p, int dim, bool pdl, cudaStream_t st);
+int attn_tc_run(const AttnParams& p, int dim, int64_t units, bool pdl, cudaStream_t st);
 
 }  // namespace tg

@@ -1,0 +1,559 @@
+// Attention of many rows at once (tcgen05): the shared prefix of a batch of more than a few
+// rows, and sequences with many query tokens.
+//
+// A CTA takes up to 256 rows (two tiles of 128) of one key head and a range of keys, 128 at a
+// time.  S = Q K^T of a tile lands in TMEM; the tile's warpgroup (one thread a row, so neither
+// the maximum nor the sum crosses lanes) turns it into P, writes P over S in the values' type,
+// and O += P V reads P from there.  While one tile's softmax runs, the tensor core works for
+// the other.
+//
+//   TMEM columns      [0,128) S0/P0   [128,256) S1/P1   [256,256+D) O0   [384,384+D) O1
+//   warps 0-3, 4-7    softmax of tile 0, 1: S -> P, the running maximum and sum, O at the end
+//   warps 8-11        K and V tiles into a ring of shared memory (cp.async: a row's address
+//                     comes from the page table, so any page size and stride will do, and rows
+//                     past the end are zeros), swizzled as the descriptors say
+//   warp 12           issues the matrix instructions
+//
+// O is rescaled only where a row's maximum has grown by more than 2^8 since the value that P is
+// taken relative to: P stays below 2^8, far inside the range of either type and of the 32-bit
+// sums, and the relative precision of P is that of any other reference.
+#include "tg_prefix_attn.cuh"
+
+namespace tg {
+namespace {
+
+// ------------------------------------------------------------------ tcgen05
+__device__ __forceinline__ void tmem_alloc(uint32_t dst, uint32_t cols) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(dst), "r"(cols) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void tmem_free(uint32_t addr, uint32_t cols) {
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(addr), "r"(cols) : "memory");
+}
+__device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void fence_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+// D (+)= A B, A and B in shared memory.
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t add) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(add)
+        : "memory");
+}
+// D (+)= A B, A in TMEM.
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t add) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(add)
+        : "memory");
+}
+// The barrier completes when the matrix instructions issued so far have.
+__device__ __forceinline__ void commit(uint32_t bar) {
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void arrive(uint32_t bar) {
+    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void tmem_ld32(uint32_t addr, uint32_t* r) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+        "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+          "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+          "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        : "r"(addr)
+        : "memory");
+}
+__device__ __forceinline__ void tmem_st32(uint32_t addr, const uint32_t* r) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
+        "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::
+            "r"(addr),
+        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+        "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]),
+        "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]),
+        "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+        : "memory");
+}
+__device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t* r) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(
+            addr),
+        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+        "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+        : "memory");
+}
+// Shared-memory operand of rows of 128 bytes, 128-byte swizzle, 8 rows 1024 bytes apart; `lead`:
+// bytes between blocks of 64 elements of the long axis of a transposed operand.
+__device__ __forceinline__ uint64_t operand(uint32_t addr, uint32_t lead) {
+    return (uint64_t)((addr & 0x3ffff) >> 4) | (uint64_t)(lead >> 4) << 16 | (uint64_t)(1024 >> 4) << 32 |
+           (uint64_t)1 << 46 | (uint64_t)2 << 61;
+}
+
+constexpr int kTile = 128;   // rows of a tile, keys of a step
+constexpr int kThreads = 512;
+constexpr uint32_t kCols = 512;
+constexpr uint32_t kColO = 256;
+constexpr float kGrow = 8.f;
+
+template <int D>
+struct TcCfg {
+    static constexpr int kBlock = kTile * D * 2;  // bytes of a tile of Q, K or V
+    static constexpr int kHalf = kTile * 128;     // of 64 of its columns
+    static constexpr int kStages = D == 128 ? 5 : 8;
+    static constexpr int kLag = 3;  // fills under way beside the one being issued
+    static constexpr int kSmem = (2 + kStages) * kBlock + 2048;
+    // A producer that waits for a free stage has delivered all but the last kLag fills, and the
+    // next to be freed is consumed once the one behind it has arrived.
+    static_assert(kLag <= kStages - 2, "the ring cannot stall");
+};
+
+struct TcShared {
+    uint64_t full[8], empty[8], s_full[2], p_full[2], o_done[2];
+    uint32_t tmem;
+    int min_seen;
+    int bad;   // a value that only some rows see is not finite
+    int fail;  // a wait ran out
+};
+
+// Bounded wait; false once one has run out in this CTA (2 s; every wait here is microseconds).
+__device__ __forceinline__ bool wait(uint32_t bar, uint32_t parity, volatile int* fail) {
+    if (mbar_try(bar, parity)) return true;
+    const uint64_t t0 = globaltimer_ns();
+    for (;;) {
+        if (mbar_try(bar, parity)) return true;
+        if (*fail) return false;
+        if (globaltimer_ns() - t0 > 2000000000ull) {
+            *fail = 1;
+            return false;
+        }
+    }
+}
+
+// One row the long way, a warp: only for a row that does not see a value that is not finite
+// while others of its tile do.  acc: D / 32 elements a lane.
+template <typename T, int D>
+__device__ __noinline__ void row_alone(const AttnParams& p, const int64_t* list, const T* q, const char* kbase,
+                                       const char* vbase, int k0, int k1, float* acc, float& m, float& l) {
+    constexpr int E = D / 32;
+    const int lane = threadIdx.x & 31;
+    m = -INFINITY, l = 0.f;
+    float x[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) x[e] = to_f32(q[lane * E + e]), acc[e] = 0.f;
+    for (int key = k0; key < k1; ++key) {
+        int page, slot;
+        locate(p, list, key, page, slot);
+        const T* kr = reinterpret_cast<const T*>(kbase) + (int64_t)page * p.k_page + slot * p.k_slot + lane * E;
+        const T* vr = reinterpret_cast<const T*>(vbase) + (int64_t)page * p.v_page + slot * p.v_slot + lane * E;
+        float s = 0.f;
+        if (page >= 0)
+#pragma unroll
+            for (int e = 0; e < E; ++e) s += x[e] * to_f32(kr[e]);
+#pragma unroll
+        for (int i = 16; i; i >>= 1) s += __shfl_xor_sync(kFull, s, i);
+        s *= p.scale_log2;
+        const float mn = fmaxf(m, s), base = mn == -INFINITY ? 0.f : mn;
+        const float keep = exp2_fast(m - base), w = exp2_fast(s - base);
+        m = mn;
+        l = l * keep + w;
+#pragma unroll
+        for (int e = 0; e < E; ++e) acc[e] = acc[e] * keep + (page >= 0 ? w * to_f32(vr[e]) : 0.f);
+    }
+}
+
+template <typename T, int D>
+__global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const AttnParams p) {
+    using C = TcCfg<D>;
+    constexpr int CH = D / 8;  // 16-byte chunks of a row
+    extern __shared__ unsigned char smem_raw[];
+    __shared__ TcShared sh;
+    unsigned char* smem = smem_raw + ((1024 - (smem_addr(smem_raw) & 1023)) & 1023);
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    pdl_trigger();
+
+    // ---- which rows, which keys (as in the kernel for few rows)
+    const int h = blockIdx.y;
+    Sequence s;
+    const int64_t* list;
+    int tile, part, keys, k0, k1;
+    if (p.over_prefix) {
+        part = blockIdx.x % p.prefix_splits;
+        tile = blockIdx.x / p.prefix_splits;
+        s.first = 0;
+        s.n = p.tokens;
+        list = p.prefix_pages;
+        keys = p.prefix_len;
+        k0 = part * p.prefix_chunk;
+        k1 = min(keys, k0 + p.prefix_chunk);
+    } else {
+        const int c = blockIdx.x % p.own_chunks, u = blockIdx.x / p.own_chunks;
+        tile = u % p.tiles;
+        s = sequence(p, u / p.tiles);
+        list = p.indices + s.page0;
+        keys = s.len;
+        k0 = c * p.own_chunk;
+        k1 = min(keys, k0 + p.own_chunk);
+        part = p.prefix_splits + c;
+    }
+    const int row0 = tile * 2 * kTile;
+    const int nrows = min(s.n * p.group - row0, 2 * kTile);
+    // grids of a call complete in order: this one, if it is the second, ends after the first
+    const bool work = nrows > 0 && (p.over_prefix || p.direct || k0 < keys);
+    if (!work) {
+        if (blockIdx.x == 0 && blockIdx.y == 0) pdl_wait();
+        return;
+    }
+    if (!p.over_prefix)  // no row sees more than the last one
+        k1 = min(k1, keys_seen(p, s, (row0 + nrows - 1) / p.group, keys, keys));
+    const int steps = k1 > k0 ? (k1 - k0 + kTile - 1) / kTile : 0;
+    const int ntiles = nrows > kTile ? 2 : 1;
+
+    const uint32_t sq = smem_addr(smem), ring = sq + 2 * C::kBlock;
+    const char* kbase = static_cast<const char*>(p.k) + h * p.k_head * 2;
+    const char* vbase = static_cast<const char*>(p.v) + h * p.v_head * 2;
+    const uint32_t b_full = smem_addr(sh.full), b_empty = smem_addr(sh.empty), b_s = smem_addr(sh.s_full),
+                   b_p = smem_addr(sh.p_full), b_o = smem_addr(sh.o_done);
+    volatile int* fail = &sh.fail;
+
+    if (warp == 12) {
+        tmem_alloc(smem_addr(&sh.tmem), kCols);
+        if (lane == 0) {
+            for (int i = 0; i < C::kStages; ++i) {
+                mbar_init(&sh.full[i], 128);
+                mbar_init(&sh.empty[i], 1);
+            }
+            for (int i = 0; i < 2; ++i) {
+                mbar_init(&sh.s_full[i], 1);
+                mbar_init(&sh.p_full[i], 128);
+                mbar_init(&sh.o_done[i], 1);
+            }
+            sh.min_seen = INT_MAX;
+            sh.bad = 0;
+            sh.fail = 0;
+            fence_mbar_init();
+        }
+    }
+    __syncthreads();
+
+    // ---- queries (swizzled, zeros where there is no row) and what each row sees
+    const int my = warp >> 2;  // the softmax tile of warps 0-7
+    const int row = tid;       // of the CTA, threads 0-255
+    int seen = 0;              // keys that the thread's row sees, up to k1
+    if (warp < 8) {
+        const int rt = tid & 127;
+        if (my < ntiles) {
+            for (int i = rt; i < kTile * CH; i += 128) {
+                const int r = i / CH, c = i % CH, f = my * kTile + r;
+                uint4 v = make_uint4(0, 0, 0, 0);
+                if (f < nrows) {
+                    const int t = s.first + (row0 + f) / p.group, qh = h * p.group + (row0 + f) % p.group;
+                    v = *reinterpret_cast<const uint4*>(static_cast<const char*>(p.q) +
+                                                        (t * p.q_tok + qh * p.q_head) * 2 + c * 16);
+                }
+                *reinterpret_cast<uint4*>(smem + my * C::kBlock + (c >> 3) * C::kHalf + r * 128 + (((c ^ r) & 7) << 4)) = v;
+            }
+            fence_async();
+        }
+        if (row < nrows) {
+            const int i = (row0 + row) / p.group;
+            if (!p.over_prefix) {
+                seen = keys_seen(p, s, i, keys, keys);
+            } else if (!p.causal) {
+                seen = keys;
+            } else {
+                const Sequence o = sequence(p, sequence_of(p.q_indptr, p.rows, i));
+                seen = keys_seen(p, o, i - o.first, (int64_t)keys + o.len, keys);
+            }
+            seen = max(min(seen, k1), 0);
+            if (seen < k1) atomicMin(&sh.min_seen, seen);
+        }
+    }
+    fence_before();
+    __syncthreads();
+    fence_after();
+    const uint32_t tmem = sh.tmem;
+
+    if (warp >= 12) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+        if (warp == 12 && lane == 0 && steps > 0) {
+            constexpr uint32_t kType = std::is_same<T, __half>::value ? 0 : 1;
+            constexpr uint32_t kBase = 1u << 4 | kType << 7 | kType << 10 | (kTile / 16) << 24;
+            constexpr uint32_t kQK = kBase | (kTile / 8) << 17;
+            constexpr uint32_t kPV = kBase | 1u << 16 | (D / 8) << 17;
+            auto qk = [&](int i, int fill) {
+                const uint32_t q = sq + i * C::kBlock, k = ring + fill % C::kStages * C::kBlock;
+#pragma unroll
+                for (int kk = 0; kk < D / 16; ++kk) {
+                    const uint32_t off = (kk >> 2) * C::kHalf + (kk & 3) * 32;
+                    mma_ss(tmem + i * kTile, operand(q + off, 16), operand(k + off, 16), kQK, kk > 0);
+                }
+                commit(b_s + i * 8);
+            };
+            auto full = [&](int fill) {
+                const bool ok = wait(b_full + fill % C::kStages * 8, fill / C::kStages & 1, fail);
+                fence_after();
+                return ok;
+            };
+            bool ok = full(0);
+            if (ok) {
+                for (int i = 0; i < ntiles; ++i) qk(i, 0);
+                commit(b_empty);
+            }
+            for (int j = 0; ok && j < steps; ++j) {
+                const int fv = 2 * j + 1, fk = 2 * j + 2;
+                ok = full(fv) && (j + 1 == steps || full(fk));
+                const uint32_t v = ring + fv % C::kStages * C::kBlock;
+                for (int i = 0; ok && i < ntiles; ++i) {
+                    ok = wait(b_p + i * 8, j & 1, fail);
+                    if (!ok) break;
+                    fence_after();
+#pragma unroll
+                    for (int kk = 0; kk < kTile / 16; ++kk)
+                        mma_ts(tmem + kColO + i * kTile, tmem + i * kTile + kk * 8, operand(v + kk * 2048, C::kHalf), kPV,
+                               j > 0 || kk > 0);
+                    commit(b_o + i * 8);
+                    // S of the next step goes over P: the tensor core works in the order of issue
+                    if (j + 1 < steps) qk(i, fk);
+                }
+                if (!ok) break;
+                commit(b_empty + fv % C::kStages * 8);
+                if (j + 1 < steps) commit(b_empty + fk % C::kStages * 8);
+            }
+        }
+    } else if (warp >= 8) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+        const int pw = warp - 8;  // rows 32 pw .. 32 pw + 31 of each tile
+        const int min_seen = sh.min_seen;
+        int page = -1, slot = 0;
+        auto find = [&](int j) {
+            const int at = k0 + j * kTile + pw * 32 + lane;
+            page = -1, slot = 0;
+            if (at < k1) locate(p, list, at, page, slot);
+        };
+        auto deliver = [&](int fill) {
+            const uint32_t dst = ring + fill % C::kStages * C::kBlock;
+            if ((fill & 1) && min_seen < min(k1, k0 + (fill / 2 + 1) * kTile)) {
+                bool bad = false;  // the values that this thread has copied
+#pragma unroll 4
+                for (int i = 0; i < CH; ++i) {
+                    const int id = i * 32 + lane, r = pw * 32 + id / CH, c = id % CH;
+                    bad |= any_nonfinite<T>(*reinterpret_cast<const uint4*>(
+                        smem + (dst - sq) + (c >> 3) * C::kHalf + r * 128 + (((c ^ r) & 7) << 4)));
+                }
+                if (bad) sh.bad = 1;
+            }
+            fence_async();
+            arrive(b_full + fill % C::kStages * 8);
+        };
+        const int fills = 2 * steps;
+        find(0);
+        int64_t ko = 0, vo = 0;
+        bool ok = true;
+        int f = 0;
+        for (; f < fills; ++f) {
+            if (f >= C::kStages && !(ok = wait(b_empty + f % C::kStages * 8, (f / C::kStages - 1) & 1, fail))) break;
+            if (!(f & 1)) {
+                ko = page < 0 ? -1 : (int64_t)page * p.k_page + slot * p.k_slot;
+                vo = page < 0 ? -1 : (int64_t)page * p.v_page + slot * p.v_slot;
+                find(f / 2 + 1);
+            }
+            const int64_t mine = (f & 1) ? vo : ko;
+            const char* base = (f & 1) ? vbase : kbase;
+            const uint32_t dst = ring + f % C::kStages * C::kBlock;
+#pragma unroll
+            for (int i = 0; i < CH; ++i) {
+                const int id = i * 32 + lane, r = id / CH, c = id % CH, rr = pw * 32 + r;
+                const int64_t off = __shfl_sync(kFull, mine, r);
+                const char* src = base + (off < 0 ? 0 : off * 2) + c * 16;
+                const int n = off < 0 ? 0 : 16;
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst + (c >> 3) * C::kHalf + rr * 128 +
+                                                                                  (((c ^ rr) & 7) << 4)),
+                             "l"(src), "r"(n)
+                             : "memory");
+            }
+            asm volatile("cp.async.commit_group;" ::: "memory");
+            if (f >= C::kLag) {
+                asm volatile("cp.async.wait_group %0;" ::"n"(C::kLag) : "memory");
+                deliver(f - C::kLag);
+            }
+        }
+        asm volatile("cp.async.wait_group 0;" ::: "memory");
+        if (ok)
+            for (f = max(0, fills - C::kLag); f < fills; ++f) deliver(f);
+    } else {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
+        if (my < ntiles) {
+            const uint32_t lanes = (uint32_t)(warp & 3) << 21;  // the warp's 32 TMEM lanes, in bits 16-31
+            const uint32_t ts = tmem + my * kTile + lanes, to = tmem + kColO + my * kTile + lanes;
+            const bool rows_here = (warp & 3) * 32 + my * kTile < nrows;  // the warp has a row
+            float m = -INFINITY, l = 0.f;  // P is taken relative to m
+            bool ok = true;
+            for (int j = 0; j < steps; ++j) {
+                if (!(ok = wait(b_s + my * 8, j & 1, fail))) break;
+                fence_after();
+                if (rows_here) {
+                    uint32_t x[kTile];
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) tmem_ld32(ts + c * 32, x + c * 32);
+                    wait_ld();
+                    const int vis = seen - (k0 + j * kTile);
+                    if (__any_sync(kFull, vis < kTile)) {
+#pragma unroll
+                        for (int c = 0; c < kTile; ++c)
+                            if (c >= vis) x[c] = 0xff800000u;  // -inf
+                    }
+                    float a0 = -INFINITY, a1 = -INFINITY, a2 = -INFINITY, a3 = -INFINITY;
+#pragma unroll
+                    for (int c = 0; c < kTile; c += 4) {
+                        a0 = fmaxf(a0, __uint_as_float(x[c]));
+                        a1 = fmaxf(a1, __uint_as_float(x[c + 1]));
+                        a2 = fmaxf(a2, __uint_as_float(x[c + 2]));
+                        a3 = fmaxf(a3, __uint_as_float(x[c + 3]));
+                    }
+                    const float top = fmaxf(fmaxf(a0, a1), fmaxf(a2, a3)) * p.scale_log2;
+                    const bool grow = top > m + kGrow || (m == -INFINITY && top > m);
+                    if (__any_sync(kFull, grow)) {
+                        const float keep = grow ? exp2_fast(m - top) : 1.f;
+                        if (grow) m = top;
+                        l *= keep;
+                        if (j > 0) {
+                            if (!(ok = wait(b_o + my * 8, (j - 1) & 1, fail))) break;
+                            fence_after();
+#pragma unroll 1
+                            for (int c = 0; c < D; c += 32) {
+                                uint32_t y[32];
+                                tmem_ld32(to + c, y);
+                                wait_ld();
+#pragma unroll
+                                for (int e = 0; e < 32; ++e) y[e] = __float_as_uint(__uint_as_float(y[e]) * keep);
+                                tmem_st32(to + c, y);
+                            }
+                        }
+                    }
+                    const float base = m == -INFINITY ? 0.f : m;
+                    float s0 = 0.f, s1 = 0.f;
+#pragma unroll
+                    for (int c = 0; c < kTile; c += 32) {
+                        uint32_t pk[16];
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) {
+                            const float u = exp2_fast(fmaf(__uint_as_float(x[c + 2 * e]), p.scale_log2, -base));
+                            const float w = exp2_fast(fmaf(__uint_as_float(x[c + 2 * e + 1]), p.scale_log2, -base));
+                            s0 += u;
+                            s1 += w;
+                            pk[e] = pack2<T>(u, w);
+                        }
+                        tmem_st16(ts + c / 2, pk);
+                    }
+                    l += s0 + s1;
+                    wait_st();
+                }
+                fence_before();
+                arrive(b_p + my * 8);
+            }
+            if (ok && steps > 0) ok = wait(b_o + my * 8, (steps - 1) & 1, fail);
+            fence_after();
+            // ---- the rows' results
+            if (!ok) l = NAN;  // loud: a wait that ran out leaves no number
+            const int f = row0 + row, t = s.first + f / p.group, qh = h * p.group + f % p.group;
+            const int64_t at = (int64_t)t * p.q_heads + qh, pat = (int64_t)part * p.tokens * p.q_heads + at;
+            const float inv = l == 0.f ? 0.f : 1.f / l;
+            if (rows_here) {
+#pragma unroll 1
+                for (int c = 0; c < D; c += 32) {
+                    uint32_t y[32];
+                    if (steps > 0) {
+                        tmem_ld32(to + c, y);
+                        wait_ld();
+                    }
+                    if (l == 0.f) {
+#pragma unroll
+                        for (int e = 0; e < 32; ++e) y[e] = 0;
+                    }
+                    if (row < nrows) {
+                        if (p.direct) {
+                            uint4* o = reinterpret_cast<uint4*>(static_cast<char*>(p.out) +
+                                                                (t * p.o_tok + qh * p.o_head + c) * 2);
+#pragma unroll
+                            for (int e = 0; e < 32; e += 8) {
+                                uint32_t w[4];
+#pragma unroll
+                                for (int i = 0; i < 4; ++i)
+                                    w[i] = pack2<T>(__uint_as_float(y[e + 2 * i]) * inv, __uint_as_float(y[e + 2 * i + 1]) * inv);
+                                o[e / 8] = make_uint4(w[0], w[1], w[2], w[3]);
+                            }
+                        } else if (l != 0.f) {
+                            uint4* o = reinterpret_cast<uint4*>(p.part_o + pat * D + c);
+#pragma unroll
+                            for (int e = 0; e < 32; e += 4) o[e / 4] = make_uint4(y[e], y[e + 1], y[e + 2], y[e + 3]);
+                        }
+                    }
+                }
+                if (row < nrows) {
+                    if (!p.direct) p.part_ml[pat] = make_float2(m, l);
+                    else if (p.lse) p.lse[at] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.69314718055994531f;
+                }
+                if (*static_cast<volatile int*>(&sh.bad)) {
+                    for (int i = 0; i < 32; ++i) {
+                        const int r = __shfl_sync(kFull, row, i), n = __shfl_sync(kFull, seen, i);
+                        if (r >= nrows || n >= k1) continue;
+                        const int g = row0 + r, tt = s.first + g / p.group, hh = h * p.group + g % p.group;
+                        float acc[D / 32], rm, rl;
+                        row_alone<T, D>(p, list, static_cast<const T*>(p.q) + tt * p.q_tok + hh * p.q_head, kbase, vbase,
+                                        k0, n, acc, rm, rl);
+                        const int64_t ra = (int64_t)tt * p.q_heads + hh, rp = (int64_t)part * p.tokens * p.q_heads + ra;
+                        const float ri = rl == 0.f ? 0.f : 1.f / rl;
+#pragma unroll
+                        for (int e = 0; e < D / 32; ++e) {
+                            if (p.direct)
+                                static_cast<T*>(p.out)[tt * p.o_tok + hh * p.o_head + lane * (D / 32) + e] = from_f32<T>(acc[e] * ri);
+                            else
+                                p.part_o[rp * D + lane * (D / 32) + e] = acc[e];
+                        }
+                        if (lane == 0) {
+                            if (!p.direct) p.part_ml[rp] = make_float2(rm, rl);
+                            else if (p.lse) p.lse[ra] = rl == 0.f ? -INFINITY : (rm + log2f(rl)) * 0.69314718055994531f;
+                        }
+                    }
+                }
+            }
+            fence_before();
+        }
+    }
+    __syncwarp();
+    __syncthreads();
+    if (warp == 12) {
+        fence_after();
+        tmem_free(tmem, kCols);
+    }
+    if (blockIdx.x == 0 && blockIdx.y == 0) pdl_wait();
+}
+
+template <typename T, int D>
+int tc_launch(const AttnParams& p, int64_t units, bool pdl, cudaStream_t st) {
+    using C = TcCfg<D>;
+    static_assert(C::kSmem + sizeof(TcShared) <= 227 * 1024, "shared memory of a CTA");
+    auto kernel = attn_tc_kernel<T, D>;
+    const int rc = check_cuda(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem),
+                              "cudaFuncSetAttribute");
+    if (rc != TG_OK) return rc;
+    const dim3 grid((unsigned)units, (unsigned)p.kv_heads);
+    if (pdl) return launch_pdl("attn_tc_kernel", kernel, grid, kThreads, C::kSmem, st, p);
+    kernel<<<grid, kThreads, C::kSmem, st>>>(p);
+    return check_launch("attn_tc_kernel");
+}
+
+}  // namespace
+
+template <typename T>
+int attn_tc_run(const AttnParams& p, int dim, int64_t units, bool pdl, cudaStream_t st) {
+    return dim == 64 ? tc_launch<T, 64>(p, units, pdl, st) : tc_launch<T, 128>(p, units, pdl, st);
+}
+template int attn_tc_run<__half>(const AttnParams&, int, int64_t, bool, cudaStream_t);
+template int attn_tc_run<__nv_bfloat16>(const AttnParams&, int, int64_t, bool, cudaStream_t);
+
+}  // namespace tg
