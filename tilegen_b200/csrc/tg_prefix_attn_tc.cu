@@ -104,11 +104,7 @@ struct TcCfg {
     static constexpr int kBlock = kTile * D * 2;  // bytes of a tile of Q, K or V
     static constexpr int kHalf = kTile * 128;     // of 64 of its columns
     static constexpr int kStages = D == 128 ? 5 : 8;
-    static constexpr int kLag = 3;  // fills under way beside the one being issued
     static constexpr int kSmem = (2 + kStages) * kBlock + 2048;
-    // A producer that waits for a free stage has delivered all but the last kLag fills, and the
-    // next to be freed is consumed once the one behind it has arrived.
-    static_assert(kLag <= kStages - 2, "the ring cannot stall");
 };
 
 struct TcShared {
@@ -295,6 +291,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const AttnParams p
             };
             auto full = [&](int fill) {
                 const bool ok = wait(b_full + fill % C::kStages * 8, fill / C::kStages & 1, fail);
+                fence_async();  // the copies wrote through the generic proxy
                 fence_after();
                 return ok;
             };
@@ -334,28 +331,22 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const AttnParams p
             page = -1, slot = 0;
             if (at < k1) locate(p, list, at, page, slot);
         };
-        auto deliver = [&](int fill) {
-            const uint32_t dst = ring + fill % C::kStages * C::kBlock;
-            if ((fill & 1) && min_seen < min(k1, k0 + (fill / 2 + 1) * kTile)) {
-                bool bad = false;  // the values that this thread has copied
+        // Whether the values of a fill that this thread has copied are finite.
+        auto look = [&](uint32_t dst) {
+            bool bad = false;
 #pragma unroll 4
-                for (int i = 0; i < CH; ++i) {
-                    const int id = i * 32 + lane, r = pw * 32 + id / CH, c = id % CH;
-                    bad |= any_nonfinite<T>(*reinterpret_cast<const uint4*>(
-                        smem + (dst - sq) + (c >> 3) * C::kHalf + r * 128 + (((c ^ r) & 7) << 4)));
-                }
-                if (bad) sh.bad = 1;
+            for (int i = 0; i < CH; ++i) {
+                const int id = i * 32 + lane, r = pw * 32 + id / CH, c = id % CH;
+                bad |= any_nonfinite<T>(*reinterpret_cast<const uint4*>(
+                    smem + (dst - sq) + (c >> 3) * C::kHalf + r * 128 + (((c ^ r) & 7) << 4)));
             }
-            fence_async();
-            arrive(b_full + fill % C::kStages * 8);
+            if (bad) sh.bad = 1;
         };
         const int fills = 2 * steps;
         find(0);
         int64_t ko = 0, vo = 0;
-        bool ok = true;
-        int f = 0;
-        for (; f < fills; ++f) {
-            if (f >= C::kStages && !(ok = wait(b_empty + f % C::kStages * 8, (f / C::kStages - 1) & 1, fail))) break;
+        for (int f = 0; f < fills; ++f) {
+            if (f >= C::kStages && !wait(b_empty + f % C::kStages * 8, (f / C::kStages - 1) & 1, fail)) break;
             if (!(f & 1)) {
                 ko = page < 0 ? -1 : (int64_t)page * p.k_page + slot * p.k_slot;
                 vo = page < 0 ? -1 : (int64_t)page * p.v_page + slot * p.v_slot;
@@ -375,15 +366,15 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const AttnParams p
                              "l"(src), "r"(n)
                              : "memory");
             }
-            asm volatile("cp.async.commit_group;" ::: "memory");
-            if (f >= C::kLag) {
-                asm volatile("cp.async.wait_group %0;" ::"n"(C::kLag) : "memory");
-                deliver(f - C::kLag);
+            if ((f & 1) && min_seen < min(k1, k0 + (f / 2 + 1) * kTile)) {
+                asm volatile("cp.async.wait_all;" ::: "memory");
+                look(dst);
             }
+            // arrives for this thread once its copies so far have landed
+            asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(b_full + f % C::kStages * 8)
+                         : "memory");
         }
-        asm volatile("cp.async.wait_group 0;" ::: "memory");
-        if (ok)
-            for (f = max(0, fills - C::kLag); f < fills; ++f) deliver(f);
+        asm volatile("cp.async.wait_all;" ::: "memory");
     } else {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
         if (my < ntiles) {
