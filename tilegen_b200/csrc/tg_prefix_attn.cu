@@ -521,9 +521,9 @@ int make_plan(const tg_prefix_attention_args* a, Plan* plan, const char* op) {
     p.causal = (a->flags & TG_FLAG_CAUSAL) != 0;
 
     // The kernel for few rows reads the keys once for each 32 rows, the tcgen05 kernel once for
-    // each 256 (it exists for heads of 64 and 128).
+    // each 256 (where it fits).
     const int64_t rows_own = max_q * p.group, rows_all = a->tokens * p.group;
-    const bool tc = c.dim == 64 || c.dim == 128;
+    const bool tc = attn_tc_fits(p, c.dim);
     plan->rt_own = tc && rows_own > 32 ? 0 : rows_own > 16 && c.dim <= 128 ? 2 : 1;
     plan->rt_prefix = tc && rows_all > 32 ? 0 : rows_all > 16 && c.dim <= 128 ? 2 : 1;
     const int64_t step_own = plan->rt_own ? 64 : 128, target_own = plan->rt_own ? kSMs * 8 : kSMs * 2;

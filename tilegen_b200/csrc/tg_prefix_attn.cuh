@@ -110,6 +110,7 @@ __device__ __forceinline__ bool any_nonfinite(uint4 v) {
 }
 
 // tg_prefix_attn_tc.cu
+bool attn_tc_fits(const AttnParams& p, int dim);
 template <typename T>
 int attn_tc_run(const AttnParams& p, int dim, int64_t units, bool pdl, cudaStream_t st);
 

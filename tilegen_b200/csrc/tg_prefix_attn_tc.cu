@@ -9,14 +9,17 @@
 //
 //   TMEM columns      [0,128) S0/P0   [128,256) S1/P1   [256,256+D) O0   [384,384+D) O1
 //   warps 0-3, 4-7    softmax of tile 0, 1: S -> P, the running maximum and sum, O at the end
-//   warps 8-11        K and V tiles into a ring of shared memory (cp.async: a row's address
-//                     comes from the page table, so any page size and stride will do, and rows
-//                     past the end are zeros), swizzled as the descriptors say
-//   warp 12           issues the matrix instructions
+//   warps 8, 10       fetch K, V tiles into a ring of shared memory by TMA, in boxes of as many
+//                     rows as divide both a page and a tile
+//   warp 9            issues the matrix instructions
 //
 // O is rescaled only where a row's maximum has grown by more than 2^8 since the value that P is
 // taken relative to: P stays below 2^8, far inside the range of either type and of the 32-bit
 // sums, and the relative precision of P is that of any other reference.
+#include <cuda.h>
+
+#include <numeric>
+
 #include "tg_prefix_attn.cuh"
 
 namespace tg {
@@ -34,24 +37,40 @@ __device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::be
 __device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+// A box of a [page][head][slot][dim] map: 64 elements from x of the rows from `slot`.
+__device__ __forceinline__ void load_box(uint32_t dst, const CUtensorMap* map, int x, int slot, int head, int page,
+                                         uint32_t bar) {
+    asm volatile(
+        "{\n\t.reg .pred e;\n\telect.sync _|e, 0xffffffff;\n\t"
+        "@e cp.async.bulk.tensor.4d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];"
+        "\n\t}" ::"r"(dst),
+        "l"(map), "r"(x), "r"(slot), "r"(head), "r"(page), "r"(bar)
+        : "memory");
+}
 __device__ __forceinline__ void fence_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+// The issuing warp runs as one, with operands the same in all lanes (so that they can live in
+// uniform registers), and one elected lane issues.
 // D (+)= A B, A and B in shared memory.
 __device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t add) {
     asm volatile(
-        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(add)
+        "{\n\t.reg .pred p, e;\n\telect.sync _|e, 0xffffffff;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(add)
         : "memory");
 }
 // D (+)= A B, A in TMEM.
 __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t add) {
     asm volatile(
-        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(add)
+        "{\n\t.reg .pred p, e;\n\telect.sync _|e, 0xffffffff;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(add)
         : "memory");
 }
-// The barrier completes when the matrix instructions issued so far have.
+// The barrier completes when the matrix instructions issued so far (by the same lane: the
+// election of a full warp is always the same) have.
 __device__ __forceinline__ void commit(uint32_t bar) {
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+    asm volatile(
+        "{\n\t.reg .pred e;\n\telect.sync _|e, 0xffffffff;\n\t"
+        "@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(bar)
+        : "memory");
 }
 __device__ __forceinline__ void arrive(uint32_t bar) {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
@@ -67,15 +86,12 @@ __device__ __forceinline__ void tmem_ld32(uint32_t addr, uint32_t* r) {
         : "r"(addr)
         : "memory");
 }
-__device__ __forceinline__ void tmem_st32(uint32_t addr, const uint32_t* r) {
+__device__ __forceinline__ void tmem_ld16(uint32_t addr, uint32_t* r) {
     asm volatile(
-        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
-        "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::
-            "r"(addr),
-        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
-        "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]),
-        "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]),
-        "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(addr)
         : "memory");
 }
 __device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t* r) {
@@ -93,11 +109,59 @@ __device__ __forceinline__ uint64_t operand(uint32_t addr, uint32_t lead) {
            (uint64_t)1 << 46 | (uint64_t)2 << 61;
 }
 
+// ------------------------------------------------------------------ pairs of 32-bit numbers
+__device__ __forceinline__ uint64_t pair(float a, float b) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ float2 both(uint64_t v) {
+    float2 r;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+    return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+// The largest of three, NaN if one of them is.
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
+// 2^x on the multiply-add units, for x <= 100 (2^-125 below -125): x = n + f with f in
+// [-1/2, 1/2], 2^f by its minimax polynomial of degree 4 (relative error 2.6e-6, a hundredth of
+// P's rounding), n added to the exponent.  The special-function unit makes 16 exponentials a
+// cycle and SM, as many cycles for a tile as its two matrix products take: what goes through
+// here shortens its queue.
+__device__ __forceinline__ float2 exp2_poly(uint64_t x) {
+    constexpr float kRound = 12582912.f;  // 1.5 * 2^23: the sum's low bits are the nearest whole number
+    float2 v = both(x);
+    x = pair(fmaxf(v.x, -125.f), fmaxf(v.y, -125.f));
+    const uint64_t t = add2(x, pair(kRound, kRound));
+    const uint64_t f = fma2(add2(t, pair(-kRound, -kRound)), pair(-1.f, -1.f), x);
+    uint64_t y = fma2(f, pair(0.009570101276f, 0.009570101276f), pair(0.055917859077f, 0.055917859077f));
+    y = fma2(y, f, pair(0.240247443318f, 0.240247443318f));
+    y = fma2(y, f, pair(0.693121790886f, 0.693121790886f));
+    y = fma2(y, f, pair(0.999999284744f, 0.999999284744f));
+    const float2 n = both(t), m = both(y);
+    return make_float2(__uint_as_float(__float_as_uint(m.x) + (__float_as_uint(n.x) << 23)),
+                       __uint_as_float(__float_as_uint(m.y) + (__float_as_uint(n.y) << 23)));
+}
+
 constexpr int kTile = 128;   // rows of a tile, keys of a step
-constexpr int kThreads = 512;
+constexpr int kThreads = 384;
 constexpr uint32_t kCols = 512;
 constexpr uint32_t kColO = 256;
 constexpr float kGrow = 8.f;
+constexpr int kPoly = 4;  // of so many pairs of scores, one goes through exp2_poly
 
 template <int D>
 struct TcCfg {
@@ -108,12 +172,14 @@ struct TcCfg {
 };
 
 struct TcShared {
-    uint64_t full[8], empty[8], s_full[2], p_full[2], o_done[2];
+    uint64_t full[8], empty[8], s_full[2], p_half[2], p_full[2], o_done[2], tail, drained;
     uint32_t tmem;
-    int min_seen;
-    int bad;   // a value that only some rows see is not finite
     int fail;  // a wait ran out
 };
+
+__device__ __forceinline__ void mbar_expect_tx(uint64_t* bar, uint32_t bytes) {
+    asm volatile("mbarrier.expect_tx.relaxed.cta.shared::cta.b64 [%0], %1;" ::"r"(smem_addr(bar)), "r"(bytes) : "memory");
+}
 
 // Bounded wait; false once one has run out in this CTA (2 s; every wait here is microseconds).
 __device__ __forceinline__ bool wait(uint32_t bar, uint32_t parity, volatile int* fail) {
@@ -162,13 +228,15 @@ __device__ __noinline__ void row_alone(const AttnParams& p, const int64_t* list,
 }
 
 template <typename T, int D>
-__global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const AttnParams p) {
+__global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const AttnParams p, const int box,
+                                                              const __grid_constant__ CUtensorMap kmap,
+                                                              const __grid_constant__ CUtensorMap vmap) {
     using C = TcCfg<D>;
     constexpr int CH = D / 8;  // 16-byte chunks of a row
     extern __shared__ unsigned char smem_raw[];
     __shared__ TcShared sh;
     unsigned char* smem = smem_raw + ((1024 - (smem_addr(smem_raw) & 1023)) & 1023);
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int tid = threadIdx.x, warp = __shfl_sync(kFull, tid >> 5, 0), lane = tid & 31;
     pdl_trigger();
 
     // ---- which rows, which keys (as in the kernel for few rows)
@@ -212,23 +280,24 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const AttnParams p
     const char* kbase = static_cast<const char*>(p.k) + h * p.k_head * 2;
     const char* vbase = static_cast<const char*>(p.v) + h * p.v_head * 2;
     const uint32_t b_full = smem_addr(sh.full), b_empty = smem_addr(sh.empty), b_s = smem_addr(sh.s_full),
-                   b_p = smem_addr(sh.p_full), b_o = smem_addr(sh.o_done);
+                   b_ph = smem_addr(sh.p_half), b_p = smem_addr(sh.p_full), b_o = smem_addr(sh.o_done);
     volatile int* fail = &sh.fail;
 
-    if (warp == 12) {
+    if (warp == 9) {
         tmem_alloc(smem_addr(&sh.tmem), kCols);
         if (lane == 0) {
             for (int i = 0; i < C::kStages; ++i) {
-                mbar_init(&sh.full[i], 128);
+                mbar_init(&sh.full[i], 1);
                 mbar_init(&sh.empty[i], 1);
             }
             for (int i = 0; i < 2; ++i) {
                 mbar_init(&sh.s_full[i], 1);
+                mbar_init(&sh.p_half[i], 128);
                 mbar_init(&sh.p_full[i], 128);
                 mbar_init(&sh.o_done[i], 1);
             }
-            sh.min_seen = INT_MAX;
-            sh.bad = 0;
+            mbar_init(&sh.tail, 1);
+            mbar_init(&sh.drained, 1);
             sh.fail = 0;
             fence_mbar_init();
         }
@@ -265,7 +334,6 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const AttnParams p
                 seen = keys_seen(p, o, i - o.first, (int64_t)keys + o.len, keys);
             }
             seen = max(min(seen, k1), 0);
-            if (seen < k1) atomicMin(&sh.min_seen, seen);
         }
     }
     fence_before();
@@ -273,9 +341,9 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const AttnParams p
     fence_after();
     const uint32_t tmem = sh.tmem;
 
-    if (warp >= 12) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
-        if (warp == 12 && lane == 0 && steps > 0) {
+    if (warp >= 8) asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+    if (warp == 9) {
+        if (steps > 0) {
             constexpr uint32_t kType = std::is_same<T, __half>::value ? 0 : 1;
             constexpr uint32_t kBase = 1u << 4 | kType << 7 | kType << 10 | (kTile / 16) << 24;
             constexpr uint32_t kQK = kBase | (kTile / 8) << 17;
@@ -290,8 +358,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const AttnParams p
                 commit(b_s + i * 8);
             };
             auto full = [&](int fill) {
-                const bool ok = wait(b_full + fill % C::kStages * 8, fill / C::kStages & 1, fail);
-                fence_async();  // the copies wrote through the generic proxy
+                const bool ok = __all_sync(kFull, wait(b_full + fill % C::kStages * 8, fill / C::kStages & 1, fail));
                 fence_after();
                 return ok;
             };
@@ -305,13 +372,17 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const AttnParams p
                 ok = full(fv) && (j + 1 == steps || full(fk));
                 const uint32_t v = ring + fv % C::kStages * C::kBlock;
                 for (int i = 0; ok && i < ntiles; ++i) {
-                    ok = wait(b_p + i * 8, j & 1, fail);
-                    if (!ok) break;
-                    fence_after();
+                    // the first half of P's columns is multiplied while the second is made
 #pragma unroll
-                    for (int kk = 0; kk < kTile / 16; ++kk)
+                    for (int kk = 0; kk < kTile / 16; ++kk) {
+                        if (kk == 0 || kk == kTile / 32) {
+                            if (!(ok = __all_sync(kFull, wait((kk ? b_p : b_ph) + i * 8, j & 1, fail)))) break;
+                            fence_after();
+                        }
                         mma_ts(tmem + kColO + i * kTile, tmem + i * kTile + kk * 8, operand(v + kk * 2048, C::kHalf), kPV,
                                j > 0 || kk > 0);
+                    }
+                    if (!ok) break;
                     commit(b_o + i * 8);
                     // S of the next step goes over P: the tensor core works in the order of issue
                     if (j + 1 < steps) qk(i, fk);
@@ -320,63 +391,68 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const AttnParams p
                 commit(b_empty + fv % C::kStages * 8);
                 if (j + 1 < steps) commit(b_empty + fk % C::kStages * 8);
             }
+            if (!ok) {  // leave no product under way
+                commit(smem_addr(&sh.drained));
+                mbar_wait(&sh.drained, 0);
+            }
         }
-    } else if (warp >= 8) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
-        const int pw = warp - 8;  // rows 32 pw .. 32 pw + 31 of each tile
-        const int min_seen = sh.min_seen;
-        int page = -1, slot = 0;
-        auto find = [&](int j) {
-            const int at = k0 + j * kTile + pw * 32 + lane;
+    } else if (warp == 8 || warp == 10) {
+        // Lane l looks up the page of box l of a tile one tile ahead; the warp issues box after
+        // box.  A box that holds no key, or whose page does not exist, is not fetched.
+        const int is_v = warp == 10, boxes = kTile / box;
+        const CUtensorMap* map = is_v ? &vmap : &kmap;
+        int page, slot;
+        auto find = [&](int at) {
             page = -1, slot = 0;
             if (at < k1) locate(p, list, at, page, slot);
         };
-        // Whether the values of a fill that this thread has copied are finite.
-        auto look = [&](uint32_t dst) {
-            bool bad = false;
-#pragma unroll 4
-            for (int i = 0; i < CH; ++i) {
-                const int id = i * 32 + lane, r = pw * 32 + id / CH, c = id % CH;
-                bad |= any_nonfinite<T>(*reinterpret_cast<const uint4*>(
-                    smem + (dst - sq) + (c >> 3) * C::kHalf + r * 128 + (((c ^ r) & 7) << 4)));
-            }
-            if (bad) sh.bad = 1;
-        };
-        const int fills = 2 * steps;
-        find(0);
-        int64_t ko = 0, vo = 0;
-        for (int f = 0; f < fills; ++f) {
-            if (f >= C::kStages && !wait(b_empty + f % C::kStages * 8, (f / C::kStages - 1) & 1, fail)) break;
-            if (!(f & 1)) {
-                ko = page < 0 ? -1 : (int64_t)page * p.k_page + slot * p.k_slot;
-                vo = page < 0 ? -1 : (int64_t)page * p.v_page + slot * p.v_slot;
-                find(f / 2 + 1);
-            }
-            const int64_t mine = (f & 1) ? vo : ko;
-            const char* base = (f & 1) ? vbase : kbase;
-            const uint32_t dst = ring + f % C::kStages * C::kBlock;
+        if (lane < boxes) find(k0 + lane * box);
+        int j = 0;
+        for (; j < steps; ++j) {
+            const int f = 2 * j + is_v, st = f % C::kStages, kt = k0 + j * kTile, have = min(k1 - kt, kTile);
+            const uint32_t dst = ring + st * C::kBlock, bar = b_full + st * 8;
+            // Values past the end must be zeros (P is zero there, but 0 * NaN is not), so the last
+            // tile lands on a barrier of its own and is delivered when they are.
+            const bool tail = is_v && have < kTile;
+            if (f >= C::kStages && !__all_sync(kFull, wait(b_empty + st * 8, (f / C::kStages - 1) & 1, fail))) break;
+            const uint32_t to = tail ? smem_addr(&sh.tail) : bar;
+            for (int g = 0; g < boxes; g += 32) {  // more than 32 boxes: pages of fewer than 4 rows in common
+                if (g > 0) find(kt + (g + lane) * box);
+                const bool mine = lane < boxes - g && page >= 0;
+                const uint32_t held = __ballot_sync(kFull, mine);
+                // the phase's one arrival comes with the last group: none completes it before
+                if (lane == 0) {
+                    const uint32_t bytes = __popc(held) * box * D * 2;
+                    if (g + 32 >= boxes) mbar_arrive_expect_tx(tail ? &sh.tail : &sh.full[st], bytes);
+                    else mbar_expect_tx(tail ? &sh.tail : &sh.full[st], bytes);
+                }
+                __syncwarp();
+                for (int i = 0; i < min(boxes - g, 32); ++i) {
+                    const int pg = __shfl_sync(kFull, page, i), sl = __shfl_sync(kFull, slot, i);
+                    if (!(held >> i & 1)) continue;
 #pragma unroll
-            for (int i = 0; i < CH; ++i) {
-                const int id = i * 32 + lane, r = id / CH, c = id % CH, rr = pw * 32 + r;
-                const int64_t off = __shfl_sync(kFull, mine, r);
-                const char* src = base + (off < 0 ? 0 : off * 2) + c * 16;
-                const int n = off < 0 ? 0 : 16;
-                asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst + (c >> 3) * C::kHalf + rr * 128 +
-                                                                                  (((c ^ rr) & 7) << 4)),
-                             "l"(src), "r"(n)
-                             : "memory");
+                    for (int half = 0; half < D / 64; ++half)
+                        load_box(dst + half * C::kHalf + (g + i) * box * 128, map, half * 64, sl, h, pg, to);
+                }
             }
-            if ((f & 1) && min_seen < min(k1, k0 + (f / 2 + 1) * kTile)) {
-                asm volatile("cp.async.wait_all;" ::: "memory");
-                look(dst);
+            if (lane < boxes) find(kt + kTile + lane * box);
+            if (tail) {
+                wait(to, 0, fail);
+                for (int i = have * 8 + lane; i < kTile * 8; i += 32)
+#pragma unroll
+                    for (int half = 0; half < D / 64; ++half)
+                        *reinterpret_cast<uint4*>(smem + (dst - sq) + half * C::kHalf + i * 16) = make_uint4(0, 0, 0, 0);
+                fence_async();
+                __syncwarp();
+                if (lane == 0) arrive(bar);
             }
-            // arrives for this thread once its copies so far have landed
-            asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(b_full + f % C::kStages * 8)
-                         : "memory");
         }
-        asm volatile("cp.async.wait_all;" ::: "memory");
-    } else {
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
+        __syncwarp();
+        if (*fail)  // leave no copy under way
+            for (int i = max(0, j - C::kStages); i < j; ++i)
+                mbar_wait(&sh.full[(2 * i + is_v) % C::kStages], (2 * i + is_v) / C::kStages & 1);
+    } else if (warp < 8) {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
         if (my < ntiles) {
             const uint32_t lanes = (uint32_t)(warp & 3) << 21;  // the warp's 32 TMEM lanes, in bits 16-31
             const uint32_t ts = tmem + my * kTile + lanes, to = tmem + kColO + my * kTile + lanes;
@@ -392,20 +468,21 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const AttnParams p
                     for (int c = 0; c < 4; ++c) tmem_ld32(ts + c * 32, x + c * 32);
                     wait_ld();
                     const int vis = seen - (k0 + j * kTile);
-                    if (__any_sync(kFull, vis < kTile)) {
+                    const bool cut = __any_sync(kFull, vis < kTile);
+                    if (cut) {
 #pragma unroll
                         for (int c = 0; c < kTile; ++c)
                             if (c >= vis) x[c] = 0xff800000u;  // -inf
                     }
                     float a0 = -INFINITY, a1 = -INFINITY, a2 = -INFINITY, a3 = -INFINITY;
 #pragma unroll
-                    for (int c = 0; c < kTile; c += 4) {
-                        a0 = fmaxf(a0, __uint_as_float(x[c]));
-                        a1 = fmaxf(a1, __uint_as_float(x[c + 1]));
-                        a2 = fmaxf(a2, __uint_as_float(x[c + 2]));
-                        a3 = fmaxf(a3, __uint_as_float(x[c + 3]));
+                    for (int c = 0; c < kTile; c += 8) {
+                        a0 = max3(a0, __uint_as_float(x[c]), __uint_as_float(x[c + 1]));
+                        a1 = max3(a1, __uint_as_float(x[c + 2]), __uint_as_float(x[c + 3]));
+                        a2 = max3(a2, __uint_as_float(x[c + 4]), __uint_as_float(x[c + 5]));
+                        a3 = max3(a3, __uint_as_float(x[c + 6]), __uint_as_float(x[c + 7]));
                     }
-                    const float top = fmaxf(fmaxf(a0, a1), fmaxf(a2, a3)) * p.scale_log2;
+                    const float top = max3(max3(a0, a1, a2), a3, a3) * p.scale_log2;
                     const bool grow = top > m + kGrow || (m == -INFINITY && top > m);
                     if (__any_sync(kFull, grow)) {
                         const float keep = grow ? exp2_fast(m - top) : 1.f;
@@ -415,33 +492,55 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const AttnParams p
                             if (!(ok = wait(b_o + my * 8, (j - 1) & 1, fail))) break;
                             fence_after();
 #pragma unroll 1
-                            for (int c = 0; c < D; c += 32) {
-                                uint32_t y[32];
-                                tmem_ld32(to + c, y);
+                            for (int c = 0; c < D; c += 16) {
+                                uint32_t y[16];
+                                tmem_ld16(to + c, y);
                                 wait_ld();
 #pragma unroll
-                                for (int e = 0; e < 32; ++e) y[e] = __float_as_uint(__uint_as_float(y[e]) * keep);
-                                tmem_st32(to + c, y);
+                                for (int e = 0; e < 16; ++e) y[e] = __float_as_uint(__uint_as_float(y[e]) * keep);
+                                tmem_st16(to + c, y);
                             }
                         }
                     }
+                    // a NaN or infinite score leaves the row's sum NaN, whatever its P
+                    if (!(top < INFINITY)) l = NAN;
                     const float base = m == -INFINITY ? 0.f : m;
-                    float s0 = 0.f, s1 = 0.f;
+                    const uint64_t scale2 = pair(p.scale_log2, p.scale_log2), base2 = pair(-base, -base);
+                    uint64_t s0 = pair(0.f, 0.f), s1 = s0;
+                    auto make_p = [&](auto whole) {
 #pragma unroll
                     for (int c = 0; c < kTile; c += 32) {
                         uint32_t pk[16];
 #pragma unroll
                         for (int e = 0; e < 16; ++e) {
-                            const float u = exp2_fast(fmaf(__uint_as_float(x[c + 2 * e]), p.scale_log2, -base));
-                            const float w = exp2_fast(fmaf(__uint_as_float(x[c + 2 * e + 1]), p.scale_log2, -base));
-                            s0 += u;
-                            s1 += w;
-                            pk[e] = pack2<T>(u, w);
+                            const uint64_t y = fma2(pair(__uint_as_float(x[c + 2 * e]), __uint_as_float(x[c + 2 * e + 1])),
+                                                    scale2, base2);
+                            float2 w;
+                            if (e % kPoly == kPoly - 1 && decltype(whole)::value) {
+                                w = exp2_poly(y);
+                            } else {
+                                w = both(y);
+                                w = make_float2(exp2_fast(w.x), exp2_fast(w.y));
+                            }
+                            if (e & 1) s1 = add2(s1, pair(w.x, w.y));
+                            else s0 = add2(s0, pair(w.x, w.y));
+                            pk[e] = pack2<T>(w.x, w.y);
                         }
                         tmem_st16(ts + c / 2, pk);
+                        if (c == 32) {
+                            wait_st();
+                            fence_before();
+                            arrive(b_ph + my * 8);
+                        }
                     }
-                    l += s0 + s1;
+                    };
+                    if (cut) make_p(std::false_type());
+                    else make_p(std::true_type());
+                    const float2 sum = both(add2(s0, s1));
+                    l += sum.x + sum.y;
                     wait_st();
+                } else {
+                    arrive(b_ph + my * 8);
                 }
                 fence_before();
                 arrive(b_p + my * 8);
@@ -453,6 +552,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const AttnParams p
             const int f = row0 + row, t = s.first + f / p.group, qh = h * p.group + f % p.group;
             const int64_t at = (int64_t)t * p.q_heads + qh, pat = (int64_t)part * p.tokens * p.q_heads + at;
             const float inv = l == 0.f ? 0.f : 1.f / l;
+            float odd = 0.f;  // NaN once an element of the row's sum is not finite
             if (rows_here) {
 #pragma unroll 1
                 for (int c = 0; c < D; c += 32) {
@@ -461,9 +561,10 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const AttnParams p
                         tmem_ld32(to + c, y);
                         wait_ld();
                     }
-                    if (l == 0.f) {
 #pragma unroll
-                        for (int e = 0; e < 32; ++e) y[e] = 0;
+                    for (int e = 0; e < 32; ++e) {
+                        odd += __uint_as_float(y[e]) * 0.f;
+                        if (l == 0.f) y[e] = 0;
                     }
                     if (row < nrows) {
                         if (p.direct) {
@@ -488,10 +589,13 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const AttnParams p
                     if (!p.direct) p.part_ml[pat] = make_float2(m, l);
                     else if (p.lse) p.lse[at] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.69314718055994531f;
                 }
-                if (*static_cast<volatile int*>(&sh.bad)) {
+                // A value that a row does not see, of a tile that it sees in part, reaches it as 0
+                // times the value: where that is NaN, the row is done again alone.
+                const bool again = row < nrows && seen < k1 && steps > 0 && odd != odd;
+                if (__any_sync(kFull, again)) {
                     for (int i = 0; i < 32; ++i) {
                         const int r = __shfl_sync(kFull, row, i), n = __shfl_sync(kFull, seen, i);
-                        if (r >= nrows || n >= k1) continue;
+                        if (!__shfl_sync(kFull, again, i)) continue;
                         const int g = row0 + r, tt = s.first + g / p.group, hh = h * p.group + g % p.group;
                         float acc[D / 32], rm, rl;
                         row_alone<T, D>(p, list, static_cast<const T*>(p.q) + tt * p.q_tok + hh * p.q_head, kbase, vbase,
@@ -517,28 +621,75 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const AttnParams p
     }
     __syncwarp();
     __syncthreads();
-    if (warp == 12) {
+    if (warp == 9) {
         fence_after();
         tmem_free(tmem, kCols);
     }
     if (blockIdx.x == 0 && blockIdx.y == 0) pdl_wait();
 }
 
+// ------------------------------------------------------------------ host
+using EncodeFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                              const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                              CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+EncodeFn encoder() {
+    static const EncodeFn fn = [] {
+        void* f = nullptr;
+        cudaDriverEntryPointQueryResult found;
+        if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &f, 12000, cudaEnableDefault, &found) != cudaSuccess ||
+            found != cudaDriverEntryPointSuccess)
+            f = nullptr;
+        return reinterpret_cast<EncodeFn>(f);
+    }();
+    return fn;
+}
+
+// Rows of a box: what a page and a tile can both be cut into.
+int box_rows(int page_size) { return std::gcd(page_size, kTile); }
+
+bool strides_fit(int64_t page, int64_t slot, int64_t head) {  // bytes below 2^40
+    return page < (1ll << 38) && slot < (1ll << 38) && head < (1ll << 38) && page >= 0 && slot >= 0 && head >= 0;
+}
+
+template <typename T>
+int cache_map(CUtensorMap* map, const AttnParams& p, const void* data, int64_t page, int64_t slot, int64_t head, int dim) {
+    if (!encoder()) return set_error(TG_ECUDA, "cuTensorMapEncodeTiled is not available");
+    const cuuint64_t size[4] = {(cuuint64_t)dim, (cuuint64_t)p.page_size, (cuuint64_t)p.kv_heads, (cuuint64_t)p.pages};
+    const cuuint64_t stride[3] = {(cuuint64_t)slot * 2, (cuuint64_t)head * 2, (cuuint64_t)page * 2};
+    const cuuint32_t box[4] = {64, (cuuint32_t)box_rows(p.page_size), 1, 1}, step[4] = {1, 1, 1, 1};
+    const CUresult r = encoder()(map, std::is_same<T, __half>::value ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16,
+                                 4, const_cast<void*>(data), size, stride, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                                 CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                                 CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    return r == CUDA_SUCCESS ? TG_OK : set_error(TG_ECUDA, "cuTensorMapEncodeTiled: CUDA error %d", (int)r);
+}
+
 template <typename T, int D>
 int tc_launch(const AttnParams& p, int64_t units, bool pdl, cudaStream_t st) {
     using C = TcCfg<D>;
     static_assert(C::kSmem + sizeof(TcShared) <= 227 * 1024, "shared memory of a CTA");
+    const int box = box_rows(p.page_size);
+    CUtensorMap kmap, vmap;
+    int rc = cache_map<T>(&kmap, p, p.k, p.k_page, p.k_slot, p.k_head, D);
+    if (rc == TG_OK) rc = cache_map<T>(&vmap, p, p.v, p.v_page, p.v_slot, p.v_head, D);
     auto kernel = attn_tc_kernel<T, D>;
-    const int rc = check_cuda(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem),
-                              "cudaFuncSetAttribute");
+    if (rc == TG_OK)
+        rc = check_cuda(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem),
+                        "cudaFuncSetAttribute");
     if (rc != TG_OK) return rc;
     const dim3 grid((unsigned)units, (unsigned)p.kv_heads);
-    if (pdl) return launch_pdl("attn_tc_kernel", kernel, grid, kThreads, C::kSmem, st, p);
-    kernel<<<grid, kThreads, C::kSmem, st>>>(p);
+    if (pdl) return launch_pdl("attn_tc_kernel", kernel, grid, kThreads, C::kSmem, st, p, box, kmap, vmap);
+    kernel<<<grid, kThreads, C::kSmem, st>>>(p, box, kmap, vmap);
     return check_launch("attn_tc_kernel");
 }
 
 }  // namespace
+
+bool attn_tc_fits(const AttnParams& p, int dim) {
+    return (dim == 64 || dim == 128) && p.pages > 0 && strides_fit(p.k_page, p.k_slot, p.k_head) &&
+           strides_fit(p.v_page, p.v_slot, p.v_head);
+}
 
 template <typename T>
 int attn_tc_run(const AttnParams& p, int dim, int64_t units, bool pdl, cudaStream_t st) {
