@@ -172,7 +172,7 @@ struct TcCfg {
 };
 
 struct TcShared {
-    uint64_t full[8], empty[8], s_full[2], p_half[2], p_full[2], o_done[2], tail, drained;
+    uint64_t q_full, full[8], empty[8], s_full[2], p_half[2], p_full[2], o_done[2], tail, drained;
     uint32_t tmem;
     int fail;  // a wait ran out
 };
@@ -296,44 +296,11 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const AttnParams p
                 mbar_init(&sh.p_full[i], 128);
                 mbar_init(&sh.o_done[i], 1);
             }
+            mbar_init(&sh.q_full, ntiles * kTile);
             mbar_init(&sh.tail, 1);
             mbar_init(&sh.drained, 1);
             sh.fail = 0;
             fence_mbar_init();
-        }
-    }
-    __syncthreads();
-
-    // ---- queries (swizzled, zeros where there is no row) and what each row sees
-    const int my = warp >> 2;  // the softmax tile of warps 0-7
-    const int row = tid;       // of the CTA, threads 0-255
-    int seen = 0;              // keys that the thread's row sees, up to k1
-    if (warp < 8) {
-        const int rt = tid & 127;
-        if (my < ntiles) {
-            for (int i = rt; i < kTile * CH; i += 128) {
-                const int r = i / CH, c = i % CH, f = my * kTile + r;
-                uint4 v = make_uint4(0, 0, 0, 0);
-                if (f < nrows) {
-                    const int t = s.first + (row0 + f) / p.group, qh = h * p.group + (row0 + f) % p.group;
-                    v = *reinterpret_cast<const uint4*>(static_cast<const char*>(p.q) +
-                                                        (t * p.q_tok + qh * p.q_head) * 2 + c * 16);
-                }
-                *reinterpret_cast<uint4*>(smem + my * C::kBlock + (c >> 3) * C::kHalf + r * 128 + (((c ^ r) & 7) << 4)) = v;
-            }
-            fence_async();
-        }
-        if (row < nrows) {
-            const int i = (row0 + row) / p.group;
-            if (!p.over_prefix) {
-                seen = keys_seen(p, s, i, keys, keys);
-            } else if (!p.causal) {
-                seen = keys;
-            } else {
-                const Sequence o = sequence(p, sequence_of(p.q_indptr, p.rows, i));
-                seen = keys_seen(p, o, i - o.first, (int64_t)keys + o.len, keys);
-            }
-            seen = max(min(seen, k1), 0);
         }
     }
     fence_before();
@@ -362,7 +329,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const AttnParams p
                 fence_after();
                 return ok;
             };
-            bool ok = full(0);
+            bool ok = __all_sync(kFull, wait(smem_addr(&sh.q_full), 0, fail)) && full(0);
             if (ok) {
                 for (int i = 0; i < ntiles; ++i) qk(i, 0);
                 commit(b_empty);
@@ -453,7 +420,48 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const AttnParams p
                 mbar_wait(&sh.full[(2 * i + is_v) % C::kStages], (2 * i + is_v) / C::kStages & 1);
     } else if (warp < 8) {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
+        const int my = warp >> 2, row = tid;  // the warp's tile, the thread's row of the CTA
         if (my < ntiles) {
+            // ---- queries, swizzled, zeros where there is no row; all loads are under way at once
+            {
+                constexpr int kStep = kTile / CH;  // rows between a thread's chunks
+                const int rt = tid & (kTile - 1), c = rt % CH, f0 = my * kTile + rt / CH;
+                const int dt = kStep / p.group, dg = kStep % p.group;
+                int t = (row0 + f0) / p.group, g = (row0 + f0) % p.group;
+                const char* q = static_cast<const char*>(p.q) + (s.first * p.q_tok + (int64_t)h * p.group * p.q_head) * 2 + c * 16;
+                uint4 v[CH];
+#pragma unroll
+                for (int i = 0; i < CH; ++i) {
+                    const bool there = f0 + i * kStep < nrows;
+                    v[i] = __ldg(reinterpret_cast<const uint4*>(q + (there ? (t * p.q_tok + g * p.q_head) * 2 : 0)));
+                    t += dt;
+                    g += dg;
+                    if (g >= p.group) g -= p.group, ++t;
+                }
+#pragma unroll
+                for (int i = 0; i < CH; ++i)
+                    if (f0 + i * kStep >= nrows) v[i] = make_uint4(0, 0, 0, 0);
+#pragma unroll
+                for (int i = 0; i < CH; ++i) {
+                    const int r = rt / CH + i * (kTile / CH);
+                    *reinterpret_cast<uint4*>(smem + my * C::kBlock + (c >> 3) * C::kHalf + r * 128 + (((c ^ r) & 7) << 4)) = v[i];
+                }
+                fence_async();
+                arrive(smem_addr(&sh.q_full));
+            }
+            int seen = 0;  // keys that the thread's row sees, up to k1
+            if (row < nrows) {
+                const int i = (row0 + row) / p.group;
+                if (!p.over_prefix) {
+                    seen = keys_seen(p, s, i, keys, keys);
+                } else if (!p.causal) {
+                    seen = keys;
+                } else {
+                    const Sequence o = sequence(p, sequence_of(p.q_indptr, p.rows, i));
+                    seen = keys_seen(p, o, i - o.first, (int64_t)keys + o.len, keys);
+                }
+                seen = max(min(seen, k1), 0);
+            }
             const uint32_t lanes = (uint32_t)(warp & 3) << 21;  // the warp's 32 TMEM lanes, in bits 16-31
             const uint32_t ts = tmem + my * kTile + lanes, to = tmem + kColO + my * kTile + lanes;
             const bool rows_here = (warp & 3) * 32 + my * kTile < nrows;  // the warp has a row
@@ -554,36 +562,49 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const AttnParams p
             const float inv = l == 0.f ? 0.f : 1.f / l;
             float odd = 0.f;  // NaN once an element of the row's sum is not finite
             if (rows_here) {
+                // The tile's queries are done with: a warp turns its 32 rows round in their place, so
+                // that stores run along the rows.  A pass: D 16-bit results or D / 2 32-bit sums.
+                unsigned char* area = smem + my * C::kBlock + (warp & 3) * (C::kBlock / 4);
+                char* to_row = p.direct ? static_cast<char*>(p.out) + (t * p.o_tok + qh * p.o_head) * 2
+                                        : reinterpret_cast<char*>(p.part_o + pat * D);
+                if (row >= nrows || (!p.direct && l == 0.f)) to_row = nullptr;
+                const int passes = p.direct ? 1 : 2;
 #pragma unroll 1
-                for (int c = 0; c < D; c += 32) {
-                    uint32_t y[32];
-                    if (steps > 0) {
-                        tmem_ld32(to + c, y);
-                        wait_ld();
-                    }
-#pragma unroll
-                    for (int e = 0; e < 32; ++e) {
-                        odd += __uint_as_float(y[e]) * 0.f;
-                        if (l == 0.f) y[e] = 0;
-                    }
-                    if (row < nrows) {
-                        if (p.direct) {
-                            uint4* o = reinterpret_cast<uint4*>(static_cast<char*>(p.out) +
-                                                                (t * p.o_tok + qh * p.o_head + c) * 2);
-#pragma unroll
-                            for (int e = 0; e < 32; e += 8) {
-                                uint32_t w[4];
-#pragma unroll
-                                for (int i = 0; i < 4; ++i)
-                                    w[i] = pack2<T>(__uint_as_float(y[e + 2 * i]) * inv, __uint_as_float(y[e + 2 * i + 1]) * inv);
-                                o[e / 8] = make_uint4(w[0], w[1], w[2], w[3]);
-                            }
-                        } else if (l != 0.f) {
-                            uint4* o = reinterpret_cast<uint4*>(p.part_o + pat * D + c);
-#pragma unroll
-                            for (int e = 0; e < 32; e += 4) o[e / 4] = make_uint4(y[e], y[e + 1], y[e + 2], y[e + 3]);
+                for (int pass = 0; pass < passes; ++pass) {
+                    const int cols = D / passes;
+#pragma unroll 1
+                    for (int c = 0; c < cols; c += 16) {
+                        uint32_t y[16];
+                        if (steps > 0) {
+                            tmem_ld16(to + pass * cols + c, y);
+                            wait_ld();
                         }
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) {
+                            odd += __uint_as_float(y[e]) * 0.f;
+                            if (l == 0.f) y[e] = 0;
+                        }
+                        if (p.direct) {
+#pragma unroll
+                            for (int e = 0; e < 8; ++e)
+                                y[e] = pack2<T>(__uint_as_float(y[2 * e]) * inv, __uint_as_float(y[2 * e + 1]) * inv);
+                        }
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            if (e < 2 || !p.direct)
+                                *reinterpret_cast<uint4*>(area + lane * D * 2 +
+                                                          ((((p.direct ? c / 8 : c / 4) + e) ^ lane) & (CH - 1)) * 16) =
+                                    make_uint4(y[4 * e], y[4 * e + 1], y[4 * e + 2], y[4 * e + 3]);
                     }
+                    __syncwarp();
+#pragma unroll 4
+                    for (int i = 0; i < CH; ++i) {
+                        const int r = (i * 32 + lane) / CH, c = lane % CH;
+                        char* dst = reinterpret_cast<char*>(__shfl_sync(kFull, reinterpret_cast<unsigned long long>(to_row), r));
+                        const uint4 v = *reinterpret_cast<const uint4*>(area + r * D * 2 + ((c ^ r) & (CH - 1)) * 16);
+                        if (dst) *reinterpret_cast<uint4*>(dst + pass * D * 2 + c * 16) = v;
+                    }
+                    __syncwarp();
                 }
                 if (row < nrows) {
                     if (!p.direct) p.part_ml[pat] = make_float2(m, l);
