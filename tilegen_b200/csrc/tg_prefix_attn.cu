@@ -392,13 +392,19 @@ __global__ void __launch_bounds__(128) attn_join_kernel(const AttnParams p) {
     pdl_wait();
     if (row >= all) return;
     const int t = (int)(row / p.q_heads), qh = (int)(row % p.q_heads);
-    int n = p.prefix_splits;
+    int np = p.prefix_splits, n;  // parts over the prefix, and all
+    if (p.prefix_ctas > 0) {
+        const int64_t u = (int64_t)(qh / p.group) * p.prefix_tiles + (t * p.group + qh % p.group) / 256;
+        np = prefix_cta(p, (u + 1) * p.prefix_steps - 1) - prefix_cta(p, u * p.prefix_steps) + 1;
+    }
+    n = np;
     if (p.own_chunks > 0) {
         const Sequence s = sequence(p, sequence_of(p.q_indptr, p.rows, t));
         if (t >= s.first && t < s.first + s.n) n += (s.len + p.own_chunk - 1) / p.own_chunk;
     }
+    auto part = [&](int i) { return (i < np ? i : i - np + p.prefix_splits) * all + row; };
     float top = -INFINITY;
-    for (int i = lane; i < n; i += 32) top = fmaxf(top, p.part_ml[i * all + row].x);
+    for (int i = lane; i < n; i += 32) top = fmaxf(top, p.part_ml[part(i)].x);
 #pragma unroll
     for (int x = 16; x; x >>= 1) top = fmaxf(top, __shfl_xor_sync(kFull, top, x));
     const float base = top == -INFINITY ? 0.f : top;
@@ -407,8 +413,8 @@ __global__ void __launch_bounds__(128) attn_join_kernel(const AttnParams p) {
     for (int i = 0; i < NV * VE; ++i) acc[i] = 0.f;
 #pragma unroll 4
     for (int i = 0; i < n; ++i) {
-        const float2 ml = p.part_ml[i * all + row];
-        const float* x = p.part_o + (i * all + row) * D;
+        const float2 ml = p.part_ml[part(i)];
+        const float* x = p.part_o + part(i) * D;
         const float f = exp2_fast(ml.x - base);
         if (ml.y == 0.f) continue;  // nothing seen there
         sum += f * ml.y;
@@ -453,24 +459,29 @@ struct Plan {
     size_t ws_bytes;
 };
 
-// Keys of a split of the prefix for the tcgen05 kernel, by the time that the whole call would
-// take: `units` CTAs for each split, one on an SM, 1.2 us for 128 keys and 5 us to begin and end;
-// the SMs that they leave, and their time after them, go to the own parts (own_bytes at 6 TB/s);
-// and each split adds a partial result of every row, written and read.
-int prefix_chunk(int64_t len, int64_t units, int64_t rows, int dim, double own_bytes) {
+// CTAs of the tcgen05 kernel over the prefix, by the time that the whole call would take: a CTA,
+// one on an SM, has an even share of the steps at 1.9 us (1.3 where there is one row tile), 5 us to
+// begin and 5 for each pair of head and row tile that it touches; the SMs that they leave, and
+// their time after them, go to the own parts (own_bytes at 6 TB/s); and each part of a row is
+// written and read once more.
+void share_prefix(AttnParams& p, int64_t rows, int dim, double own_bytes) {
+    const int64_t units = (int64_t)p.prefix_tiles * p.kv_heads;
+    p.prefix_steps = (int)ceil_div(p.prefix_len, 128);
+    p.prefix_work = units * p.prefix_steps;
+    const double step = rows > 128 ? 1.9 : 1.3;
     double best = 1e30;
-    int64_t chunk = 0;
-    for (int64_t n = 1; n <= 128; ++n) {
-        const int64_t c = ceil_div(ceil_div(len, n), 128) * 128, ctas = units * ceil_div(len, c);
-        const double cta = 5.0 + 1.2 * (double)(c / 128);
-        const double prefix = cta * (double)ceil_div(ctas, kSMs);
-        const double all = own_bytes / 6e6 + cta * (double)ctas / kSMs;
-        const double join = (double)ceil_div(len, c) * (double)rows * dim * 8 / 6e6;
-        const double t = std::max(prefix, all) + join;
-        if (t < best * 0.999) best = t, chunk = c;
-        if (c == 128) break;
+    int ctas = 1;
+    for (int64_t n = 1; n <= std::min<int64_t>(kSMs, p.prefix_work); ++n) {
+        const double cta = 5.0 + step * (double)ceil_div(p.prefix_work, n) + 5.0 * (double)(ceil_div(units, n) + (units % n != 0));
+        const double all = own_bytes / 6e6 + cta * (double)n / kSMs;
+        const double parts = 1.0 + (double)n / (double)units;
+        const double t = std::max(cta, all) + parts * (double)rows * p.kv_heads * dim * 8 / 6e6;
+        if (t < best * 0.999) best = t, ctas = (int)n;
     }
-    return (int)chunk;
+    p.prefix_ctas = ctas;
+    p.prefix_splits = 1;
+    for (int64_t u = 0; u < units; ++u)
+        p.prefix_splits = std::max(p.prefix_splits, prefix_cta(p, (u + 1) * p.prefix_steps - 1) - prefix_cta(p, u * p.prefix_steps) + 1);
 }
 
 int make_plan(const tg_prefix_attention_args* a, Plan* plan, const char* op) {
@@ -533,11 +544,11 @@ int make_plan(const tg_prefix_attention_args* a, Plan* plan, const char* op) {
         if (plan->rt_prefix) {
             const int64_t n = std::max<int64_t>(1, kSMs * 8 / (tiles_all * c.heads));
             p.prefix_chunk = (int)std::max<int64_t>(256, ceil_div(ceil_div(p.prefix_len, n), 64) * 64);
+            p.prefix_splits = (int)ceil_div(p.prefix_len, p.prefix_chunk);
         } else {
-            p.prefix_chunk = prefix_chunk(p.prefix_len, tiles_all * c.heads, rows_all * c.heads, c.dim,
-                                          (double)t.nnz * c.page_size * c.heads * c.dim * 4);
+            p.prefix_tiles = (int)tiles_all;
+            share_prefix(p, rows_all, c.dim, (double)t.nnz * c.page_size * c.heads * c.dim * 4);
         }
-        p.prefix_splits = (int)ceil_div(p.prefix_len, p.prefix_chunk);
     }
     if (max_seq > 0 || p.prefix_len == 0) {
         const int64_t n = std::max<int64_t>(1, target_own / std::max<int64_t>(1, t.rows * tiles_own * c.heads));
@@ -545,7 +556,7 @@ int make_plan(const tg_prefix_attention_args* a, Plan* plan, const char* op) {
         p.own_chunks = (int)std::max<int64_t>(1, ceil_div(max_seq, p.own_chunk));
     }
     plan->own_units = t.rows * tiles_own * p.own_chunks;
-    plan->prefix_units = tiles_all * p.prefix_splits;
+    plan->prefix_units = p.prefix_ctas ? p.prefix_ctas : tiles_all * p.prefix_splits;
     if (plan->own_units > INT32_MAX || plan->prefix_units > INT32_MAX || c.heads > 65535)
         return set_error(TG_EUNSUPPORTED, "%s: too many rows for one launch", op);
     p.tiles = (int)tiles_own;
@@ -593,6 +604,7 @@ int attn_run(const Plan& plan, void* ws, cudaStream_t st) {
     if (p.prefix_splits > 0) {
         AttnParams q = p;
         q.over_prefix = 1;
+        q.tiles = p.prefix_tiles;
         const int rc = launch(q, plan.rt_prefix, plan.prefix_units);
         if (rc != TG_OK) return rc;
     }

@@ -26,7 +26,11 @@ struct AttnParams {
     float scale_log2;
     int causal;
     // parts
-    int prefix_splits, prefix_chunk;  // keys of a split
+    int prefix_splits, prefix_chunk;  // most parts of a row over the prefix; keys of a split
+    // the tcgen05 kernel over the prefix: its CTAs share prefix_work steps of 128 keys evenly,
+    // prefix_steps for each (head, row tile) in turn, prefix_tiles row tiles
+    int64_t prefix_work;
+    int prefix_ctas, prefix_steps, prefix_tiles;  // prefix_ctas 0: splits of prefix_chunk keys
     int own_chunks, own_chunk;        // most chunks of a sequence, keys of a chunk
     int tiles;                        // row tiles of a sequence (own) or of all rows (prefix)
     int over_prefix;                  // this launch: the prefix, else the sequences' own pages
@@ -57,6 +61,11 @@ __device__ __forceinline__ Sequence sequence(const AttnParams& p, int64_t b) {
 __device__ __forceinline__ int keys_seen(const AttnParams& p, const Sequence& s, int i, int64_t total, int whole) {
     if (!p.causal) return whole;
     return (int)min(max(total - s.n + i + 1, (int64_t)0), (int64_t)whole);
+}
+
+// The CTA that has step x of the prefix.
+__host__ __device__ __forceinline__ int prefix_cta(const AttnParams& p, int64_t x) {
+    return (int)(((x + 1) * p.prefix_ctas - 1) / p.prefix_work);
 }
 
 // Page and slot of token `at` of a page list; page -1 where the list names no page of the cache.

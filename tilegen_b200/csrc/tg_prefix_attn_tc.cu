@@ -172,7 +172,7 @@ struct TcCfg {
 };
 
 struct TcShared {
-    uint64_t q_full, full[8], empty[8], s_full[2], p_half[2], p_full[2], o_done[2], tail, drained;
+    uint64_t q_full[2], full[8], empty[8], s_full[2], p_half[2], p_full[2], o_done[2], tail, drained;
     uint32_t tmem;
     int fail;  // a wait ran out
 };
@@ -192,6 +192,13 @@ __device__ __forceinline__ bool wait(uint32_t bar, uint32_t parity, volatile int
             *fail = 1;
             return false;
         }
+    }
+}
+
+// As mbar_wait, for at most a millisecond: to let copies land before a kernel that gave up ends.
+__device__ __forceinline__ void mbar_wait_brief(uint64_t* bar, uint32_t parity) {
+    const uint64_t t0 = globaltimer_ns();
+    while (!mbar_try(smem_addr(bar), parity) && globaltimer_ns() - t0 < 1000000ull) {
     }
 }
 
@@ -227,6 +234,65 @@ __device__ __noinline__ void row_alone(const AttnParams& p, const int64_t* list,
     }
 }
 
+// Up to 256 rows over a range of keys, as all warps of a CTA see it.
+struct Segment {
+    Sequence s;
+    const int64_t* list;
+    int h, part, row0, nrows, k0, k1, keys, steps, ntiles;
+};
+
+// The CTA's segments, one after the other.  Over the prefix a CTA has an even share of all steps
+// of all (head, row tile) pairs, so it ends one pair and begins another where its share does; the
+// parts of a pair are numbered by CTA.  Over own pages it has one segment.
+struct Segments {
+    int64_t at, end;
+    __device__ __forceinline__ explicit Segments(const AttnParams& p) {
+        at = p.over_prefix ? blockIdx.x * p.prefix_work / p.prefix_ctas : 0;
+        end = p.over_prefix ? (blockIdx.x + 1) * p.prefix_work / p.prefix_ctas : 1;
+    }
+    __device__ __forceinline__ bool next(const AttnParams& p, Segment& g) {
+        if (at >= end) return false;
+        int tile;
+        if (p.over_prefix) {
+            const int64_t u = at / p.prefix_steps;
+            const int first = (int)(at - u * p.prefix_steps);
+            g.steps = (int)min((int64_t)(p.prefix_steps - first), end - at);
+            at += g.steps;
+            g.h = (int)(u / p.tiles);
+            tile = (int)(u - (int64_t)g.h * p.tiles);
+            g.part = blockIdx.x - prefix_cta(p, u * p.prefix_steps);
+            g.s.first = 0;
+            g.s.n = p.tokens;
+            g.list = p.prefix_pages;
+            g.keys = p.prefix_len;
+            g.k0 = first * kTile;
+            g.k1 = min(g.keys, g.k0 + g.steps * kTile);
+        } else {
+            at = end;
+            const int c = blockIdx.x % p.own_chunks, u = blockIdx.x / p.own_chunks;
+            g.h = blockIdx.y;
+            tile = u % p.tiles;
+            g.s = sequence(p, u / p.tiles);
+            g.list = p.indices + g.s.page0;
+            g.keys = g.s.len;
+            g.k0 = c * p.own_chunk;
+            g.k1 = min(g.keys, g.k0 + p.own_chunk);
+            g.part = p.prefix_splits + c;
+        }
+        g.row0 = tile * 2 * kTile;
+        g.nrows = min(g.s.n * p.group - g.row0, 2 * kTile);
+        if (g.nrows <= 0) return false;
+        g.ntiles = g.nrows > kTile ? 2 : 1;
+        if (!p.over_prefix) {
+            if (g.k0 >= g.keys && !p.direct) return false;  // no such chunk: the join does not ask for it
+            // no row sees more than the last one
+            g.k1 = min(g.k1, keys_seen(p, g.s, (g.row0 + g.nrows - 1) / p.group, g.keys, g.keys));
+            g.steps = g.k1 > g.k0 ? (g.k1 - g.k0 + kTile - 1) / kTile : 0;
+        }
+        return true;
+    }
+};
+
 template <typename T, int D>
 __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const AttnParams p, const int box,
                                                               const __grid_constant__ CUtensorMap kmap,
@@ -238,49 +304,19 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const AttnParams p
     unsigned char* smem = smem_raw + ((1024 - (smem_addr(smem_raw) & 1023)) & 1023);
     const int tid = threadIdx.x, warp = __shfl_sync(kFull, tid >> 5, 0), lane = tid & 31;
     pdl_trigger();
-
-    // ---- which rows, which keys (as in the kernel for few rows)
-    const int h = blockIdx.y;
-    Sequence s;
-    const int64_t* list;
-    int tile, part, keys, k0, k1;
-    if (p.over_prefix) {
-        part = blockIdx.x % p.prefix_splits;
-        tile = blockIdx.x / p.prefix_splits;
-        s.first = 0;
-        s.n = p.tokens;
-        list = p.prefix_pages;
-        keys = p.prefix_len;
-        k0 = part * p.prefix_chunk;
-        k1 = min(keys, k0 + p.prefix_chunk);
-    } else {
-        const int c = blockIdx.x % p.own_chunks, u = blockIdx.x / p.own_chunks;
-        tile = u % p.tiles;
-        s = sequence(p, u / p.tiles);
-        list = p.indices + s.page0;
-        keys = s.len;
-        k0 = c * p.own_chunk;
-        k1 = min(keys, k0 + p.own_chunk);
-        part = p.prefix_splits + c;
+    if (!p.over_prefix) {
+        Segments some(p);
+        Segment g;
+        if (!some.next(p, g)) {
+            if (blockIdx.x == 0 && blockIdx.y == 0) pdl_wait();
+            return;
+        }
     }
-    const int row0 = tile * 2 * kTile;
-    const int nrows = min(s.n * p.group - row0, 2 * kTile);
-    // grids of a call complete in order: this one, if it is the second, ends after the first
-    const bool work = nrows > 0 && (p.over_prefix || p.direct || k0 < keys);
-    if (!work) {
-        if (blockIdx.x == 0 && blockIdx.y == 0) pdl_wait();
-        return;
-    }
-    if (!p.over_prefix)  // no row sees more than the last one
-        k1 = min(k1, keys_seen(p, s, (row0 + nrows - 1) / p.group, keys, keys));
-    const int steps = k1 > k0 ? (k1 - k0 + kTile - 1) / kTile : 0;
-    const int ntiles = nrows > kTile ? 2 : 1;
 
     const uint32_t sq = smem_addr(smem), ring = sq + 2 * C::kBlock;
-    const char* kbase = static_cast<const char*>(p.k) + h * p.k_head * 2;
-    const char* vbase = static_cast<const char*>(p.v) + h * p.v_head * 2;
-    const uint32_t b_full = smem_addr(sh.full), b_empty = smem_addr(sh.empty), b_s = smem_addr(sh.s_full),
-                   b_ph = smem_addr(sh.p_half), b_p = smem_addr(sh.p_full), b_o = smem_addr(sh.o_done);
+    const uint32_t b_q = smem_addr(sh.q_full), b_full = smem_addr(sh.full), b_empty = smem_addr(sh.empty),
+                   b_s = smem_addr(sh.s_full), b_ph = smem_addr(sh.p_half), b_p = smem_addr(sh.p_full),
+                   b_o = smem_addr(sh.o_done);
     volatile int* fail = &sh.fail;
 
     if (warp == 9) {
@@ -291,12 +327,12 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const AttnParams p
                 mbar_init(&sh.empty[i], 1);
             }
             for (int i = 0; i < 2; ++i) {
+                mbar_init(&sh.q_full[i], kTile);
                 mbar_init(&sh.s_full[i], 1);
-                mbar_init(&sh.p_half[i], 128);
-                mbar_init(&sh.p_full[i], 128);
+                mbar_init(&sh.p_half[i], kTile);
+                mbar_init(&sh.p_full[i], kTile);
                 mbar_init(&sh.o_done[i], 1);
             }
-            mbar_init(&sh.q_full, ntiles * kTile);
             mbar_init(&sh.tail, 1);
             mbar_init(&sh.drained, 1);
             sh.fail = 0;
@@ -307,43 +343,50 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const AttnParams p
     __syncthreads();
     fence_after();
     const uint32_t tmem = sh.tmem;
+    Segments segments(p);
+    Segment g;
 
     if (warp >= 8) asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
     if (warp == 9) {
-        if (steps > 0) {
-            constexpr uint32_t kType = std::is_same<T, __half>::value ? 0 : 1;
-            constexpr uint32_t kBase = 1u << 4 | kType << 7 | kType << 10 | (kTile / 16) << 24;
-            constexpr uint32_t kQK = kBase | (kTile / 8) << 17;
-            constexpr uint32_t kPV = kBase | 1u << 16 | (D / 8) << 17;
-            auto qk = [&](int i, int fill) {
-                const uint32_t q = sq + i * C::kBlock, k = ring + fill % C::kStages * C::kBlock;
+        constexpr uint32_t kType = std::is_same<T, __half>::value ? 0 : 1;
+        constexpr uint32_t kBase = 1u << 4 | kType << 7 | kType << 10 | (kTile / 16) << 24;
+        constexpr uint32_t kQK = kBase | (kTile / 8) << 17;
+        constexpr uint32_t kPV = kBase | 1u << 16 | (D / 8) << 17;
+        auto qk = [&](int i, int fill) {
+            const uint32_t q = sq + i * C::kBlock, k = ring + fill % C::kStages * C::kBlock;
 #pragma unroll
-                for (int kk = 0; kk < D / 16; ++kk) {
-                    const uint32_t off = (kk >> 2) * C::kHalf + (kk & 3) * 32;
-                    mma_ss(tmem + i * kTile, operand(q + off, 16), operand(k + off, 16), kQK, kk > 0);
-                }
-                commit(b_s + i * 8);
-            };
-            auto full = [&](int fill) {
-                const bool ok = __all_sync(kFull, wait(b_full + fill % C::kStages * 8, fill / C::kStages & 1, fail));
-                fence_after();
-                return ok;
-            };
-            bool ok = __all_sync(kFull, wait(smem_addr(&sh.q_full), 0, fail)) && full(0);
-            if (ok) {
-                for (int i = 0; i < ntiles; ++i) qk(i, 0);
-                commit(b_empty);
+            for (int kk = 0; kk < D / 16; ++kk) {
+                const uint32_t off = (kk >> 2) * C::kHalf + (kk & 3) * 32;
+                mma_ss(tmem + i * kTile, operand(q + off, 16), operand(k + off, 16), kQK, kk > 0);
             }
-            for (int j = 0; ok && j < steps; ++j) {
-                const int fv = 2 * j + 1, fk = 2 * j + 2;
-                ok = full(fv) && (j + 1 == steps || full(fk));
+            commit(b_s + i * 8);
+        };
+        auto full = [&](int fill) {
+            const bool ok = __all_sync(kFull, wait(b_full + fill % C::kStages * 8, fill / C::kStages & 1, fail));
+            fence_after();
+            return ok;
+        };
+        auto holds = [&](uint32_t bar, int parity) { return __all_sync(kFull, wait(bar, parity & 1, fail)); };
+        bool ok = true;
+        int f = 0, done0 = 0, done1 = 0, seg0 = 0, seg1 = 0;  // fills; steps and segments of each tile
+        while (ok && segments.next(p, g)) {
+            if (g.steps == 0) continue;
+            ok = holds(b_q, seg0++) && (g.ntiles == 1 || holds(b_q + 8, seg1++)) && full(f);
+            if (!ok) break;
+            for (int i = 0; i < g.ntiles; ++i) qk(i, f);
+            commit(b_empty + f % C::kStages * 8);
+            for (int j = 0; j < g.steps; ++j) {
+                const int fv = f + 2 * j + 1, fk = fv + 1;
+                const bool more = j + 1 < g.steps;
+                ok = full(fv) && (!more || full(fk));
                 const uint32_t v = ring + fv % C::kStages * C::kBlock;
-                for (int i = 0; ok && i < ntiles; ++i) {
+                for (int i = 0; ok && i < g.ntiles; ++i) {
+                    const int turn = (i ? done1 : done0) + j;
                     // the first half of P's columns is multiplied while the second is made
 #pragma unroll
                     for (int kk = 0; kk < kTile / 16; ++kk) {
                         if (kk == 0 || kk == kTile / 32) {
-                            if (!(ok = __all_sync(kFull, wait((kk ? b_p : b_ph) + i * 8, j & 1, fail)))) break;
+                            if (!(ok = holds((kk ? b_p : b_ph) + i * 8, turn))) break;
                             fence_after();
                         }
                         mma_ts(tmem + kColO + i * kTile, tmem + i * kTile + kk * 8, operand(v + kk * 2048, C::kHalf), kPV,
@@ -352,78 +395,92 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const AttnParams p
                     if (!ok) break;
                     commit(b_o + i * 8);
                     // S of the next step goes over P: the tensor core works in the order of issue
-                    if (j + 1 < steps) qk(i, fk);
+                    if (more) qk(i, fk);
                 }
                 if (!ok) break;
                 commit(b_empty + fv % C::kStages * 8);
-                if (j + 1 < steps) commit(b_empty + fk % C::kStages * 8);
+                if (more) commit(b_empty + fk % C::kStages * 8);
             }
-            if (!ok) {  // leave no product under way
-                commit(smem_addr(&sh.drained));
-                mbar_wait(&sh.drained, 0);
-            }
+            f += 2 * g.steps;
+            done0 += g.steps;
+            if (g.ntiles == 2) done1 += g.steps;
+        }
+        if (!ok) {  // leave no product under way
+            commit(smem_addr(&sh.drained));
+            mbar_wait(&sh.drained, 0);
         }
     } else if (warp == 8 || warp == 10) {
         // Lane l looks up the page of box l of a tile one tile ahead; the warp issues box after
         // box.  A box that holds no key, or whose page does not exist, is not fetched.
         const int is_v = warp == 10, boxes = kTile / box;
         const CUtensorMap* map = is_v ? &vmap : &kmap;
-        int page, slot;
-        auto find = [&](int at) {
-            page = -1, slot = 0;
-            if (at < k1) locate(p, list, at, page, slot);
-        };
-        if (lane < boxes) find(k0 + lane * box);
-        int j = 0;
-        for (; j < steps; ++j) {
-            const int f = 2 * j + is_v, st = f % C::kStages, kt = k0 + j * kTile, have = min(k1 - kt, kTile);
-            const uint32_t dst = ring + st * C::kBlock, bar = b_full + st * 8;
-            // Values past the end must be zeros (P is zero there, but 0 * NaN is not), so the last
-            // tile lands on a barrier of its own and is delivered when they are.
-            const bool tail = is_v && have < kTile;
-            if (f >= C::kStages && !__all_sync(kFull, wait(b_empty + st * 8, (f / C::kStages - 1) & 1, fail))) break;
-            const uint32_t to = tail ? smem_addr(&sh.tail) : bar;
-            for (int g = 0; g < boxes; g += 32) {  // more than 32 boxes: pages of fewer than 4 rows in common
-                if (g > 0) find(kt + (g + lane) * box);
-                const bool mine = lane < boxes - g && page >= 0;
-                const uint32_t held = __ballot_sync(kFull, mine);
-                // the phase's one arrival comes with the last group: none completes it before
-                if (lane == 0) {
-                    const uint32_t bytes = __popc(held) * box * D * 2;
-                    if (g + 32 >= boxes) mbar_arrive_expect_tx(tail ? &sh.tail : &sh.full[st], bytes);
-                    else mbar_expect_tx(tail ? &sh.tail : &sh.full[st], bytes);
-                }
-                __syncwarp();
-                for (int i = 0; i < min(boxes - g, 32); ++i) {
-                    const int pg = __shfl_sync(kFull, page, i), sl = __shfl_sync(kFull, slot, i);
-                    if (!(held >> i & 1)) continue;
+        int f0 = 0, tails = 0;  // fills before this segment, tails so far
+        bool ok = true;
+        while (ok && segments.next(p, g)) {
+            int page, slot;
+            auto find = [&](int at) {
+                page = -1, slot = 0;
+                if (at < g.k1) locate(p, g.list, at, page, slot);
+            };
+            if (lane < boxes) find(g.k0 + lane * box);
+            for (int j = 0; j < g.steps; ++j) {
+                const int f = f0 + 2 * j + is_v, st = f % C::kStages, kt = g.k0 + j * kTile, have = min(g.k1 - kt, kTile);
+                const uint32_t dst = ring + st * C::kBlock, bar = b_full + st * 8;
+                // Values past the end must be zeros (P is zero there, but 0 * NaN is not), so the
+                // last tile lands on a barrier of its own and is delivered when they are.
+                const bool tail = is_v && have < kTile;
+                if (f >= C::kStages && !(ok = __all_sync(kFull, wait(b_empty + st * 8, (f / C::kStages - 1) & 1, fail)))) break;
+                uint64_t* const land = tail ? &sh.tail : &sh.full[st];
+                for (int b = 0; b < boxes; b += 32) {  // more than 32: page and tile have fewer than 4 rows in common
+                    if (b > 0) find(kt + (b + lane) * box);
+                    const uint32_t held = __ballot_sync(kFull, lane < boxes - b && page >= 0);
+                    // the phase's one arrival comes with the last boxes: none completes it before
+                    if (lane == 0) {
+                        const uint32_t bytes = __popc(held) * box * D * 2;
+                        if (b + 32 >= boxes) mbar_arrive_expect_tx(land, bytes);
+                        else mbar_expect_tx(land, bytes);
+                    }
+                    __syncwarp();
+                    for (int i = 0; i < min(boxes - b, 32); ++i) {
+                        const int pg = __shfl_sync(kFull, page, i), sl = __shfl_sync(kFull, slot, i);
+                        if (!(held >> i & 1)) continue;
 #pragma unroll
-                    for (int half = 0; half < D / 64; ++half)
-                        load_box(dst + half * C::kHalf + (g + i) * box * 128, map, half * 64, sl, h, pg, to);
+                        for (int half = 0; half < D / 64; ++half)
+                            load_box(dst + half * C::kHalf + (b + i) * box * 128, map, half * 64, sl, g.h, pg, smem_addr(land));
+                    }
+                }
+                if (lane < boxes) find(kt + kTile + lane * box);
+                if (tail) {
+                    wait(smem_addr(&sh.tail), tails++ & 1, fail);
+                    for (int i = have * 8 + lane; i < kTile * 8; i += 32)
+#pragma unroll
+                        for (int half = 0; half < D / 64; ++half)
+                            *reinterpret_cast<uint4*>(smem + (dst - sq) + half * C::kHalf + i * 16) = make_uint4(0, 0, 0, 0);
+                    fence_async();
+                    __syncwarp();
+                    if (lane == 0) arrive(bar);
                 }
             }
-            if (lane < boxes) find(kt + kTile + lane * box);
-            if (tail) {
-                wait(to, 0, fail);
-                for (int i = have * 8 + lane; i < kTile * 8; i += 32)
-#pragma unroll
-                    for (int half = 0; half < D / 64; ++half)
-                        *reinterpret_cast<uint4*>(smem + (dst - sq) + half * C::kHalf + i * 16) = make_uint4(0, 0, 0, 0);
-                fence_async();
-                __syncwarp();
-                if (lane == 0) arrive(bar);
-            }
+            if (ok) f0 += 2 * g.steps;
         }
         __syncwarp();
         if (*fail)  // leave no copy under way
-            for (int i = max(0, j - C::kStages); i < j; ++i)
-                mbar_wait(&sh.full[(2 * i + is_v) % C::kStages], (2 * i + is_v) / C::kStages & 1);
+            for (int f = max(0, f0 - C::kStages); f < f0 + C::kStages; ++f)
+                if ((f & 1) == is_v) mbar_wait_brief(&sh.full[f % C::kStages], f / C::kStages & 1);
     } else if (warp < 8) {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
         const int my = warp >> 2, row = tid;  // the warp's tile, the thread's row of the CTA
-        if (my < ntiles) {
+        int done = 0;                         // steps of the tile so far
+        while (segments.next(p, g)) {
+            if (my >= g.ntiles) continue;
+            const Sequence& s = g.s;
+            const int h = g.h, row0 = g.row0, nrows = g.nrows, steps = g.steps, k0 = g.k0, k1 = g.k1, keys = g.keys;
+            const int part = g.part;
+            const int64_t* list = g.list;
+            const char* kbase = static_cast<const char*>(p.k) + h * p.k_head * 2;
+            const char* vbase = static_cast<const char*>(p.v) + h * p.v_head * 2;
             // ---- queries, swizzled, zeros where there is no row; all loads are under way at once
-            {
+            if (steps > 0) {
                 constexpr int kStep = kTile / CH;  // rows between a thread's chunks
                 const int rt = tid & (kTile - 1), c = rt % CH, f0 = my * kTile + rt / CH;
                 const int dt = kStep / p.group, dg = kStep % p.group;
@@ -447,7 +504,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const AttnParams p
                     *reinterpret_cast<uint4*>(smem + my * C::kBlock + (c >> 3) * C::kHalf + r * 128 + (((c ^ r) & 7) << 4)) = v[i];
                 }
                 fence_async();
-                arrive(smem_addr(&sh.q_full));
+                arrive(b_q + my * 8);
             }
             int seen = 0;  // keys that the thread's row sees, up to k1
             if (row < nrows) {
@@ -468,7 +525,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const AttnParams p
             float m = -INFINITY, l = 0.f;  // P is taken relative to m
             bool ok = true;
             for (int j = 0; j < steps; ++j) {
-                if (!(ok = wait(b_s + my * 8, j & 1, fail))) break;
+                if (!(ok = wait(b_s + my * 8, (done + j) & 1, fail))) break;
                 fence_after();
                 if (rows_here) {
                     uint32_t x[kTile];
@@ -497,7 +554,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const AttnParams p
                         if (grow) m = top;
                         l *= keep;
                         if (j > 0) {
-                            if (!(ok = wait(b_o + my * 8, (j - 1) & 1, fail))) break;
+                            if (!(ok = wait(b_o + my * 8, (done + j - 1) & 1, fail))) break;
                             fence_after();
 #pragma unroll 1
                             for (int c = 0; c < D; c += 16) {
@@ -553,7 +610,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const AttnParams p
                 fence_before();
                 arrive(b_p + my * 8);
             }
-            if (ok && steps > 0) ok = wait(b_o + my * 8, (steps - 1) & 1, fail);
+            if (ok && steps > 0) ok = wait(b_o + my * 8, (done + steps - 1) & 1, fail);
             fence_after();
             // ---- the rows' results
             if (!ok) l = NAN;  // loud: a wait that ran out leaves no number
@@ -638,6 +695,9 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const AttnParams p
                 }
             }
             fence_before();
+            done += steps;
+            // the tile's memory and TMEM may be written again
+            asm volatile("bar.sync %0, 128;" ::"r"(my + 1) : "memory");
         }
     }
     __syncwarp();
@@ -646,6 +706,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const AttnParams p
         fence_after();
         tmem_free(tmem, kCols);
     }
+    // grids of a call complete in order: this one, if it is the second, ends after the first
     if (blockIdx.x == 0 && blockIdx.y == 0) pdl_wait();
 }
 
@@ -699,7 +760,7 @@ int tc_launch(const AttnParams& p, int64_t units, bool pdl, cudaStream_t st) {
         rc = check_cuda(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem),
                         "cudaFuncSetAttribute");
     if (rc != TG_OK) return rc;
-    const dim3 grid((unsigned)units, (unsigned)p.kv_heads);
+    const dim3 grid((unsigned)units, p.over_prefix ? 1u : (unsigned)p.kv_heads);
     if (pdl) return launch_pdl("attn_tc_kernel", kernel, grid, kThreads, C::kSmem, st, p, box, kmap, vmap);
     kernel<<<grid, kThreads, C::kSmem, st>>>(p, box, kmap, vmap);
     return check_launch("attn_tc_kernel");
