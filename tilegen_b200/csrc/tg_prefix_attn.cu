@@ -33,37 +33,43 @@ __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], 
     }
 }
 // ------------------------------------------------------------------ few rows
-// One CTA: RT*16 rows (of one sequence's tokens x group, or of all tokens over the prefix),
-// one key head, one chunk of keys.  Its four warps take 16 keys in turn, each with its own
-// ring of K and V tiles and its own running maximum and sum, so nothing but the end
-// synchronises the CTA; the four results are joined in shared memory.
+// One warp: RT*16 rows (of one sequence's tokens x group, or of all tokens over the prefix), one
+// key head, one chunk of keys, 16 at a time.
 //
-// Bound: HBM (the keys and values of a chunk are read once for 16 RT rows).  The rows are
-// the 16 rows of mma.m16n8k16; S stays in registers and is the A operand of the second
-// product as it lies.  Rows of shared memory are padded by 16 bytes, which makes every
-// ldmatrix free of bank conflicts for any head dim.
-constexpr int kRowWarps = 4;
+// Bound: HBM (the keys and values of a chunk are read once for 16 RT rows).  A row of K or V is
+// one bulk copy, one lane each, into the warp's ring; nothing synchronises warps, so an SM holds
+// as many as its shared memory does, at different places of their chunks, and the chain of page
+// table, page and result is hidden.  (Four warps of a CTA with 16-byte copies and a joint end
+// took 700 instructions a step instead of 200 and reached 4.1 TB/s.)  The rows are the 16 rows of
+// mma.m16n8k16; S stays in registers and is the A operand of the second product as it lies.
+// Rows of shared memory are padded by 16 bytes, which makes every ldmatrix free of bank conflicts
+// for any head dim.
 constexpr int kStepKeys = 16;
 
 template <int D, int RT>
 struct RowCfg {
     static constexpr int kPitch = D * 2 + 16;
     static constexpr int kStage = 2 * kStepKeys * kPitch;  // K then V
-    static constexpr int kStages = D <= 64 ? 6 : D <= 96 ? 4 : 3;
-    static constexpr int kQ = RT * 16 * kPitch;
-    static constexpr int kSmem = kQ + kRowWarps * kStages * kStage;
-    static_assert(kRowWarps * RT * 16 * D * 4 <= kRowWarps * kStages * kStage, "the join reuses the ring");
+    static constexpr int kStages = 3;
+    static constexpr int kQ = RT == 1 ? 0 : RT * 16 * kPitch;
+    static constexpr int kSmem = kQ + kStages * kStage;
     static_assert(RT * 16 * kStepKeys * 4 <= kStepKeys * kPitch, "a step's P fits its K tile");
 };
 
+__device__ __forceinline__ void bulk_row(uint32_t dst, const void* src, uint32_t bytes, uint64_t* bar) {
+    asm volatile("cp.async.bulk.shared::cta.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src),
+                 "r"(bytes), "r"(smem_addr(bar))
+                 : "memory");
+}
+
 template <typename T, int D, int RT>
-__global__ void __launch_bounds__(kRowWarps * 32) attn_rows_kernel(const AttnParams p) {
+__global__ void __launch_bounds__(32) attn_rows_kernel(const AttnParams p) {
     using C = RowCfg<D, RT>;
     constexpr int CH = D / 8;  // 16-byte chunks of a row
     constexpr int S = C::kStages;
     extern __shared__ __align__(16) unsigned char smem[];
-    __shared__ float s_m[kRowWarps][RT * 16], s_l[kRowWarps][RT * 16];
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    __shared__ uint64_t bar[S];
+    const int lane = threadIdx.x;
     pdl_trigger();
     // The grids of a call complete in order: this one (the second) ends after the first.
     struct AtEnd {
@@ -76,7 +82,7 @@ __global__ void __launch_bounds__(kRowWarps * 32) attn_rows_kernel(const AttnPar
     const int h = blockIdx.y;
     Sequence s;
     const int64_t* list;
-    int tile, part, nrows, keys, k0, k1;
+    int tile, part, keys, k0, k1;
     if (p.over_prefix) {
         part = blockIdx.x % p.prefix_splits;
         tile = blockIdx.x / p.prefix_splits;
@@ -97,34 +103,37 @@ __global__ void __launch_bounds__(kRowWarps * 32) attn_rows_kernel(const AttnPar
         part = p.prefix_splits + c;
         if (k0 >= keys && !p.direct) return;  // no such chunk: the join does not ask for it
     }
-    nrows = s.n * p.group - tile * RT * 16;
+    const int row0 = tile * RT * 16, nrows = min(s.n * p.group - row0, RT * 16);
     if (nrows <= 0) return;
-    nrows = min(nrows, RT * 16);
-    const int row0 = tile * RT * 16;
+    if (!p.over_prefix)  // no row sees more than the last one
+        k1 = min(k1, keys_seen(p, s, (row0 + nrows - 1) / p.group, keys, keys));
+    const int steps = max(0, (k1 - k0 + kStepKeys - 1) / kStepKeys);
 
-    const char* kbase = static_cast<const char*>(p.k) + h * p.k_head * 2;
-    const char* vbase = static_cast<const char*>(p.v) + h * p.v_head * 2;
-    const uint32_t ring = smem_addr(smem) + C::kQ + warp * S * C::kStage;
-    const int kw = k0 + warp * kStepKeys;  // this warp's first key; its steps are 64 keys apart
-    const int steps = max(0, (k1 - kw + kRowWarps * kStepKeys - 1) / (kRowWarps * kStepKeys));
-
-    // lane & 15: the key of a step whose page this lane looks up
+    if (lane == 0) {
+        for (int i = 0; i < S; ++i) mbar_init(&bar[i], 1);
+        fence_mbar_init();
+    }
+    __syncwarp();
+    const bool is_v = lane >= kStepKeys;  // lanes 0-15: the rows of K, 16-31: of V
+    const char* base = is_v ? static_cast<const char*>(p.v) + h * p.v_head * 2 : static_cast<const char*>(p.k) + h * p.k_head * 2;
+    const int64_t page_stride = is_v ? p.v_page : p.k_page, slot_stride = is_v ? p.v_slot : p.k_slot;
+    const uint32_t ring = smem_addr(smem) + C::kQ;
     auto find = [&](int i, int& page, int& slot) {
-        const int at = kw + i * kRowWarps * kStepKeys + (lane & 15);
+        const int at = k0 + i * kStepKeys + (lane & 15);
         page = -1;
         slot = 0;
         if (at < k1) locate(p, list, at, page, slot);
     };
     auto fetch = [&](int stage, int page, int slot) {
-        const uint32_t dst = ring + stage * C::kStage;
-#pragma unroll
-        for (int i = 0; i < kStepKeys * CH / 32; ++i) {
-            const int id = i * 32 + lane, r = id / CH, c = id % CH;
-            const int pg = __shfl_sync(kFull, page, r), sl = __shfl_sync(kFull, slot, r);
-            const bool ok = pg >= 0;
-            const int64_t ko = ok ? pg * p.k_page + sl * p.k_slot : 0, vo = ok ? pg * p.v_page + sl * p.v_slot : 0;
-            cp_async16(dst + r * C::kPitch + c * 16, kbase + ko * 2 + c * 16, ok);
-            cp_async16(dst + (kStepKeys + r) * C::kPitch + c * 16, vbase + vo * 2 + c * 16, ok);
+        const uint32_t at = C::kQ + stage * C::kStage + lane * C::kPitch;
+        const uint32_t there = __ballot_sync(kFull, page >= 0);
+        if (lane == 0) mbar_arrive_expect_tx(&bar[stage], __popc(there) * D * 2);
+        __syncwarp();
+        if (page >= 0) {
+            bulk_row(smem_addr(smem) + at, base + (page * page_stride + slot * slot_stride) * 2, D * 2, &bar[stage]);
+        } else {  // past the end: zeros, so that no 0 * NaN arises
+#pragma unroll 1
+            for (int c = 0; c < CH; ++c) *reinterpret_cast<uint4*>(smem + at + c * 16) = make_uint4(0, 0, 0, 0);
         }
     };
     {
@@ -132,21 +141,36 @@ __global__ void __launch_bounds__(kRowWarps * 32) attn_rows_kernel(const AttnPar
 #pragma unroll
         for (int i = 0; i < S; ++i) find(i, page[i], slot[i]);
 #pragma unroll
-        for (int i = 0; i < S; ++i) {
+        for (int i = 0; i < S; ++i)
             if (i < steps) fetch(i, page[i], slot[i]);
-            cp_async_commit();
-        }
     }
 
-    // ---- queries to shared memory, zeros for rows that are not there
-    for (int i = tid; i < RT * 16 * CH; i += kRowWarps * 32) {
-        const int r = i / CH, c = i % CH;
-        uint4 v = make_uint4(0, 0, 0, 0);
-        if (r < nrows) {
-            const int f = row0 + r, t = s.first + f / p.group, qh = h * p.group + f % p.group;
-            v = *reinterpret_cast<const uint4*>(static_cast<const char*>(p.q) + (t * p.q_tok + qh * p.q_head) * 2 + c * 16);
+    // ---- queries: fragments in registers for one row tile, in shared memory for two; zeros for
+    // rows that are not there
+    uint32_t qf[RT == 1 ? D / 16 : 1][4];
+    const uint32_t qaddr = smem_addr(smem) + (lane & 15) * C::kPitch + (lane >> 4) * 16;
+    const char* qbase = static_cast<const char*>(p.q) + (int64_t)h * p.group * p.q_head * 2;
+    if constexpr (RT == 1) {
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            const int r = (lane >> 2) + 8 * e, f = row0 + (r < nrows ? r : 0);
+            const char* q = qbase + ((int64_t)(s.first + f / p.group) * p.q_tok + f % p.group * p.q_head + 2 * (lane & 3)) * 2;
+#pragma unroll
+            for (int kk = 0; kk < D / 16; ++kk)
+#pragma unroll
+                for (int x = 0; x < 2; ++x)
+                    qf[kk][2 * x + e] = r < nrows ? __ldg(reinterpret_cast<const uint32_t*>(q + kk * 32 + x * 16)) : 0;
         }
-        *reinterpret_cast<uint4*>(smem + r * C::kPitch + c * 16) = v;
+    } else {
+#pragma unroll 4
+        for (int i = lane; i < RT * 16 * CH; i += 32) {
+            const int r = i / CH, c = i % CH, f = row0 + (r < nrows ? r : 0);
+            uint4 v = __ldg(reinterpret_cast<const uint4*>(
+                qbase + ((int64_t)(s.first + f / p.group) * p.q_tok + f % p.group * p.q_head) * 2 + c * 16));
+            if (r >= nrows) v = make_uint4(0, 0, 0, 0);
+            *reinterpret_cast<uint4*>(smem + r * C::kPitch + c * 16) = v;
+        }
+        __syncwarp();
     }
     // ---- keys that each of the thread's rows sees (none where there is no row)
     int seen[RT][2];
@@ -168,14 +192,6 @@ __global__ void __launch_bounds__(kRowWarps * 32) attn_rows_kernel(const AttnPar
                 }
             }
         }
-    __syncthreads();
-
-    uint32_t qf[RT == 1 ? D / 16 : 1][4];
-    const uint32_t qaddr = smem_addr(smem) + (lane & 15) * C::kPitch + (lane >> 4) * 16;
-    if constexpr (RT == 1) {
-#pragma unroll
-        for (int kk = 0; kk < D / 16; ++kk) ldmatrix4(qaddr + kk * 32, qf[kk]);
-    }
 
     float o[RT][D / 8][4], m[RT][2], l[RT][2];
 #pragma unroll
@@ -188,14 +204,17 @@ __global__ void __launch_bounds__(kRowWarps * 32) attn_rows_kernel(const AttnPar
             for (int e = 0; e < 4; ++e) o[rt][n][e] = 0.f;
     }
 
-    int stage = 0;
+    int stage = 0, phase = 0;
+    bool ok = true;
     for (int it = 0; it < steps; ++it) {
         int page, slot;
         find(it + S, page, slot);
-        cp_async_wait<S - 1>();
-        __syncwarp();
+        if (!__all_sync(kFull, mbar_wait(&bar[stage], phase))) {
+            ok = false;
+            break;
+        }
         const uint32_t kt = ring + stage * C::kStage, vt = kt + kStepKeys * C::kPitch;
-        const int key0 = kw + it * kRowWarps * kStepKeys;
+        const int key0 = k0 + it * kStepKeys;
 
         float sc[RT][2][4];
 #pragma unroll
@@ -321,14 +340,12 @@ __global__ void __launch_bounds__(kRowWarps * 32) attn_rows_kernel(const AttnPar
         }
         __syncwarp();
         if (it + S < steps) fetch(stage, page, slot);
-        cp_async_commit();
-        stage = stage + 1 == S ? 0 : stage + 1;
+        if (++stage == S) stage = 0, phase ^= 1;
     }
-    cp_async_wait<0>();
-    __syncthreads();  // the rings are free
+    if (!ok)  // a copy that has not landed in 2 s: leave none under way, and no number
+        for (int i = 0; i < S; ++i) mbar_wait(&bar[i], phase ^ (i < stage));
 
-    // ---- join the four warps
-    float* so = reinterpret_cast<float*>(smem + C::kQ) + warp * RT * 16 * D;
+    // ---- results
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
@@ -336,59 +353,40 @@ __global__ void __launch_bounds__(kRowWarps * 32) attn_rows_kernel(const AttnPar
             float sum = l[rt][e];
             sum += __shfl_xor_sync(kFull, sum, 1);
             sum += __shfl_xor_sync(kFull, sum, 2);
+            if (!ok) sum = NAN;
             const int r = rt * 16 + (lane >> 2) + 8 * e;
-            if ((lane & 3) == 0) {
-                s_m[warp][r] = m[rt][e];
-                s_l[warp][r] = sum;
+            if (r >= nrows) continue;
+            const int f = row0 + r, t = s.first + f / p.group, qh = h * p.group + f % p.group;
+            const int64_t row = (int64_t)t * p.q_heads + qh;
+            if (p.direct) {
+                const float inv = sum == 0.f ? 0.f : 1.f / sum;
+                T* out = static_cast<T*>(p.out) + t * p.o_tok + qh * p.o_head + 2 * (lane & 3);
+#pragma unroll
+                for (int n = 0; n < D / 8; ++n)
+                    *reinterpret_cast<uint32_t*>(out + n * 8) = pack2<T>(o[rt][n][2 * e] * inv, o[rt][n][2 * e + 1] * inv);
+                if (p.lse && (lane & 3) == 0)
+                    p.lse[row] = sum == 0.f ? -INFINITY : (m[rt][e] + log2f(sum)) * 0.69314718055994531f;
+            } else {
+                const int64_t at = (int64_t)part * p.tokens * p.q_heads + row;
+                float* out = p.part_o + at * D + 2 * (lane & 3);
+#pragma unroll
+                for (int n = 0; n < D / 8; ++n)
+                    *reinterpret_cast<float2*>(out + n * 8) = make_float2(o[rt][n][2 * e], o[rt][n][2 * e + 1]);
+                if ((lane & 3) == 0) p.part_ml[at] = make_float2(m[rt][e], sum);
             }
-#pragma unroll
-            for (int n = 0; n < D / 8; ++n)
-                *reinterpret_cast<float2*>(so + r * D + n * 8 + 2 * (lane & 3)) =
-                    make_float2(o[rt][n][2 * e], o[rt][n][2 * e + 1]);
         }
-    __syncthreads();
-    const float* all = reinterpret_cast<const float*>(smem + C::kQ);
-    for (int i = tid; i < nrows * (D / 4); i += kRowWarps * 32) {
-        const int r = i / (D / 4), c = i % (D / 4) * 4;
-        float top = s_m[0][r];
-#pragma unroll
-        for (int w = 1; w < kRowWarps; ++w) top = fmaxf(top, s_m[w][r]);
-        const float base = top == -INFINITY ? 0.f : top;
-        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-        float sum = 0.f;
-#pragma unroll
-        for (int w = 0; w < kRowWarps; ++w) {
-            const float f = exp2_fast(s_m[w][r] - base);
-            const float4 x = *reinterpret_cast<const float4*>(all + (w * RT * 16 + r) * D + c);
-            if (s_l[w][r] == 0.f) continue;  // no key of this warp is seen (a NaN score leaves l NaN)
-            acc.x += f * x.x, acc.y += f * x.y, acc.z += f * x.z, acc.w += f * x.w;
-            sum += f * s_l[w][r];
-        }
-        const int f = row0 + r, t = s.first + f / p.group, qh = h * p.group + f % p.group;
-        const int64_t row = (int64_t)t * p.q_heads + qh;
-        if (p.direct) {
-            const float inv = sum == 0.f ? 0.f : 1.f / sum;
-            uint2 y;
-            y.x = pack2<T>(acc.x * inv, acc.y * inv);
-            y.y = pack2<T>(acc.z * inv, acc.w * inv);
-            *reinterpret_cast<uint2*>(static_cast<char*>(p.out) + (t * p.o_tok + qh * p.o_head + c) * 2) = y;
-            if (p.lse && c == 0) p.lse[row] = sum == 0.f ? -INFINITY : (top + log2f(sum)) * 0.69314718055994531f;
-        } else {
-            const int64_t at = (int64_t)part * p.tokens * p.q_heads + row;
-            *reinterpret_cast<float4*>(p.part_o + at * D + c) = acc;
-            if (c == 0) p.part_ml[at] = make_float2(top, sum);
-        }
-    }
 }
 
 // ------------------------------------------------------------------ joining the parts
-// One warp a row.  Bound: L2 (the parts were just written), so loads are 16 bytes a lane and
-// four parts are in flight.
-template <typename T, int D>
+// WPR warps a row, each with every WPR-th part: one where rows are many, all four where parts
+// are (147 parts of 64 rows: 63 us by one warp a row, DRAM latency after latency).  Bound: L2 (the
+// parts were just written), so loads are 16 bytes a lane and eight parts are in flight.
+template <typename T, int D, int WPR>
 __global__ void __launch_bounds__(128) attn_join_kernel(const AttnParams p) {
     constexpr int VE = D % 128 == 0 ? 4 : D % 64 == 0 ? 2 : 1, NV = D / (32 * VE);
-    const int lane = threadIdx.x & 31;
-    const int64_t all = (int64_t)p.tokens * p.q_heads, row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
+    __shared__ float s_acc[WPR == 1 ? 1 : 4][D], s_sum[4], s_top[4];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, mine = WPR == 1 ? 0 : warp;
+    const int64_t all = (int64_t)p.tokens * p.q_heads, row = WPR == 1 ? (int64_t)blockIdx.x * 4 + warp : blockIdx.x;
     pdl_wait();
     if (row >= all) return;
     const int t = (int)(row / p.q_heads), qh = (int)(row % p.q_heads);
@@ -404,15 +402,15 @@ __global__ void __launch_bounds__(128) attn_join_kernel(const AttnParams p) {
     }
     auto part = [&](int i) { return (i < np ? i : i - np + p.prefix_splits) * all + row; };
     float top = -INFINITY;
-    for (int i = lane; i < n; i += 32) top = fmaxf(top, p.part_ml[part(i)].x);
+    for (int i = lane * WPR + mine; i < n; i += 32 * WPR) top = fmaxf(top, p.part_ml[part(i)].x);
 #pragma unroll
     for (int x = 16; x; x >>= 1) top = fmaxf(top, __shfl_xor_sync(kFull, top, x));
     const float base = top == -INFINITY ? 0.f : top;
     float acc[NV * VE], sum = 0.f;
 #pragma unroll
     for (int i = 0; i < NV * VE; ++i) acc[i] = 0.f;
-#pragma unroll 4
-    for (int i = 0; i < n; ++i) {
+#pragma unroll 8
+    for (int i = mine; i < n; i += WPR) {
         const float2 ml = p.part_ml[part(i)];
         const float* x = p.part_o + part(i) * D;
         const float f = exp2_fast(ml.x - base);
@@ -432,6 +430,29 @@ __global__ void __launch_bounds__(128) attn_join_kernel(const AttnParams p) {
             }
 #pragma unroll
             for (int e = 0; e < VE; ++e) acc[j * VE + e] += f * v[e];
+        }
+    }
+    if constexpr (WPR > 1) {
+#pragma unroll
+        for (int j = 0; j < NV; ++j)
+#pragma unroll
+            for (int e = 0; e < VE; ++e) s_acc[warp][(j * 32 + lane) * VE + e] = acc[j * VE + e];
+        if (lane == 0) s_sum[warp] = sum, s_top[warp] = top;
+        __syncthreads();
+        if (warp > 0) return;
+        top = fmaxf(fmaxf(s_top[0], s_top[1]), fmaxf(s_top[2], s_top[3]));
+        const float all_base = top == -INFINITY ? 0.f : top;
+        sum = 0.f;
+#pragma unroll
+        for (int i = 0; i < NV * VE; ++i) acc[i] = 0.f;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+            const float f = s_sum[w] == 0.f ? 0.f : exp2_fast(s_top[w] - all_base);
+            sum += f * s_sum[w];
+#pragma unroll
+            for (int j = 0; j < NV; ++j)
+#pragma unroll
+                for (int e = 0; e < VE; ++e) acc[j * VE + e] += f * s_acc[w][(j * 32 + lane) * VE + e];
         }
     }
     const float inv = sum == 0.f ? 0.f : 1.f / sum;
@@ -537,13 +558,13 @@ int make_plan(const tg_prefix_attention_args* a, Plan* plan, const char* op) {
     const bool tc = attn_tc_fits(p, c.dim);
     plan->rt_own = tc && rows_own > 32 ? 0 : rows_own > 16 && c.dim <= 128 ? 2 : 1;
     plan->rt_prefix = tc && rows_all > 32 ? 0 : rows_all > 16 && c.dim <= 128 ? 2 : 1;
-    const int64_t step_own = plan->rt_own ? 64 : 128, target_own = plan->rt_own ? kSMs * 8 : kSMs * 2;
+    const int64_t warps = kSMs * 7;  // warps of the kernel for few rows that run at once (heads of 128)
     const int64_t tiles_own = ceil_div(std::max<int64_t>(rows_own, 1), plan->rt_own ? 16 * plan->rt_own : 256);
     const int64_t tiles_all = ceil_div(std::max<int64_t>(rows_all, 1), plan->rt_prefix ? 16 * plan->rt_prefix : 256);
     if (p.prefix_len > 0) {
         if (plan->rt_prefix) {
-            const int64_t n = std::max<int64_t>(1, kSMs * 8 / (tiles_all * c.heads));
-            p.prefix_chunk = (int)std::max<int64_t>(256, ceil_div(ceil_div(p.prefix_len, n), 64) * 64);
+            const int64_t n = std::max<int64_t>(1, warps / (tiles_all * c.heads));
+            p.prefix_chunk = (int)std::max<int64_t>(128, ceil_div(ceil_div(p.prefix_len, n), 16) * 16);
             p.prefix_splits = (int)ceil_div(p.prefix_len, p.prefix_chunk);
         } else {
             p.prefix_tiles = (int)tiles_all;
@@ -551,8 +572,17 @@ int make_plan(const tg_prefix_attention_args* a, Plan* plan, const char* op) {
         }
     }
     if (max_seq > 0 || p.prefix_len == 0) {
-        const int64_t n = std::max<int64_t>(1, target_own / std::max<int64_t>(1, t.rows * tiles_own * c.heads));
-        p.own_chunk = (int)std::max<int64_t>(256, ceil_div(ceil_div(max_seq, n), step_own) * step_own);
+        // The kernel for few rows: two rounds of its warps, in chunks of 128 to 512 keys (or 64
+        // chunks, for sequences that may be long) so that long sequences do not end alone.  The
+        // tcgen05 kernel: two CTAs an SM.
+        const int64_t units = std::max<int64_t>(1, t.rows * tiles_own * c.heads);
+        if (plan->rt_own) {
+            const int64_t even = ceil_div(ceil_div(max_seq, std::max<int64_t>(1, 2 * warps / units)), 16) * 16;
+            p.own_chunk = (int)std::min(std::max<int64_t>(128, even), std::max<int64_t>(512, ceil_div(max_seq, 64 * 16) * 16));
+        } else {
+            const int64_t n = std::max<int64_t>(1, 2 * kSMs / units);
+            p.own_chunk = (int)std::max<int64_t>(256, ceil_div(ceil_div(max_seq, n), 128) * 128);
+        }
         p.own_chunks = (int)std::max<int64_t>(1, ceil_div(max_seq, p.own_chunk));
     }
     plan->own_units = t.rows * tiles_own * p.own_chunks;
@@ -571,14 +601,13 @@ int make_plan(const tg_prefix_attention_args* a, Plan* plan, const char* op) {
 template <typename T, int D, int RT>
 int rows_launch(const AttnParams& p, int64_t units, bool pdl, cudaStream_t st) {
     using C = RowCfg<D, RT>;
-    static_assert(C::kSmem <= 227 * 1024 - 1024, "shared memory of a CTA");
     auto kernel = attn_rows_kernel<T, D, RT>;
     const int rc = check_cuda(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem),
                               "cudaFuncSetAttribute");
     if (rc != TG_OK) return rc;
     const dim3 grid((unsigned)units, (unsigned)p.kv_heads);
-    if (pdl) return launch_pdl("attn_rows_kernel", kernel, grid, kRowWarps * 32, C::kSmem, st, p);
-    kernel<<<grid, kRowWarps * 32, C::kSmem, st>>>(p);
+    if (pdl) return launch_pdl("attn_rows_kernel", kernel, grid, 32, C::kSmem, st, p);
+    kernel<<<grid, 32, C::kSmem, st>>>(p);
     return check_launch("attn_rows_kernel");
 }
 
@@ -613,8 +642,9 @@ int attn_run(const Plan& plan, void* ws, cudaStream_t st) {
         if (rc != TG_OK) return rc;
     }
     if (p.direct) return TG_OK;
-    return launch_pdl("attn_join_kernel", attn_join_kernel<T, D>, dim3((unsigned)ceil_div((int64_t)rows, 4)), 128, 0, st,
-                      p);
+    if (parts > 8 && rows < 4 * kSMs * 16)
+        return launch_pdl("attn_join_kernel", attn_join_kernel<T, D, 4>, dim3((unsigned)rows), 128, 0, st, p);
+    return launch_pdl("attn_join_kernel", attn_join_kernel<T, D, 1>, dim3((unsigned)ceil_div((int64_t)rows, 4)), 128, 0, st, p);
 }
 
 template <typename T>
