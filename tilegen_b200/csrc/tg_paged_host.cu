@@ -1,7 +1,7 @@
 // Argument and index checks shared by the paged operators.
 #include <algorithm>
 
-#include "tg_paged.cuh"
+#include "tg_prefix_attn.cuh"
 
 namespace tg {
 
@@ -105,6 +105,49 @@ int paged_bounds_check(const tg_csr& t, int64_t page_size, const int64_t* seq_le
                          (h & 4) ? " indptr[rows]!=nnz" : "", (h & 8) ? " page out of range" : "",
                          (h & 16) ? " seq_len out of range" : "", (h & 32) ? " q_indptr" : "",
                          (h & 64) ? " prefix page out of range" : "", (h & 128) ? " more new tokens than seq_len" : "");
+    return TG_OK;
+}
+
+// ------------------------------------------------------------------ tensor maps
+namespace {
+
+using EncodeFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                              const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                              CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+EncodeFn encoder() {
+    static const EncodeFn fn = [] {
+        void* f = nullptr;
+        cudaDriverEntryPointQueryResult found;
+        if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &f, 12000, cudaEnableDefault, &found) != cudaSuccess ||
+            found != cudaDriverEntryPointSuccess)
+            f = nullptr;
+        return reinterpret_cast<EncodeFn>(f);
+    }();
+    return fn;
+}
+
+}  // namespace
+
+int cache_maps(const AttnParams& p, bool is_half, int dim, int box_rows, CUtensorMap* k, CUtensorMap* v) {
+    *k = *v = CUtensorMap{};
+    if (p.pages == 0) return TG_OK;  // no page, no box
+    if (!encoder()) return set_error(TG_ECUDA, "cuTensorMapEncodeTiled is not available");
+    // the stride of a dimension of one is of no use to anyone and may be anything
+    const auto bytes = [&](int64_t n, int64_t stride) { return (cuuint64_t)(n > 1 ? stride : dim) * 2; };
+    for (int i = 0; i < 2; ++i) {
+        const int64_t page = i ? p.v_page : p.k_page, slot = i ? p.v_slot : p.k_slot, head = i ? p.v_head : p.k_head;
+        const cuuint64_t size[4] = {(cuuint64_t)dim, (cuuint64_t)p.page_size, (cuuint64_t)p.kv_heads, (cuuint64_t)p.pages};
+        const cuuint64_t stride[3] = {bytes(p.page_size, slot), bytes(p.kv_heads, head), bytes(p.pages, page)};
+        const cuuint32_t box[4] = {64, (cuuint32_t)box_rows, 1, 1}, step[4] = {1, 1, 1, 1};
+        const CUresult r = encoder()(i ? v : k, is_half ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4,
+                                     const_cast<void*>(i ? p.v : p.k), size, stride, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                                     CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                                     CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+        if (r != CUDA_SUCCESS)
+            return set_error(TG_ECUDA, "cuTensorMapEncodeTiled: CUDA error %d (page_size=%d strides %lld %lld %lld)", (int)r,
+                             p.page_size, (long long)page, (long long)slot, (long long)head);
+    }
     return TG_OK;
 }
 

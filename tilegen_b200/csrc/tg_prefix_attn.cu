@@ -1,6 +1,7 @@
 // Attention of a batch that shares a prefix (tg_prefix_attention_*): the kernel for few
 // rows, the join of the parts, planning and the C entry points.
 #include <algorithm>
+#include <numeric>
 
 #include "tg_prefix_attn.cuh"
 
@@ -36,39 +37,36 @@ __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], 
 // One warp: RT*16 rows (of one sequence's tokens x group, or of all tokens over the prefix), one
 // key head, one chunk of keys, 16 at a time.
 //
-// Bound: HBM (the keys and values of a chunk are read once for 16 RT rows).  A row of K or V is
-// one bulk copy, one lane each, into the warp's ring; nothing synchronises warps, so an SM holds
-// as many as its shared memory does, at different places of their chunks, and the chain of page
-// table, page and result is hidden.  (Four warps of a CTA with 16-byte copies and a joint end
-// took 700 instructions a step instead of 200 and reached 4.1 TB/s.)  The rows are the 16 rows of
-// mma.m16n8k16; S stays in registers and is the A operand of the second product as it lies.
-// Rows of shared memory are padded by 16 bytes, which makes every ldmatrix free of bank conflicts
-// for any head dim.
+// Bound: HBM (the keys and values of a chunk are read once for 16 RT rows).  16 keys are a TMA box
+// of 64 columns (or as many boxes as pages cut them into), which lands swizzled, free of bank
+// conflicts for ldmatrix; nothing synchronises warps, so an SM holds as many as its shared memory
+// does, at different places of their chunks, and the chain of page table, page and result is
+// hidden.  The rows are the 16 rows of mma.m16n8k16; S stays in registers and is the A operand of
+// the second product as it lies.
 constexpr int kStepKeys = 16;
 
 template <int D, int RT>
 struct RowCfg {
-    static constexpr int kPitch = D * 2 + 16;
-    static constexpr int kStage = 2 * kStepKeys * kPitch;  // K then V
+    static constexpr int kHalves = (D + 63) / 64;
+    static constexpr int kBox = kStepKeys * 128;  // bytes of 64 columns of 16 rows
+    static constexpr int kStage = 2 * kHalves * kBox;  // K then V
     static constexpr int kStages = 3;
+    static constexpr int kPitch = D * 2 + 16;  // of the queries, padded
     static constexpr int kQ = RT == 1 ? 0 : RT * 16 * kPitch;
-    static constexpr int kSmem = kQ + kStages * kStage;
-    static_assert(RT * 16 * kStepKeys * 4 <= kStepKeys * kPitch, "a step's P fits its K tile");
+    static constexpr int kSmem = kStages * kStage + kQ + 64;  // and the barriers
+    static_assert(RT * 16 * kStepKeys * 4 <= kHalves * kBox, "a step's P fits its K tile");
 };
 
-__device__ __forceinline__ void bulk_row(uint32_t dst, const void* src, uint32_t bytes, uint64_t* bar) {
-    asm volatile("cp.async.bulk.shared::cta.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src),
-                 "r"(bytes), "r"(smem_addr(bar))
-                 : "memory");
-}
-
 template <typename T, int D, int RT>
-__global__ void __launch_bounds__(32) attn_rows_kernel(const AttnParams p) {
+__global__ void __launch_bounds__(32) attn_rows_kernel(const AttnParams p, const int box,
+                                                       const __grid_constant__ CUtensorMap kmap,
+                                                       const __grid_constant__ CUtensorMap vmap) {
     using C = RowCfg<D, RT>;
     constexpr int CH = D / 8;  // 16-byte chunks of a row
     constexpr int S = C::kStages;
-    extern __shared__ __align__(16) unsigned char smem[];
-    __shared__ uint64_t bar[S];
+    extern __shared__ __align__(1024) unsigned char smem[];
+    unsigned char* const sq = smem + S * C::kStage;
+    uint64_t* const bar = reinterpret_cast<uint64_t*>(sq + C::kQ);
     const int lane = threadIdx.x;
     pdl_trigger();
     // The grids of a call complete in order: this one (the second) ends after the first.
@@ -114,28 +112,33 @@ __global__ void __launch_bounds__(32) attn_rows_kernel(const AttnParams p) {
         fence_mbar_init();
     }
     __syncwarp();
-    const bool is_v = lane >= kStepKeys;  // lanes 0-15: the rows of K, 16-31: of V
-    const char* base = is_v ? static_cast<const char*>(p.v) + h * p.v_head * 2 : static_cast<const char*>(p.k) + h * p.k_head * 2;
-    const int64_t page_stride = is_v ? p.v_page : p.k_page, slot_stride = is_v ? p.v_slot : p.k_slot;
-    const uint32_t ring = smem_addr(smem) + C::kQ;
+    const uint32_t ring = smem_addr(smem);
+    const int boxes = kStepKeys / box;
+    uint32_t missing = 0;  // stages of which a box was not fetched
+    // lane l: the page of box l of a step
     auto find = [&](int i, int& page, int& slot) {
-        const int at = k0 + i * kStepKeys + (lane & 15);
+        const int at = k0 + i * kStepKeys + lane * box;
         page = -1;
         slot = 0;
-        if (at < k1) locate(p, list, at, page, slot);
+        if (lane < boxes && at < k1) locate(p, list, at, page, slot);
     };
     auto fetch = [&](int stage, int page, int slot) {
-        const uint32_t at = C::kQ + stage * C::kStage + lane * C::kPitch;
-        const uint32_t there = __ballot_sync(kFull, page >= 0);
-        if (lane == 0) mbar_arrive_expect_tx(&bar[stage], __popc(there) * D * 2);
+        const uint32_t dst = ring + stage * C::kStage, there = __ballot_sync(kFull, page >= 0);
+        missing = (missing & ~(1u << stage)) | (uint32_t)(__popc(there) < boxes) << stage;
+        if (lane == 0) mbar_arrive_expect_tx(&bar[stage], __popc(there) * box * C::kHalves * 256);
         __syncwarp();
-        if (page >= 0) {
-            bulk_row(smem_addr(smem) + at, base + (page * page_stride + slot * slot_stride) * 2, D * 2, &bar[stage]);
-        } else {  // past the end: zeros, so that no 0 * NaN arises
-#pragma unroll 1
-            for (int c = 0; c < CH; ++c) *reinterpret_cast<uint4*>(smem + at + c * 16) = make_uint4(0, 0, 0, 0);
+        for (int i = 0; i < boxes; ++i) {
+            const int pg = __shfl_sync(kFull, page, i), sl = __shfl_sync(kFull, slot, i);
+            if (!(there >> i & 1)) continue;
+#pragma unroll
+            for (int half = 0; half < C::kHalves; ++half) {
+                load_box(dst + half * C::kBox + i * box * 128, &kmap, half * 64, sl, h, pg, smem_addr(&bar[stage]));
+                load_box(dst + (C::kHalves + half) * C::kBox + i * box * 128, &vmap, half * 64, sl, h, pg, smem_addr(&bar[stage]));
+            }
         }
     };
+    // A 16-byte chunk of a row of a tile; rows of 128 bytes, chunks swizzled by the row.
+    auto chunk_at = [&](uint32_t tile_at, int r, int c) { return tile_at + (c >> 3) * C::kBox + r * 128 + (((c ^ r) & 7) << 4); };
     {
         int page[S], slot[S];
 #pragma unroll
@@ -148,7 +151,7 @@ __global__ void __launch_bounds__(32) attn_rows_kernel(const AttnParams p) {
     // ---- queries: fragments in registers for one row tile, in shared memory for two; zeros for
     // rows that are not there
     uint32_t qf[RT == 1 ? D / 16 : 1][4];
-    const uint32_t qaddr = smem_addr(smem) + (lane & 15) * C::kPitch + (lane >> 4) * 16;
+    const uint32_t qaddr = smem_addr(sq) + (lane & 15) * C::kPitch + (lane >> 4) * 16;
     const char* qbase = static_cast<const char*>(p.q) + (int64_t)h * p.group * p.q_head * 2;
     if constexpr (RT == 1) {
 #pragma unroll
@@ -168,7 +171,7 @@ __global__ void __launch_bounds__(32) attn_rows_kernel(const AttnParams p) {
             uint4 v = __ldg(reinterpret_cast<const uint4*>(
                 qbase + ((int64_t)(s.first + f / p.group) * p.q_tok + f % p.group * p.q_head) * 2 + c * 16));
             if (r >= nrows) v = make_uint4(0, 0, 0, 0);
-            *reinterpret_cast<uint4*>(smem + r * C::kPitch + c * 16) = v;
+            *reinterpret_cast<uint4*>(sq + r * C::kPitch + c * 16) = v;
         }
         __syncwarp();
     }
@@ -213,8 +216,21 @@ __global__ void __launch_bounds__(32) attn_rows_kernel(const AttnParams p) {
             ok = false;
             break;
         }
-        const uint32_t kt = ring + stage * C::kStage, vt = kt + kStepKeys * C::kPitch;
-        const int key0 = k0 + it * kStepKeys;
+        const uint32_t kt = ring + stage * C::kStage, vt = kt + C::kHalves * C::kBox;
+        const int key0 = k0 + it * kStepKeys, step_end = min(key0 + kStepKeys, k1);
+        // Keys and values past the end, or of pages that do not exist, are zeros: a box may hold
+        // anything there, and 0 * NaN is not 0.
+        if (key0 + kStepKeys > k1 || missing & 1u << stage) {
+            for (int r = 0; r < kStepKeys; ++r) {
+                int pg = -1, sl;
+                if (key0 + r < k1) locate(p, list, key0 + r, pg, sl);
+                if (pg < 0)
+                    for (int c = lane; c < 2 * C::kHalves * 8; c += 32)
+                        *reinterpret_cast<uint4*>(smem + (kt - ring) + (c >> 3) * C::kBox + r * 128 + (c & 7) * 16) = make_uint4(0, 0, 0, 0);
+            }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // a later box may land here
+            __syncwarp();
+        }
 
         float sc[RT][2][4];
 #pragma unroll
@@ -223,11 +239,10 @@ __global__ void __launch_bounds__(32) attn_rows_kernel(const AttnParams p) {
             for (int n = 0; n < 2; ++n)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) sc[rt][n][e] = 0.f;
-        const uint32_t kaddr = kt + ((lane & 7) + ((lane >> 4) << 3)) * C::kPitch + ((lane >> 3) & 1) * 16;
 #pragma unroll
         for (int kk = 0; kk < D / 16; ++kk) {
             uint32_t b[4];
-            ldmatrix4(kaddr + kk * 32, b);
+            ldmatrix4(chunk_at(kt, (lane & 7) + ((lane >> 4) << 3), kk * 2 + ((lane >> 3) & 1)), b);
 #pragma unroll
             for (int rt = 0; rt < RT; ++rt) {
                 if constexpr (RT == 1) {
@@ -244,7 +259,6 @@ __global__ void __launch_bounds__(32) attn_rows_kernel(const AttnParams p) {
 
         uint32_t pf[RT][4];
         bool part_seen = false;  // a row of this lane sees only some of the step's keys
-        const int step_end = min(key0 + kStepKeys, k1);
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
@@ -294,13 +308,12 @@ __global__ void __launch_bounds__(32) attn_rows_kernel(const AttnParams p) {
         if (__any_sync(kFull, part_seen)) {
             bool bad = false;
             for (int i = lane; i < kStepKeys * CH; i += 32)
-                bad |= any_nonfinite<T>(*reinterpret_cast<const uint4*>(smem + (vt - smem_addr(smem)) + (i / CH) * C::kPitch +
-                                                                      (i % CH) * 16));
+                bad |= any_nonfinite<T>(*reinterpret_cast<const uint4*>(smem + (chunk_at(vt, i / CH, i % CH) - ring)));
             by_rows = __any_sync(kFull, bad);
         }
         if (by_rows) {
             __syncwarp();
-            float* sp = reinterpret_cast<float*>(smem + (kt - smem_addr(smem)));  // the K tile is done with
+            float* sp = reinterpret_cast<float*>(smem + (kt - ring));  // the K tile is done with
 #pragma unroll
             for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
@@ -311,7 +324,6 @@ __global__ void __launch_bounds__(32) attn_rows_kernel(const AttnParams p) {
             __syncwarp();
 #pragma unroll 1
             for (int key = 0; key < kStepKeys; ++key) {
-                const T* vr = reinterpret_cast<const T*>(smem + (vt - smem_addr(smem)) + key * C::kPitch) + 2 * (lane & 3);
 #pragma unroll
                 for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
@@ -320,17 +332,17 @@ __global__ void __launch_bounds__(32) attn_rows_kernel(const AttnParams p) {
                         const float w = sp[(rt * 16 + (lane >> 2) + 8 * e) * kStepKeys + key];
 #pragma unroll
                         for (int n = 0; n < D / 8; ++n) {
-                            o[rt][n][2 * e] += w * to_f32(vr[n * 8]);
-                            o[rt][n][2 * e + 1] += w * to_f32(vr[n * 8 + 1]);
+                            const T* vr = reinterpret_cast<const T*>(smem + (chunk_at(vt, key, n) - ring)) + 2 * (lane & 3);
+                            o[rt][n][2 * e] += w * to_f32(vr[0]);
+                            o[rt][n][2 * e + 1] += w * to_f32(vr[1]);
                         }
                     }
             }
         } else {
-            const uint32_t vaddr = vt + (lane & 15) * C::kPitch + (lane >> 4) * 16;
 #pragma unroll
             for (int dn = 0; dn < D / 16; ++dn) {
                 uint32_t b[4];
-                ldmatrix4_trans(vaddr + dn * 32, b);
+                ldmatrix4_trans(chunk_at(vt, lane & 15, dn * 2 + (lane >> 4)), b);
 #pragma unroll
                 for (int rt = 0; rt < RT; ++rt) {
                     mma16816<T>(o[rt][2 * dn], pf[rt], b[0], b[1]);
@@ -553,9 +565,9 @@ int make_plan(const tg_prefix_attention_args* a, Plan* plan, const char* op) {
     p.causal = (a->flags & TG_FLAG_CAUSAL) != 0;
 
     // The kernel for few rows reads the keys once for each 32 rows, the tcgen05 kernel once for
-    // each 256 (where it fits).
+    // each 256 (it exists for heads of 64 and 128).
     const int64_t rows_own = max_q * p.group, rows_all = a->tokens * p.group;
-    const bool tc = attn_tc_fits(p, c.dim);
+    const bool tc = c.dim == 64 || c.dim == 128;
     plan->rt_own = tc && rows_own > 32 ? 0 : rows_own > 16 && c.dim <= 128 ? 2 : 1;
     plan->rt_prefix = tc && rows_all > 32 ? 0 : rows_all > 16 && c.dim <= 128 ? 2 : 1;
     const int64_t warps = kSMs * 7;  // warps of the kernel for few rows that run at once (heads of 128)
@@ -602,12 +614,16 @@ template <typename T, int D, int RT>
 int rows_launch(const AttnParams& p, int64_t units, bool pdl, cudaStream_t st) {
     using C = RowCfg<D, RT>;
     auto kernel = attn_rows_kernel<T, D, RT>;
-    const int rc = check_cuda(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem),
+    const int box = std::gcd(p.page_size, kStepKeys);
+    CUtensorMap kmap, vmap;
+    int rc = cache_maps(p, std::is_same<T, __half>::value, D, box, &kmap, &vmap);
+    if (rc != TG_OK) return rc;
+    rc = check_cuda(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem),
                               "cudaFuncSetAttribute");
     if (rc != TG_OK) return rc;
     const dim3 grid((unsigned)units, (unsigned)p.kv_heads);
-    if (pdl) return launch_pdl("attn_rows_kernel", kernel, grid, 32, C::kSmem, st, p);
-    kernel<<<grid, 32, C::kSmem, st>>>(p);
+    if (pdl) return launch_pdl("attn_rows_kernel", kernel, grid, 32, C::kSmem, st, p, box, kmap, vmap);
+    kernel<<<grid, 32, C::kSmem, st>>>(p, box, kmap, vmap);
     return check_launch("attn_rows_kernel");
 }
 

@@ -7,6 +7,8 @@
 //   M = max m_i,  out = sum_i exp2(m_i - M) o_i / sum_i exp2(m_i - M) l_i.
 #pragma once
 
+#include <cuda.h>
+
 #include "tg_paged.cuh"
 
 namespace tg {
@@ -108,8 +110,25 @@ __device__ __forceinline__ bool any_nonfinite(uint4 v) {
     return bad;
 }
 
+// A box of a [page][head][slot][dim] map: 64 elements from x of the rows from `slot`.
+__device__ __forceinline__ void load_box(uint32_t dst, const CUtensorMap* map, int x, int slot, int head, int page,
+                                         uint32_t bar) {
+    asm volatile(
+        "{\n\t.reg .pred e;\n\telect.sync _|e, 0xffffffff;\n\t"
+        "@e cp.async.bulk.tensor.4d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];"
+        "\n\t}" ::"r"(dst),
+        "l"(map), "r"(x), "r"(slot), "r"(head), "r"(page), "r"(bar)
+        : "memory");
+}
+__device__ __forceinline__ void mbar_expect_tx(uint64_t* bar, uint32_t bytes) {
+    asm volatile("mbarrier.expect_tx.relaxed.cta.shared::cta.b64 [%0], %1;" ::"r"(smem_addr(bar)), "r"(bytes) : "memory");
+}
+
+// Tensor maps of the keys and values as [page][head][slot][dim], boxes of box_rows slots of 64
+// elements of one head, rows of 128 bytes swizzled by 128 bytes (tg_paged_host.cu).
+int cache_maps(const AttnParams& p, bool is_half, int dim, int box_rows, CUtensorMap* k, CUtensorMap* v);
+
 // tg_prefix_attn_tc.cu
-bool attn_tc_fits(const AttnParams& p, int dim);
 template <typename T>
 int attn_tc_run(const AttnParams& p, int dim, int64_t units, bool pdl, cudaStream_t st);
 

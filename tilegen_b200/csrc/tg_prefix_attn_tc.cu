@@ -16,8 +16,6 @@
 // O is rescaled only where a row's maximum has grown by more than 2^8 since the value that P is
 // taken relative to: P stays below 2^8, far inside the range of either type and of the 32-bit
 // sums, and the relative precision of P is that of any other reference.
-#include <cuda.h>
-
 #include <numeric>
 
 #include "tg_prefix_attn.cuh"
@@ -37,16 +35,6 @@ __device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::be
 __device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
-// A box of a [page][head][slot][dim] map: 64 elements from x of the rows from `slot`.
-__device__ __forceinline__ void load_box(uint32_t dst, const CUtensorMap* map, int x, int slot, int head, int page,
-                                         uint32_t bar) {
-    asm volatile(
-        "{\n\t.reg .pred e;\n\telect.sync _|e, 0xffffffff;\n\t"
-        "@e cp.async.bulk.tensor.4d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];"
-        "\n\t}" ::"r"(dst),
-        "l"(map), "r"(x), "r"(slot), "r"(head), "r"(page), "r"(bar)
-        : "memory");
-}
 __device__ __forceinline__ void fence_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 // The issuing warp runs as one, with operands the same in all lanes (so that they can live in
 // uniform registers), and one elected lane issues.
@@ -176,10 +164,6 @@ struct TcShared {
     uint32_t tmem;
     int fail;  // a wait ran out
 };
-
-__device__ __forceinline__ void mbar_expect_tx(uint64_t* bar, uint32_t bytes) {
-    asm volatile("mbarrier.expect_tx.relaxed.cta.shared::cta.b64 [%0], %1;" ::"r"(smem_addr(bar)), "r"(bytes) : "memory");
-}
 
 // Bounded wait; false once one has run out in this CTA (2 s; every wait here is microseconds).
 __device__ __forceinline__ bool wait(uint32_t bar, uint32_t parity, volatile int* fail) {
@@ -711,50 +695,13 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const AttnParams p
 }
 
 // ------------------------------------------------------------------ host
-using EncodeFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
-                              const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
-                              CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-
-EncodeFn encoder() {
-    static const EncodeFn fn = [] {
-        void* f = nullptr;
-        cudaDriverEntryPointQueryResult found;
-        if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &f, 12000, cudaEnableDefault, &found) != cudaSuccess ||
-            found != cudaDriverEntryPointSuccess)
-            f = nullptr;
-        return reinterpret_cast<EncodeFn>(f);
-    }();
-    return fn;
-}
-
-// Rows of a box: what a page and a tile can both be cut into.
-int box_rows(int page_size) { return std::gcd(page_size, kTile); }
-
-bool strides_fit(int64_t page, int64_t slot, int64_t head) {  // bytes below 2^40
-    return page < (1ll << 38) && slot < (1ll << 38) && head < (1ll << 38) && page >= 0 && slot >= 0 && head >= 0;
-}
-
-template <typename T>
-int cache_map(CUtensorMap* map, const AttnParams& p, const void* data, int64_t page, int64_t slot, int64_t head, int dim) {
-    if (!encoder()) return set_error(TG_ECUDA, "cuTensorMapEncodeTiled is not available");
-    const cuuint64_t size[4] = {(cuuint64_t)dim, (cuuint64_t)p.page_size, (cuuint64_t)p.kv_heads, (cuuint64_t)p.pages};
-    const cuuint64_t stride[3] = {(cuuint64_t)slot * 2, (cuuint64_t)head * 2, (cuuint64_t)page * 2};
-    const cuuint32_t box[4] = {64, (cuuint32_t)box_rows(p.page_size), 1, 1}, step[4] = {1, 1, 1, 1};
-    const CUresult r = encoder()(map, std::is_same<T, __half>::value ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16,
-                                 4, const_cast<void*>(data), size, stride, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                                 CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                                 CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-    return r == CUDA_SUCCESS ? TG_OK : set_error(TG_ECUDA, "cuTensorMapEncodeTiled: CUDA error %d", (int)r);
-}
-
 template <typename T, int D>
 int tc_launch(const AttnParams& p, int64_t units, bool pdl, cudaStream_t st) {
     using C = TcCfg<D>;
     static_assert(C::kSmem + sizeof(TcShared) <= 227 * 1024, "shared memory of a CTA");
-    const int box = box_rows(p.page_size);
+    const int box = std::gcd(p.page_size, kTile);
     CUtensorMap kmap, vmap;
-    int rc = cache_map<T>(&kmap, p, p.k, p.k_page, p.k_slot, p.k_head, D);
-    if (rc == TG_OK) rc = cache_map<T>(&vmap, p, p.v, p.v_page, p.v_slot, p.v_head, D);
+    int rc = cache_maps(p, std::is_same<T, __half>::value, D, box, &kmap, &vmap);
     auto kernel = attn_tc_kernel<T, D>;
     if (rc == TG_OK)
         rc = check_cuda(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem),
@@ -767,11 +714,6 @@ int tc_launch(const AttnParams& p, int64_t units, bool pdl, cudaStream_t st) {
 }
 
 }  // namespace
-
-bool attn_tc_fits(const AttnParams& p, int dim) {
-    return (dim == 64 || dim == 128) && p.pages > 0 && strides_fit(p.k_page, p.k_slot, p.k_head) &&
-           strides_fit(p.v_page, p.v_slot, p.v_head);
-}
 
 template <typename T>
 int attn_tc_run(const AttnParams& p, int dim, int64_t units, bool pdl, cudaStream_t st) {
