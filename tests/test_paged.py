@@ -81,7 +81,8 @@ def _table(**kw):
 
 def _attention(cache=None, table=None, **kw):
     a = lib.TgPrefixAttentionArgs()
-    a.cache, a.pages = ctypes.pointer(cache or _cache()), ctypes.pointer(table or _table())
+    a.held = cache or _cache(), table or _table()
+    a.cache, a.pages = (ctypes.addressof(x) for x in a.held)
     fields = dict(seq_len=4096, max_seq_len=96, prefix_pages=4096, n_prefix_pages=4, prefix_len=50, tokens=3,
                   q_indptr=None, max_q_len=1, q_heads=4, q=lib.TgRows(4096, 256, 64), out=lib.TgRows(4096, 256, 64),
                   lse=None, scale=0.125, flags=lib.TG_FLAG_CAUSAL)
@@ -143,11 +144,15 @@ def test_attention_refuses_a_missing_or_small_workspace():
     _refused(lib.TG_EINVAL, _attention(), "16-byte", 4100, n)
 
 
+_Q = lib.TgRows(4096, 128, 64)
+
+
 def _append(cache=None, table=None, rope=None, **kw):
     a = lib.TgKvAppendArgs()
-    a.cache, a.pages = ctypes.pointer(cache or _cache()), ctypes.pointer(table or _table())
+    a.held = cache or _cache(), table or _table(), rope
+    a.cache, a.pages = (ctypes.addressof(x) for x in a.held[:2])
     if rope is not None:
-        a.rope = ctypes.pointer(rope)
+        a.rope = ctypes.addressof(rope)
     fields = dict(seq_len=4096, tokens=3, q_indptr=None, k=lib.TgRows(4096, 128, 64), v=lib.TgRows(4096, 128, 64))
     fields.update(kw)
     for k, v in fields.items():
@@ -162,7 +167,7 @@ def _append(cache=None, table=None, rope=None, **kw):
     (dict(rope=lib.TgRope(4096, 31, 0, 1.0)), "rot_dim"),
     (dict(rope=lib.TgRope(4096, 32, 2, 1.0)), "layout"),
     (dict(rope=lib.TgRope(None, 32, 0, 1.0)), "freq"),
-    (dict(q=ctypes.pointer(lib.TgRows(4096, 128, 64)), q_heads=2), "q_out"),
+    (dict(q=ctypes.addressof(_Q), q_heads=2), "q_out"),
     (dict(flags=lib.TG_FLAG_CAUSAL), "flags"),
     (dict(table=_table(rows=0), tokens=3, q_indptr=4096), "sequence"),
 ])

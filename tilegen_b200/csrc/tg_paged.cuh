@@ -5,6 +5,7 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <atomic>
 #include <climits>
 
 #include "../../include/tilegen_b200_paged.h"
@@ -70,6 +71,20 @@ int paged_bounds_check(const tg_csr& t, int64_t page_size, const int64_t* seq_le
                        bool append, const char* op, cudaStream_t st);
 // The device word that bounds checks report into (tg_abi.cu).
 int bounds_word(uint32_t** err);
+
+// Raises a kernel's limit of dynamic shared memory, once on each device.
+struct SmemOnce {
+    std::atomic<uint64_t> done{0};  // devices, by bit
+    int raise(const void* kernel, int bytes) {
+        int dev = 0;
+        const int rc = check_cuda(cudaGetDevice(&dev), "cudaGetDevice");
+        if (rc != TG_OK || (dev < 64 && done.load(std::memory_order_relaxed) >> dev & 1)) return rc;
+        const int set = check_cuda(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes),
+                                   "cudaFuncSetAttribute");
+        if (set == TG_OK && dev < 64) done.fetch_or(1ull << dev, std::memory_order_relaxed);
+        return set;
+    }
+};
 
 // Launch with the programmatic-dependency attribute: the kernel may start while the one
 // before it on the stream still runs, and orders itself with pdl_wait().

@@ -78,10 +78,11 @@ __global__ void __launch_bounds__(32) attn_rows_kernel(const AttnParams p, const
 
     // ---- which rows, which keys
     const int h = blockIdx.y;
+    const bool over_prefix = blockIdx.x < p.prefix_units;
     Sequence s;
     const int64_t* list;
     int tile, part, keys, k0, k1;
-    if (p.over_prefix) {
+    if (over_prefix) {
         part = blockIdx.x % p.prefix_splits;
         tile = blockIdx.x / p.prefix_splits;
         s.first = 0;
@@ -91,7 +92,7 @@ __global__ void __launch_bounds__(32) attn_rows_kernel(const AttnParams p, const
         k0 = part * p.prefix_chunk;
         k1 = min(keys, k0 + p.prefix_chunk);
     } else {
-        const int c = blockIdx.x % p.own_chunks, u = blockIdx.x / p.own_chunks;
+        const int x = blockIdx.x - p.prefix_units, c = x % p.own_chunks, u = x / p.own_chunks;
         tile = u % p.tiles;
         s = sequence(p, u / p.tiles);
         list = p.indices + s.page0;
@@ -103,7 +104,7 @@ __global__ void __launch_bounds__(32) attn_rows_kernel(const AttnParams p, const
     }
     const int row0 = tile * RT * 16, nrows = min(s.n * p.group - row0, RT * 16);
     if (nrows <= 0) return;
-    if (!p.over_prefix)  // no row sees more than the last one
+    if (!over_prefix)  // no row sees more than the last one
         k1 = min(k1, keys_seen(p, s, (row0 + nrows - 1) / p.group, keys, keys));
     const int steps = max(0, (k1 - k0 + kStepKeys - 1) / kStepKeys);
 
@@ -185,7 +186,7 @@ __global__ void __launch_bounds__(32) attn_rows_kernel(const AttnParams p, const
             seen[rt][e] = 0;
             if (r < nrows) {
                 const int i = (row0 + r) / p.group;
-                if (!p.over_prefix) {
+                if (!over_prefix) {
                     seen[rt][e] = keys_seen(p, s, i, keys, keys);
                 } else if (!p.causal) {
                     seen[rt][e] = keys;
@@ -412,38 +413,49 @@ __global__ void __launch_bounds__(128) attn_join_kernel(const AttnParams p) {
         const Sequence s = sequence(p, sequence_of(p.q_indptr, p.rows, t));
         if (t >= s.first && t < s.first + s.n) n += (s.len + p.own_chunk - 1) / p.own_chunk;
     }
+    // lane l holds the maximum and sum of the l-th of 32 of the warp's parts at a time
     auto part = [&](int i) { return (i < np ? i : i - np + p.prefix_splits) * all + row; };
-    float top = -INFINITY;
-    for (int i = lane * WPR + mine; i < n; i += 32 * WPR) top = fmaxf(top, p.part_ml[part(i)].x);
+    const int count = (n - mine + WPR - 1) / WPR;
+    float2 first = make_float2(-INFINITY, 0.f);
+    if (lane < count) first = p.part_ml[part(lane * WPR + mine)];
+    float top = first.x;
+    for (int i = lane + 32; i < count; i += 32) top = fmaxf(top, p.part_ml[part(i * WPR + mine)].x);
 #pragma unroll
     for (int x = 16; x; x >>= 1) top = fmaxf(top, __shfl_xor_sync(kFull, top, x));
     const float base = top == -INFINITY ? 0.f : top;
     float acc[NV * VE], sum = 0.f;
 #pragma unroll
     for (int i = 0; i < NV * VE; ++i) acc[i] = 0.f;
+    for (int i0 = 0; i0 < count; i0 += 32) {
+        float2 ml = first;
+        if (i0 > 0) ml = i0 + lane < count ? p.part_ml[part((i0 + lane) * WPR + mine)] : make_float2(-INFINITY, 0.f);
+        // 0: nothing seen there, nothing written; a NaN score leaves the sum NaN
+        const float mine_f = ml.y == 0.f ? 0.f : ml.y != ml.y ? NAN : exp2_fast(ml.x - base);
+        sum += mine_f == 0.f ? 0.f : mine_f * ml.y;
+        const int here = min(32, count - i0);
 #pragma unroll 8
-    for (int i = mine; i < n; i += WPR) {
-        const float2 ml = p.part_ml[part(i)];
-        const float* x = p.part_o + part(i) * D;
-        const float f = exp2_fast(ml.x - base);
-        if (ml.y == 0.f) continue;  // nothing seen there
-        sum += f * ml.y;
+        for (int i = 0; i < here; ++i) {
+            const float f = __shfl_sync(kFull, mine_f, i);
+            const float* x = p.part_o + part((i0 + i) * WPR + mine) * D;
 #pragma unroll
-        for (int j = 0; j < NV; ++j) {
-            float v[VE];
-            if constexpr (VE == 4) {
-                const float4 y = *reinterpret_cast<const float4*>(x + (j * 32 + lane) * 4);
-                v[0] = y.x, v[1] = y.y, v[2] = y.z, v[3] = y.w;
-            } else if constexpr (VE == 2) {
-                const float2 y = *reinterpret_cast<const float2*>(x + (j * 32 + lane) * 2);
-                v[0] = y.x, v[1] = y.y;
-            } else {
-                v[0] = x[j * 32 + lane];
+            for (int j = 0; j < NV; ++j) {
+                float v[VE];
+                if constexpr (VE == 4) {
+                    const float4 y = *reinterpret_cast<const float4*>(x + (j * 32 + lane) * 4);
+                    v[0] = y.x, v[1] = y.y, v[2] = y.z, v[3] = y.w;
+                } else if constexpr (VE == 2) {
+                    const float2 y = *reinterpret_cast<const float2*>(x + (j * 32 + lane) * 2);
+                    v[0] = y.x, v[1] = y.y;
+                } else {
+                    v[0] = x[j * 32 + lane];
+                }
+#pragma unroll
+                for (int e = 0; e < VE; ++e) acc[j * VE + e] += f == 0.f ? 0.f : f * v[e];
             }
-#pragma unroll
-            for (int e = 0; e < VE; ++e) acc[j * VE + e] += f * v[e];
         }
     }
+#pragma unroll
+    for (int x = 16; x; x >>= 1) sum += __shfl_xor_sync(kFull, sum, x);
     if constexpr (WPR > 1) {
 #pragma unroll
         for (int j = 0; j < NV; ++j)
@@ -505,7 +517,9 @@ void share_prefix(AttnParams& p, int64_t rows, int dim, double own_bytes) {
     double best = 1e30;
     int ctas = 1;
     for (int64_t n = 1; n <= std::min<int64_t>(kSMs, p.prefix_work); ++n) {
-        const double cta = 5.0 + step * (double)ceil_div(p.prefix_work, n) + 5.0 * (double)(ceil_div(units, n) + (units % n != 0));
+        // an even share that does not end where a pair does is in one more pair
+        const bool even = n >= units ? n % units == 0 : units % n == 0;
+        const double cta = 5.0 + step * (double)ceil_div(p.prefix_work, n) + 5.0 * (double)(ceil_div(units, n) + !even);
         const double all = own_bytes / 6e6 + cta * (double)n / kSMs;
         const double parts = 1.0 + (double)n / (double)units;
         const double t = std::max(cta, all) + parts * (double)rows * p.kv_heads * dim * 8 / 6e6;
@@ -565,21 +579,23 @@ int make_plan(const tg_prefix_attention_args* a, Plan* plan, const char* op) {
     p.causal = (a->flags & TG_FLAG_CAUSAL) != 0;
 
     // The kernel for few rows reads the keys once for each 32 rows, the tcgen05 kernel once for
-    // each 256 (it exists for heads of 64 and 128).
+    // each 256 (it exists for heads of 64 and 128) but begins and ends for 10 us.  Own parts of 320
+    // keys, 48 sequences: 56 rows 58 against 64 us, 80 rows 79 against 74 us.
     const int64_t rows_own = max_q * p.group, rows_all = a->tokens * p.group;
     const bool tc = c.dim == 64 || c.dim == 128;
-    plan->rt_own = tc && rows_own > 32 ? 0 : rows_own > 16 && c.dim <= 128 ? 2 : 1;
+    plan->rt_own = tc && rows_own > 64 ? 0 : rows_own > 16 && c.dim <= 128 ? 2 : 1;
     plan->rt_prefix = tc && rows_all > 32 ? 0 : rows_all > 16 && c.dim <= 128 ? 2 : 1;
+    if (p.prefix_len > 0 && plan->rt_prefix) plan->rt_own = plan->rt_prefix;  // one launch for both
     const int64_t warps = kSMs * 7;  // warps of the kernel for few rows that run at once (heads of 128)
     const int64_t tiles_own = ceil_div(std::max<int64_t>(rows_own, 1), plan->rt_own ? 16 * plan->rt_own : 256);
     const int64_t tiles_all = ceil_div(std::max<int64_t>(rows_all, 1), plan->rt_prefix ? 16 * plan->rt_prefix : 256);
     if (p.prefix_len > 0) {
+        p.prefix_tiles = (int)tiles_all;
         if (plan->rt_prefix) {
             const int64_t n = std::max<int64_t>(1, warps / (tiles_all * c.heads));
             p.prefix_chunk = (int)std::max<int64_t>(128, ceil_div(ceil_div(p.prefix_len, n), 16) * 16);
             p.prefix_splits = (int)ceil_div(p.prefix_len, p.prefix_chunk);
         } else {
-            p.prefix_tiles = (int)tiles_all;
             share_prefix(p, rows_all, c.dim, (double)t.nnz * c.page_size * c.heads * c.dim * 4);
         }
     }
@@ -599,7 +615,7 @@ int make_plan(const tg_prefix_attention_args* a, Plan* plan, const char* op) {
     }
     plan->own_units = t.rows * tiles_own * p.own_chunks;
     plan->prefix_units = p.prefix_ctas ? p.prefix_ctas : tiles_all * p.prefix_splits;
-    if (plan->own_units > INT32_MAX || plan->prefix_units > INT32_MAX || c.heads > 65535)
+    if (plan->own_units + plan->prefix_units > INT32_MAX || c.heads > 65535)
         return set_error(TG_EUNSUPPORTED, "%s: too many rows for one launch", op);
     p.tiles = (int)tiles_own;
     const int parts = p.prefix_splits + p.own_chunks;
@@ -634,29 +650,30 @@ int attn_run(const Plan& plan, void* ws, cudaStream_t st) {
     const size_t parts = p.prefix_splits + p.own_chunks;
     p.part_o = static_cast<float*>(ws);
     p.part_ml = reinterpret_cast<float2*>(static_cast<char*>(ws) + (parts * rows * D * sizeof(float) + 255) / 256 * 256);
-    bool first = true;
-    auto launch = [&](const AttnParams& q, int rt, int64_t units) {
-        const bool pdl = !first;
-        first = false;
+    int rc = TG_OK;
+    bool second = false;
+    if (p.prefix_ctas > 0) {
         if constexpr (D == 64 || D == 128) {
-            if (rt == 0) return attn_tc_run<T>(q, D, units, pdl, st);
+            AttnParams q = p;
+            q.over_prefix = 1;
+            q.tiles = p.prefix_tiles;
+            rc = attn_tc_run<T>(q, D, p.prefix_ctas, false, st);
         }
-        if constexpr (D <= 128) {
-            if (rt == 2) return rows_launch<T, D, 2>(q, units, pdl, st);
+        second = true;
+    } else {
+        p.prefix_units = (int)plan.prefix_units;
+    }
+    const int64_t units = plan.own_units + p.prefix_units;
+    if (rc == TG_OK && units > 0) {
+        if (plan.rt_own == 0) {
+            if constexpr (D == 64 || D == 128) rc = attn_tc_run<T>(p, D, units, second, st);
+        } else if (plan.rt_own == 2) {
+            if constexpr (D <= 128) rc = rows_launch<T, D, 2>(p, units, second, st);
+        } else {
+            rc = rows_launch<T, D, 1>(p, units, second, st);
         }
-        return rows_launch<T, D, 1>(q, units, pdl, st);
-    };
-    if (p.prefix_splits > 0) {
-        AttnParams q = p;
-        q.over_prefix = 1;
-        q.tiles = p.prefix_tiles;
-        const int rc = launch(q, plan.rt_prefix, plan.prefix_units);
-        if (rc != TG_OK) return rc;
     }
-    if (p.own_chunks > 0) {
-        const int rc = launch(p, plan.rt_own, plan.own_units);
-        if (rc != TG_OK) return rc;
-    }
+    if (rc != TG_OK) return rc;
     if (p.direct) return TG_OK;
     if (parts > 8 && rows < 4 * kSMs * 16)
         return launch_pdl("attn_join_kernel", attn_join_kernel<T, D, 4>, dim3((unsigned)rows), 128, 0, st, p);

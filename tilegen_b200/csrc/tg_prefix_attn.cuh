@@ -35,7 +35,8 @@ struct AttnParams {
     int prefix_ctas, prefix_steps, prefix_tiles;  // prefix_ctas 0: splits of prefix_chunk keys
     int own_chunks, own_chunk;        // most chunks of a sequence, keys of a chunk
     int tiles;                        // row tiles of a sequence (own) or of all rows (prefix)
-    int over_prefix;                  // this launch: the prefix, else the sequences' own pages
+    int over_prefix;                  // the tcgen05 kernel: the prefix, else the sequences' own pages
+    int prefix_units;                 // the kernel for few rows: its first blocks go over the prefix
     int direct;                       // the only part: rows are finished here
     float* part_o;                    // [part][token][head][dim]
     float2* part_ml;                  // [part][token][head]: m, l

@@ -703,9 +703,9 @@ int tc_launch(const AttnParams& p, int64_t units, bool pdl, cudaStream_t st) {
     CUtensorMap kmap, vmap;
     int rc = cache_maps(p, std::is_same<T, __half>::value, D, box, &kmap, &vmap);
     auto kernel = attn_tc_kernel<T, D>;
+    static SmemOnce once;
     if (rc == TG_OK)
-        rc = check_cuda(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem),
-                        "cudaFuncSetAttribute");
+        rc = once.raise(reinterpret_cast<const void*>(kernel), C::kSmem);
     if (rc != TG_OK) return rc;
     const dim3 grid((unsigned)units, p.over_prefix ? 1u : (unsigned)p.kv_heads);
     if (pdl) return launch_pdl("attn_tc_kernel", kernel, grid, kThreads, C::kSmem, st, p, box, kmap, vmap);

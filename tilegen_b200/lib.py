@@ -127,16 +127,16 @@ class TgPagedKV(ctypes.Structure):
 
 class TgKvAppendArgs(ctypes.Structure):
     _fields_ = [
-        ("cache", ctypes.POINTER(TgPagedKV)),
-        ("pages", ctypes.POINTER(TgCsr)),
+        ("cache", ctypes.c_void_p),  # TgPagedKV
+        ("pages", ctypes.c_void_p),  # TgCsr
         ("seq_len", ctypes.c_void_p),
         ("tokens", ctypes.c_int64),
         ("q_indptr", ctypes.c_void_p),
         ("k", TgRows),
         ("v", TgRows),
-        ("rope", ctypes.POINTER(TgRope)),
-        ("q", ctypes.POINTER(TgRows)),
-        ("q_out", ctypes.POINTER(TgRows)),
+        ("rope", ctypes.c_void_p),  # TgRope
+        ("q", ctypes.c_void_p),  # TgRows
+        ("q_out", ctypes.c_void_p),  # TgRows
         ("q_heads", ctypes.c_int32),
         ("position_base", ctypes.c_int64),
         ("positions", ctypes.c_void_p),
@@ -146,8 +146,8 @@ class TgKvAppendArgs(ctypes.Structure):
 
 class TgPrefixAttentionArgs(ctypes.Structure):
     _fields_ = [
-        ("cache", ctypes.POINTER(TgPagedKV)),
-        ("pages", ctypes.POINTER(TgCsr)),
+        ("cache", ctypes.c_void_p),  # TgPagedKV
+        ("pages", ctypes.c_void_p),  # TgCsr
         ("seq_len", ctypes.c_void_p),
         ("max_seq_len", ctypes.c_int64),
         ("prefix_pages", ctypes.c_void_p),

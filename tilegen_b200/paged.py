@@ -15,7 +15,6 @@ and the prefix itself is written once, as a table of one row.
 
 from __future__ import annotations
 
-import contextlib
 import ctypes
 import math
 from dataclasses import dataclass
@@ -31,6 +30,17 @@ __all__ = ["Rope", "rope_frequencies", "rope", "rope_backward", "PagedKV", "Page
 
 _SUFFIX = {torch.float32: "f32", torch.float16: "f16", torch.bfloat16: "bf16"}
 _LAYOUT = {"half": _lib.TG_ROPE_HALF, "interleaved": _lib.TG_ROPE_INTERLEAVED}
+
+
+_CALLS: dict = {}
+
+
+def _call(name: str):
+    """A function of the library, looked up once."""
+    fn = _CALLS.get(name)
+    if fn is None:
+        fn = _CALLS[name] = getattr(_lib.load(), name)
+    return fn
 
 
 def rope_frequencies(rot_dim: int, base: float = 10000.0, *, scaling: Optional[str] = None, factor: float = 1.0,
@@ -90,14 +100,14 @@ class Rope:
     layout: str = "half"
     scale: float = 1.0
 
-    def desc(self, device: torch.device) -> _lib.TgRope:
-        f = self.freq
-        if f.dtype != torch.float64 or f.dim() != 1 or not f.is_contiguous() or f.device != device:
-            raise ValueError("freq must be a contiguous float64 vector on %s (got %s %s on %s)"
-                             % (device, tuple(f.shape), f.dtype, f.device))
-        if self.layout not in _LAYOUT:
+    def desc(self, index: int) -> _lib.TgRope:
+        f, layout = self.freq, _LAYOUT.get(self.layout)
+        if f.dtype is not torch.float64 or f.dim() != 1 or not f.is_contiguous() or f.get_device() != index:
+            raise ValueError("freq must be a contiguous float64 vector on cuda:%d (got %s %s on %s)"
+                             % (index, tuple(f.shape), f.dtype, f.device))
+        if layout is None:
             raise ValueError("layout must be 'half' or 'interleaved' (got %r)" % (self.layout,))
-        return _lib.TgRope(f.data_ptr(), 2 * f.numel(), _LAYOUT[self.layout], float(self.scale))
+        return _lib.TgRope(f.data_ptr(), 2 * f.shape[0], layout, self.scale)
 
 
 @dataclass
@@ -118,18 +128,16 @@ class PagedKV:
 
     def desc(self) -> _lib.TgPagedKV:
         k, v = self.k, self.v
-        if k.dim() != 4 or k.shape != v.shape or k.dtype != v.dtype or k.device != v.device:
+        shape, ks, vs = k.shape, k.stride(), v.stride()
+        if len(shape) != 4 or shape != v.shape or k.dtype != v.dtype or k.get_device() != v.get_device():
             raise ValueError("k and v must be [pages, page_size, heads, dim] of one type on one device (got %s %s and "
                              "%s %s)" % (tuple(k.shape), k.dtype, tuple(v.shape), v.dtype))
         if not k.is_cuda or k.dtype not in _SUFFIX:
             raise ValueError("the cache must be float32, float16 or bfloat16 on a CUDA device (got %s on %s)"
                              % (k.dtype, k.device))
-        pages, size, heads, dim = k.shape
-        ks, vs = k.stride(), v.stride()
-        if dim > 1 and (ks[3] != 1 or vs[3] != 1):
+        if shape[3] > 1 and (ks[3] != 1 or vs[3] != 1):
             raise ValueError("the cache's last stride must be 1")
-        return _lib.TgPagedKV(k.data_ptr(), v.data_ptr(), pages, size, heads, dim, ks[0], ks[1], ks[2], vs[0], vs[1],
-                              vs[2])
+        return _lib.TgPagedKV(k.data_ptr(), v.data_ptr(), *shape, ks[0], ks[1], ks[2], vs[0], vs[1], vs[2])
 
 
 @dataclass
@@ -154,71 +162,80 @@ class PageTable:
             indptr.append(len(flat))
         return cls(torch.tensor(indptr, dtype=torch.int64).to(d), torch.tensor(flat, dtype=torch.int64).to(d))
 
-    def desc(self, device: torch.device, pages: int) -> _lib.TgCsr:
-        ip, ix = self.indptr, self.indices
-        _vector(ip, "indptr", device)
-        _vector(ix, "indices", device)
-        if ip.numel() < 1:
+    def desc(self, index: int, pages: int) -> _lib.TgCsr:
+        ip, ix = _vector(self.indptr, "indptr", index), _vector(self.indices, "indices", index)
+        rows = self.indptr.shape[0] - 1
+        if rows < 0:
             raise ValueError("indptr must have at least one entry")
-        return _lib.TgCsr(ip.numel() - 1, pages, ix.numel(), ip.data_ptr(), ix.data_ptr(), None)
+        return _lib.TgCsr(rows, pages, self.indices.shape[0], ip, ix, None)
 
 
-def _vector(t: torch.Tensor, name: str, device: torch.device, n: Optional[int] = None) -> int:
-    if t.dtype != torch.int64 or t.dim() != 1 or not t.is_contiguous() or t.device != device:
-        raise ValueError("%s must be a contiguous int64 vector on %s (got %s %s on %s)"
-                         % (name, device, tuple(t.shape), t.dtype, t.device))
-    if n is not None and t.numel() != n:
-        raise ValueError("%s must have %d entries (got %d)" % (name, n, t.numel()))
+# The calls below are made between the kernels of a decoding step, so their checks read what a
+# tensor gives without making an object of it (device numbers instead of devices, for one).
+def _vector(t: torch.Tensor, name: str, index: int, n: Optional[int] = None) -> int:
+    if t.dtype is not torch.int64 or t.dim() != 1 or not t.is_contiguous() or t.get_device() != index:
+        raise ValueError("%s must be a contiguous int64 vector on cuda:%d (got %s %s on %s)"
+                         % (name, index, tuple(t.shape), t.dtype, t.device))
+    if n is not None and t.shape[0] != n:
+        raise ValueError("%s must have %d entries (got %d)" % (name, n, t.shape[0]))
     return t.data_ptr()
 
 
-def _rows(t: torch.Tensor, name: str, shape: Tuple, dtype: torch.dtype, device: torch.device) -> _lib.TgRows:
-    if t.shape != shape or t.dtype != dtype or t.device != device:
-        raise ValueError("%s must be a %s tensor of shape %s on %s (got %s %s on %s)"
-                         % (name, dtype, tuple(shape), device, t.dtype, tuple(t.shape), t.device))
+def _rows(t: torch.Tensor, name: str, shape: Tuple, dtype: torch.dtype, index: int) -> _lib.TgRows:
+    if t.shape != shape or t.dtype is not dtype or t.get_device() != index:
+        raise ValueError("%s must be a %s tensor of shape %s on cuda:%d (got %s %s on %s)"
+                         % (name, dtype, tuple(shape), index, t.dtype, tuple(t.shape), t.device))
     st = t.stride()
     if st[2] != 1 and shape[2] > 1:
         raise ValueError("%s: the last stride must be 1 (got %d)" % (name, st[2]))
     return _lib.TgRows(t.data_ptr(), st[0], st[1])
 
 
-@contextlib.contextmanager
-def _on(stream: torch.cuda.Stream):
-    with torch.cuda.stream(stream):
-        yield
+def _like(t: torch.Tensor) -> torch.Tensor:
+    return torch.empty_like(t) if t.is_contiguous() else torch.empty(t.shape, dtype=t.dtype, device=t.device)
 
 
-def _place(device: torch.device, stream: Optional[torch.cuda.Stream]):
-    """(context, stream pointer): the context makes the device and the stream current, so that
-    outputs and workspaces allocated inside belong to that stream.  Nothing is entered where
-    both are current already."""
+def _stream(index: int, stream: Optional[torch.cuda.Stream]) -> int:
+    """The stream's handle; raises unless it is on device `index`."""
+    if stream is None:
+        return torch._C._cuda_getCurrentRawStream(index)  # current_stream(index).cuda_stream, made once a step
+    if stream.device.index != index:
+        raise ValueError("the stream is on %s and the tensors on cuda:%d" % (stream.device, index))
+    return int(stream.cuda_stream)
+
+
+def _elsewhere(index: int, stream: Optional[torch.cuda.Stream]):
+    """The context in which a call's outputs and workspace are allocated and its kernels launched:
+    they belong to the call's stream and device.  None where both are current already."""
     if stream is not None:
-        if stream.device != device:
-            raise ValueError("the stream is on %s and the tensors on %s" % (stream.device, device))
-        return _on(stream), int(stream.cuda_stream)
-    if torch.cuda.current_device() != device.index:
-        return torch.cuda.device(device), int(torch.cuda.current_stream(device).cuda_stream)
-    return contextlib.nullcontext(), int(torch.cuda.current_stream(device).cuda_stream)
+        return torch.cuda.stream(stream)
+    return torch.cuda.device(index) if torch.cuda.current_device() != index else None
 
 
 def _rope_call(x: torch.Tensor, r: Rope, positions: torch.Tensor, out: Optional[torch.Tensor], flags: int,
                stream) -> torch.Tensor:
-    L = _lib.load()
-    dev = x.device
-    if x.dim() != 3 or dev.type != "cuda" or x.dtype not in _SUFFIX:
+    suffix = _SUFFIX.get(x.dtype)
+    if x.dim() != 3 or not x.is_cuda or suffix is None:
         raise ValueError("x must be [tokens, heads, dim], float32, float16 or bfloat16, on a CUDA device (got %s %s on "
-                         "%s)" % (tuple(x.shape), x.dtype, dev))
+                         "%s)" % (tuple(x.shape), x.dtype, x.device))
+    index, shape = x.get_device(), x.shape
+    xr = _rows(x, "x", shape, x.dtype, index)
+    rd = r.desc(index)
+    pos = _vector(positions, "positions", index, shape[0])
+    sp = _stream(index, stream)
+    where = _elsewhere(index, stream)
+    if where is not None:
+        with where:
+            return _rope_launch(suffix, x, out, xr, rd, pos, flags, sp)
+    return _rope_launch(suffix, x, out, xr, rd, pos, flags, sp)
+
+
+def _rope_launch(suffix, x, out, xr, rd, pos, flags, sp) -> torch.Tensor:
+    if out is None:
+        out = _like(x)
+    yr = _rows(out, "out", x.shape, x.dtype, x.get_device())
     tokens, heads, dim = x.shape
-    xr = _rows(x, "x", x.shape, x.dtype, dev)
-    rd = r.desc(dev)
-    pos = _vector(positions, "positions", dev, tokens)
-    ctx, sp = _place(dev, stream)
-    with ctx:
-        if out is None:
-            out = torch.empty(x.shape, dtype=x.dtype, device=dev)
-        yr = _rows(out, "out", x.shape, x.dtype, dev)
-        fn = getattr(L, "tg_rope_" + _SUFFIX[x.dtype])
-        _lib.check(fn(rd, xr, yr, tokens, heads, dim, pos, flags, sp), "tg_rope")
+    _lib.check(_call("tg_rope_" + suffix)(rd, xr, yr, tokens, heads, dim, pos, flags, sp), "tg_rope")
     return out
 
 
@@ -247,77 +264,82 @@ def kv_append(cache: PagedKV, table: PageTable, seq_len: torch.Tensor, k: torch.
     seq_len[b] tokens long after them; its new token i is token a = seq_len[b] - n + i of its
     pages, at position positions[t] or position_base + a.  ``check`` checks the index arrays
     first (and synchronises)."""
-    L = _lib.load()
     kv = cache.desc()
-    dev, dt = cache.k.device, cache.k.dtype
-    tb = table.desc(dev, kv.pages)
+    index, dt = cache.k.get_device(), cache.k.dtype
+    tb = table.desc(index, kv.pages)
     if k.dim() != 3:
         raise ValueError("k must be [tokens, heads, dim] (got %s)" % (tuple(k.shape),))
-    tokens = int(k.shape[0])
+    tokens, rows = k.shape[0], tb.rows
     shape = (tokens, kv.heads, kv.dim)
-    a = _lib.TgKvAppendArgs()
-    a.cache, a.pages = ctypes.pointer(kv), ctypes.pointer(tb)
-    a.seq_len = _vector(seq_len, "seq_len", dev, tb.rows)
-    a.tokens = tokens
+    a = _lib.TgKvAppendArgs(ctypes.addressof(kv), ctypes.addressof(tb), _vector(seq_len, "seq_len", index, rows), tokens)
     if q_indptr is not None:
-        a.q_indptr = _vector(q_indptr, "q_indptr", dev, tb.rows + 1)
-    elif tokens != tb.rows:
-        raise ValueError("%d tokens for %d sequences need a q_indptr" % (tokens, tb.rows))
-    a.k, a.v = _rows(k, "k", shape, dt, dev), _rows(v, "v", shape, dt, dev)
+        a.q_indptr = _vector(q_indptr, "q_indptr", index, rows + 1)
+    elif tokens != rows:
+        raise ValueError("%d tokens for %d sequences need a q_indptr" % (tokens, rows))
+    a.k, a.v = _rows(k, "k", shape, dt, index), _rows(v, "v", shape, dt, index)
     if rope is not None:
-        a.rope = ctypes.pointer(rope.desc(dev))
-    a.position_base = int(position_base)
+        rd = rope.desc(index)
+        a.rope = ctypes.addressof(rd)
+    a.position_base = position_base
     if positions is not None:
-        a.positions = _vector(positions, "positions", dev, tokens)
-    a.flags = _lib.TG_FLAG_BOUNDS_CHECK if check else 0
-    ctx, sp = _place(dev, stream)
-    with ctx:
-        if q is not None:
-            if q.dim() != 3:
-                raise ValueError("q must be [tokens, q_heads, dim] (got %s)" % (tuple(q.shape),))
-            qshape = (tokens, int(q.shape[1]), kv.dim)
-            if q_out is None:
-                q_out = torch.empty(qshape, dtype=dt, device=dev)
-            a.q = ctypes.pointer(_rows(q, "q", qshape, dt, dev))
-            a.q_out = ctypes.pointer(_rows(q_out, "q_out", qshape, dt, dev))
-            a.q_heads = qshape[1]
-        elif q_out is not None:
-            raise ValueError("q_out without q")
-        _lib.check(getattr(L, "tg_kv_append_" + _SUFFIX[dt])(a, sp), "tg_kv_append")
+        a.positions = _vector(positions, "positions", index, tokens)
+    if check:
+        a.flags = _lib.TG_FLAG_BOUNDS_CHECK
+    if q is not None:
+        if q.dim() != 3:
+            raise ValueError("q must be [tokens, q_heads, dim] (got %s)" % (tuple(q.shape),))
+        a.q_heads = q.shape[1]
+    elif q_out is not None:
+        raise ValueError("q_out without q")
+    sp = _stream(index, stream)
+    where = _elsewhere(index, stream)
+    if where is not None:
+        with where:
+            return _append_launch(a, q, q_out, (tokens, a.q_heads, kv.dim), dt, index, sp)
+    return _append_launch(a, q, q_out, (tokens, a.q_heads, kv.dim), dt, index, sp)
+
+
+def _append_launch(a, q, q_out, qshape, dt, index, sp) -> Optional[torch.Tensor]:
+    if q is not None:
+        qr = _rows(q, "q", qshape, dt, index)
+        if q_out is None:
+            q_out = _like(q)
+        qo = _rows(q_out, "q_out", qshape, dt, index)
+        a.q, a.q_out = ctypes.addressof(qr), ctypes.addressof(qo)
+    _lib.check(_call("tg_kv_append_" + _SUFFIX[dt])(a, sp), "tg_kv_append")
     return q_out
 
 
 def _attention_args(q, cache, table, seq_len, prefix_pages, prefix_len, q_indptr, max_q_len, max_seq_len, scale,
                     causal, check):
+    """(arguments for the library, the descriptors that they point to)."""
     kv = cache.desc()
-    dev, dt = cache.k.device, cache.k.dtype
-    if dt == torch.float32:
+    index, dt = cache.k.get_device(), cache.k.dtype
+    if dt is torch.float32:
         raise ValueError("attention takes float16 or bfloat16 caches (got %s)" % dt)
-    tb = table.desc(dev, kv.pages)
+    tb = table.desc(index, kv.pages)
     if q.dim() != 3:
         raise ValueError("q must be [tokens, q_heads, dim] (got %s)" % (tuple(q.shape),))
-    tokens, heads = int(q.shape[0]), int(q.shape[1])
-    a = _lib.TgPrefixAttentionArgs()
-    a.cache, a.pages = ctypes.pointer(kv), ctypes.pointer(tb)
-    a.seq_len = _vector(seq_len, "seq_len", dev, tb.rows)
-    slots = tb.nnz * kv.page_size
-    a.max_seq_len = slots if max_seq_len is None else int(max_seq_len)
+    tokens, heads, _ = q.shape
+    rows = tb.rows
+    a = _lib.TgPrefixAttentionArgs(ctypes.addressof(kv), ctypes.addressof(tb), _vector(seq_len, "seq_len", index, rows),
+                                   tb.nnz * kv.page_size if max_seq_len is None else max_seq_len)
     if prefix_pages is not None:
-        a.prefix_pages, a.n_prefix_pages = _vector(prefix_pages, "prefix_pages", dev), prefix_pages.numel()
-    a.prefix_len = int(prefix_len)
+        a.prefix_pages, a.n_prefix_pages = _vector(prefix_pages, "prefix_pages", index), prefix_pages.shape[0]
+    a.prefix_len = prefix_len
     a.tokens = tokens
     if q_indptr is not None:
-        a.q_indptr = _vector(q_indptr, "q_indptr", dev, tb.rows + 1)
-        a.max_q_len = tokens if max_q_len is None else int(max_q_len)
+        a.q_indptr = _vector(q_indptr, "q_indptr", index, rows + 1)
+        a.max_q_len = tokens if max_q_len is None else max_q_len
     else:
-        if tokens != tb.rows:
-            raise ValueError("%d tokens for %d sequences need a q_indptr" % (tokens, tb.rows))
+        if tokens != rows:
+            raise ValueError("%d tokens for %d sequences need a q_indptr" % (tokens, rows))
         a.max_q_len = 1
     a.q_heads = heads
-    a.q = _rows(q, "q", (tokens, heads, kv.dim), dt, dev)
-    a.scale = kv.dim ** -0.5 if scale is None else float(scale)
+    a.q = _rows(q, "q", (tokens, heads, kv.dim), dt, index)
+    a.scale = kv.dim ** -0.5 if scale is None else scale
     a.flags = (_lib.TG_FLAG_CAUSAL if causal else 0) | (_lib.TG_FLAG_BOUNDS_CHECK if check else 0)
-    return a
+    return a, (kv, tb)
 
 
 def prefix_attention_workspace_bytes(q: torch.Tensor, cache: PagedKV, table: PageTable, seq_len: torch.Tensor,
@@ -325,9 +347,9 @@ def prefix_attention_workspace_bytes(q: torch.Tensor, cache: PagedKV, table: Pag
                                      q_indptr: Optional[torch.Tensor] = None, max_q_len: Optional[int] = None,
                                      max_seq_len: Optional[int] = None) -> int:
     """Bytes of workspace that prefix_attention needs with these arguments."""
-    a = _attention_args(q, cache, table, seq_len, prefix_pages, prefix_len, q_indptr, max_q_len, max_seq_len, None,
-                        True, False)
-    return int(_lib.load().tg_prefix_attention_workspace_bytes(a))
+    a, _held = _attention_args(q, cache, table, seq_len, prefix_pages, prefix_len, q_indptr, max_q_len, max_seq_len,
+                               None, True, False)
+    return int(_call("tg_prefix_attention_workspace_bytes")(a))
 
 
 def prefix_attention(q: torch.Tensor, cache: PagedKV, table: PageTable, seq_len: torch.Tensor,
@@ -349,28 +371,37 @@ def prefix_attention(q: torch.Tensor, cache: PagedKV, table: PageTable, seq_len:
     (out, log of the softmax's sum).  ``workspace`` (prefix_attention_workspace_bytes) is
     allocated on the call's stream where it is not given; ``check`` checks the index arrays
     first (and synchronises)."""
-    L = _lib.load()
-    a = _attention_args(q, cache, table, seq_len, prefix_pages, prefix_len, q_indptr, max_q_len, max_seq_len, scale,
-                        causal, check)
-    dev, dt = q.device, q.dtype
-    ctx, sp = _place(dev, stream)
-    with ctx:
-        if out is None:
-            out = torch.empty(q.shape, dtype=dt, device=dev)
-        a.out = _rows(out, "out", q.shape, dt, dev)
-        if lse is True:
-            lse = torch.empty(q.shape[:2], dtype=torch.float32, device=dev)
-        if isinstance(lse, torch.Tensor):
-            if lse.shape != q.shape[:2] or lse.dtype != torch.float32 or lse.device != dev or not lse.is_contiguous():
-                raise ValueError("lse must be a contiguous float32 tensor of shape %s on %s" % (tuple(q.shape[:2]), dev))
-            a.lse = lse.data_ptr()
-        nbytes = L.tg_prefix_attention_workspace_bytes(a)
-        if workspace is None and nbytes:
-            workspace = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-        wp, wn = (0, 0) if workspace is None else (workspace.data_ptr(), workspace.numel() * workspace.element_size())
-        if workspace is not None and workspace.device != dev:
-            raise ValueError("the workspace must be on %s (got %s)" % (dev, workspace.device))
-        if wn < nbytes:
-            raise ValueError("workspace too small: need %d bytes" % nbytes)
-        _lib.check(getattr(L, "tg_prefix_attention_" + _SUFFIX[dt])(a, wp, wn, sp), "tg_prefix_attention")
+    a, _held = _attention_args(q, cache, table, seq_len, prefix_pages, prefix_len, q_indptr, max_q_len, max_seq_len,
+                               scale, causal, check)
+    index = q.get_device()
+    sp = _stream(index, stream)
+    where = _elsewhere(index, stream)
+    if where is not None:
+        with where:
+            return _attention_launch(a, q, out, lse, workspace, index, sp)
+    return _attention_launch(a, q, out, lse, workspace, index, sp)
+
+
+def _attention_launch(a, q, out, lse, workspace, index, sp):
+    if out is None:
+        out = _like(q)
+    a.out = _rows(out, "out", q.shape, q.dtype, index)
+    if lse is True:
+        lse = torch.empty(q.shape[:2], dtype=torch.float32, device=q.device)
+    if isinstance(lse, torch.Tensor):
+        if lse.shape != q.shape[:2] or lse.dtype != torch.float32 or lse.get_device() != index or not lse.is_contiguous():
+            raise ValueError("lse must be a contiguous float32 tensor of shape %s on cuda:%d" % (tuple(q.shape[:2]), index))
+        a.lse = lse.data_ptr()
+    need = _call("tg_prefix_attention_workspace_bytes")(a)
+    ws = size = 0
+    if workspace is None and need:
+        workspace, size = torch.empty(need, dtype=torch.uint8, device=q.device), need
+        ws = workspace.data_ptr()
+    elif workspace is not None:
+        if workspace.get_device() != index:
+            raise ValueError("the workspace must be on cuda:%d (got %s)" % (index, workspace.device))
+        ws, size = workspace.data_ptr(), workspace.numel() * workspace.element_size()
+        if size < need:
+            raise ValueError("workspace too small: need %d bytes" % need)
+    _lib.check(_call("tg_prefix_attention_" + _SUFFIX[q.dtype])(a, ws, size, sp), "tg_prefix_attention")
     return (out, lse) if isinstance(lse, torch.Tensor) else out
