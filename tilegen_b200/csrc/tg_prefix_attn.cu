@@ -405,7 +405,7 @@ __global__ void __launch_bounds__(128) attn_join_kernel(const AttnParams p) {
     const int t = (int)(row / p.q_heads), qh = (int)(row % p.q_heads);
     int np = p.prefix_splits, n;  // parts over the prefix, and all
     if (p.prefix_ctas > 0) {
-        const int64_t u = (int64_t)(qh / p.group) * p.prefix_tiles + (t * p.group + qh % p.group) / 256;
+        const int u = qh / p.group * p.prefix_tiles + (t * p.group + qh % p.group) / 256;
         np = prefix_cta(p, (u + 1) * p.prefix_steps - 1) - prefix_cta(p, u * p.prefix_steps) + 1;
     }
     n = np;
@@ -512,7 +512,7 @@ struct Plan {
 void share_prefix(AttnParams& p, int64_t rows, int dim, double own_bytes) {
     const int64_t units = (int64_t)p.prefix_tiles * p.kv_heads;
     p.prefix_steps = (int)ceil_div(p.prefix_len, 128);
-    p.prefix_work = units * p.prefix_steps;
+    p.prefix_work = (int)(units * p.prefix_steps);
     const double step = rows > 128 ? 1.9 : 1.3;
     double best = 1e30;
     int ctas = 1;
@@ -527,7 +527,7 @@ void share_prefix(AttnParams& p, int64_t rows, int dim, double own_bytes) {
     }
     p.prefix_ctas = ctas;
     p.prefix_splits = 1;
-    for (int64_t u = 0; u < units; ++u)
+    for (int u = 0; u < (int)units; ++u)
         p.prefix_splits = std::max(p.prefix_splits, prefix_cta(p, (u + 1) * p.prefix_steps - 1) - prefix_cta(p, u * p.prefix_steps) + 1);
 }
 
@@ -596,6 +596,8 @@ int make_plan(const tg_prefix_attention_args* a, Plan* plan, const char* op) {
             p.prefix_chunk = (int)std::max<int64_t>(128, ceil_div(ceil_div(p.prefix_len, n), 16) * 16);
             p.prefix_splits = (int)ceil_div(p.prefix_len, p.prefix_chunk);
         } else {
+            if (tiles_all * c.heads > INT32_MAX / ceil_div(p.prefix_len, 128))
+                return set_error(TG_EUNSUPPORTED, "%s: too many rows for one launch", op);
             share_prefix(p, rows_all, c.dim, (double)t.nnz * c.page_size * c.heads * c.dim * 4);
         }
     }

@@ -31,8 +31,7 @@ struct AttnParams {
     int prefix_splits, prefix_chunk;  // most parts of a row over the prefix; keys of a split
     // the tcgen05 kernel over the prefix: its CTAs share prefix_work steps of 128 keys evenly,
     // prefix_steps for each (head, row tile) in turn, prefix_tiles row tiles
-    int64_t prefix_work;
-    int prefix_ctas, prefix_steps, prefix_tiles;  // prefix_ctas 0: splits of prefix_chunk keys
+    int prefix_work, prefix_ctas, prefix_steps, prefix_tiles;  // prefix_ctas 0: splits of prefix_chunk keys
     int own_chunks, own_chunk;        // most chunks of a sequence, keys of a chunk
     int tiles;                        // row tiles of a sequence (own) or of all rows (prefix)
     int over_prefix;                  // the tcgen05 kernel: the prefix, else the sequences' own pages
@@ -66,9 +65,15 @@ __device__ __forceinline__ int keys_seen(const AttnParams& p, const Sequence& s,
     return (int)min(max(total - s.n + i + 1, (int64_t)0), (int64_t)whole);
 }
 
-// The CTA that has step x of the prefix.
-__host__ __device__ __forceinline__ int prefix_cta(const AttnParams& p, int64_t x) {
-    return (int)(((x + 1) * p.prefix_ctas - 1) / p.prefix_work);
+// The first step of a CTA's share of the prefix (the first prefix_work % prefix_ctas have one more),
+// and the CTA that has step x.
+__host__ __device__ __forceinline__ int prefix_start(const AttnParams& p, int cta) {
+    const int q = p.prefix_work / p.prefix_ctas, more = p.prefix_work - q * p.prefix_ctas;
+    return cta * q + (cta < more ? cta : more);
+}
+__host__ __device__ __forceinline__ int prefix_cta(const AttnParams& p, int x) {
+    const int q = p.prefix_work / p.prefix_ctas, more = p.prefix_work - q * p.prefix_ctas;
+    return x < more * (q + 1) ? x / (q + 1) : more + (x - more * (q + 1)) / q;
 }
 
 // Page and slot of token `at` of a page list; page -1 where the list names no page of the cache.

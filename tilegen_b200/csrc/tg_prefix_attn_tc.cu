@@ -12,6 +12,7 @@
 //   warps 8, 10       fetch K, V tiles into a ring of shared memory by TMA, in boxes of as many
 //                     rows as divide both a page and a tile
 //   warp 9            issues the matrix instructions
+//   warp 11           how many keys each row sees
 //
 // O is rescaled only where a row's maximum has grown by more than 2^8 since the value that P is
 // taken relative to: P stays below 2^8, far inside the range of either type and of the 32-bit
@@ -156,13 +157,14 @@ struct TcCfg {
     static constexpr int kBlock = kTile * D * 2;  // bytes of a tile of Q, K or V
     static constexpr int kHalf = kTile * 128;     // of 64 of its columns
     static constexpr int kStages = D == 128 ? 5 : 8;
-    static constexpr int kSmem = (2 + kStages) * kBlock + 2048;
+    static constexpr int kSmem = (2 + kStages) * kBlock + 2048;  // and a TcShared
 };
 
 struct TcShared {
-    uint64_t q_full[2], full[8], empty[8], s_full[2], p_half[2], p_full[2], o_done[2], tail, drained;
+    uint64_t q_full[2], full[8], empty[8], s_full[2], p_half[2], p_full[2], o_done[2], seen_full, seen_free, tail, drained;
     uint32_t tmem;
     int fail;  // a wait ran out
+    int seen[2 * kTile];
 };
 
 // Bounded wait; false once one has run out in this CTA (2 s; every wait here is microseconds).
@@ -186,22 +188,29 @@ __device__ __forceinline__ void mbar_wait_brief(uint64_t* bar, uint32_t parity) 
     }
 }
 
-// One row the long way, a warp: only for a row that does not see a value that is not finite
-// while others of its tile do.  acc: D / 32 elements a lane.
+// Up to 256 rows over a range of keys, as all warps of a CTA see it.
+struct Segment {
+    Sequence s;
+    const int64_t* list;
+    int h, part, row0, nrows, k0, k1, keys, steps, ntiles;
+};
+
+// Row r of the segment, which sees the keys up to n, the long way, by a warp: only for a row that
+// does not see a value that is not finite while others of its tile do.  (Inlined: a call would put
+// the parameters on the stack of every thread.)
 template <typename T, int D>
-__device__ __noinline__ void row_alone(const AttnParams& p, const int64_t* list, const T* q, const char* kbase,
-                                       const char* vbase, int k0, int k1, float* acc, float& m, float& l) {
-    constexpr int E = D / 32;
-    const int lane = threadIdx.x & 31;
-    m = -INFINITY, l = 0.f;
-    float x[E];
+__device__ __forceinline__ void row_alone(const AttnParams& p, const Segment& g, int r, int n) {
+    constexpr int E = D / 32;  // elements of a lane
+    const int lane = threadIdx.x & 31, f = g.row0 + r, t = g.s.first + f / p.group, qh = g.h * p.group + f % p.group;
+    const T* q = static_cast<const T*>(p.q) + t * p.q_tok + qh * p.q_head;
+    float x[E], acc[E], m = -INFINITY, l = 0.f;
 #pragma unroll
     for (int e = 0; e < E; ++e) x[e] = to_f32(q[lane * E + e]), acc[e] = 0.f;
-    for (int key = k0; key < k1; ++key) {
+    for (int key = g.k0; key < n; ++key) {
         int page, slot;
-        locate(p, list, key, page, slot);
-        const T* kr = reinterpret_cast<const T*>(kbase) + (int64_t)page * p.k_page + slot * p.k_slot + lane * E;
-        const T* vr = reinterpret_cast<const T*>(vbase) + (int64_t)page * p.v_page + slot * p.v_slot + lane * E;
+        locate(p, g.list, key, page, slot);
+        const T* kr = static_cast<const T*>(p.k) + g.h * p.k_head + page * p.k_page + slot * p.k_slot + lane * E;
+        const T* vr = static_cast<const T*>(p.v) + g.h * p.v_head + page * p.v_page + slot * p.v_slot + lane * E;
         float s = 0.f;
         if (page >= 0)
 #pragma unroll
@@ -216,34 +225,37 @@ __device__ __noinline__ void row_alone(const AttnParams& p, const int64_t* list,
 #pragma unroll
         for (int e = 0; e < E; ++e) acc[e] = acc[e] * keep + (page >= 0 ? w * to_f32(vr[e]) : 0.f);
     }
+    const int64_t at = (int64_t)t * p.q_heads + qh, pat = (int64_t)g.part * p.tokens * p.q_heads + at;
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+        if (p.direct) static_cast<T*>(p.out)[t * p.o_tok + qh * p.o_head + lane * E + e] = from_f32<T>(acc[e] * inv);
+        else p.part_o[pat * D + lane * E + e] = acc[e];
+    }
+    if (lane == 0) {
+        if (!p.direct) p.part_ml[pat] = make_float2(m, l);
+        else if (p.lse) p.lse[at] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.69314718055994531f;
+    }
 }
-
-// Up to 256 rows over a range of keys, as all warps of a CTA see it.
-struct Segment {
-    Sequence s;
-    const int64_t* list;
-    int h, part, row0, nrows, k0, k1, keys, steps, ntiles;
-};
 
 // The CTA's segments, one after the other.  Over the prefix a CTA has an even share of all steps
 // of all (head, row tile) pairs, so it ends one pair and begins another where its share does; the
 // parts of a pair are numbered by CTA.  Over own pages it has one segment.
 struct Segments {
-    int64_t at, end;
+    int at, end;
     __device__ __forceinline__ explicit Segments(const AttnParams& p) {
-        at = p.over_prefix ? blockIdx.x * p.prefix_work / p.prefix_ctas : 0;
-        end = p.over_prefix ? (blockIdx.x + 1) * p.prefix_work / p.prefix_ctas : 1;
+        at = p.over_prefix ? prefix_start(p, blockIdx.x) : 0;
+        end = p.over_prefix ? prefix_start(p, blockIdx.x + 1) : 1;
     }
     __device__ __forceinline__ bool next(const AttnParams& p, Segment& g) {
         if (at >= end) return false;
         int tile;
         if (p.over_prefix) {
-            const int64_t u = at / p.prefix_steps;
-            const int first = (int)(at - u * p.prefix_steps);
-            g.steps = (int)min((int64_t)(p.prefix_steps - first), end - at);
+            const int u = at / p.prefix_steps, first = at - u * p.prefix_steps;
+            g.steps = min(p.prefix_steps - first, end - at);
             at += g.steps;
-            g.h = (int)(u / p.tiles);
-            tile = (int)(u - (int64_t)g.h * p.tiles);
+            g.h = u / p.tiles;
+            tile = u - g.h * p.tiles;
             g.part = blockIdx.x - prefix_cta(p, u * p.prefix_steps);
             g.s.first = 0;
             g.s.n = p.tokens;
@@ -283,9 +295,8 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const AttnParams p
                                                               const __grid_constant__ CUtensorMap vmap) {
     using C = TcCfg<D>;
     constexpr int CH = D / 8;  // 16-byte chunks of a row
-    extern __shared__ unsigned char smem_raw[];
-    __shared__ TcShared sh;
-    unsigned char* smem = smem_raw + ((1024 - (smem_addr(smem_raw) & 1023)) & 1023);
+    extern __shared__ __align__(1024) unsigned char smem[];
+    TcShared& sh = *reinterpret_cast<TcShared*>(smem + (2 + C::kStages) * C::kBlock);
     const int tid = threadIdx.x, warp = __shfl_sync(kFull, tid >> 5, 0), lane = tid & 31;
     pdl_trigger();
     if (!p.over_prefix) {
@@ -317,6 +328,8 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const AttnParams p
                 mbar_init(&sh.p_full[i], kTile);
                 mbar_init(&sh.o_done[i], 1);
             }
+            mbar_init(&sh.seen_full, 32);
+            mbar_init(&sh.seen_free, 2 * kTile);
             mbar_init(&sh.tail, 1);
             mbar_init(&sh.drained, 1);
             sh.fail = 0;
@@ -451,64 +464,98 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const AttnParams p
         if (*fail)  // leave no copy under way
             for (int f = max(0, f0 - C::kStages); f < f0 + C::kStages; ++f)
                 if ((f & 1) == is_v) mbar_wait_brief(&sh.full[f % C::kStages], f / C::kStages & 1);
-    } else if (warp < 8) {
+    } else if (warp == 11) {
+        // Keys that each row sees, up to the segment's end: eight rows a lane, the searches of four
+        // side by side.
+        int turn = 0;
+        bool ok = true;
+        while (ok && segments.next(p, g)) {
+            if (g.steps == 0) continue;
+            if (turn > 0) ok = __all_sync(kFull, wait(smem_addr(&sh.seen_free), (turn - 1) & 1, fail));
+#pragma unroll 1
+            for (int r0 = lane; r0 < 2 * kTile; r0 += 4 * 32) {
+                int seen[4];
+                if (p.over_prefix && p.causal) {
+                    int t[4], lo[4];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const int r = r0 + i * 32;
+                        t[i] = (g.row0 + (r < g.nrows ? r : 0)) / p.group;
+                        lo[i] = p.q_indptr ? 0 : t[i];
+                    }
+                    if (p.q_indptr) {  // the last lo with q_indptr[lo] <= t
+                        for (int step = 1 << (31 - __clz(p.rows)); step > 0; step >>= 1)
+#pragma unroll
+                            for (int i = 0; i < 4; ++i)
+                                if (lo[i] + step < p.rows && p.q_indptr[lo[i] + step] <= t[i]) lo[i] += step;
+                    }
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const Sequence o = sequence(p, lo[i]);
+                        seen[i] = keys_seen(p, o, t[i] - o.first, (int64_t)g.keys + o.len, g.keys);
+                    }
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        seen[i] = p.over_prefix ? g.keys : keys_seen(p, g.s, (g.row0 + r0 + i * 32) / p.group, g.keys, g.keys);
+                }
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int r = r0 + i * 32;
+                    sh.seen[r] = r < g.nrows ? max(min(seen[i], g.k1), 0) : 0;
+                }
+            }
+            arrive(smem_addr(&sh.seen_full));
+            ++turn;
+        }
+    } else {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
-        const int my = warp >> 2, row = tid;  // the warp's tile, the thread's row of the CTA
-        int done = 0;                         // steps of the tile so far
+        const int my = warp >> 2, quarter = warp & 3, row = tid;  // tile, 32 rows of it, row of the CTA
+        const uint32_t lanes = (uint32_t)quarter << 21;           // the warp's TMEM lanes, in bits 16-31
+        const uint32_t ts = tmem + my * kTile + lanes, to = tmem + kColO + my * kTile + lanes;
+        int done = 0, turn = 0;  // steps of the tile so far, segments
         while (segments.next(p, g)) {
-            if (my >= g.ntiles) continue;
-            const Sequence& s = g.s;
-            const int h = g.h, row0 = g.row0, nrows = g.nrows, steps = g.steps, k0 = g.k0, k1 = g.k1, keys = g.keys;
-            const int part = g.part;
-            const int64_t* list = g.list;
-            const char* kbase = static_cast<const char*>(p.k) + h * p.k_head * 2;
-            const char* vbase = static_cast<const char*>(p.v) + h * p.v_head * 2;
-            // ---- queries, swizzled, zeros where there is no row; all loads are under way at once
+            if (my >= g.ntiles) {
+                if (g.steps > 0) {
+                    wait(smem_addr(&sh.seen_full), turn++ & 1, fail);
+                    arrive(smem_addr(&sh.seen_free));
+                }
+                continue;
+            }
+            const int h = g.h, row0 = g.row0, nrows = g.nrows, steps = g.steps, k0 = g.k0, k1 = g.k1, first = g.s.first;
+            int seen = 0;
+            bool ok = true;
             if (steps > 0) {
+                // ---- queries, swizzled, zeros where there is no row; all loads are under way at once
                 constexpr int kStep = kTile / CH;  // rows between a thread's chunks
                 const int rt = tid & (kTile - 1), c = rt % CH, f0 = my * kTile + rt / CH;
                 const int dt = kStep / p.group, dg = kStep % p.group;
-                int t = (row0 + f0) / p.group, g = (row0 + f0) % p.group;
-                const char* q = static_cast<const char*>(p.q) + (s.first * p.q_tok + (int64_t)h * p.group * p.q_head) * 2 + c * 16;
+                int t = (row0 + f0) / p.group, x = (row0 + f0) % p.group;
+                const char* q = static_cast<const char*>(p.q) + (first * p.q_tok + (int64_t)h * p.group * p.q_head) * 2 + c * 16;
                 uint4 v[CH];
 #pragma unroll
                 for (int i = 0; i < CH; ++i) {
                     const bool there = f0 + i * kStep < nrows;
-                    v[i] = __ldg(reinterpret_cast<const uint4*>(q + (there ? (t * p.q_tok + g * p.q_head) * 2 : 0)));
+                    v[i] = __ldg(reinterpret_cast<const uint4*>(q + (there ? (t * p.q_tok + x * p.q_head) * 2 : 0)));
                     t += dt;
-                    g += dg;
-                    if (g >= p.group) g -= p.group, ++t;
+                    x += dg;
+                    if (x >= p.group) x -= p.group, ++t;
                 }
 #pragma unroll
-                for (int i = 0; i < CH; ++i)
-                    if (f0 + i * kStep >= nrows) v[i] = make_uint4(0, 0, 0, 0);
-#pragma unroll
                 for (int i = 0; i < CH; ++i) {
-                    const int r = rt / CH + i * (kTile / CH);
+                    const int r = rt / CH + i * kStep;
+                    if (f0 + i * kStep >= nrows) v[i] = make_uint4(0, 0, 0, 0);
                     *reinterpret_cast<uint4*>(smem + my * C::kBlock + (c >> 3) * C::kHalf + r * 128 + (((c ^ r) & 7) << 4)) = v[i];
                 }
                 fence_async();
                 arrive(b_q + my * 8);
+                ok = wait(smem_addr(&sh.seen_full), turn++ & 1, fail);
+                seen = sh.seen[row];
+                arrive(smem_addr(&sh.seen_free));
             }
-            int seen = 0;  // keys that the thread's row sees, up to k1
-            if (row < nrows) {
-                const int i = (row0 + row) / p.group;
-                if (!p.over_prefix) {
-                    seen = keys_seen(p, s, i, keys, keys);
-                } else if (!p.causal) {
-                    seen = keys;
-                } else {
-                    const Sequence o = sequence(p, sequence_of(p.q_indptr, p.rows, i));
-                    seen = keys_seen(p, o, i - o.first, (int64_t)keys + o.len, keys);
-                }
-                seen = max(min(seen, k1), 0);
-            }
-            const uint32_t lanes = (uint32_t)(warp & 3) << 21;  // the warp's 32 TMEM lanes, in bits 16-31
-            const uint32_t ts = tmem + my * kTile + lanes, to = tmem + kColO + my * kTile + lanes;
-            const bool rows_here = (warp & 3) * 32 + my * kTile < nrows;  // the warp has a row
-            float m = -INFINITY, l = 0.f;  // P is taken relative to m
-            bool ok = true;
-            for (int j = 0; j < steps; ++j) {
+            const bool rows_here = quarter * 32 + my * kTile < nrows;  // the warp has a row
+            float m = -INFINITY, l = 0.f;                              // P is taken relative to m
+            for (int j = 0; ok && j < steps; ++j) {
                 if (!(ok = wait(b_s + my * 8, (done + j) & 1, fail))) break;
                 fence_after();
                 if (rows_here) {
@@ -598,14 +645,14 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const AttnParams p
             fence_after();
             // ---- the rows' results
             if (!ok) l = NAN;  // loud: a wait that ran out leaves no number
-            const int f = row0 + row, t = s.first + f / p.group, qh = h * p.group + f % p.group;
-            const int64_t at = (int64_t)t * p.q_heads + qh, pat = (int64_t)part * p.tokens * p.q_heads + at;
+            const int f = row0 + row, t = first + f / p.group, qh = h * p.group + f % p.group;
+            const int64_t at = (int64_t)t * p.q_heads + qh, pat = (int64_t)g.part * p.tokens * p.q_heads + at;
             const float inv = l == 0.f ? 0.f : 1.f / l;
             float odd = 0.f;  // NaN once an element of the row's sum is not finite
             if (rows_here) {
                 // The tile's queries are done with: a warp turns its 32 rows round in their place, so
                 // that stores run along the rows.  A pass: D 16-bit results or D / 2 32-bit sums.
-                unsigned char* area = smem + my * C::kBlock + (warp & 3) * (C::kBlock / 4);
+                unsigned char* area = smem + my * C::kBlock + quarter * (C::kBlock / 4);
                 char* to_row = p.direct ? static_cast<char*>(p.out) + (t * p.o_tok + qh * p.o_head) * 2
                                         : reinterpret_cast<char*>(p.part_o + pat * D);
                 if (row >= nrows || (!p.direct && l == 0.f)) to_row = nullptr;
@@ -614,31 +661,36 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const AttnParams p
                 for (int pass = 0; pass < passes; ++pass) {
                     const int cols = D / passes;
 #pragma unroll 1
-                    for (int c = 0; c < cols; c += 16) {
-                        uint32_t y[16];
+                    for (int c = 0; c < cols; c += 32) {
+                        uint32_t y[32];
                         if (steps > 0) {
-                            tmem_ld16(to + pass * cols + c, y);
+                            tmem_ld32(to + pass * cols + c, y);
                             wait_ld();
                         }
+                        float o0 = 0.f, o1 = 0.f;
 #pragma unroll
-                        for (int e = 0; e < 16; ++e) {
-                            odd += __uint_as_float(y[e]) * 0.f;
-                            if (l == 0.f) y[e] = 0;
+                        for (int e = 0; e < 32; e += 2) {
+                            o0 = fmaf(__uint_as_float(y[e]), 0.f, o0);
+                            o1 = fmaf(__uint_as_float(y[e + 1]), 0.f, o1);
                         }
+                        odd += o0 + o1;
+#pragma unroll
+                        for (int e = 0; e < 32; ++e)
+                            if (l == 0.f) y[e] = 0;
                         if (p.direct) {
 #pragma unroll
-                            for (int e = 0; e < 8; ++e)
+                            for (int e = 0; e < 16; ++e)
                                 y[e] = pack2<T>(__uint_as_float(y[2 * e]) * inv, __uint_as_float(y[2 * e + 1]) * inv);
                         }
 #pragma unroll
-                        for (int e = 0; e < 4; ++e)
-                            if (e < 2 || !p.direct)
+                        for (int e = 0; e < 8; ++e)
+                            if (e < 4 || !p.direct)
                                 *reinterpret_cast<uint4*>(area + lane * D * 2 +
                                                           ((((p.direct ? c / 8 : c / 4) + e) ^ lane) & (CH - 1)) * 16) =
                                     make_uint4(y[4 * e], y[4 * e + 1], y[4 * e + 2], y[4 * e + 3]);
                     }
                     __syncwarp();
-#pragma unroll 4
+#pragma unroll
                     for (int i = 0; i < CH; ++i) {
                         const int r = (i * 32 + lane) / CH, c = lane % CH;
                         char* dst = reinterpret_cast<char*>(__shfl_sync(kFull, reinterpret_cast<unsigned long long>(to_row), r));
@@ -647,41 +699,24 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const AttnParams p
                     }
                     __syncwarp();
                 }
-                if (row < nrows) {
-                    if (!p.direct) p.part_ml[pat] = make_float2(m, l);
-                    else if (p.lse) p.lse[at] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.69314718055994531f;
-                }
                 // A value that a row does not see, of a tile that it sees in part, reaches it as 0
                 // times the value: where that is NaN, the row is done again alone.
                 const bool again = row < nrows && seen < k1 && steps > 0 && odd != odd;
+                if (row < nrows && !again) {
+                    if (!p.direct) p.part_ml[pat] = make_float2(m, l);
+                    else if (p.lse) p.lse[at] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.69314718055994531f;
+                }
                 if (__any_sync(kFull, again)) {
                     for (int i = 0; i < 32; ++i) {
                         const int r = __shfl_sync(kFull, row, i), n = __shfl_sync(kFull, seen, i);
-                        if (!__shfl_sync(kFull, again, i)) continue;
-                        const int g = row0 + r, tt = s.first + g / p.group, hh = h * p.group + g % p.group;
-                        float acc[D / 32], rm, rl;
-                        row_alone<T, D>(p, list, static_cast<const T*>(p.q) + tt * p.q_tok + hh * p.q_head, kbase, vbase,
-                                        k0, n, acc, rm, rl);
-                        const int64_t ra = (int64_t)tt * p.q_heads + hh, rp = (int64_t)part * p.tokens * p.q_heads + ra;
-                        const float ri = rl == 0.f ? 0.f : 1.f / rl;
-#pragma unroll
-                        for (int e = 0; e < D / 32; ++e) {
-                            if (p.direct)
-                                static_cast<T*>(p.out)[tt * p.o_tok + hh * p.o_head + lane * (D / 32) + e] = from_f32<T>(acc[e] * ri);
-                            else
-                                p.part_o[rp * D + lane * (D / 32) + e] = acc[e];
-                        }
-                        if (lane == 0) {
-                            if (!p.direct) p.part_ml[rp] = make_float2(rm, rl);
-                            else if (p.lse) p.lse[ra] = rl == 0.f ? -INFINITY : (rm + log2f(rl)) * 0.69314718055994531f;
-                        }
+                        if (__shfl_sync(kFull, again, i)) row_alone<T, D>(p, g, r, n);
                     }
                 }
             }
             fence_before();
             done += steps;
             // the tile's memory and TMEM may be written again
-            asm volatile("bar.sync %0, 128;" ::"r"(my + 1) : "memory");
+            asm volatile("bar.sync %0, 128;" ::"r"(1 + my) : "memory");
         }
     }
     __syncwarp();
@@ -698,7 +733,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const AttnParams p
 template <typename T, int D>
 int tc_launch(const AttnParams& p, int64_t units, bool pdl, cudaStream_t st) {
     using C = TcCfg<D>;
-    static_assert(C::kSmem + sizeof(TcShared) <= 227 * 1024, "shared memory of a CTA");
+    static_assert(C::kSmem <= 227 * 1024 && sizeof(TcShared) <= 2048, "shared memory of a CTA");
     const int box = std::gcd(p.page_size, kTile);
     CUtensorMap kmap, vmap;
     int rc = cache_maps(p, std::is_same<T, __half>::value, D, box, &kmap, &vmap);
