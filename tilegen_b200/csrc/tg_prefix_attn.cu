@@ -505,27 +505,32 @@ struct Plan {
 };
 
 // CTAs of the tcgen05 kernel over the prefix, by the time that the whole call would take: a CTA,
-// one on an SM, has an even share of the steps at 1.9 us (1.3 where there is one row tile), 5 us to
-// begin and 5 for each pair of head and row tile that it touches; the SMs that they leave, and
-// their time after them, go to the own parts (own_bytes at 6 TB/s); and each part of a row is
-// written and read once more.
+// one on an SM, has its steps at 1.75 us (1.2 where there is one row tile), 10 us to begin and end
+// (18 where the own parts keep the memory busy) and 8 for each pair of head and row tile that it
+// goes on to; the SMs that they leave, and their time after them, go to the own parts (own_bytes at
+// 6 TB/s, 12 us at least); and each part of a row is written and read once more.  As many CTAs for
+// each pair, or fewer than pairs and even shares.  It finds the best of a sweep of 64 sequences of
+// 540 keys behind 8192 (56 CTAs: 56 us; 32: 69, 128: 75), of 256 behind 32768 (128: 172; 64: 243,
+// 144: 180) and of 48 of 5 tokens and 320 keys behind 5003 (96: 49; 64: 58, 128: 59).
 void share_prefix(AttnParams& p, int64_t rows, int dim, double own_bytes) {
     const int64_t units = (int64_t)p.prefix_tiles * p.kv_heads;
     p.prefix_steps = (int)ceil_div(p.prefix_len, 128);
     p.prefix_work = (int)(units * p.prefix_steps);
-    const double step = rows > 128 ? 1.9 : 1.3;
+    const double step = rows > 128 ? 1.75 : 1.2, begin = own_bytes > 0 ? 18.0 : 10.0;
+    const double own = own_bytes > 0 ? std::max(own_bytes / 6e6, 12.0) : 0.0;
     double best = 1e30;
-    int ctas = 1;
+    int64_t ctas = 1;
     for (int64_t n = 1; n <= std::min<int64_t>(kSMs, p.prefix_work); ++n) {
-        // an even share that does not end where a pair does is in one more pair
-        const bool even = n >= units ? n % units == 0 : units % n == 0;
-        const double cta = 5.0 + step * (double)ceil_div(p.prefix_work, n) + 5.0 * (double)(ceil_div(units, n) + !even);
-        const double all = own_bytes / 6e6 + cta * (double)n / kSMs;
-        const double parts = 1.0 + (double)n / (double)units;
+        if (n > units && (n % units || n / units > p.prefix_steps)) continue;
+        const double more = n >= units ? 0.0 : (double)(ceil_div(units, n) - (units % n == 0));
+        const double cta = begin + step * (double)ceil_div(p.prefix_work, n) + 8.0 * more;
+        const double all = own + cta * (double)n / kSMs;
+        const double parts = n >= units ? (double)(n / units) : 1.0 + (double)n / (double)units;
         const double t = std::max(cta, all) + parts * (double)rows * p.kv_heads * dim * 8 / 6e6;
-        if (t < best * 0.999) best = t, ctas = (int)n;
+        if (t < best * 0.999) best = t, ctas = n;
     }
-    p.prefix_ctas = ctas;
+    p.prefix_ctas = (int)ctas;
+    p.prefix_per_unit = ctas % units == 0 ? (int)(ctas / units) : 0;
     p.prefix_splits = 1;
     for (int u = 0; u < (int)units; ++u)
         p.prefix_splits = std::max(p.prefix_splits, prefix_cta(p, (u + 1) * p.prefix_steps - 1) - prefix_cta(p, u * p.prefix_steps) + 1);

@@ -31,7 +31,7 @@ struct AttnParams {
     int prefix_splits, prefix_chunk;  // most parts of a row over the prefix; keys of a split
     // the tcgen05 kernel over the prefix: its CTAs share prefix_work steps of 128 keys evenly,
     // prefix_steps for each (head, row tile) in turn, prefix_tiles row tiles
-    int prefix_work, prefix_ctas, prefix_steps, prefix_tiles;  // prefix_ctas 0: splits of prefix_chunk keys
+    int prefix_work, prefix_per_unit, prefix_ctas, prefix_steps, prefix_tiles;  // prefix_ctas 0: splits of prefix_chunk keys
     int own_chunks, own_chunk;        // most chunks of a sequence, keys of a chunk
     int tiles;                        // row tiles of a sequence (own) or of all rows (prefix)
     int over_prefix;                  // the tcgen05 kernel: the prefix, else the sequences' own pages
@@ -65,15 +65,27 @@ __device__ __forceinline__ int keys_seen(const AttnParams& p, const Sequence& s,
     return (int)min(max(total - s.n + i + 1, (int64_t)0), (int64_t)whole);
 }
 
-// The first step of a CTA's share of the prefix (the first prefix_work % prefix_ctas have one more),
-// and the CTA that has step x.
+// The first step of part i of n near-even shares of `all` steps (the first all % n have one more),
+// and the share that has step x.
+__host__ __device__ __forceinline__ int share_start(int all, int n, int i) {
+    const int q = all / n, more = all - q * n;
+    return i * q + (i < more ? i : more);
+}
+__host__ __device__ __forceinline__ int share_of(int all, int n, int x) {
+    const int q = all / n, more = all - q * n;
+    return x < more * (q + 1) ? x / (q + 1) : more + (x - more * (q + 1)) / q;
+}
+// The same for the CTAs over the prefix: prefix_per_unit of them for each (head, row tile), or even
+// shares of all steps where that is 0.
 __host__ __device__ __forceinline__ int prefix_start(const AttnParams& p, int cta) {
-    const int q = p.prefix_work / p.prefix_ctas, more = p.prefix_work - q * p.prefix_ctas;
-    return cta * q + (cta < more ? cta : more);
+    if (!p.prefix_per_unit) return share_start(p.prefix_work, p.prefix_ctas, cta);
+    const int u = cta / p.prefix_per_unit;
+    return u * p.prefix_steps + share_start(p.prefix_steps, p.prefix_per_unit, cta - u * p.prefix_per_unit);
 }
 __host__ __device__ __forceinline__ int prefix_cta(const AttnParams& p, int x) {
-    const int q = p.prefix_work / p.prefix_ctas, more = p.prefix_work - q * p.prefix_ctas;
-    return x < more * (q + 1) ? x / (q + 1) : more + (x - more * (q + 1)) / q;
+    if (!p.prefix_per_unit) return share_of(p.prefix_work, p.prefix_ctas, x);
+    const int u = x / p.prefix_steps;
+    return u * p.prefix_per_unit + share_of(p.prefix_steps, p.prefix_per_unit, x - u * p.prefix_steps);
 }
 
 // Page and slot of token `at` of a page list; page -1 where the list names no page of the cache.
