@@ -102,16 +102,6 @@ __device__ __forceinline__ void locate(const AttnParams& p, const int64_t* list,
     page = id >= 0 && id < p.pages ? (int)id : -1;
 }
 
-template <typename T>
-__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
-    if constexpr (std::is_same<T, __half>::value) {
-        const __half2 h = __floats2half2_rn(lo, hi);
-        return *reinterpret_cast<const uint32_t*>(&h);
-    } else {
-        const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
-        return *reinterpret_cast<const uint32_t*>(&h);
-    }
-}
 __device__ __forceinline__ float exp2_fast(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));

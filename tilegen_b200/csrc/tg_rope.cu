@@ -37,27 +37,54 @@ struct RopeParams {
     int64_t position_base;
     const int64_t *q_indptr, *seq_len, *indptr, *indices;
     int64_t rows, pages, nnz, page_size;
-    int lanes;  // threads along a row
+    int lanes, chunks, blocks;  // threads along a row, items of a row, rounds of the threads over them
 };
 
 template <typename T, int VEC>
 struct alignas(sizeof(T) * VEC) Pack {
     T v[VEC];
+    __device__ __forceinline__ void get(float (&f)[VEC]) const {
+        if constexpr (VEC > 1 && sizeof(T) == 2) {
+#pragma unroll
+            for (int i = 0; i < VEC; i += 2) {
+                const float2 x = unpack2<T>(reinterpret_cast<const uint32_t*>(v)[i / 2]);
+                f[i] = x.x, f[i + 1] = x.y;
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) f[i] = to_f32(v[i]);
+        }
+    }
+    __device__ __forceinline__ void put(const float (&f)[VEC]) {
+        if constexpr (VEC > 1 && sizeof(T) == 2) {
+#pragma unroll
+            for (int i = 0; i < VEC; i += 2) reinterpret_cast<uint32_t*>(v)[i / 2] = pack2<T>(f[i], f[i + 1]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) v[i] = from_f32<T>(f[i]);
+        }
+    }
 };
 
 constexpr int kRopeThreads = 256;
 constexpr int kRopeTile = 32;         // most tokens of a CTA
 constexpr int kRopeSmem = 32 * 1024;  // most bytes of cosines and sines of a CTA
 
-// VEC elements are moved at once: 16 bytes where rows, strides and the parts of a row are
-// multiples of that, else single elements.
+// VEC elements (a pack) are moved at once: 16 bytes where rows, strides and the parts of a row are
+// multiples of that, else single elements.  A thread's item is two packs of a row: the two halves
+// of its pairs (HALF, or single elements of neighbouring pairs), or two packs of whole pairs or
+// copied elements, a stretch of a row apart so that the threads' packs lie side by side.  The
+// packs of its next item are under way while one is turned, the first while the sines are made.
 template <typename T, int VEC, bool HALF, bool APPEND>
-__global__ void __launch_bounds__(kRopeThreads) rope_kernel(const RopeParams<T> p) {
-    extern __shared__ float2 s_turn[];  // [tile][pairs] scale * (cos, sin)
+__global__ void __launch_bounds__(kRopeThreads, 5) rope_kernel(const RopeParams<T> p) {
+    extern __shared__ float4 s_turn4[];  // scale * (cos, sin) of [tile][pairs], two pairs in one float4
+    float2* const s_turn = reinterpret_cast<float2*>(s_turn4);
     __shared__ double s_pos[kRopeTile];
     __shared__ int64_t s_page[kRopeTile];  // the token's cache page, -1: no such slot
     __shared__ int64_t s_slot[kRopeTile];
     using P = Pack<T, VEC>;
+    constexpr bool kApart = HALF || VEC == 1;  // a pair's elements are in different packs
+    constexpr int kPairs = kApart ? VEC : VEC / 2;  // of an item's pack
     const int tid = threadIdx.x;
     const int64_t t0 = (int64_t)blockIdx.x * p.tile;
     const int tile = (int)min((int64_t)p.tile, p.tokens - t0);
@@ -83,81 +110,138 @@ __global__ void __launch_bounds__(kRopeThreads) rope_kernel(const RopeParams<T> 
         }
     }
     __syncthreads();
-    const int pairs = p.rot / 2;
+
+    const int pairs = p.rot / 2, packs = p.dim / VEC;
+    const int turning = kApart ? pairs / VEC : p.rot / VEC;  // packs (or pairs of packs) that turn
+    const int rows = (p.q_rows + (APPEND ? 2 * p.kv_rows : 0)) * p.blocks, step = blockDim.x / p.lanes;
+    struct Item {
+        P a, b;
+        T* out;
+        int ia, ib;  // places of the packs; ib < 0: none
+        int tt;      // token of the tile, -1: nothing turns
+    };
+    int tt = 0, row = tid / p.lanes - step;
+    auto next = [&](Item& x) {  // the thread's next item, its loads under way
+        for (;;) {
+            row += step;
+            while (row >= rows) {
+                row -= rows;
+                ++tt;
+            }
+            if (tt >= tile) return false;
+            const int r = p.blocks == 1 ? row : row / p.blocks;
+            const int c = tid % p.lanes + (p.blocks == 1 ? 0 : (row - r * p.blocks) * p.lanes);
+            if (c >= p.chunks) continue;
+            const int64_t t = t0 + tt;
+            const T* in;
+            bool turns = true;
+            if (!APPEND || r < p.q_rows) {
+                in = p.q + t * p.q_tok + r * p.q_head;
+                x.out = p.qo + t * p.qo_tok + r * p.qo_head;
+            } else {
+                const int64_t page = s_page[tt];
+                if (page < 0) continue;
+                const int h = r - p.q_rows;
+                turns = h < p.kv_rows;
+                if (turns) {
+                    in = p.k + t * p.k_tok + h * p.k_head;
+                    x.out = p.ko + page * p.ko_page + s_slot[tt] * p.ko_slot + h * p.ko_head;
+                } else {
+                    in = p.v + t * p.v_tok + (h - p.kv_rows) * p.v_head;
+                    x.out = p.vo + page * p.vo_page + s_slot[tt] * p.vo_slot + (h - p.kv_rows) * p.vo_head;
+                }
+            }
+            x.tt = turns ? tt : -1;
+            if (kApart && turns) {
+                if (c < turning) {
+                    x.ia = HALF ? c : 2 * c;
+                    x.ib = HALF ? turning + c : 2 * c + 1;
+                } else {  // copied, behind the turning ones
+                    const int rest = p.chunks - turning;
+                    x.ia = turning + c;
+                    x.ib = x.ia + rest < packs ? x.ia + rest : -1;
+                    x.tt = -1;
+                }
+            } else {
+                x.ia = c;
+                x.ib = c + p.chunks < packs ? c + p.chunks : -1;
+            }
+            x.a = reinterpret_cast<const P*>(in)[x.ia];
+            if (x.ib >= 0) x.b = reinterpret_cast<const P*>(in)[x.ib];
+            return true;
+        }
+    };
+    // The sines of pair j of pack c of a token: float4 j / 2 of all packs side by side, so that lanes
+    // read them without bank conflicts.
+    auto place = [&](int c, int j) { return kPairs == 1 ? c : ((j >> 1) * turning + c) * 2 + (j & 1); };
+    auto sines = [&](const float2* turn, int c, float2* cs) {
+        if constexpr (kPairs == 1) {
+            cs[0] = turn[c];
+        } else {
+#pragma unroll
+            for (int j = 0; j < kPairs; j += 2) {
+                const float4 v = *reinterpret_cast<const float4*>(turn + place(c, j));
+                cs[j] = make_float2(v.x, v.y);
+                cs[j + 1] = make_float2(v.z, v.w);
+            }
+        }
+    };
+    auto turn_pack = [&](P& v, int i, const float2* turn) {  // whole pairs
+        if (i >= turning) return;
+        float2 cs[kPairs];
+        float f[VEC];
+        sines(turn, i, cs);
+        v.get(f);
+#pragma unroll
+        for (int j = 0; j < VEC / 2; ++j) {
+            const float u = f[2 * j], w = f[2 * j + 1];
+            f[2 * j] = u * cs[j].x - w * cs[j].y;
+            f[2 * j + 1] = w * cs[j].x + u * cs[j].y;
+        }
+        v.put(f);
+    };
+    Item x;
+    bool have = next(x);
+
     for (int i = tid; i < tile * pairs; i += blockDim.x) {
-        const int tt = i / pairs;
-        const double t = s_pos[tt] * p.freq[i - tt * pairs];
-        const double k = rint(t * 0.15915494309189533577);  // whole turns
-        const double rest = fma(-k, 2.4492935982947064e-16, fma(-k, 6.283185307179586, t));  // 2 pi in two parts
+        const int k = i / pairs;
+        const double t = s_pos[k] * p.freq[i - k * pairs];
+        const double whole = rint(t * 0.15915494309189533577);  // turns
+        const double rest = fma(-whole, 2.4492935982947064e-16, fma(-whole, 6.283185307179586, t));  // 2 pi in two parts
         float s, c;
         sincospif((float)(rest * 0.31830988618379067154), &s, &c);
-        s_turn[i] = make_float2(c * p.scale, s * p.scale * p.sign);
+        const int pair = i - k * pairs;
+        s_turn[k * pairs + place(pair / kPairs, pair % kPairs)] = make_float2(c * p.scale, s * p.scale * p.sign);
     }
     __syncthreads();
 
-    const int rows = p.q_rows + (APPEND ? 2 * p.kv_rows : 0);
-    const int lane = tid % p.lanes, step = blockDim.x / p.lanes;
-    const int turning = pairs / VEC;                         // chunks of pairs in a row
-    const int chunks = turning + (p.dim - p.rot) / VEC;      // and of copied elements behind them
-    int tt = 0, row = tid / p.lanes;
-    for (;; row += step) {
-        while (row >= rows) {
-            row -= rows;
-            ++tt;
-        }
-        if (tt >= tile) break;
-        const T* in;
-        T* out;
-        const int64_t t = t0 + tt;
-        if (!APPEND || row < p.q_rows) {
-            in = p.q + t * p.q_tok + row * p.q_head;
-            out = p.qo + t * p.qo_tok + row * p.qo_head;
-        } else {
-            const int64_t page = s_page[tt];
-            if (page < 0) continue;
-            const int h = row - p.q_rows;
-            if (h >= p.kv_rows) {
-                in = p.v + t * p.v_tok + (h - p.kv_rows) * p.v_head;
-                out = p.vo + page * p.vo_page + s_slot[tt] * p.vo_slot + (h - p.kv_rows) * p.vo_head;
-                for (int c = lane; c < p.dim / VEC; c += p.lanes)
-                    reinterpret_cast<P*>(out)[c] = reinterpret_cast<const P*>(in)[c];
-                continue;
-            }
-            in = p.k + t * p.k_tok + h * p.k_head;
-            out = p.ko + page * p.ko_page + s_slot[tt] * p.ko_slot + h * p.ko_head;
-        }
-        const float2* turn = s_turn + tt * pairs;
-        for (int c = lane; c < chunks; c += p.lanes) {
-            if (c >= turning) {
-                const int at = p.rot / VEC + c - turning;
-                reinterpret_cast<P*>(out)[at] = reinterpret_cast<const P*>(in)[at];
-                continue;
-            }
-            // two packs hold VEC pairs: halves apart, or neighbours
-            const int ia = HALF ? c : 2 * c, ib = HALF ? turning + c : 2 * c + 1;
-            P a = reinterpret_cast<const P*>(in)[ia], b = reinterpret_cast<const P*>(in)[ib];
-            float x[2 * VEC];
+    while (have) {
+        Item y;
+        have = next(y);
+        if (x.tt >= 0) {
+            const float2* turn = s_turn + x.tt * pairs;
+            if constexpr (kApart) {
+                float2 cs[kPairs];
+                sines(turn, HALF ? x.ia : x.ia / 2, cs);
+                float f[VEC], g[VEC];
+                x.a.get(f);
+                x.b.get(g);
 #pragma unroll
-            for (int j = 0; j < VEC; ++j) {
-                x[j] = to_f32(a.v[j]);
-                x[VEC + j] = to_f32(b.v[j]);
+                for (int j = 0; j < VEC; ++j) {
+                    const float u = f[j], w = g[j];
+                    f[j] = u * cs[j].x - w * cs[j].y;
+                    g[j] = w * cs[j].x + u * cs[j].y;
+                }
+                x.a.put(f);
+                x.b.put(g);
+            } else {
+                turn_pack(x.a, x.ia, turn);
+                if (x.ib >= 0) turn_pack(x.b, x.ib, turn);
             }
-#pragma unroll
-            for (int j = 0; j < VEC; ++j) {
-                const float2 cs = turn[c * VEC + j];
-                const int k0 = HALF ? j : 2 * j, k1 = HALF ? VEC + j : 2 * j + 1;
-                const float u = x[k0], w = x[k1];
-                x[k0] = u * cs.x - w * cs.y;
-                x[k1] = w * cs.x + u * cs.y;
-            }
-#pragma unroll
-            for (int j = 0; j < VEC; ++j) {
-                a.v[j] = from_f32<T>(x[j]);
-                b.v[j] = from_f32<T>(x[VEC + j]);
-            }
-            reinterpret_cast<P*>(out)[ia] = a;
-            reinterpret_cast<P*>(out)[ib] = b;
         }
+        reinterpret_cast<P*>(x.out)[x.ia] = x.a;
+        if (x.ib >= 0) reinterpret_cast<P*>(x.out)[x.ib] = x.b;
+        x = y;
     }
 }
 
@@ -172,10 +256,12 @@ int rope_run(RopeParams<T> p, int layout, cudaStream_t st, const char* what) {
     uint64_t all = 0;
     for (const void* a : at) all |= reinterpret_cast<uint64_t>(a);
     for (const int64_t s : strides) all |= (uint64_t)s * sizeof(T);
-    const bool wide = all % 16 == 0 && p.rot % (2 * WIDE) == 0 && (p.dim - p.rot) % WIDE == 0;
+    const bool half = layout == TG_ROPE_HALF;
+    const bool wide = all % 16 == 0 && p.dim % WIDE == 0 && p.rot % (half ? 2 * WIDE : WIDE) == 0;
     const int vec = wide ? WIDE : 1;
-    const int chunks = (p.rot / 2 + p.dim - p.rot) / vec;
-    p.lanes = std::min(chunks, kRopeThreads);
+    p.chunks = half || !wide ? p.rot / 2 / vec + ((p.dim - p.rot) / vec + 1) / 2 : (p.dim / vec + 1) / 2;
+    p.lanes = std::min(p.chunks, kRopeThreads);
+    p.blocks = (p.chunks + p.lanes - 1) / p.lanes;
     const int rows = p.q_rows + (APPEND ? 2 * p.kv_rows : 0);
     const int block = p.lanes * std::min(kRopeThreads / p.lanes, std::max(rows, 1) * kRopeTile);
     // Tokens of a CTA: enough that each thread moves a few rows for its share of the sines, but
@@ -187,7 +273,6 @@ int rope_run(RopeParams<T> p, int layout, cudaStream_t st, const char* what) {
     p.tile = (int)tile;
     const size_t smem = (size_t)tile * pairs * sizeof(float2);
     const unsigned grid = (unsigned)ceil_div(p.tokens, tile);
-    const bool half = layout == TG_ROPE_HALF;
     auto kernel = wide ? (half ? rope_kernel<T, WIDE, true, APPEND> : rope_kernel<T, WIDE, false, APPEND>)
                        : (half ? rope_kernel<T, 1, true, APPEND> : rope_kernel<T, 1, false, APPEND>);
     kernel<<<grid, block, smem, st>>>(p);
