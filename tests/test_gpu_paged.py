@@ -548,3 +548,17 @@ def test_prompts_then_decoding_steps():
         b.q = q
         b.check(P.prefix_attention(q, cache, table, seq_len, prefix_pages=torch.tensor(pre, device="cuda"), prefix_len=prefix,
                                    q_indptr=indptr, max_q_len=max(news)))
+
+
+@pytest.mark.parametrize("kw", [dict(batch=5, prefix=100, steps=3), dict(batch=40, prefix=515, steps=20, prompt=(1, 30)),
+                                dict(batch=2, prefix=1, steps=2, heads=8, kv_heads=8, dim=128, page=8)])
+def test_the_decoding_example(kw):
+    """Three 16-bit roundings of the block's output (projections, attention, sum): 4 half ulps."""
+    import importlib.util
+    import os
+
+    path = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "examples", "shared_prefix_decode.py")
+    spec = importlib.util.spec_from_file_location("shared_prefix_decode", path)
+    example = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(example)
+    assert example.check(*example.generate(**kw)) < 4 * U[BF16]
