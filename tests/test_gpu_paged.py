@@ -356,6 +356,31 @@ def test_cache_offsets_beyond_32_bits():
     assert torch.equal(flat[last[0], 99 % page], k[0]) and torch.equal(other[last[1], 129 % page], k[2])
 
 
+@pytest.mark.parametrize("news,dim,page", [([1, 1], 128, 16), ([1, 1], 64, 7), ([40, 30], 128, 16), ([40, 90], 64, 24), ([200, 9], 64, 8)])
+def test_pages_outside_the_cache_read_as_zeros(news, dim, page):
+    """Lengths beyond the listed pages are cut to them, pages that do not exist hold zeros."""
+    b = Batch(news, [200, 150], 90, 8, 2, dim, page, BF16, seed=3)
+    bad = b.table.indices.clone()
+    bad[1], bad[int(b.table.indptr[1]) + 2] = b.cache.pages + 3, -2
+    b.table = P.PageTable(b.table.indptr, bad)
+    pre = b.prefix_pages.clone()
+    pre[-1] = 1 << 40
+    b.prefix_pages = pre
+    for s, i in ((0, 1), (1, 2)):
+        for x in b.own[s]:
+            x[i * page:(i + 1) * page] = 0
+    for x in b.shared:
+        x[(len(pre) - 1) * page:] = 0
+    b.check(b.run())
+    b.seq_len = torch.tensor([10 ** 12, -4], device="cuda")
+    b.lens = [len(b.rows[0]) * page, 0]
+    b.own[1] = [x[:0] for x in b.own[1]]
+    for x in (b.cache.k, b.cache.v):  # the last page's free slots are seen now
+        x[b.rows[0][-1]] = x[b.rows[0][-1]].nan_to_num(0.0)
+    b.own[0] = [torch.cat((x, x.new_zeros(b.lens[0] - x.shape[0], *x.shape[1:]))) for x in b.own[0]]
+    b.check(b.run())
+
+
 def test_attention_on_another_stream_and_workspace():
     b = Batch(*ATTEND[9], BF16, seed=4)
     st = torch.cuda.Stream()

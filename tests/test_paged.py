@@ -128,6 +128,8 @@ def test_attention_workspace_size():
     (dict(cache=_cache(dim=80)), lib.TG_EUNSUPPORTED, "head dim"),
     (dict(cache=_cache(page_size=0)), lib.TG_EINVAL, "page_size"),
     (dict(cache=_cache(k=None)), lib.TG_EINVAL, "null cache"),
+    (dict(cache=_cache(pages=0), table=_table(cols=0)), lib.TG_EINVAL, "without pages"),
+    (dict(tokens=1 << 30, q_indptr=4096, max_q_len=1, q_heads=64), lib.TG_EUNSUPPORTED, "too many rows"),
     (dict(cache=_cache(v_slot_stride=129)), lib.TG_EINVAL, "aligned"),
     (dict(table=_table(cols=9)), lib.TG_EINVAL, "columns"),
     (dict(table=_table(indptr=None)), lib.TG_EINVAL, "indptr"),

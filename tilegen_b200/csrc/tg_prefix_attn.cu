@@ -115,17 +115,19 @@ __global__ void __launch_bounds__(32) attn_rows_kernel(const AttnParams p, const
     __syncwarp();
     const uint32_t ring = smem_addr(smem);
     const int boxes = kStepKeys / box;
-    uint32_t missing = 0;  // stages of which a box was not fetched
-    // lane l: the page of box l of a step
+    // Lane l: the page of box l of a step, -1 past the end.  A page that does not exist is fetched
+    // from behind the last one, which reads as zeros.
     auto find = [&](int i, int& page, int& slot) {
         const int at = k0 + i * kStepKeys + lane * box;
         page = -1;
         slot = 0;
-        if (lane < boxes && at < k1) locate(p, list, at, page, slot);
+        if (lane < boxes && at < k1) {
+            locate(p, list, at, page, slot);
+            if (page < 0) page = p.pages;
+        }
     };
     auto fetch = [&](int stage, int page, int slot) {
         const uint32_t dst = ring + stage * C::kStage, there = __ballot_sync(kFull, page >= 0);
-        missing = (missing & ~(1u << stage)) | (uint32_t)(__popc(there) < boxes) << stage;
         if (lane == 0) mbar_arrive_expect_tx(&bar[stage], __popc(there) * box * C::kHalves * 256);
         __syncwarp();
         for (int i = 0; i < boxes; ++i) {
@@ -219,17 +221,13 @@ __global__ void __launch_bounds__(32) attn_rows_kernel(const AttnParams p, const
         }
         const uint32_t kt = ring + stage * C::kStage, vt = kt + C::kHalves * C::kBox;
         const int key0 = k0 + it * kStepKeys, step_end = min(key0 + kStepKeys, k1);
-        // Keys and values past the end, or of pages that do not exist, are zeros: a box may hold
-        // anything there, and 0 * NaN is not 0.
-        if (key0 + kStepKeys > k1 || missing & 1u << stage) {
-            for (int r = 0; r < kStepKeys; ++r) {
-                int pg = -1, sl;
-                if (key0 + r < k1) locate(p, list, key0 + r, pg, sl);
-                if (pg < 0)
-                    for (int c = lane; c < 2 * C::kHalves * 8; c += 32)
-                        *reinterpret_cast<uint4*>(smem + (kt - ring) + (c >> 3) * C::kBox + r * 128 + (c & 7) * 16) = make_uint4(0, 0, 0, 0);
-            }
-            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // a later box may land here
+        // Values past the end are zeros: a box may hold anything there, and 0 * NaN is not 0 (it is
+        // the last step, so no later box lands on what is written here).
+        if (key0 + kStepKeys > k1) {
+            for (int i = (k1 - key0) * 8 + lane; i < kStepKeys * 8; i += 32)
+#pragma unroll
+                for (int half = 0; half < C::kHalves; ++half)
+                    *reinterpret_cast<uint4*>(smem + (vt - ring) + half * C::kBox + i * 16) = make_uint4(0, 0, 0, 0);
             __syncwarp();
         }
 
@@ -560,7 +558,10 @@ int make_plan(const tg_prefix_attention_args* a, Plan* plan, const char* op) {
     if (!(a->scale > 0.0) || a->scale > 1e30) return set_error(TG_EINVAL, "%s: scale must be positive", op);
     if (a->flags & ~(TG_FLAG_CAUSAL | TG_FLAG_BOUNDS_CHECK))
         return set_error(TG_EINVAL, "%s: unknown flags 0x%x", op, a->flags);
-    const int64_t slots = t.nnz > INT32_MAX / c.page_size ? INT32_MAX / 2 : t.nnz * c.page_size;
+    if (a->prefix_len > 0 && c.pages == 0) return set_error(TG_EINVAL, "%s: a prefix in a cache without pages", op);
+    if (a->tokens * (a->q_heads / c.heads) > INT32_MAX)
+        return set_error(TG_EUNSUPPORTED, "%s: too many rows for one launch", op);
+    const int64_t slots = c.pages == 0 ? 0 : t.nnz > INT32_MAX / c.page_size ? INT32_MAX / 2 : t.nnz * c.page_size;
     const int64_t max_seq = std::min({a->max_seq_len, slots, (int64_t)INT32_MAX / 2});
     const int64_t max_q = a->q_indptr ? std::min(a->max_q_len, a->tokens) : 1;
 

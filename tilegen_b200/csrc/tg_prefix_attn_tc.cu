@@ -408,7 +408,8 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const AttnParams p
         }
     } else if (warp == 8 || warp == 10) {
         // Lane l looks up the page of box l of a tile one tile ahead; the warp issues box after
-        // box.  A box that holds no key, or whose page does not exist, is not fetched.
+        // box.  A box past the end is not fetched; a page that does not exist is fetched from behind
+        // the last one, which reads as zeros.
         const int is_v = warp == 10, boxes = kTile / box;
         const CUtensorMap* map = is_v ? &vmap : &kmap;
         int f0 = 0, tails = 0;  // fills before this segment, tails so far
@@ -417,7 +418,10 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const AttnParams p
             int page, slot;
             auto find = [&](int at) {
                 page = -1, slot = 0;
-                if (at < g.k1) locate(p, g.list, at, page, slot);
+                if (at < g.k1) {
+                    locate(p, g.list, at, page, slot);
+                    if (page < 0) page = p.pages;
+                }
             };
             if (lane < boxes) find(g.k0 + lane * box);
             for (int j = 0; j < g.steps; ++j) {
