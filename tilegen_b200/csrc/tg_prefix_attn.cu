@@ -389,13 +389,13 @@ __global__ void __launch_bounds__(32) attn_rows_kernel(const AttnParams p, const
 }
 
 // ------------------------------------------------------------------ joining the parts
-// WPR warps a row, each with every WPR-th part: one where rows are many, all four where parts
-// are (147 parts of 64 rows: 63 us by one warp a row, DRAM latency after latency).  Bound: L2 (the
-// parts were just written), so loads are 16 bytes a lane and eight parts are in flight.
+// WPR warps a row, each with every WPR-th part: one where rows are many, 4 or 16 where parts are
+// (147 parts of 64 rows: 63 us by one warp a row, latency after latency).  Bound: L2 (the parts were
+// just written), so loads are 16 bytes a lane and eight parts are in flight.
 template <typename T, int D, int WPR>
-__global__ void __launch_bounds__(128) attn_join_kernel(const AttnParams p) {
+__global__ void __launch_bounds__(WPR == 16 ? 512 : 128) attn_join_kernel(const AttnParams p) {
     constexpr int VE = D % 128 == 0 ? 4 : D % 64 == 0 ? 2 : 1, NV = D / (32 * VE);
-    __shared__ float s_acc[WPR == 1 ? 1 : 4][D], s_sum[4], s_top[4];
+    __shared__ float s_acc[WPR][D], s_sum[WPR], s_top[WPR];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, mine = WPR == 1 ? 0 : warp;
     const int64_t all = (int64_t)p.tokens * p.q_heads, row = WPR == 1 ? (int64_t)blockIdx.x * 4 + warp : blockIdx.x;
     pdl_wait();
@@ -462,13 +462,15 @@ __global__ void __launch_bounds__(128) attn_join_kernel(const AttnParams p) {
         if (lane == 0) s_sum[warp] = sum, s_top[warp] = top;
         __syncthreads();
         if (warp > 0) return;
-        top = fmaxf(fmaxf(s_top[0], s_top[1]), fmaxf(s_top[2], s_top[3]));
+        top = s_top[0];
+#pragma unroll
+        for (int w = 1; w < WPR; ++w) top = fmaxf(top, s_top[w]);
         const float all_base = top == -INFINITY ? 0.f : top;
         sum = 0.f;
 #pragma unroll
         for (int i = 0; i < NV * VE; ++i) acc[i] = 0.f;
 #pragma unroll
-        for (int w = 0; w < 4; ++w) {
+        for (int w = 0; w < WPR; ++w) {
             const float f = s_sum[w] == 0.f ? 0.f : exp2_fast(s_top[w] - all_base);
             sum += f * s_sum[w];
 #pragma unroll
@@ -683,6 +685,8 @@ int attn_run(const Plan& plan, void* ws, cudaStream_t st) {
     }
     if (rc != TG_OK) return rc;
     if (p.direct) return TG_OK;
+    if (parts > 32 && rows < kSMs * 8)
+        return launch_pdl("attn_join_kernel", attn_join_kernel<T, D, 16>, dim3((unsigned)rows), 512, 0, st, p);
     if (parts > 8 && rows < 4 * kSMs * 16)
         return launch_pdl("attn_join_kernel", attn_join_kernel<T, D, 4>, dim3((unsigned)rows), 128, 0, st, p);
     return launch_pdl("attn_join_kernel", attn_join_kernel<T, D, 1>, dim3((unsigned)ceil_div((int64_t)rows, 4)), 128, 0, st, p);
