@@ -496,6 +496,100 @@ __global__ void __launch_bounds__(WPR == 16 ? 512 : 128) attn_join_kernel(const 
     if (p.lse && lane == 0) p.lse[row] = sum == 0.f ? -INFINITY : (top + log2f(sum)) * 0.69314718055994531f;
 }
 
+// At most eight parts, many rows: a warp joins four heads of a token.  What the chain of the sequence's place
+// and length, m and l, and the sums costs is paid once for the four, and their loads are under way
+// together (a warp a row: 92 us for 119,040 rows of three parts, 183 MB).
+template <typename T, int D>
+__global__ void __launch_bounds__(128) attn_join_few_kernel(const AttnParams p) {
+    constexpr int VE = D % 128 == 0 ? 4 : D % 64 == 0 ? 2 : 1, NV = D / (32 * VE), kHeads = 4, kParts = 8;
+    const int lane = threadIdx.x & 31;
+    const int groups = (p.q_heads + kHeads - 1) / kHeads;
+    const int64_t id = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5), all = (int64_t)p.tokens * p.q_heads;
+    const int t = (int)(id / groups), h0 = (int)(id % groups) * kHeads;
+    pdl_wait();
+    if (t >= p.tokens) return;
+    int own = 0;
+    if (p.own_chunks > 0) {
+        const Sequence s = sequence(p, sequence_of(p.q_indptr, p.rows, t));
+        if (t >= s.first && t < s.first + s.n) own = (s.len + p.own_chunk - 1) / p.own_chunk;
+    }
+    // lane 8 k + i: part i of head h0 + k
+    const int h = min(h0 + lane / kParts, p.q_heads - 1), i = lane % kParts;
+    int np = p.prefix_splits;  // parts over the prefix
+    if (p.prefix_ctas > 0) {
+        const int u = h / p.group * p.prefix_tiles + (t * p.group + h % p.group) / 256;
+        np = prefix_cta(p, (u + 1) * p.prefix_steps - 1) - prefix_cta(p, u * p.prefix_steps) + 1;
+    }
+    const int n = np + own, place = i < np ? i : i - np + p.prefix_splits;
+    const int64_t at = place * all + (int64_t)t * p.q_heads + h;
+    float2 ml = make_float2(-INFINITY, 0.f);
+    if (i < n) ml = p.part_ml[at];
+    float top = ml.x;
+#pragma unroll
+    for (int x = kParts / 2; x; x >>= 1) top = fmaxf(top, __shfl_xor_sync(kFull, top, x));
+    // 0: nothing seen there, nothing written; a NaN score leaves the sum NaN
+    float f = ml.y == 0.f ? 0.f : ml.y != ml.y ? NAN : exp2_fast(ml.x - (top == -INFINITY ? 0.f : top));
+    float sum = f == 0.f ? 0.f : f * ml.y;
+#pragma unroll
+    for (int x = kParts / 2; x; x >>= 1) sum += __shfl_xor_sync(kFull, sum, x);
+    if (p.lse && i == 0 && h0 + lane / kParts < p.q_heads)
+        p.lse[(int64_t)t * p.q_heads + h] = sum == 0.f ? -INFINITY : (top + log2f(sum)) * 0.69314718055994531f;
+    f *= sum == 0.f ? 0.f : 1.f / sum;
+    float acc[kHeads][NV * VE];
+#pragma unroll
+    for (int k = 0; k < kHeads; ++k)
+#pragma unroll
+        for (int e = 0; e < NV * VE; ++e) acc[k][e] = 0.f;
+    const int most = __reduce_max_sync(kFull, n);
+#pragma unroll 2
+    for (int j = 0; j < most; ++j) {
+        float v[kHeads][NV * VE], w[kHeads];
+#pragma unroll
+        for (int k = 0; k < kHeads; ++k) {
+            w[k] = __shfl_sync(kFull, f, k * kParts + j);
+            const int64_t from = __shfl_sync(kFull, at, k * kParts + j);
+            const float* x = p.part_o + from * D;
+#pragma unroll
+            for (int e = 0; e < NV * VE; ++e) v[k][e] = 0.f;
+            if (w[k] != 0.f) {
+#pragma unroll
+                for (int q = 0; q < NV; ++q) {
+                    if constexpr (VE == 4) {
+                        const float4 y = *reinterpret_cast<const float4*>(x + (q * 32 + lane) * 4);
+                        v[k][q * 4] = y.x, v[k][q * 4 + 1] = y.y, v[k][q * 4 + 2] = y.z, v[k][q * 4 + 3] = y.w;
+                    } else if constexpr (VE == 2) {
+                        const float2 y = *reinterpret_cast<const float2*>(x + (q * 32 + lane) * 2);
+                        v[k][q * 2] = y.x, v[k][q * 2 + 1] = y.y;
+                    } else {
+                        v[k][q] = x[q * 32 + lane];
+                    }
+                }
+            }
+        }
+#pragma unroll
+        for (int k = 0; k < kHeads; ++k)
+#pragma unroll
+            for (int e = 0; e < NV * VE; ++e) acc[k][e] += w[k] * v[k][e];
+    }
+#pragma unroll
+    for (int k = 0; k < kHeads; ++k) {
+        if (h0 + k >= p.q_heads) break;
+        T* out = static_cast<T*>(p.out) + t * p.o_tok + (h0 + k) * p.o_head;
+#pragma unroll
+        for (int q = 0; q < NV; ++q) {
+            T* y = out + (q * 32 + lane) * VE;
+            if constexpr (VE == 4) {
+                *reinterpret_cast<uint2*>(y) = make_uint2(pack2<T>(acc[k][q * 4], acc[k][q * 4 + 1]),
+                                                          pack2<T>(acc[k][q * 4 + 2], acc[k][q * 4 + 3]));
+            } else if constexpr (VE == 2) {
+                *reinterpret_cast<uint32_t*>(y) = pack2<T>(acc[k][q * 2], acc[k][q * 2 + 1]);
+            } else {
+                *y = from_f32<T>(acc[k][q]);
+            }
+        }
+    }
+}
+
 // ------------------------------------------------------------------ host
 struct Plan {
     AttnParams p;
@@ -625,9 +719,10 @@ int make_plan(const tg_prefix_attention_args* a, Plan* plan, const char* op) {
     }
     plan->own_units = t.rows * tiles_own * p.own_chunks;
     plan->prefix_units = p.prefix_ctas ? p.prefix_ctas : tiles_all * p.prefix_splits;
-    if (plan->own_units + plan->prefix_units > INT32_MAX || c.heads > 65535)
+    if ((plan->own_units + plan->prefix_units) * c.heads > INT32_MAX - kSMs || c.heads > 65535)
         return set_error(TG_EUNSUPPORTED, "%s: too many rows for one launch", op);
     p.tiles = (int)tiles_own;
+    p.own_pieces = (int)(plan->own_units * c.heads);
     const int parts = p.prefix_splits + p.own_chunks;
     p.direct = parts == 1;
     const size_t rows = (size_t)a->tokens * a->q_heads;
@@ -676,7 +771,7 @@ int attn_run(const Plan& plan, void* ws, cudaStream_t st) {
     const int64_t units = plan.own_units + p.prefix_units;
     if (rc == TG_OK && units > 0) {
         if (plan.rt_own == 0) {
-            if constexpr (D == 64 || D == 128) rc = attn_tc_run<T>(p, D, units, second, st);
+            if constexpr (D == 64 || D == 128) rc = attn_tc_run<T>(p, D, std::min(p.own_pieces, kSMs), second, st);
         } else if (plan.rt_own == 2) {
             if constexpr (D <= 128) rc = rows_launch<T, D, 2>(p, units, second, st);
         } else {
@@ -685,6 +780,10 @@ int attn_run(const Plan& plan, void* ws, cudaStream_t st) {
     }
     if (rc != TG_OK) return rc;
     if (p.direct) return TG_OK;
+    if (parts <= 8 && rows >= (size_t)kSMs * 128) {  // fewer rows do better with a warp each
+        const int64_t warps = p.tokens * ceil_div(p.q_heads, 4);
+        return launch_pdl("attn_join_few_kernel", attn_join_few_kernel<T, D>, dim3((unsigned)ceil_div(warps, 4)), 128, 0, st, p);
+    }
     if (parts > 32 && rows < kSMs * 8)
         return launch_pdl("attn_join_kernel", attn_join_kernel<T, D, 16>, dim3((unsigned)rows), 512, 0, st, p);
     if (parts > 8 && rows < 4 * kSMs * 16)

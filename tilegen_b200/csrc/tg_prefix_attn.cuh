@@ -33,6 +33,7 @@ struct AttnParams {
     // prefix_steps for each (head, row tile) in turn, prefix_tiles row tiles
     int prefix_work, prefix_per_unit, prefix_ctas, prefix_steps, prefix_tiles;  // prefix_ctas 0: splits of prefix_chunk keys
     int own_chunks, own_chunk;        // most chunks of a sequence, keys of a chunk
+    int own_pieces;                   // the tcgen05 kernel: (head, chunk, sequence, row tile)
     int tiles;                        // row tiles of a sequence (own) or of all rows (prefix)
     int over_prefix;                  // the tcgen05 kernel: the prefix, else the sequences' own pages
     int prefix_units;                 // the kernel for few rows: its first blocks go over the prefix
@@ -138,6 +139,6 @@ int cache_maps(const AttnParams& p, bool is_half, int dim, int box_rows, CUtenso
 
 // tg_prefix_attn_tc.cu
 template <typename T>
-int attn_tc_run(const AttnParams& p, int dim, int64_t units, bool pdl, cudaStream_t st);
+int attn_tc_run(const AttnParams& p, int dim, int ctas, bool pdl, cudaStream_t st);
 
 }  // namespace tg

@@ -238,54 +238,57 @@ __device__ __forceinline__ void row_alone(const AttnParams& p, const Segment& g,
     }
 }
 
-// The CTA's segments, one after the other.  Over the prefix a CTA has an even share of all steps
-// of all (head, row tile) pairs, so it ends one pair and begins another where its share does; the
-// parts of a pair are numbered by CTA.  Over own pages it has one segment.
+// The CTA's segments, one after the other, so that the keys of the next are under way while the
+// results of one are written.  Over the prefix a CTA has a share of the steps of the (head, row
+// tile) pairs; it may end one pair and begin another, and the parts of a pair are numbered by CTA.
+// Over own pages it has every gridDim.x-th of the pieces (head, chunk, row tile, sequence), the
+// last rows first: they see the most keys, and rounds of the CTAs are of like length.
 struct Segments {
     int at, end;
     __device__ __forceinline__ explicit Segments(const AttnParams& p) {
-        at = p.over_prefix ? prefix_start(p, blockIdx.x) : 0;
-        end = p.over_prefix ? prefix_start(p, blockIdx.x + 1) : 1;
+        at = p.over_prefix ? prefix_start(p, blockIdx.x) : blockIdx.x;
+        end = p.over_prefix ? prefix_start(p, blockIdx.x + 1) : p.own_pieces;
     }
     __device__ __forceinline__ bool next(const AttnParams& p, Segment& g) {
-        if (at >= end) return false;
-        int tile;
-        if (p.over_prefix) {
-            const int u = at / p.prefix_steps, first = at - u * p.prefix_steps;
-            g.steps = min(p.prefix_steps - first, end - at);
-            at += g.steps;
-            g.h = u / p.tiles;
-            tile = u - g.h * p.tiles;
-            g.part = blockIdx.x - prefix_cta(p, u * p.prefix_steps);
-            g.s.first = 0;
-            g.s.n = p.tokens;
-            g.list = p.prefix_pages;
-            g.keys = p.prefix_len;
-            g.k0 = first * kTile;
-            g.k1 = min(g.keys, g.k0 + g.steps * kTile);
-        } else {
-            at = end;
-            const int c = blockIdx.x % p.own_chunks, u = blockIdx.x / p.own_chunks;
-            g.h = blockIdx.y;
-            tile = u % p.tiles;
-            g.s = sequence(p, u / p.tiles);
-            g.list = p.indices + g.s.page0;
-            g.keys = g.s.len;
-            g.k0 = c * p.own_chunk;
-            g.k1 = min(g.keys, g.k0 + p.own_chunk);
-            g.part = p.prefix_splits + c;
+        for (;;) {
+            if (at >= end) return false;
+            if (p.over_prefix) {
+                const int u = at / p.prefix_steps, first = at - u * p.prefix_steps;
+                g.steps = min(p.prefix_steps - first, end - at);
+                at += g.steps;
+                g.h = u / p.tiles;
+                g.row0 = (u - g.h * p.tiles) * 2 * kTile;
+                g.part = blockIdx.x - prefix_cta(p, u * p.prefix_steps);
+                g.s.first = 0;
+                g.s.n = p.tokens;
+                g.nrows = min(p.tokens * p.group - g.row0, 2 * kTile);
+                g.list = p.prefix_pages;
+                g.keys = p.prefix_len;
+                g.k0 = first * kTile;
+                g.k1 = min(g.keys, g.k0 + g.steps * kTile);
+            } else {
+                int x = at;
+                at += gridDim.x;
+                g.h = x % p.kv_heads, x /= p.kv_heads;
+                const int c = x % p.own_chunks;
+                x /= p.own_chunks;
+                const int b = x % p.rows;
+                g.row0 = (p.tiles - 1 - x / p.rows) * 2 * kTile;
+                g.s = sequence(p, b);
+                g.nrows = min(g.s.n * p.group - g.row0, 2 * kTile);
+                g.list = p.indices + g.s.page0;
+                g.keys = g.s.len;
+                g.k0 = c * p.own_chunk;
+                g.part = p.prefix_splits + c;
+                // no rows, or no such chunk (the join does not ask for it)
+                if (g.nrows <= 0 || (g.k0 >= g.keys && !p.direct)) continue;
+                // no row sees more than the last one
+                g.k1 = min(min(g.keys, g.k0 + p.own_chunk), keys_seen(p, g.s, (g.row0 + g.nrows - 1) / p.group, g.keys, g.keys));
+                g.steps = g.k1 > g.k0 ? (g.k1 - g.k0 + kTile - 1) / kTile : 0;
+            }
+            g.ntiles = g.nrows > kTile ? 2 : 1;
+            return true;
         }
-        g.row0 = tile * 2 * kTile;
-        g.nrows = min(g.s.n * p.group - g.row0, 2 * kTile);
-        if (g.nrows <= 0) return false;
-        g.ntiles = g.nrows > kTile ? 2 : 1;
-        if (!p.over_prefix) {
-            if (g.k0 >= g.keys && !p.direct) return false;  // no such chunk: the join does not ask for it
-            // no row sees more than the last one
-            g.k1 = min(g.k1, keys_seen(p, g.s, (g.row0 + g.nrows - 1) / p.group, g.keys, g.keys));
-            g.steps = g.k1 > g.k0 ? (g.k1 - g.k0 + kTile - 1) / kTile : 0;
-        }
-        return true;
     }
 };
 
@@ -303,7 +306,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const AttnParams p
         Segments some(p);
         Segment g;
         if (!some.next(p, g)) {
-            if (blockIdx.x == 0 && blockIdx.y == 0) pdl_wait();
+            if (blockIdx.x == 0) pdl_wait();
             return;
         }
     }
@@ -730,12 +733,12 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const AttnParams p
         tmem_free(tmem, kCols);
     }
     // grids of a call complete in order: this one, if it is the second, ends after the first
-    if (blockIdx.x == 0 && blockIdx.y == 0) pdl_wait();
+    if (blockIdx.x == 0) pdl_wait();
 }
 
 // ------------------------------------------------------------------ host
 template <typename T, int D>
-int tc_launch(const AttnParams& p, int64_t units, bool pdl, cudaStream_t st) {
+int tc_launch(const AttnParams& p, int ctas, bool pdl, cudaStream_t st) {
     using C = TcCfg<D>;
     static_assert(C::kSmem <= 227 * 1024 && sizeof(TcShared) <= 2048, "shared memory of a CTA");
     const int box = std::gcd(p.page_size, kTile);
@@ -746,7 +749,7 @@ int tc_launch(const AttnParams& p, int64_t units, bool pdl, cudaStream_t st) {
     if (rc == TG_OK)
         rc = once.raise(reinterpret_cast<const void*>(kernel), C::kSmem);
     if (rc != TG_OK) return rc;
-    const dim3 grid((unsigned)units, p.over_prefix ? 1u : (unsigned)p.kv_heads);
+    const dim3 grid((unsigned)ctas);
     if (pdl) return launch_pdl("attn_tc_kernel", kernel, grid, kThreads, C::kSmem, st, p, box, kmap, vmap);
     kernel<<<grid, kThreads, C::kSmem, st>>>(p, box, kmap, vmap);
     return check_launch("attn_tc_kernel");
@@ -755,10 +758,10 @@ int tc_launch(const AttnParams& p, int64_t units, bool pdl, cudaStream_t st) {
 }  // namespace
 
 template <typename T>
-int attn_tc_run(const AttnParams& p, int dim, int64_t units, bool pdl, cudaStream_t st) {
-    return dim == 64 ? tc_launch<T, 64>(p, units, pdl, st) : tc_launch<T, 128>(p, units, pdl, st);
+int attn_tc_run(const AttnParams& p, int dim, int ctas, bool pdl, cudaStream_t st) {
+    return dim == 64 ? tc_launch<T, 64>(p, ctas, pdl, st) : tc_launch<T, 128>(p, ctas, pdl, st);
 }
-template int attn_tc_run<__half>(const AttnParams&, int, int64_t, bool, cudaStream_t);
-template int attn_tc_run<__nv_bfloat16>(const AttnParams&, int, int64_t, bool, cudaStream_t);
+template int attn_tc_run<__half>(const AttnParams&, int, int, bool, cudaStream_t);
+template int attn_tc_run<__nv_bfloat16>(const AttnParams&, int, int, bool, cudaStream_t);
 
 }  // namespace tg
