@@ -74,9 +74,9 @@ constexpr int kRopeSmem = 32 * 1024;  // most bytes of cosines and sines of a CT
 // multiples of that, else single elements.  A thread's item is two packs of a row: the two halves
 // of its pairs (HALF, or single elements of neighbouring pairs), or two packs of whole pairs or
 // copied elements, a stretch of a row apart so that the threads' packs lie side by side.  The
-// packs of its next item are under way while one is turned, the first while the sines are made.
+// first item's packs are under way while the sines are made.
 template <typename T, int VEC, bool HALF, bool APPEND>
-__global__ void __launch_bounds__(kRopeThreads, 5) rope_kernel(const RopeParams<T> p) {
+__global__ void __launch_bounds__(kRopeThreads, APPEND ? 6 : 5) rope_kernel(const RopeParams<T> p) {
     extern __shared__ float4 s_turn4[];  // scale * (cos, sin) of [tile][pairs], two pairs in one float4
     float2* const s_turn = reinterpret_cast<float2*>(s_turn4);
     __shared__ double s_pos[kRopeTile];
@@ -84,6 +84,10 @@ __global__ void __launch_bounds__(kRopeThreads, 5) rope_kernel(const RopeParams<
     __shared__ int64_t s_slot[kRopeTile];
     using P = Pack<T, VEC>;
     constexpr bool kApart = HALF || VEC == 1;  // a pair's elements are in different packs
+    // The next packs under way cost 10 registers, a CTA on an SM: worth it for the rotation alone
+    // (47 against 54 us for 268 MB), not for the append (106 against 98 us for 572 MB), which waits for
+    // page numbers too.
+    constexpr bool kAhead = !APPEND;
     constexpr int kPairs = kApart ? VEC : VEC / 2;  // of an item's pack
     const int tid = threadIdx.x;
     const int64_t t0 = (int64_t)blockIdx.x * p.tile;
@@ -217,7 +221,7 @@ __global__ void __launch_bounds__(kRopeThreads, 5) rope_kernel(const RopeParams<
 
     while (have) {
         Item y;
-        have = next(y);
+        if constexpr (kAhead) have = next(y);
         if (x.tt >= 0) {
             const float2* turn = s_turn + x.tt * pairs;
             if constexpr (kApart) {
@@ -241,7 +245,8 @@ __global__ void __launch_bounds__(kRopeThreads, 5) rope_kernel(const RopeParams<
         }
         reinterpret_cast<P*>(x.out)[x.ia] = x.a;
         if (x.ib >= 0) reinterpret_cast<P*>(x.out)[x.ib] = x.b;
-        x = y;
+        if constexpr (kAhead) x = y;
+        else have = next(x);
     }
 }
 
