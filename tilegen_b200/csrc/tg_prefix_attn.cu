@@ -625,9 +625,9 @@ void share_prefix(AttnParams& p, int64_t rows, int dim, double own_bytes) {
     }
     p.prefix_ctas = (int)ctas;
     p.prefix_per_unit = ctas % units == 0 ? (int)(ctas / units) : 0;
-    p.prefix_splits = 1;
-    for (int u = 0; u < (int)units; ++u)
-        p.prefix_splits = std::max(p.prefix_splits, prefix_cta(p, (u + 1) * p.prefix_steps - 1) - prefix_cta(p, u * p.prefix_steps) + 1);
+    // a pair's steps lie in at most so many shares of at least prefix_work / ctas steps
+    const int least = p.prefix_work / p.prefix_ctas;
+    p.prefix_splits = p.prefix_per_unit ? p.prefix_per_unit : (p.prefix_steps + least - 2) / least + 1;
 }
 
 int make_plan(const tg_prefix_attention_args* a, Plan* plan, const char* op) {
