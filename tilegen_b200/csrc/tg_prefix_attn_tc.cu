@@ -125,32 +125,12 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
     asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
     return r;
 }
-// 2^x on the multiply-add units, for x <= 100 (2^-125 below -125): x = n + f with f in
-// [-1/2, 1/2], 2^f by its minimax polynomial of degree 4 (relative error 2.6e-6, a hundredth of
-// P's rounding), n added to the exponent.  The special-function unit makes 16 exponentials a
-// cycle and SM, as many cycles for a tile as its two matrix products take: what goes through
-// here shortens its queue.
-__device__ __forceinline__ float2 exp2_poly(uint64_t x) {
-    constexpr float kRound = 12582912.f;  // 1.5 * 2^23: the sum's low bits are the nearest whole number
-    float2 v = both(x);
-    x = pair(fmaxf(v.x, -125.f), fmaxf(v.y, -125.f));
-    const uint64_t t = add2(x, pair(kRound, kRound));
-    const uint64_t f = fma2(add2(t, pair(-kRound, -kRound)), pair(-1.f, -1.f), x);
-    uint64_t y = fma2(f, pair(0.009570101276f, 0.009570101276f), pair(0.055917859077f, 0.055917859077f));
-    y = fma2(y, f, pair(0.240247443318f, 0.240247443318f));
-    y = fma2(y, f, pair(0.693121790886f, 0.693121790886f));
-    y = fma2(y, f, pair(0.999999284744f, 0.999999284744f));
-    const float2 n = both(t), m = both(y);
-    return make_float2(__uint_as_float(__float_as_uint(m.x) + (__float_as_uint(n.x) << 23)),
-                       __uint_as_float(__float_as_uint(m.y) + (__float_as_uint(n.y) << 23)));
-}
-
 constexpr int kTile = 128;   // rows of a tile, keys of a step
 constexpr int kThreads = 384;
 constexpr uint32_t kCols = 512;
 constexpr uint32_t kColO = 256;
 constexpr float kGrow = 8.f;
-constexpr int kPoly = 4;  // of so many pairs of scores, one goes through exp2_poly
+constexpr int kFirst = 64;  // columns of P that are multiplied while the others are made
 
 template <int D>
 struct TcCfg {
@@ -382,10 +362,10 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const AttnParams p
                 const uint32_t v = ring + fv % C::kStages * C::kBlock;
                 for (int i = 0; ok && i < g.ntiles; ++i) {
                     const int turn = (i ? done1 : done0) + j;
-                    // the first half of P's columns is multiplied while the second is made
+                    // the first columns of P are multiplied while the others are made
 #pragma unroll
                     for (int kk = 0; kk < kTile / 16; ++kk) {
-                        if (kk == 0 || kk == kTile / 32) {
+                        if (kk == 0 || kk == kFirst / 16) {
                             if (!(ok = holds((kk ? b_p : b_ph) + i * 8, turn))) break;
                             fence_after();
                         }
@@ -610,35 +590,24 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const AttnParams p
                     const float base = m == -INFINITY ? 0.f : m;
                     const uint64_t scale2 = pair(p.scale_log2, p.scale_log2), base2 = pair(-base, -base);
                     uint64_t s0 = pair(0.f, 0.f), s1 = s0;
-                    auto make_p = [&](auto whole) {
 #pragma unroll
                     for (int c = 0; c < kTile; c += 32) {
                         uint32_t pk[16];
 #pragma unroll
                         for (int e = 0; e < 16; ++e) {
-                            const uint64_t y = fma2(pair(__uint_as_float(x[c + 2 * e]), __uint_as_float(x[c + 2 * e + 1])),
-                                                    scale2, base2);
-                            float2 w;
-                            if (e % kPoly == kPoly - 1 && decltype(whole)::value) {
-                                w = exp2_poly(y);
-                            } else {
-                                w = both(y);
-                                w = make_float2(exp2_fast(w.x), exp2_fast(w.y));
-                            }
+                            float2 w = both(fma2(pair(__uint_as_float(x[c + 2 * e]), __uint_as_float(x[c + 2 * e + 1])), scale2, base2));
+                            w = make_float2(exp2_fast(w.x), exp2_fast(w.y));
                             if (e & 1) s1 = add2(s1, pair(w.x, w.y));
                             else s0 = add2(s0, pair(w.x, w.y));
                             pk[e] = pack2<T>(w.x, w.y);
                         }
                         tmem_st16(ts + c / 2, pk);
-                        if (c == 32) {
+                        if (c == kFirst - 32) {
                             wait_st();
                             fence_before();
                             arrive(b_ph + my * 8);
                         }
                     }
-                    };
-                    if (cut) make_p(std::false_type());
-                    else make_p(std::true_type());
                     const float2 sum = both(add2(s0, s1));
                     l += sum.x + sum.y;
                     wait_st();
