@@ -61,6 +61,22 @@ __device__ __forceinline__ int64_t sequence_of(const int64_t* q_indptr, int64_t 
     return lo;
 }
 
+// The same for a token that is the same in all lanes of a full warp: 32 places at a time, so that
+// a batch of 1024 takes two loads one after the other instead of ten.
+__device__ __forceinline__ int64_t sequence_of_warp(const int64_t* q_indptr, int rows, int t) {
+    if (!q_indptr) return t;
+    const int lane = threadIdx.x & 31;
+    int lo = 0, n = rows;
+    while (n > 1) {
+        const int step = (n + 31) / 32, at = lane * step;
+        const uint32_t below = __ballot_sync(kFull, at < n && q_indptr[lo + at] <= t);
+        const int k = below ? 31 - __clz(below) : 0;
+        lo += k * step;
+        n = min(step, n - k * step);
+    }
+    return lo;
+}
+
 // First token and number of tokens of sequence b, inside [0, tokens] whatever q_indptr holds.
 __device__ __forceinline__ void tokens_of(const int64_t* q_indptr, int64_t tokens, int64_t b, int64_t& first,
                                           int64_t& n) {

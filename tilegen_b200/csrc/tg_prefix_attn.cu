@@ -410,7 +410,7 @@ __global__ void __launch_bounds__(WPR == 16 ? 512 : 128) attn_join_kernel(const 
     }
     n = np;
     if (p.own_chunks > 0) {
-        const Sequence s = sequence(p, sequence_of(p.q_indptr, p.rows, t));
+        const Sequence s = sequence(p, sequence_of_warp(p.q_indptr, p.rows, t));
         if (t >= s.first && t < s.first + s.n) n += (s.len + p.own_chunk - 1) / p.own_chunk;
     }
     // lane l holds the maximum and sum of the l-th of 32 of the warp's parts at a time
@@ -512,7 +512,7 @@ __global__ void __launch_bounds__(128) attn_join_few_kernel(const AttnParams p) 
     if (t >= p.tokens) return;
     int own = 0;
     if (p.own_chunks > 0) {
-        const Sequence s = sequence(p, sequence_of(p.q_indptr, p.rows, t));
+        const Sequence s = sequence(p, sequence_of_warp(p.q_indptr, p.rows, t));
         if (t >= s.first && t < s.first + s.n) own = (s.len + p.own_chunk - 1) / p.own_chunk;
     }
     // lane 8 k + i: part i of head h0 + k
