@@ -339,6 +339,7 @@ __global__ void __launch_bounds__(32) attn_rows_kernel(const AttnParams p, const
                         }
                     }
             }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // a box will land where P is
         } else {
 #pragma unroll
             for (int dn = 0; dn < D / 16; ++dn) {
