@@ -371,7 +371,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const AttnParams p
             for (int j = 0; j < g.steps; ++j) {
                 const int fv = f + 2 * j + 1, fk = fv + 1;
                 const bool more = j + 1 < g.steps;
-                ok = full(fv) && (!more || full(fk));
+                ok = full(fv);
                 const uint32_t v = ring + fv % C::kStages * C::kBlock;
                 for (int i = 0; ok && i < g.ntiles; ++i) {
                     const int turn = (i ? done1 : done0) + j;
@@ -388,6 +388,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const AttnParams p
                     if (!ok) break;
                     commit(b_o + i * 8);
                     // S of the next step goes over P: the tensor core works in the order of issue
+                    if (more && i == 0 && !(ok = full(fk))) break;
                     if (more) qk(i, fk);
                 }
                 if (!ok) break;
