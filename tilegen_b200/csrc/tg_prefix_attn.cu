@@ -685,7 +685,8 @@ int make_plan(const tg_prefix_attention_args* a, Plan* plan, const char* op) {
 
     // The kernel for few rows reads the keys once for each 32 rows, the tcgen05 kernel once for
     // each 256 (it exists for heads of 64 and 128) but begins and ends for 10 us.  Own parts of 320
-    // keys, 48 sequences: 56 rows 58 against 64 us, 80 rows 79 against 74 us.
+    // keys, 48 sequences: 56 rows 58 against 64 us, 80 rows 79 against 74 us.  A prefix of 16384
+    // keys: 40 rows 60 against 39 us, 64 rows 64 against 37 us (one of 2000: 29 against 35).
     const int64_t rows_own = max_q * p.group, rows_all = a->tokens * p.group;
     const bool tc = c.dim == 64 || c.dim == 128;
     plan->rt_own = tc && rows_own > 64 ? 0 : rows_own > 16 && c.dim <= 128 ? 2 : 1;
@@ -707,13 +708,15 @@ int make_plan(const tg_prefix_attention_args* a, Plan* plan, const char* op) {
         }
     }
     if (max_seq > 0 || p.prefix_len == 0) {
-        // The kernel for few rows: two rounds of its warps, in chunks of 128 to 512 keys (or 64
-        // chunks, for sequences that may be long) so that long sequences do not end alone.  The
-        // tcgen05 kernel: two CTAs an SM.
+        // The kernel for few rows: two rounds of its warps, in chunks of 256 to 512 keys (or 64
+        // chunks, for sequences that may be long) so that long sequences do not end alone.  One
+        // sequence of 32768 keys: 34 us in chunks of 256, 38 in chunks of 128 (the join has 256
+        // parts); 64 sequences of 4096: 184 to 188 us for any bounds from 128 to 1024.  The tcgen05
+        // kernel: two pieces an SM.
         const int64_t units = std::max<int64_t>(1, t.rows * tiles_own * c.heads);
         if (plan->rt_own) {
             const int64_t even = ceil_div(ceil_div(max_seq, std::max<int64_t>(1, 2 * warps / units)), 16) * 16;
-            p.own_chunk = (int)std::min(std::max<int64_t>(128, even), std::max<int64_t>(512, ceil_div(max_seq, 64 * 16) * 16));
+            p.own_chunk = (int)std::min(std::max<int64_t>(256, even), std::max<int64_t>(512, ceil_div(max_seq, 64 * 16) * 16));
         } else {
             const int64_t n = std::max<int64_t>(1, 2 * kSMs / units);
             p.own_chunk = (int)std::max<int64_t>(256, ceil_div(ceil_div(max_seq, n), 128) * 128);
@@ -783,10 +786,13 @@ int attn_run(const Plan& plan, void* ws, cudaStream_t st) {
     }
     if (rc != TG_OK) return rc;
     if (p.direct) return TG_OK;
-    if (parts <= 8 && rows >= (size_t)kSMs * 128) {  // fewer rows do better with a warp each
+    // Four heads a warp, for many rows: 119,040 of 3 parts 38 us against 92 with a warp a row; 8192 of
+    // 5 parts do better with a warp each (167 against 174 us for the call).
+    if (parts <= 8 && rows >= (size_t)kSMs * 128) {
         const int64_t warps = p.tokens * ceil_div(p.q_heads, 4);
         return launch_pdl("attn_join_few_kernel", attn_join_few_kernel<T, D>, dim3((unsigned)ceil_div(warps, 4)), 128, 0, st, p);
     }
+    // 64 rows of 130 parts: 99 us for the call with 16 warps a row, 102 with 4.
     if (parts > 32 && rows < kSMs * 8)
         return launch_pdl("attn_join_kernel", attn_join_kernel<T, D, 16>, dim3((unsigned)rows), 512, 0, st, p);
     if (parts > 8 && rows < 4 * kSMs * 16)
