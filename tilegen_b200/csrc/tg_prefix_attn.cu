@@ -709,14 +709,16 @@ int make_plan(const tg_prefix_attention_args* a, Plan* plan, const char* op) {
     }
     if (max_seq > 0 || p.prefix_len == 0) {
         // The kernel for few rows: two rounds of its warps, in chunks of 256 to 512 keys (or 64
-        // chunks, for sequences that may be long) so that long sequences do not end alone.  One
+        // chunks, for sequences that may be long; 16 where sequences and heads alone make two rounds,
+        // as each chunk costs workspace) so that long sequences do not end alone.  One
         // sequence of 32768 keys: 34 us in chunks of 256, 38 in chunks of 128 (the join has 256
         // parts); 64 sequences of 4096: 184 to 188 us for any bounds from 128 to 1024.  The tcgen05
         // kernel: two pieces an SM.
         const int64_t units = std::max<int64_t>(1, t.rows * tiles_own * c.heads);
         if (plan->rt_own) {
             const int64_t even = ceil_div(ceil_div(max_seq, std::max<int64_t>(1, 2 * warps / units)), 16) * 16;
-            p.own_chunk = (int)std::min(std::max<int64_t>(256, even), std::max<int64_t>(512, ceil_div(max_seq, 64 * 16) * 16));
+            const int64_t most = units >= 2 * warps ? 16 : 64;
+            p.own_chunk = (int)std::min(std::max<int64_t>(256, even), std::max<int64_t>(512, ceil_div(max_seq, most * 16) * 16));
         } else {
             const int64_t n = std::max<int64_t>(1, 2 * kSMs / units);
             p.own_chunk = (int)std::max<int64_t>(256, ceil_div(ceil_div(max_seq, n), 128) * 128);
