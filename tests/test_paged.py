@@ -200,3 +200,25 @@ def test_cpu_tensors_are_refused():
         P.kv_append(kv, table, torch.zeros(0, dtype=torch.int64), x, x)
     with pytest.raises(ValueError, match="CUDA"):
         P.prefix_attention(x, kv, table, torch.zeros(0, dtype=torch.int64))
+
+
+def test_a_workspace_is_contiguous_and_on_the_calls_device():
+    """One byte expanded to many is no workspace: a kernel writes from its address on."""
+    from tilegen_b200 import device as D
+
+    cpu = torch.device("cpu")
+    ok = torch.empty(512, dtype=torch.uint8)
+    assert P._workspace(ok, 512, -1) == (ok.data_ptr(), 512)  # -1: the device number of a CPU tensor
+    assert D._ws(512, cpu, ok) == (ok.data_ptr(), 512)
+    for bad in (torch.empty(1, dtype=torch.uint8).expand(512), torch.empty(1024, dtype=torch.uint8)[::2],
+                torch.empty(32, 32, dtype=torch.uint8).t()[:, ::2]):
+        with pytest.raises(ValueError, match="contiguous"):
+            P._workspace(bad, 512, -1)
+        with pytest.raises(ValueError, match="contiguous"):
+            D._ws(512, cpu, bad)
+    with pytest.raises(ValueError, match="cuda:0"):
+        P._workspace(ok, 512, 0)
+    with pytest.raises(ValueError, match="cuda:0"):
+        D._ws(512, torch.device("cuda", 0), ok)
+    with pytest.raises(ValueError, match="small"):
+        P._workspace(ok, 513, -1)

@@ -116,6 +116,9 @@ def _check_vec(t: torch.Tensor, n: int, dtype: torch.dtype, device: torch.device
 
 def _ws(nbytes: int, device, workspace) -> Tuple[int, int]:
     if workspace is not None:
+        if workspace.device != device or not workspace.is_contiguous():
+            raise ValueError("the workspace must be a contiguous tensor on %s (got strides %s of shape %s on %s)"
+                             % (device, tuple(workspace.stride()), tuple(workspace.shape), workspace.device))
         if workspace.numel() * workspace.element_size() < nbytes:
             raise ValueError("workspace too small: need %d bytes" % nbytes)
         return workspace.data_ptr(), workspace.numel() * workspace.element_size()

@@ -382,6 +382,19 @@ def prefix_attention(q: torch.Tensor, cache: PagedKV, table: PageTable, seq_len:
     return _attention_launch(a, q, out, lse, workspace, index, sp)
 
 
+def _workspace(workspace: torch.Tensor, need: int, index: int) -> Tuple[int, int]:
+    """Address and bytes of a caller's workspace of at least `need` bytes."""
+    if workspace.get_device() != index:
+        raise ValueError("the workspace must be on cuda:%d (got %s)" % (index, workspace.device))
+    if not workspace.is_contiguous():  # its bytes would not be the ones from its address on
+        raise ValueError("the workspace must be contiguous (got strides %s of shape %s)"
+                         % (tuple(workspace.stride()), tuple(workspace.shape)))
+    size = workspace.numel() * workspace.element_size()
+    if size < need:
+        raise ValueError("workspace too small: need %d bytes" % need)
+    return workspace.data_ptr(), size
+
+
 def _attention_launch(a, q, out, lse, workspace, index, sp):
     if out is None:
         out = _like(q)
@@ -398,10 +411,6 @@ def _attention_launch(a, q, out, lse, workspace, index, sp):
         workspace, size = torch.empty(need, dtype=torch.uint8, device=q.device), need
         ws = workspace.data_ptr()
     elif workspace is not None:
-        if workspace.get_device() != index:
-            raise ValueError("the workspace must be on cuda:%d (got %s)" % (index, workspace.device))
-        ws, size = workspace.data_ptr(), workspace.numel() * workspace.element_size()
-        if size < need:
-            raise ValueError("workspace too small: need %d bytes" % need)
+        ws, size = _workspace(workspace, need, index)
     _lib.check(_call("tg_prefix_attention_" + _SUFFIX[q.dtype])(a, ws, size, sp), "tg_prefix_attention")
     return (out, lse) if isinstance(lse, torch.Tensor) else out
