@@ -468,6 +468,52 @@ def test_index_check():
         P.kv_append(b.cache, b.table, torch.tensor([0, 5], device="cuda"), k, k, q_indptr=good[3], check=True)
 
 
+def test_index_checks_of_several_threads_keep_apart():
+    """Checked calls of good and bad tables, paged and sparse, each from a thread and a stream of its
+    own: every bad one is refused and no good one.  (The bad matrix is bad by its column count alone,
+    and a page outside the cache reads as zeros, so a check that failed to tell would do no harm.)"""
+    import threading
+
+    from tilegen_b200 import codegen, device
+
+    b = Batch([1, 2], [5, 16], 20, 4, 2, 64, 16, BF16)
+    (q, cache, table, seq_len), named = b.args()
+    off = P.PageTable(table.indptr, torch.full_like(table.indices, cache.pages))
+    sched = codegen.generate("spmv", codegen.Config(bounds_check=True))
+    ip = torch.arange(0, 2 * 500 + 1, 2, device="cuda")
+    ix = torch.arange(1000, device="cuda") % 400
+    x = torch.ones(400, dtype=torch.float64, device="cuda")
+    good = device.DeviceCSR(ip, ix, torch.ones(1000, dtype=torch.float64, device="cuda"), (500, 400))
+    bad = device.DeviceCSR(ip, ix, good.data, (500, 399))
+    calls = [(True, lambda st: P.prefix_attention(q, cache, table, seq_len, check=True, stream=st, **named)),
+             (False, lambda st: P.prefix_attention(q, cache, off, seq_len, check=True, stream=st, **named)),
+             (True, lambda st: device.spmv(good, x, sched=sched, stream=st)),
+             (False, lambda st: device.spmv(bad, x[:399], sched=sched, stream=st))] * 2
+    wrong = []
+
+    def work(fine, call):
+        st = torch.cuda.Stream()
+        for _ in range(300):
+            try:
+                call(st)
+                refused = False
+            except lib.TgError as e:
+                refused = e.status == lib.TG_EBOUNDS
+                if not refused:
+                    wrong.append(str(e))
+            if refused == fine:
+                wrong.append("refused" if refused else "let pass")
+        st.synchronize()
+
+    torch.cuda.synchronize()
+    threads = [threading.Thread(target=work, args=c) for c in calls]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong, "%d of %d: %s" % (len(wrong), 300 * len(calls), sorted(set(wrong)))
+
+
 # ------------------------------------------------------------------ append
 @pytest.mark.parametrize("dtype", [BF16, F16, F32])
 @pytest.mark.parametrize("news,lens,page,dim,rot,layout,heads_first", [

@@ -98,8 +98,10 @@ tg_sched g_sched = {32, 1, 1, 1, 128, TG_SPLIT_ROWWISE, 0, 0u};
 struct DeviceScratch {
     void* ws = nullptr;  // workspace cache of the launch_* launchers (grow-only)
     size_t ws_bytes = 0;
-    uint32_t* err = nullptr;  // bounds-check word
+    uint32_t* words = nullptr;  // kCheckWords words that index checks report into
+    uint64_t words_taken = 0;   // by checks under way, a bit each
 };
+constexpr int kCheckWords = 64;
 std::vector<DeviceScratch> g_dev;
 
 DeviceScratch* device_scratch() {
@@ -111,17 +113,35 @@ DeviceScratch* device_scratch() {
 
 }  // namespace
 
-// The current device's bounds-check word, allocated at its first use.
-int bounds_word(uint32_t** err) {
+// One word of the current device for one check, so that checks of other threads and streams neither
+// clear nor raise it.  No lock is held while the check waits for its stream, which may itself wait
+// for work that another thread has yet to submit.  More checks at once than words: one of its own.
+int CheckWord::take() {
     std::lock_guard<std::mutex> lk(g_mu);
     DeviceScratch* d = device_scratch();
     if (!d) return set_error(TG_ECUDA, "cudaGetDevice failed");
-    if (!d->err) {
-        int rc = check_cuda(cudaMalloc(&d->err, sizeof(uint32_t)), "cudaMalloc(bounds word)");
+    if (!d->words) {
+        const int rc = check_cuda(cudaMalloc(&d->words, kCheckWords * sizeof(uint32_t)), "cudaMalloc(check words)");
         if (rc != TG_OK) return rc;
     }
-    *err = d->err;
-    return TG_OK;
+    for (int i = 0; i < kCheckWords; ++i)
+        if (!(d->words_taken >> i & 1)) {
+            d->words_taken |= 1ull << i;
+            dev_ = (int)(d - g_dev.data());
+            slot_ = i;
+            at = d->words + i;
+            return TG_OK;
+        }
+    return check_cuda(cudaMalloc(&at, sizeof(uint32_t)), "cudaMalloc(check word)");
+}
+
+CheckWord::~CheckWord() {
+    if (slot_ >= 0) {
+        std::lock_guard<std::mutex> lk(g_mu);
+        g_dev[dev_].words_taken &= ~(1ull << slot_);
+    } else if (at) {
+        cudaFree(at);
+    }
 }
 
 // Fills *out from `in` (NULL: the process schedule of tg_set_schedule) with every zero
@@ -181,9 +201,10 @@ int check_csr(const tg_csr* A, const char* op) {
 
 // Bounds-checked calls validate the CSR structure first and are synchronous on `st`.
 int bounds_check(const tg_csr& A, cudaStream_t st) {
-    uint32_t* err = nullptr;
-    int rc = bounds_word(&err);
+    CheckWord word;
+    int rc = word.take();
     if (rc != TG_OK) return rc;
+    uint32_t* const err = word.at;
     rc = check_cuda(cudaMemsetAsync(err, 0, sizeof(uint32_t), st), "cudaMemsetAsync");
     if (rc != TG_OK) return rc;
     int64_t blocks = std::min<int64_t>(ceil_div(std::max(A.rows, A.nnz) + 1, 256), 148 * 16);

@@ -20,6 +20,20 @@ namespace tg {
 // ------------------------------------------------------------------ host errors
 int set_error(int status, const char* fmt, ...);
 int check_cuda(cudaError_t e, const char* what);
+
+// A device word that an index check reports into, the check's own while this lives (tg_abi.cu).
+class CheckWord {
+public:
+    CheckWord() = default;
+    CheckWord(const CheckWord&) = delete;
+    CheckWord& operator=(const CheckWord&) = delete;
+    ~CheckWord();
+    int take();
+    uint32_t* at = nullptr;
+
+private:
+    int dev_ = 0, slot_ = -1;
+};
 int check_launch(const char* what);
 
 constexpr int kWarp = 32;

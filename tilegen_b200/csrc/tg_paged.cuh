@@ -106,9 +106,6 @@ int check_rope(const tg_rope* r, int32_t dim, const char* op);
 int paged_bounds_check(const tg_csr& t, int64_t page_size, const int64_t* seq_len, int64_t max_seq_len, int64_t tokens,
                        const int64_t* q_indptr, int64_t max_q_len, const int64_t* prefix_pages, int64_t n_prefix,
                        bool append, const char* op, cudaStream_t st);
-// The device word that bounds checks report into (tg_abi.cu).
-int bounds_word(uint32_t** err);
-
 // Raises a kernel's limit of dynamic shared memory, once on each device.
 struct SmemOnce {
     std::atomic<uint64_t> done{0};  // devices, by bit

@@ -84,9 +84,10 @@ int paged_bounds_check(const tg_csr& t, int64_t page_size, const int64_t* seq_le
                        const int64_t* q_indptr, int64_t max_q_len, const int64_t* prefix_pages, int64_t n_prefix,
                        bool append, const char* op, cudaStream_t st) {
     if (t.rows == 0) return TG_OK;
-    uint32_t* err = nullptr;
-    int rc = bounds_word(&err);
+    CheckWord word;
+    int rc = word.take();
     if (rc != TG_OK) return rc;
+    uint32_t* const err = word.at;
     rc = check_cuda(cudaMemsetAsync(err, 0, sizeof(uint32_t), st), "cudaMemsetAsync");
     if (rc != TG_OK) return rc;
     const int64_t blocks = std::min<int64_t>(ceil_div(std::max({t.rows, t.nnz, n_prefix}) + 1, 256), kSMs * 16);
