@@ -108,9 +108,10 @@ TG_API int tg_kv_append_bf16(const tg_kv_append_args* a, tg_stream_t stream);
  * keys, without it all; a query that sees none gives zeros.  What lies in the cache beyond
  * what a query sees (NaN and infinities included) has no effect on it.  lse, where not
  * NULL, receives log(sum(exp(scale * q k^T))) of each (token, head), -inf where nothing is
- * seen.  max_seq_len and max_q_len bound the entries of seq_len and the tokens of one
- * sequence; longer ones are cut to them.  Dim 64, 96, 128 or 256; all strides multiples of
- * 8 elements and all rows 16-byte aligned. */
+ * seen.  max_seq_len bounds the entries of seq_len; a longer one counts as max_seq_len.
+ * max_q_len (not 0) bounds the tokens of one sequence: the first max_q_len see what they see
+ * without the bound, those after them, and tokens that no sequence holds, see nothing.  Dim 64,
+ * 96, 128 or 256; all strides multiples of 8 elements and all rows 16-byte aligned. */
 typedef struct tg_prefix_attention_args {
     const tg_paged_kv* cache;
     const tg_csr* pages;

@@ -514,6 +514,51 @@ def test_index_checks_of_several_threads_keep_apart():
     assert not wrong, "%d of %d: %s" % (len(wrong), 300 * len(calls), sorted(set(wrong)))
 
 
+@pytest.mark.parametrize("prefix", [0, 90])
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("dim,heads,news,lens,max_q", [
+    (64, 8, [3, 1, 2], [20, 9, 2], 2),          # the kernel for few rows, one part without a prefix
+    (96, 4, [40, 7], [300, 7], 12),             # several chunks of own keys
+    (128, 16, [150, 40], [150, 210], 70),       # the tcgen05 kernel, one part without a prefix
+    (64, 16, [200, 3, 0, 90], [700, 3, 5, 90], 128),
+])
+def test_more_tokens_than_max_q_len(dim, heads, news, lens, max_q, causal, prefix):
+    """The first max_q_len tokens of a sequence see what they see without the bound; the others,
+    and tokens that no sequence holds, see nothing: zeros, and -inf in lse."""
+    b = Batch(news, lens, prefix, heads, 2, dim, 16, BF16, seed=7)
+    whole, whole_lse = b.run(lse=True, causal=causal)
+    b.check(whole, whole_lse, causal=causal)
+    head, tail = 3, 5  # tokens before the first sequence and after the last one
+    q = torch.cat((normal(gen(1), head, heads, dim, dtype=BF16), b.q, normal(gen(2), tail, heads, dim, dtype=BF16)))
+    indptr = b.q_indptr + head
+    out = torch.full_like(q, math.nan)
+    lse = torch.full(q.shape[:2], math.nan, device="cuda")
+    P.prefix_attention(q, b.cache, b.table, b.seq_len, prefix_pages=b.prefix_pages, prefix_len=prefix, q_indptr=indptr,
+                       max_q_len=max_q, causal=causal, out=out, lse=lse)
+    held = torch.zeros(q.shape[0], dtype=torch.bool, device="cuda")
+    for first, n in zip(indptr[:-1].tolist(), news):
+        held[first:first + min(n, max_q)] = True
+    inside = held[head:head + sum(news)]
+    got = torch.where(inside[:, None, None], out[head:head + sum(news)], whole)
+    b.check(got, torch.where(inside[:, None], lse[head:head + sum(news)], whole_lse), causal=causal)
+    assert bool((out[~held] == 0).all()) and bool((lse[~held] == -math.inf).all())
+
+
+@pytest.mark.parametrize("dim,n,max_q", [(64, 3, 4), (128, 150, 160), (256, 3, 4)])
+@pytest.mark.parametrize("own", [True, False])
+def test_tokens_past_the_last_sequence(dim, n, max_q, own):
+    """A padded batch, with a prefix alone and with own pages alone."""
+    b = Batch([n, 2], [n, 2] if own else [0, 0], 0 if own else 40, 8, 2, dim, 16, F16, seed=3)
+    pad = 700
+    q = torch.cat((b.q, normal(gen(1), pad, 8, dim, dtype=F16)))
+    for causal in (True, False):
+        out, lse = torch.full_like(q, math.nan), torch.full(q.shape[:2], math.nan, device="cuda")
+        P.prefix_attention(q, b.cache, b.table, b.seq_len, prefix_pages=b.prefix_pages, prefix_len=b.prefix,
+                           q_indptr=b.q_indptr, max_q_len=max_q, max_seq_len=max(b.lens), causal=causal, out=out, lse=lse)
+        b.check(out[:n + 2], lse[:n + 2], causal=causal)
+        assert bool((out[n + 2:] == 0).all()) and bool((lse[n + 2:] == -math.inf).all())
+
+
 # ------------------------------------------------------------------ append
 @pytest.mark.parametrize("dtype", [BF16, F16, F32])
 @pytest.mark.parametrize("news,lens,page,dim,rot,layout,heads_first", [

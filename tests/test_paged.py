@@ -222,3 +222,9 @@ def test_a_workspace_is_contiguous_and_on_the_calls_device():
         D._ws(512, torch.device("cuda", 0), ok)
     with pytest.raises(ValueError, match="small"):
         P._workspace(ok, 513, -1)
+
+
+def test_attention_refuses_a_max_q_len_of_zero():
+    _refused(lib.TG_EINVAL, _attention(q_indptr=4096, max_q_len=0), "max_q_len")
+    empty = _attention(q_indptr=4096, max_q_len=0, tokens=0)
+    assert lib.load().tg_prefix_attention_bf16(empty, None, 0, None) == lib.TG_OK

@@ -59,7 +59,7 @@ struct RowCfg {
     static_assert(RT * 16 * kStepKeys * 4 <= kHalves * kBox, "a step's P fits its K tile");
 };
 
-template <typename T, int D, int RT>
+template <typename T, int D, int RT, bool FILL>
 __global__ void __launch_bounds__(32) attn_rows_kernel(const AttnParams p, const int box,
                                                        const __grid_constant__ CUtensorMap kmap,
                                                        const __grid_constant__ CUtensorMap vmap) {
@@ -73,10 +73,13 @@ __global__ void __launch_bounds__(32) attn_rows_kernel(const AttnParams p, const
     pdl_trigger();
     // The grids of a call complete in order: this one (the second) ends after the first.
     struct AtEnd {
+        const AttnParams& p;
         __device__ ~AtEnd() {
+            if constexpr (FILL)
+                fill_unanswered<T, D>(p, (int64_t)blockIdx.y * gridDim.x + blockIdx.x, (int64_t)gridDim.y * gridDim.x);
             if (blockIdx.x == 0 && blockIdx.y == 0) pdl_wait();
         }
-    } at_end;
+    } at_end{p};
 
     // ---- which rows, which keys
     const int h = blockIdx.y;
@@ -88,7 +91,7 @@ __global__ void __launch_bounds__(32) attn_rows_kernel(const AttnParams p, const
         part = blockIdx.x % p.prefix_splits;
         tile = blockIdx.x / p.prefix_splits;
         s.first = 0;
-        s.n = p.tokens;
+        s.n = s.asked = p.tokens;
         list = p.prefix_pages;
         keys = p.prefix_len;
         k0 = part * p.prefix_chunk;
@@ -104,7 +107,7 @@ __global__ void __launch_bounds__(32) attn_rows_kernel(const AttnParams p, const
         part = p.prefix_splits + c;
         if (k0 >= keys && !p.direct) return;  // no such chunk: the join does not ask for it
     }
-    const int row0 = tile * RT * 16, nrows = min(s.n * p.group - row0, RT * 16);
+    const int row0 = tile * RT * 16, nrows = min(s.asked * p.group - row0, RT * 16);
     if (nrows <= 0) return;
     if (!over_prefix)  // no row sees more than the last one
         k1 = min(k1, keys_seen(p, s, (row0 + nrows - 1) / p.group, keys, keys));
@@ -192,11 +195,10 @@ __global__ void __launch_bounds__(32) attn_rows_kernel(const AttnParams p, const
                 const int i = (row0 + r) / p.group;
                 if (!over_prefix) {
                     seen[rt][e] = keys_seen(p, s, i, keys, keys);
-                } else if (!p.causal) {
+                } else if (!p.causal && !p.q_indptr) {
                     seen[rt][e] = keys;
                 } else {
-                    const Sequence o = sequence(p, sequence_of(p.q_indptr, p.rows, i));
-                    seen[rt][e] = keys_seen(p, o, i - o.first, (int64_t)keys + o.len, keys);
+                    seen[rt][e] = prefix_seen(p, sequence(p, sequence_of(p.q_indptr, p.rows, i)), i, keys);
                 }
             }
         }
@@ -412,7 +414,7 @@ __global__ void __launch_bounds__(WPR == 16 ? 512 : 128) attn_join_kernel(const 
     n = np;
     if (p.own_chunks > 0) {
         const Sequence s = sequence(p, sequence_of_warp(p.q_indptr, p.rows, t));
-        if (t >= s.first && t < s.first + s.n) n += (s.len + p.own_chunk - 1) / p.own_chunk;
+        if (t >= s.first && t < s.first + s.asked) n += (s.len + p.own_chunk - 1) / p.own_chunk;
     }
     // lane l holds the maximum and sum of the l-th of 32 of the warp's parts at a time
     auto part = [&](int i) { return (i < np ? i : i - np + p.prefix_splits) * all + row; };
@@ -514,7 +516,7 @@ __global__ void __launch_bounds__(128) attn_join_few_kernel(const AttnParams p) 
     int own = 0;
     if (p.own_chunks > 0) {
         const Sequence s = sequence(p, sequence_of_warp(p.q_indptr, p.rows, t));
-        if (t >= s.first && t < s.first + s.n) own = (s.len + p.own_chunk - 1) / p.own_chunk;
+        if (t >= s.first && t < s.first + s.asked) own = (s.len + p.own_chunk - 1) / p.own_chunk;
     }
     // lane 8 k + i: part i of head h0 + k
     const int h = min(h0 + lane / kParts, p.q_heads - 1), i = lane % kParts;
@@ -654,6 +656,8 @@ int make_plan(const tg_prefix_attention_args* a, Plan* plan, const char* op) {
                          (long long)a->prefix_len, (long long)a->n_prefix_pages, (long long)c.page_size);
     if (a->max_seq_len < 0 || a->max_q_len < 0)
         return set_error(TG_EINVAL, "%s: negative max_seq_len or max_q_len", op);
+    if (a->q_indptr && a->tokens > 0 && a->max_q_len == 0)
+        return set_error(TG_EINVAL, "%s: a max_q_len of 0 answers none of the %lld tokens", op, (long long)a->tokens);
     if (!(a->scale > 0.0) || a->scale > 1e30) return set_error(TG_EINVAL, "%s: scale must be positive", op);
     if (a->flags & ~(TG_FLAG_CAUSAL | TG_FLAG_BOUNDS_CHECK))
         return set_error(TG_EINVAL, "%s: unknown flags 0x%x", op, a->flags);
@@ -733,6 +737,7 @@ int make_plan(const tg_prefix_attention_args* a, Plan* plan, const char* op) {
     p.own_pieces = (int)(plan->own_units * c.heads);
     const int parts = p.prefix_splits + p.own_chunks;
     p.direct = parts == 1;
+    p.fill = p.direct && p.q_indptr && p.prefix_len == 0;
     const size_t rows = (size_t)a->tokens * a->q_heads;
     const size_t o_bytes = (parts * rows * c.dim * sizeof(float) + 255) / 256 * 256;
     plan->ws_bytes = p.direct || rows == 0 ? 0 : o_bytes + (parts * rows * sizeof(float2) + 255) / 256 * 256;
@@ -742,7 +747,7 @@ int make_plan(const tg_prefix_attention_args* a, Plan* plan, const char* op) {
 template <typename T, int D, int RT>
 int rows_launch(const AttnParams& p, int64_t units, bool pdl, cudaStream_t st) {
     using C = RowCfg<D, RT>;
-    auto kernel = attn_rows_kernel<T, D, RT>;
+    auto kernel = p.fill ? attn_rows_kernel<T, D, RT, true> : attn_rows_kernel<T, D, RT, false>;
     const int box = std::gcd(p.page_size, kStepKeys);
     CUtensorMap kmap, vmap;
     int rc = cache_maps(p, std::is_same<T, __half>::value, D, box, &kmap, &vmap);

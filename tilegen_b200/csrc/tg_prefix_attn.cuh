@@ -37,15 +37,17 @@ struct AttnParams {
     int tiles;                        // row tiles of a sequence (own) or of all rows (prefix)
     int over_prefix;                  // the tcgen05 kernel: the prefix, else the sequences' own pages
     int prefix_units;                 // the kernel for few rows: its first blocks go over the prefix
+    int fill;                         // the only part, of own pages, tokens by q_indptr: fill_unanswered
     int direct;                       // the only part: rows are finished here
     float* part_o;                    // [part][token][head][dim]
     float2* part_ml;                  // [part][token][head]: m, l
 };
 
-// One sequence as the kernels see it: its tokens, its own pages and length.
+// One sequence as the kernels see it: its tokens, how many of them are answered (the first max_q),
+// its own pages and length.
 struct Sequence {
     int64_t page0;
-    int first, n, len;
+    int first, n, asked, len;
 };
 
 __device__ __forceinline__ Sequence sequence(const AttnParams& p, int64_t b) {
@@ -54,7 +56,8 @@ __device__ __forceinline__ Sequence sequence(const AttnParams& p, int64_t b) {
     tokens_of(p.q_indptr, p.tokens, b, first, n);
     pages_of(p.indptr, p.nnz, b, s.page0, npages);
     s.first = (int)first;
-    s.n = (int)min(n, (int64_t)p.max_q);
+    s.n = (int)n;
+    s.asked = min(s.n, p.max_q);
     const int64_t len = min(min(p.seq_len[b], npages * p.page_size), (int64_t)p.max_seq);
     s.len = (int)max(len, (int64_t)0);
     return s;
@@ -64,6 +67,39 @@ __device__ __forceinline__ Sequence sequence(const AttnParams& p, int64_t b) {
 __device__ __forceinline__ int keys_seen(const AttnParams& p, const Sequence& s, int i, int64_t total, int whole) {
     if (!p.causal) return whole;
     return (int)min(max(total - s.n + i + 1, (int64_t)0), (int64_t)whole);
+}
+
+// Keys of the prefix (`whole` keys) that token t of sequence s sees: none where s does not answer it.
+__device__ __forceinline__ int prefix_seen(const AttnParams& p, const Sequence& s, int t, int whole) {
+    const int i = t - s.first;
+    return i < 0 || i >= s.asked ? 0 : keys_seen(p, s, i, (int64_t)whole + s.len, whole);
+}
+
+// A call without a join: the rows of tokens that no sequence answers (past its first max_q, before
+// the first sequence or after the last one) are no CTA's of the kernel over the own pages, so warp
+// `warp` of `warps` writes its share of them at its end, zeros and -inf: one sequence after the
+// other, and all warps share the tokens of none.  Instances of their own have it: calls with a join
+// took 53 us for 50 and 60 for 55 with this code in the kernel, run or not, and a launch of its own
+// costs small calls 2 to 4 of 21 to 24 us.
+template <typename T, int D>
+__device__ __forceinline__ void fill_unanswered(const AttnParams& p, int64_t warp, int64_t warps) {
+    const int lane = threadIdx.x & 31;
+    auto fill = [&](int64_t t0, int64_t t1, int64_t mine, int64_t all) {
+        for (int64_t t = t0 + mine; t < t1; t += all)
+            for (int h = 0; h < p.q_heads; ++h) {
+                if (lane < D / 8)
+                    *reinterpret_cast<uint4*>(static_cast<T*>(p.out) + t * p.o_tok + h * p.o_head + lane * 8) = make_uint4(0, 0, 0, 0);
+                if (p.lse && lane == 0) p.lse[t * p.q_heads + h] = -INFINITY;
+            }
+    };
+    const int64_t all = p.tokens, begin = min(max(p.q_indptr[0], (int64_t)0), all), end = max(min(p.q_indptr[p.rows], all), begin);
+    fill(0, begin, warp, warps);
+    fill(end, all, warp, warps);
+    for (int64_t b = warp; b < p.rows; b += warps) {
+        int64_t first, n;
+        tokens_of(p.q_indptr, p.tokens, b, first, n);
+        if (n > p.max_q) fill(first + p.max_q, first + n, 0, 1);
+    }
 }
 
 // The first step of part i of n near-even shares of `all` steps (the first all % n have one more),

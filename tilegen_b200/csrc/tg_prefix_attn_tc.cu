@@ -253,7 +253,7 @@ struct Segments {
                 g.row0 = (u - g.h * p.tiles) * 2 * kTile;
                 g.part = blockIdx.x - prefix_cta(p, u * p.prefix_steps);
                 g.s.first = 0;
-                g.s.n = p.tokens;
+                g.s.n = g.s.asked = p.tokens;
                 g.nrows = min(p.tokens * p.group - g.row0, 2 * kTile);
                 g.list = p.prefix_pages;
                 g.keys = p.prefix_len;
@@ -268,7 +268,7 @@ struct Segments {
                 const int b = x % p.rows;
                 g.row0 = (p.tiles - 1 - x / p.rows) * 2 * kTile;
                 g.s = sequence(p, b);
-                g.nrows = min(g.s.n * p.group - g.row0, 2 * kTile);
+                g.nrows = min(g.s.asked * p.group - g.row0, 2 * kTile);
                 g.list = p.indices + g.s.page0;
                 g.keys = g.s.len;
                 g.k0 = c * p.own_chunk;
@@ -285,7 +285,7 @@ struct Segments {
     }
 };
 
-template <typename T, int D>
+template <typename T, int D, bool FILL>
 __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const AttnParams p, const int box,
                                                               const __grid_constant__ CUtensorMap kmap,
                                                               const __grid_constant__ CUtensorMap vmap) {
@@ -295,13 +295,19 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const AttnParams p
     TcShared& sh = *reinterpret_cast<TcShared*>(smem + (2 + C::kStages) * C::kBlock);
     const int tid = threadIdx.x, warp = __shfl_sync(kFull, tid >> 5, 0), lane = tid & 31;
     pdl_trigger();
+    struct AtEnd {
+        const AttnParams& p;
+        __device__ ~AtEnd() {
+            if constexpr (FILL)
+                fill_unanswered<T, D>(p, blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5), gridDim.x * (kThreads / 32));
+            // grids of a call complete in order: this one, if it is the second, ends after the first
+            if (blockIdx.x == 0) pdl_wait();
+        }
+    } at_end{p};
     if (!p.over_prefix) {
         Segments some(p);
         Segment g;
-        if (!some.next(p, g)) {
-            if (blockIdx.x == 0) pdl_wait();
-            return;
-        }
+        if (!some.next(p, g)) return;
     }
 
     const uint32_t sq = smem_addr(smem), ring = sq + 2 * C::kBlock;
@@ -476,7 +482,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const AttnParams p
 #pragma unroll 1
             for (int r0 = lane; r0 < 2 * kTile; r0 += 4 * 32) {
                 int seen[4];
-                if (p.over_prefix && p.causal) {
+                if (p.over_prefix && (p.causal || p.q_indptr)) {
                     int t[4], lo[4];
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
@@ -491,10 +497,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const AttnParams p
                                 if (lo[i] + step < p.rows && p.q_indptr[lo[i] + step] <= t[i]) lo[i] += step;
                     }
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const Sequence o = sequence(p, lo[i]);
-                        seen[i] = keys_seen(p, o, t[i] - o.first, (int64_t)g.keys + o.len, g.keys);
-                    }
+                    for (int i = 0; i < 4; ++i) seen[i] = prefix_seen(p, sequence(p, lo[i]), t[i], g.keys);
                 } else {
 #pragma unroll
                     for (int i = 0; i < 4; ++i)
@@ -715,8 +718,6 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const AttnParams p
         fence_after();
         tmem_free(tmem, kCols);
     }
-    // grids of a call complete in order: this one, if it is the second, ends after the first
-    if (blockIdx.x == 0) pdl_wait();
 }
 
 // ------------------------------------------------------------------ host
@@ -727,10 +728,10 @@ int tc_launch(const AttnParams& p, int ctas, bool pdl, cudaStream_t st) {
     const int box = std::gcd(p.page_size, kTile);
     CUtensorMap kmap, vmap;
     int rc = cache_maps(p, std::is_same<T, __half>::value, D, box, &kmap, &vmap);
-    auto kernel = attn_tc_kernel<T, D>;
-    static SmemOnce once;
+    auto kernel = p.fill ? attn_tc_kernel<T, D, true> : attn_tc_kernel<T, D, false>;
+    static SmemOnce once[2];
     if (rc == TG_OK)
-        rc = once.raise(reinterpret_cast<const void*>(kernel), C::kSmem);
+        rc = once[p.fill].raise(reinterpret_cast<const void*>(kernel), C::kSmem);
     if (rc != TG_OK) return rc;
     const dim3 grid((unsigned)ctas);
     if (pdl) return launch_pdl("attn_tc_kernel", kernel, grid, kThreads, C::kSmem, st, p, box, kmap, vmap);

@@ -365,8 +365,10 @@ def prefix_attention(q: torch.Tensor, cache: PagedKV, table: PageTable, seq_len:
 
     Queries are given as for kv_append: q_indptr, or one for each sequence.  With ``causal`` the
     last query of a sequence sees all its keys, the one before it one key less, and so on; a
-    query that sees nothing gives zeros.  max_q_len and max_seq_len bound the tokens and the own
-    length of a sequence (defaults: what the arrays' sizes allow; tighter bounds plan better).
+    query that sees nothing gives zeros, and so does one that no sequence holds.  max_q_len and
+    max_seq_len bound the tokens and the own length of a sequence (defaults: what the arrays' sizes
+    allow; tighter bounds plan better): tokens past the first max_q_len see nothing, a longer
+    sequence counts as max_seq_len.
     scale defaults to dim ** -0.5.  ``lse=True`` (or a float32 [tokens, q_heads] tensor) returns
     (out, log of the softmax's sum).  ``workspace`` (prefix_attention_workspace_bytes) is
     allocated on the call's stream where it is not given; ``check`` checks the index arrays
