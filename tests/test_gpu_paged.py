@@ -559,6 +559,44 @@ def test_tokens_past_the_last_sequence(dim, n, max_q, own):
         assert bool((out[n + 2:] == 0).all()) and bool((lse[n + 2:] == -math.inf).all())
 
 
+@pytest.mark.parametrize("many", [False, True])
+@pytest.mark.parametrize("dtype", [F16, BF16])
+def test_many_small_weights_beside_a_large_one(dtype, many):
+    """One key takes nearly all of the softmax, and all others 2^-26 of it each: together, they are
+    what the output is made of (their values are 8, the large key's are 0).  A weight rounded to
+    float16 beside a largest weight of 1 would be lost, being below half of the type's smallest
+    number.  The kernels keep the largest weight of a part at 2^7 or above in float16, so that what
+    rounding to a multiple of 2^-24 may cost is keys * 2^-32 of the largest value."""
+    heads, dim, page = 64, 64, 256
+    gap = 26 * math.log(2.0)
+    if many:  # one CTA a pair of head and row tile goes over all of the prefix
+        rows, prefix, own = 300, 65536, 0
+    else:     # as many (sequence, head) pairs as fill the GPU: few and long chunks of own keys
+        rows, prefix, own = 40, 0, 65536
+    pages = 65536 // page
+    k = torch.zeros(pages, page, heads, dim, dtype=dtype, device="cuda")
+    v = torch.full_like(k, 8.0)
+    k[0, 0, :, 0] = 16.0
+    v[0, 0] = 0.0
+    q = torch.zeros(rows, heads, dim, dtype=dtype, device="cuda")
+    q[..., 0] = 16.0
+    ids = torch.arange(pages, device="cuda")
+    if many:
+        table = P.PageTable(torch.zeros(rows + 1, dtype=torch.int64, device="cuda"), ids[:0])
+        named = dict(prefix_pages=ids, prefix_len=prefix)
+    else:     # all sequences list the same pages
+        table = P.PageTable(torch.arange(rows + 1, device="cuda") * pages, ids.repeat(rows))
+        named = dict(max_seq_len=own)
+    seq_len = torch.full((rows,), own, device="cuda")
+    out, lse = P.prefix_attention(q, P.PagedKV(k, v), table, seq_len, scale=gap / 256, lse=True, **named)
+    w = 65535 * 2.0 ** -26
+    ref = 8 * w / (1 + w)
+    u, e = U[dtype], 2.0 ** -18 * (1 + gap)
+    tol = u * ref + (u + 4 * e) * ref + (2.0 ** -25 + 65536 * 2.0 ** -32 * 8 if dtype == F16 else 0)
+    assert float((out.double() - ref).abs().max()) <= tol
+    assert float((lse.double() - (gap + math.log1p(w))).abs().max()) <= 4 * e
+
+
 # ------------------------------------------------------------------ append
 @pytest.mark.parametrize("dtype", [BF16, F16, F32])
 @pytest.mark.parametrize("news,lens,page,dim,rot,layout,heads_first", [

@@ -279,7 +279,7 @@ __global__ void __launch_bounds__(32) attn_rows_kernel(const AttnParams p, const
                     }
                 mx = fmaxf(mx, __shfl_xor_sync(kFull, mx, 1));
                 mx = fmaxf(mx, __shfl_xor_sync(kFull, mx, 2));
-                const float mn = fmaxf(m[rt][e], mx), base = mn == -INFINITY ? 0.f : mn;
+                const float mn = fmaxf(m[rt][e], reference<T, 15>(mx)), base = mn == -INFINITY ? 0.f : mn;
                 const float keep = exp2_fast(m[rt][e] - base);
                 m[rt][e] = mn;
                 float sum = 0.f;
@@ -300,7 +300,8 @@ __global__ void __launch_bounds__(32) attn_rows_kernel(const AttnParams p, const
                     }
                 }
                 // P is rounded to the values' type for the product, as the output is: relative
-                // errors of half an ulp that average out over the keys.  l sums the unrounded P.
+                // errors of half an ulp that average out over the keys (in float16, weights below
+                // 2^-40 of a part's largest are lost).  l sums the unrounded P.
                 pf[rt][e] = pack2<T>(sc[rt][0][2 * e], sc[rt][0][2 * e + 1]);
                 pf[rt][2 + e] = pack2<T>(sc[rt][1][2 * e], sc[rt][1][2 * e + 1]);
             }

@@ -144,6 +144,15 @@ __device__ __forceinline__ float exp2_fast(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
+// The value that P is taken relative to, for a row's maximum `top`.  float16 has no number below
+// 2^-24: beside a largest weight of 1, thousands of weights of 2^-26 would all round to nothing.
+// LIFT (15 or less) puts the largest weight at 2^LIFT instead.  Maxima of 2^20 and above, where top -
+// LIFT would be rounded, stay as they are.
+template <typename T, int LIFT>
+__device__ __forceinline__ float reference(float top) {
+    if constexpr (std::is_same<T, __half>::value) return fabsf(top) < 1048576.f ? top - (float)LIFT : top;
+    else return top;
+}
 // Whether one of the eight 16-bit numbers in v is an infinity or NaN.
 template <typename T>
 __device__ __forceinline__ bool any_nonfinite(uint4 v) {

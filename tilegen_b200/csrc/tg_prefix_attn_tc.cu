@@ -22,8 +22,10 @@
 // unit 48 %, issue slots 48 %.
 //
 // O is rescaled only where a row's maximum has grown by more than 2^8 since the value that P is
-// taken relative to: P stays below 2^8, far inside the range of either type and of the 32-bit
-// sums, and the relative precision of P is that of any other reference.
+// taken relative to: P stays below 2^8 (2^15 in float16, where the largest weight is at least 2^7, so
+// that small weights keep their bits: what they may lose is keys * 2^-32 of the largest value),
+// inside the range of either type and of the 32-bit sums, and the relative precision of P is that of
+// any other reference.
 #include <numeric>
 
 #include "tg_prefix_attn.cuh"
@@ -137,7 +139,8 @@ constexpr int kTile = 128;   // rows of a tile, keys of a step
 constexpr int kThreads = 384;
 constexpr uint32_t kCols = 512;
 constexpr uint32_t kColO = 256;
-constexpr float kGrow = 8.f;  // log2 of how far the maximum may pass the value that P is taken relative to
+constexpr float kGrow = 8.f;  // log2 of how far the maximum may grow before P is taken relative to a new one
+constexpr int kLift = 7;      // float16: log2 of the largest P at first
 constexpr int kFirst = 64;  // columns of P that are multiplied while the others are made
 
 template <int D>
@@ -583,10 +586,11 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const AttnParams p
                         a3 = max3(a3, __uint_as_float(x[c + 6]), __uint_as_float(x[c + 7]));
                     }
                     const float top = max3(max3(a0, a1, a2), a3, a3) * p.scale_log2;
-                    const bool grow = top > m + kGrow || (m == -INFINITY && top > m);
+                    const float ref = reference<T, kLift>(top);
+                    const bool grow = ref > m + kGrow || (m == -INFINITY && ref > m);
                     if (__any_sync(kFull, grow)) {
-                        const float keep = grow ? exp2_fast(m - top) : 1.f;
-                        if (grow) m = top;
+                        const float keep = grow ? exp2_fast(m - ref) : 1.f;
+                        if (grow) m = ref;
                         l *= keep;
                         if (j > 0) {
                             if (!(ok = wait_warp(b_o + my * 8, (done + j - 1) & 1, fail))) break;
