@@ -228,3 +228,17 @@ def test_attention_refuses_a_max_q_len_of_zero():
     _refused(lib.TG_EINVAL, _attention(q_indptr=4096, max_q_len=0), "max_q_len")
     empty = _attention(q_indptr=4096, max_q_len=0, tokens=0)
     assert lib.load().tg_prefix_attention_bf16(empty, None, 0, None) == lib.TG_OK
+
+
+@pytest.mark.parametrize("rows,tokens,heads,kv_heads,dim,seq,listed", [
+    (1, 32768, 32, 8, 256, 32768, 32768),            # a long prompt
+    (1, 16384, 32, 8, 96, 16384, 16384),
+    (1024, 16384, 32, 8, 128, 8192, 1024 * 8192),    # 16 tokens for each of many sequences
+    (256, 2048, 32, 8, 128, 65536, 65536 + 255 * 512),  # one long sequence among short ones
+    (1024, 16384, 32, 8, 64, 65536, 65536 + 1023 * 512),
+])
+def test_attention_workspace_stays_small(rows, tokens, heads, kv_heads, dim, seq, listed):
+    """Own parts take 1 GiB at most, or one part of each row, whatever the sizes."""
+    a = _attention(cache=_cache(pages=1 << 20, heads=kv_heads, dim=dim), table=_table(rows=rows, cols=1 << 20, nnz=listed // 16),
+                   tokens=tokens, q_indptr=4096, max_q_len=tokens // rows, q_heads=heads, max_seq_len=seq, prefix_len=0)
+    assert lib.load().tg_prefix_attention_workspace_bytes(a) <= max(1 << 30, tokens * heads * (4 * dim + 8)) + 512

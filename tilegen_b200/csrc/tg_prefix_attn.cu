@@ -597,6 +597,18 @@ __global__ void __launch_bounds__(128) attn_join_few_kernel(const AttnParams p) 
 }
 
 // ------------------------------------------------------------------ host
+// Bytes of own parts.  A prompt of 8192 tokens, 16 heads of 256 on 4: 4.4 ms with 256 MiB, 5.3 with 16
+// chunks in 2 GiB.  256 sequences of 8 tokens and 500 keys, one of 65536: 0.46 ms with 32 chunks in 1 GiB,
+// 0.45 with 64 in 2 GiB, 0.82 with 8 in 256 MiB; 1024 of 16 tokens with one such: 2.9 ms with 4 chunks, 2.2
+// with 16 in 4 GiB.
+constexpr int64_t kFewParts = 256ll << 20, kMostParts = 1ll << 30;
+
+// Keys of a chunk so that the parts of `rows` rows take `bytes` at most (or are one for each row).
+int64_t fit_chunk(int64_t max_seq, int64_t rows, int64_t bytes, int dim) {
+    const int64_t parts = std::max<int64_t>(1, bytes / (std::max<int64_t>(1, rows) * (dim * 4 + 8)));
+    return ceil_div(max_seq, parts * 16) * 16;
+}
+
 struct Plan {
     AttnParams p;
     int rt_own, rt_prefix;  // 16-row tiles of a CTA of the kernel for few rows; 0: the tcgen05 kernel
@@ -719,11 +731,20 @@ int make_plan(const tg_prefix_attention_args* a, Plan* plan, const char* op) {
         // sequence of 32768 keys: 34 us in chunks of 256, 38 in chunks of 128 (the join has 256
         // parts); 64 sequences of 4096: 184 to 188 us for any bounds from 128 to 1024.  The tcgen05
         // kernel: two pieces an SM.
-        const int64_t units = std::max<int64_t>(1, t.rows * tiles_own * c.heads);
+        const int64_t units = std::max<int64_t>(1, t.rows * tiles_own * c.heads), part_rows = a->tokens * a->q_heads;
         if (plan->rt_own) {
             const int64_t even = ceil_div(ceil_div(max_seq, std::max<int64_t>(1, 2 * warps / units)), 16) * 16;
             const int64_t most = units >= 2 * warps ? 16 : 64;
             p.own_chunk = (int)std::min(std::max<int64_t>(256, even), std::max<int64_t>(512, ceil_div(max_seq, most * 16) * 16));
+            // Chunks of every sequence have their place in the workspace, as many as the longest may
+            // have.  Above kFewParts chunks grow until it fits there, but not beyond what even shares
+            // of all listed keys would be; above kMostParts they grow whatever it costs.
+            const int64_t keys = std::min(slots, t.rows * max_seq);
+            const double share = (double)keys * tiles_own * c.heads / (2 * warps);
+            const int64_t few = fit_chunk(max_seq, part_rows, kFewParts, c.dim);
+            const int64_t chunk = std::max({(int64_t)p.own_chunk, share < (double)few ? ((int64_t)share + 15) / 16 * 16 : few,
+                                            fit_chunk(max_seq, part_rows, kMostParts, c.dim)});
+            p.own_chunk = (int)chunk;
         } else {
             const int64_t n = std::max<int64_t>(1, 2 * kSMs / units);
             p.own_chunk = (int)std::max<int64_t>(256, ceil_div(ceil_div(max_seq, n), 128) * 128);
