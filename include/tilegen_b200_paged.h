@@ -129,9 +129,14 @@ typedef struct tg_prefix_attention_args {
     double scale; /* > 0 */
     uint32_t flags;
 } tg_prefix_attention_args;
-/* Bytes of workspace for a call with these arguments (pointers are not read); 0 also where
- * the arguments are not valid. */
+/* Bytes of a workspace to keep: enough for a call with these arguments and for any with the
+ * same head sizes and at most as many tokens, sequences, listed pages and prefix tokens and
+ * no larger max_seq_len and max_q_len (pointers are not read); 0 also where the arguments are
+ * not valid.  It stays below 1.1 GiB and three parts of each row together. */
 TG_API size_t tg_prefix_attention_workspace_bytes(const tg_prefix_attention_args* a);
+/* What a call with these very arguments takes, at most the former: for one that allocates.
+ * A smaller call may take more. */
+TG_API size_t tg_prefix_attention_needed_bytes(const tg_prefix_attention_args* a);
 TG_API int tg_prefix_attention_f16(const tg_prefix_attention_args* a, void* workspace, size_t workspace_bytes,
                                    tg_stream_t stream);
 TG_API int tg_prefix_attention_bf16(const tg_prefix_attention_args* a, void* workspace, size_t workspace_bytes,

@@ -242,3 +242,34 @@ def test_attention_workspace_stays_small(rows, tokens, heads, kv_heads, dim, seq
     a = _attention(cache=_cache(pages=1 << 20, heads=kv_heads, dim=dim), table=_table(rows=rows, cols=1 << 20, nnz=listed // 16),
                    tokens=tokens, q_indptr=4096, max_q_len=tokens // rows, q_heads=heads, max_seq_len=seq, prefix_len=0)
     assert lib.load().tg_prefix_attention_workspace_bytes(a) <= max(1 << 30, tokens * heads * (4 * dim + 8)) + 512
+
+
+def test_a_workspace_serves_every_smaller_call():
+    """A buffer taken at the largest sizes of a server, and calls with fewer of everything."""
+    import random
+
+    rng = random.Random(5)
+    ask = lib.load().tg_prefix_attention_workspace_bytes
+
+    def below(n):
+        return rng.choice([n, rng.randint(0, n), int(n ** rng.random())])
+
+    def args(rows, tokens, nnz, heads, kv_heads, dim, page, prefix, seq, q, ragged):
+        return _attention(cache=_cache(pages=1 << 24, heads=kv_heads, dim=dim, page_size=page), table=_table(rows=rows, cols=1 << 24, nnz=nnz),
+                          tokens=tokens if ragged else rows, q_indptr=4096 if ragged else None, max_q_len=q, q_heads=heads,
+                          max_seq_len=seq, prefix_len=prefix, n_prefix_pages=-(-prefix // page))
+
+    for _ in range(300):
+        kv_heads, page = rng.choice([1, 2, 8]), rng.choice([1, 7, 16, 64])
+        heads, dim = kv_heads * rng.choice([1, 4, 8]), rng.choice([64, 96, 128, 256])
+        rows, seq = rng.choice([1, 4, 64, 130, 1024]), rng.choice([1, 256, 2000, 8192, 131072])
+        q, prefix = rng.choice([1, 5, 300, 4096]), rng.choice([0, 0, 100, 8192, 131072])
+        tokens, nnz = rows + rng.randint(0, rows * (q - 1)), rows * -(-seq // page)
+        kept = ask(args(rows, tokens, nnz, heads, kv_heads, dim, page, prefix, seq, q, True))
+        for _ in range(30):
+            r = max(1, below(rows))
+            small = args(r, max(1, below(tokens)), below(nnz), heads, kv_heads, dim, page, below(prefix), below(seq), max(1, below(q)),
+                         rng.random() < 0.7)
+            assert ask(small) <= kept
+            needed = lib.load().tg_prefix_attention_needed_bytes(small)
+            assert needed <= ask(small)

@@ -613,8 +613,13 @@ struct Plan {
     AttnParams p;
     int rt_own, rt_prefix;  // 16-row tiles of a CTA of the kernel for few rows; 0: the tcgen05 kernel
     int64_t own_units, prefix_units;
-    size_t ws_bytes;
+    size_t ws_bytes;   // what the call takes
+    size_t ws_enough;  // what a call of these sizes or of any smaller ones takes at most
 };
+
+// Bytes of so many rows of parts: the sums, then m and l.
+size_t sum_bytes(int64_t rows, int dim) { return ((size_t)rows * dim * sizeof(float) + 255) / 256 * 256; }
+size_t parts_bytes(int64_t rows, int dim) { return sum_bytes(rows, dim) + ((size_t)rows * sizeof(float2) + 255) / 256 * 256; }
 
 // CTAs of the tcgen05 kernel over the prefix, by the time that the whole call would take: a CTA,
 // one on an SM, has its steps at 1.75 us (1.2 where there is one row tile), 10 us to begin and end
@@ -747,7 +752,8 @@ int make_plan(const tg_prefix_attention_args* a, Plan* plan, const char* op) {
             p.own_chunk = (int)chunk;
         } else {
             const int64_t n = std::max<int64_t>(1, 2 * kSMs / units);
-            p.own_chunk = (int)std::max<int64_t>(256, ceil_div(ceil_div(max_seq, n), 128) * 128);
+            const int64_t most = fit_chunk(max_seq, part_rows, kMostParts, c.dim);  // many tokens of no sequence
+            p.own_chunk = (int)std::max<int64_t>(256, ceil_div(std::max(ceil_div(max_seq, n), most), 128) * 128);
         }
         p.own_chunks = (int)std::max<int64_t>(1, ceil_div(max_seq, p.own_chunk));
     }
@@ -760,9 +766,16 @@ int make_plan(const tg_prefix_attention_args* a, Plan* plan, const char* op) {
     const int parts = p.prefix_splits + p.own_chunks;
     p.direct = parts == 1;
     p.fill = p.direct && p.q_indptr && p.prefix_len == 0;
-    const size_t rows = (size_t)a->tokens * a->q_heads;
-    const size_t o_bytes = (parts * rows * c.dim * sizeof(float) + 255) / 256 * 256;
-    plan->ws_bytes = p.direct || rows == 0 ? 0 : o_bytes + (parts * rows * sizeof(float2) + 255) / 256 * 256;
+    const int64_t rows = a->tokens * a->q_heads;
+    plan->ws_bytes = p.direct ? 0 : parts_bytes(parts * rows, c.dim);
+    // Fewer sequences or listed pages are cut into more parts, so what this call takes is no bound for
+    // smaller ones.  A part has 128 keys of the prefix or 256 own keys, or the last of them.  Over the
+    // prefix, more than two parts of a row are one for each of so many warps (or CTAs) that together
+    // have 32 (or 256) rows each; own parts fit kMostParts.
+    const int64_t of_prefix = ceil_div(p.prefix_len, 128), of_own = ceil_div(max_seq, 256);
+    const int64_t prefix_rows = std::min(of_prefix * rows, std::max<int64_t>({2 * rows, warps * 32, (int64_t)kSMs * 256}));
+    const int64_t own_rows = std::min(of_own * rows, std::max<int64_t>(rows, kMostParts / (c.dim * 4 + 8)));
+    plan->ws_enough = of_prefix + of_own <= 1 ? 0 : parts_bytes(prefix_rows + own_rows, c.dim);
     return TG_OK;
 }
 
@@ -789,7 +802,7 @@ int attn_run(const Plan& plan, void* ws, cudaStream_t st) {
     const size_t rows = (size_t)p.tokens * p.q_heads;
     const size_t parts = p.prefix_splits + p.own_chunks;
     p.part_o = static_cast<float*>(ws);
-    p.part_ml = reinterpret_cast<float2*>(static_cast<char*>(ws) + (parts * rows * D * sizeof(float) + 255) / 256 * 256);
+    p.part_ml = reinterpret_cast<float2*>(static_cast<char*>(ws) + sum_bytes((int64_t)(parts * rows), D));
     int rc = TG_OK;
     bool second = false;
     if (p.prefix_ctas > 0) {
@@ -872,6 +885,11 @@ int attention(const tg_prefix_attention_args* a, void* ws, size_t ws_bytes, tg_s
 extern "C" {
 
 size_t tg_prefix_attention_workspace_bytes(const tg_prefix_attention_args* a) {
+    tg::Plan plan;
+    return tg::make_plan(a, &plan, "tg_prefix_attention") == TG_OK ? plan.ws_enough : 0;
+}
+
+size_t tg_prefix_attention_needed_bytes(const tg_prefix_attention_args* a) {
     tg::Plan plan;
     return tg::make_plan(a, &plan, "tg_prefix_attention") == TG_OK ? plan.ws_bytes : 0;
 }

@@ -244,6 +244,7 @@ SIGNATURES_PAGED = {
     "tg_kv_append_f16": (ctypes.c_int, [ctypes.POINTER(TgKvAppendArgs), _P]),
     "tg_kv_append_bf16": (ctypes.c_int, [ctypes.POINTER(TgKvAppendArgs), _P]),
     "tg_prefix_attention_workspace_bytes": (_SZ, [ctypes.POINTER(TgPrefixAttentionArgs)]),
+    "tg_prefix_attention_needed_bytes": (_SZ, [ctypes.POINTER(TgPrefixAttentionArgs)]),
     "tg_prefix_attention_f16": (ctypes.c_int, [ctypes.POINTER(TgPrefixAttentionArgs), _P, _SZ, _P]),
     "tg_prefix_attention_bf16": (ctypes.c_int, [ctypes.POINTER(TgPrefixAttentionArgs), _P, _SZ, _P]),
 }

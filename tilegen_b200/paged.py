@@ -346,7 +346,9 @@ def prefix_attention_workspace_bytes(q: torch.Tensor, cache: PagedKV, table: Pag
                                      prefix_pages: Optional[torch.Tensor] = None, prefix_len: int = 0,
                                      q_indptr: Optional[torch.Tensor] = None, max_q_len: Optional[int] = None,
                                      max_seq_len: Optional[int] = None) -> int:
-    """Bytes of workspace that prefix_attention needs with these arguments."""
+    """Bytes of a workspace to keep for prefix_attention: enough for a call with these arguments and
+    for any of the same head sizes that is smaller (fewer tokens, sequences, listed pages or prefix
+    tokens, smaller bounds)."""
     a, _held = _attention_args(q, cache, table, seq_len, prefix_pages, prefix_len, q_indptr, max_q_len, max_seq_len,
                                None, True, False)
     return int(_call("tg_prefix_attention_workspace_bytes")(a))
@@ -370,8 +372,8 @@ def prefix_attention(q: torch.Tensor, cache: PagedKV, table: PageTable, seq_len:
     allow; tighter bounds plan better): tokens past the first max_q_len see nothing, a longer
     sequence counts as max_seq_len.
     scale defaults to dim ** -0.5.  ``lse=True`` (or a float32 [tokens, q_heads] tensor) returns
-    (out, log of the softmax's sum).  ``workspace`` (prefix_attention_workspace_bytes) is
-    allocated on the call's stream where it is not given; ``check`` checks the index arrays
+    (out, log of the softmax's sum).  ``workspace`` (prefix_attention_workspace_bytes for one to
+    keep) is allocated on the call's stream where it is not given; ``check`` checks the index arrays
     first (and synchronises)."""
     a, _held = _attention_args(q, cache, table, seq_len, prefix_pages, prefix_len, q_indptr, max_q_len, max_seq_len,
                                scale, causal, check)
@@ -407,7 +409,7 @@ def _attention_launch(a, q, out, lse, workspace, index, sp):
         if lse.shape != q.shape[:2] or lse.dtype != torch.float32 or lse.get_device() != index or not lse.is_contiguous():
             raise ValueError("lse must be a contiguous float32 tensor of shape %s on cuda:%d" % (tuple(q.shape[:2]), index))
         a.lse = lse.data_ptr()
-    need = _call("tg_prefix_attention_workspace_bytes")(a)
+    need = _call("tg_prefix_attention_needed_bytes")(a)
     ws = size = 0
     if workspace is None and need:
         workspace, size = torch.empty(need, dtype=torch.uint8, device=q.device), need
