@@ -111,7 +111,8 @@ TG_API int tg_kv_append_bf16(const tg_kv_append_args* a, tg_stream_t stream);
  * seen.  max_seq_len bounds the entries of seq_len; a longer one counts as max_seq_len.
  * max_q_len (not 0) bounds the tokens of one sequence: the first max_q_len see what they see
  * without the bound, those after them, and tokens that no sequence holds, see nothing.  Dim 64,
- * 96, 128 or 256; all strides multiples of 8 elements and all rows 16-byte aligned. */
+ * 96, 128 or 256; all rows 16-byte aligned and all strides multiples of 8 elements, but those
+ * of dimensions of one, which are not read. */
 typedef struct tg_prefix_attention_args {
     const tg_paged_kv* cache;
     const tg_csr* pages;

@@ -597,6 +597,27 @@ def test_many_small_weights_beside_a_large_one(dtype, many):
     assert float((lse.double() - (gap + math.log1p(w))).abs().max()) <= 4 * e
 
 
+def test_strides_of_dimensions_of_one():
+    """Nothing is multiplied by the stride of a dimension of one, so it may be anything: one token or
+    one page cut out of a buffer whose rows are off the 16-byte grid."""
+    b = Batch([1], [11], 20, 4, 1, 64, 32, BF16, seed=6)
+    q, out = (torch.zeros(5, 259, dtype=BF16, device="cuda")[:, :256].unflatten(1, (4, 64))[:1] for _ in range(2))
+    q.copy_(b.q)
+    b.q = q
+    assert q.stride() == (259, 64, 1)
+    assert b.run(out=out) is out
+    b.check(out)
+    lone = Batch([2], [11], 0, 1, 1, 64, 32, BF16, seed=6, spare=0)
+    assert lone.cache.pages == 1
+    odd = [torch.as_strided(x, x.shape, (x.stride(0) + 1, 64, 3, 1)) for x in (lone.cache.k, lone.cache.v)]
+    lone.cache = P.PagedKV(*odd)
+    lone.q = torch.as_strided(lone.q, lone.q.shape, (64, 5, 1))
+    lone.check(lone.run())
+    r = P.Rope(P.rope_frequencies(64))
+    pos = torch.tensor([9], device="cuda")
+    check_rotated(P.rope(q, r, pos), *rotate64(q, pos, r), BF16)
+
+
 # ------------------------------------------------------------------ append
 @pytest.mark.parametrize("dtype", [BF16, F16, F32])
 @pytest.mark.parametrize("news,lens,page,dim,rot,layout,heads_first", [

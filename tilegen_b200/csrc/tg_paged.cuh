@@ -97,6 +97,10 @@ __device__ __forceinline__ void pages_of(const int64_t* indptr, int64_t nnz, int
     n = min(max(e, first), nnz) - first;
 }
 
+// The stride of a dimension of n: nothing is multiplied by that of a dimension of one, which may be
+// anything and must not decide how rows are moved or whether they are refused.
+inline int64_t stride_of(int64_t n, int64_t stride) { return n > 1 ? stride : 0; }
+
 // host side (tg_paged_host.cu)
 int check_cache(const tg_paged_kv* c, const char* op);
 int check_table(const tg_csr* t, const tg_paged_kv* c, int64_t tokens, const int64_t* q_indptr, const int64_t* seq_len,

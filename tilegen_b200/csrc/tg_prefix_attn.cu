@@ -689,10 +689,11 @@ int make_plan(const tg_prefix_attention_args* a, Plan* plan, const char* op) {
     AttnParams& p = plan->p;
     p = {};
     p.q = a->q.data, p.k = c.k, p.v = c.v, p.out = a->out.data, p.lse = a->lse;
-    p.q_tok = a->q.token_stride, p.q_head = a->q.head_stride;
-    p.o_tok = a->out.token_stride, p.o_head = a->out.head_stride;
-    p.k_page = c.k_page_stride, p.k_slot = c.k_slot_stride, p.k_head = c.k_head_stride;
-    p.v_page = c.v_page_stride, p.v_slot = c.v_slot_stride, p.v_head = c.v_head_stride;
+    p.q_tok = stride_of(a->tokens, a->q.token_stride), p.q_head = stride_of(a->q_heads, a->q.head_stride);
+    p.o_tok = stride_of(a->tokens, a->out.token_stride), p.o_head = stride_of(a->q_heads, a->out.head_stride);
+    p.k_page = stride_of(c.pages, c.k_page_stride), p.v_page = stride_of(c.pages, c.v_page_stride);
+    p.k_slot = stride_of(c.page_size, c.k_slot_stride), p.v_slot = stride_of(c.page_size, c.v_slot_stride);
+    p.k_head = stride_of(c.heads, c.k_head_stride), p.v_head = stride_of(c.heads, c.v_head_stride);
     p.pages = (int)c.pages, p.page_size = (int)c.page_size;
     p.page_shift = -1;
     for (int i = 0; i < 31; ++i)
@@ -854,9 +855,9 @@ int attention(const tg_prefix_attention_args* a, void* ws, size_t ws_bytes, tg_s
     if (a->prefix_len > 0 && !a->prefix_pages) return set_error(TG_EINVAL, "%s: null prefix_pages", op);
     const uint64_t at = reinterpret_cast<uint64_t>(a->q.data) | reinterpret_cast<uint64_t>(a->out.data) |
                         reinterpret_cast<uint64_t>(c.k) | reinterpret_cast<uint64_t>(c.v);
-    const uint64_t strides = (uint64_t)(a->q.token_stride | a->q.head_stride | a->out.token_stride | a->out.head_stride |
-                                        c.k_page_stride | c.k_slot_stride | c.k_head_stride | c.v_page_stride |
-                                        c.v_slot_stride | c.v_head_stride);
+    const AttnParams& p = plan.p;
+    const uint64_t strides = (uint64_t)(p.q_tok | p.q_head | p.o_tok | p.o_head | p.k_page | p.k_slot | p.k_head |
+                                        p.v_page | p.v_slot | p.v_head);
     if (at % 16 || strides % 8)
         return set_error(TG_EINVAL, "%s: rows must be 16-byte aligned (strides multiples of 8 elements)", op);
     if (ws_bytes < plan.ws_bytes || (plan.ws_bytes && !ws))

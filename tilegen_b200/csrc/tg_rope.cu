@@ -308,8 +308,8 @@ int rope(const tg_rope* r, const tg_rows* x, const tg_rows* y, int64_t tokens, i
     RopeParams<T> p = {};
     p.q = static_cast<const T*>(x->data);
     p.qo = static_cast<T*>(y->data);
-    p.q_tok = x->token_stride, p.q_head = x->head_stride;
-    p.qo_tok = y->token_stride, p.qo_head = y->head_stride;
+    p.q_tok = stride_of(tokens, x->token_stride), p.q_head = stride_of(heads, x->head_stride);
+    p.qo_tok = stride_of(tokens, y->token_stride), p.qo_head = stride_of(heads, y->head_stride);
     p.q_rows = heads;
     p.dim = dim, p.rot = r->rot_dim;
     p.freq = r->freq, p.scale = (float)r->scale;
@@ -343,15 +343,16 @@ int append(const tg_kv_append_args* a, tg_stream_t stream, const char* op) {
     RopeParams<T> p = {};
     p.k = static_cast<const T*>(a->k.data), p.ko = static_cast<T*>(c.k);
     p.v = static_cast<const T*>(a->v.data), p.vo = static_cast<T*>(c.v);
-    p.k_tok = a->k.token_stride, p.k_head = a->k.head_stride;
-    p.v_tok = a->v.token_stride, p.v_head = a->v.head_stride;
-    p.ko_page = c.k_page_stride, p.ko_slot = c.k_slot_stride, p.ko_head = c.k_head_stride;
-    p.vo_page = c.v_page_stride, p.vo_slot = c.v_slot_stride, p.vo_head = c.v_head_stride;
+    p.k_tok = stride_of(a->tokens, a->k.token_stride), p.k_head = stride_of(c.heads, a->k.head_stride);
+    p.v_tok = stride_of(a->tokens, a->v.token_stride), p.v_head = stride_of(c.heads, a->v.head_stride);
+    p.ko_page = stride_of(c.pages, c.k_page_stride), p.vo_page = stride_of(c.pages, c.v_page_stride);
+    p.ko_slot = stride_of(c.page_size, c.k_slot_stride), p.vo_slot = stride_of(c.page_size, c.v_slot_stride);
+    p.ko_head = stride_of(c.heads, c.k_head_stride), p.vo_head = stride_of(c.heads, c.v_head_stride);
     p.kv_rows = c.heads, p.dim = c.dim;
     if (with_q) {
         p.q = static_cast<const T*>(a->q->data), p.qo = static_cast<T*>(a->q_out->data);
-        p.q_tok = a->q->token_stride, p.q_head = a->q->head_stride;
-        p.qo_tok = a->q_out->token_stride, p.qo_head = a->q_out->head_stride;
+        p.q_tok = stride_of(a->tokens, a->q->token_stride), p.q_head = stride_of(a->q_heads, a->q->head_stride);
+        p.qo_tok = stride_of(a->tokens, a->q_out->token_stride), p.qo_head = stride_of(a->q_heads, a->q_out->head_stride);
         p.q_rows = a->q_heads;
     }
     if (a->rope) {
