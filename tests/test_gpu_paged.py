@@ -117,6 +117,36 @@ def test_rope_gradient_against_autograd_and_differences(layout):
     assert abs(float(num - (dx.double() * step.double()).sum())) < 6 * 3 * 24 * 8 * 16 * 2.0 ** -22
 
 
+@pytest.mark.parametrize("layout", ["half", "interleaved"])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_rope_takes_part_in_autograd(layout, dtype):
+    """The gradient that reaches x is rope_backward's, of a whole tensor, of a joint projection's
+    view and of an expanded number; without a gradient asked for, the result has none."""
+    g = gen(13)
+    r = P.Rope(P.rope_frequencies(40), layout, 1.5)
+    pos = torch.randint(0, 9000, (33,), generator=g, device="cuda")
+    qkv = normal(g, 33, 6, 64, dtype=dtype).requires_grad_()
+    x, dy = qkv[:, 1:5], normal(g, 33, 4, 64, dtype=dtype)
+    y = P.rope(x, r, pos)
+    assert torch.equal(y, P.rope(x.detach(), r, pos))
+    (grad,) = torch.autograd.grad(y, qkv, dy, retain_graph=True)
+    assert torch.equal(grad[:, 1:5], P.rope_backward(dy, r, pos)) and not bool(grad[:, 0].any() | grad[:, 5].any())
+    (grad,) = torch.autograd.grad(y.sum(), qkv)
+    assert torch.equal(grad[:, 1:5], P.rope_backward(torch.ones_like(dy), r, pos))
+    # of the gradient in turn, and on another stream
+    st = torch.cuda.Stream()
+    st.wait_stream(torch.cuda.current_stream())
+    y = P.rope(x, r, pos, stream=st)
+    torch.cuda.current_stream().wait_stream(st)
+    up = dy.clone().requires_grad_()
+    (grad,) = torch.autograd.grad(y, x, up, create_graph=True)
+    (back,) = torch.autograd.grad(grad, up, x.detach())
+    assert torch.equal(back, y.detach())
+    with torch.no_grad():
+        assert not P.rope(x, r, pos).requires_grad
+    assert not P.rope(x, r, pos, out=torch.empty_like(dy)).requires_grad
+
+
 def test_rope_empty_and_refusals():
     r = P.Rope(P.rope_frequencies(8))
     pos = torch.zeros(4, dtype=torch.int64, device="cuda")

@@ -239,17 +239,45 @@ def _rope_launch(suffix, x, out, xr, rd, pos, flags, sp) -> torch.Tensor:
     return out
 
 
+class _Turn(torch.autograd.Function):
+    """The rotation, or with TG_FLAG_ROPE_INVERSE its transpose: each is the other's gradient."""
+
+    @staticmethod
+    def forward(ctx, x, freq, positions, layout, scale, flags):
+        ctx.save_for_backward(freq, positions)
+        ctx.how = layout, scale, flags
+        return _rope_call(x, Rope(freq, layout, scale), positions, None, flags, None)
+
+    @staticmethod
+    def backward(ctx, dy):
+        layout, scale, flags = ctx.how
+        if dy.shape[2] > 1 and dy.stride(2) != 1:  # the gradient of a sum is one number, expanded
+            dy = dy.contiguous()
+        return (_Turn.apply(dy, *ctx.saved_tensors, layout, scale, flags ^ _lib.TG_FLAG_ROPE_INVERSE),) + (None,) * 5
+
+
+def _turn(x, r, positions, out, flags, stream) -> torch.Tensor:
+    if out is None and x.requires_grad and torch.is_grad_enabled():
+        if stream is not None:
+            _stream(x.get_device(), stream)  # it is on x's device
+        with torch.cuda.stream(stream):  # the gradient is taken on the stream of the call (None: no change)
+            return _Turn.apply(x, r.freq, positions, r.layout, r.scale, flags)
+    return _rope_call(x, r, positions, out, flags, stream)
+
+
 def rope(x: torch.Tensor, r: Rope, positions: torch.Tensor, out: Optional[torch.Tensor] = None,
          stream: Optional[torch.cuda.Stream] = None) -> torch.Tensor:
-    """x [tokens, heads, dim] rotated at positions [tokens] (int64); out may be x."""
-    return _rope_call(x, r, positions, out, 0, stream)
+    """x [tokens, heads, dim] rotated at positions [tokens] (int64); out may be x.
+
+    Differentiable with respect to x, unless the result is written to a given out."""
+    return _turn(x, r, positions, out, 0, stream)
 
 
 def rope_backward(dout: torch.Tensor, r: Rope, positions: torch.Tensor, out: Optional[torch.Tensor] = None,
                   stream: Optional[torch.cuda.Stream] = None) -> torch.Tensor:
     """The gradient with respect to x of rope(x, r, positions), for the gradient dout of its
-    output; out may be dout."""
-    return _rope_call(dout, r, positions, out, _lib.TG_FLAG_ROPE_INVERSE, stream)
+    output; out may be dout.  (What autograd calls for rope; differentiable as rope is.)"""
+    return _turn(dout, r, positions, out, _lib.TG_FLAG_ROPE_INVERSE, stream)
 
 
 def kv_append(cache: PagedKV, table: PageTable, seq_len: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
@@ -263,7 +291,7 @@ def kv_append(cache: PagedKV, table: PageTable, seq_len: torch.Tensor, k: torch.
     Sequence b brings the tokens q_indptr[b]:q_indptr[b + 1] (without q_indptr: token b) and is
     seq_len[b] tokens long after them; its new token i is token a = seq_len[b] - n + i of its
     pages, at position positions[t] or position_base + a.  ``check`` checks the index arrays
-    first (and synchronises)."""
+    first (and synchronises).  A call for serving: no gradient goes through it."""
     kv = cache.desc()
     index, dt = cache.k.get_device(), cache.k.dtype
     tb = table.desc(index, kv.pages)
@@ -374,7 +402,7 @@ def prefix_attention(q: torch.Tensor, cache: PagedKV, table: PageTable, seq_len:
     scale defaults to dim ** -0.5.  ``lse=True`` (or a float32 [tokens, q_heads] tensor) returns
     (out, log of the softmax's sum).  ``workspace`` (prefix_attention_workspace_bytes for one to
     keep) is allocated on the call's stream where it is not given; ``check`` checks the index arrays
-    first (and synchronises)."""
+    first (and synchronises).  A call for serving: no gradient goes through it."""
     a, _held = _attention_args(q, cache, table, seq_len, prefix_pages, prefix_len, q_indptr, max_q_len, max_seq_len,
                                scale, causal, check)
     index = q.get_device()
