@@ -648,6 +648,29 @@ def test_strides_of_dimensions_of_one():
     check_rotated(P.rope(q, r, pos), *rotate64(q, pos, r), BF16)
 
 
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("page", [1, 6, 7, 130])
+@pytest.mark.parametrize("news,lens,prefix", [([150, 129, 1], [150, 400, 90], 333), ([90, 70], [290, 71], 0), ([1] * 50, [9] * 50, 300)])
+def test_pages_with_few_rows_in_common_with_a_tile(news, lens, prefix, page, dim, dtype):
+    """The tcgen05 kernel with 64 or 128 boxes a tile of 128 keys, lengths that end inside one, and
+    pages outside the cache, which read as zeros."""
+    b = Batch(news, lens, prefix, 8, 2, dim, page, dtype, seed=page)
+    out, lse = b.run(lse=True)
+    b.check(out, lse)
+    bad = b.table.indices.clone()
+    bad[0] = b.cache.pages
+    b.table = P.PageTable(b.table.indptr, bad)
+    for x in b.own[0]:
+        x[:page] = 0
+    if prefix:
+        b.prefix_pages = b.prefix_pages.clone()
+        b.prefix_pages[2] = -1
+        for x in b.shared:
+            x[2 * page:3 * page] = 0
+    b.check(b.run())
+
+
 # ------------------------------------------------------------------ append
 @pytest.mark.parametrize("dtype", [BF16, F16, F32])
 @pytest.mark.parametrize("news,lens,page,dim,rot,layout,heads_first", [
