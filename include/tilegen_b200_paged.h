@@ -102,17 +102,25 @@ TG_API int tg_kv_append_bf16(const tg_kv_append_args* a, tg_stream_t stream);
 
 /* out = softmax(scale * q k^T) v for the queries of a batch (tokens by q_indptr as above).
  * The keys of sequence b are the prefix_len tokens of the prefix pages, shared by the whole
- * batch, followed by the seq_len[b] tokens of its own pages; the prefix is read once for
- * all.  Query head j uses key head j / (q_heads / cache->heads).  With TG_FLAG_CAUSAL the
- * i-th of the n queries of sequence b sees the first prefix_len + seq_len[b] - n + i + 1
- * keys, without it all; a query that sees none gives zeros.  What lies in the cache beyond
- * what a query sees (NaN and infinities included) has no effect on it.  lse, where not
- * NULL, receives log(sum(exp(scale * q k^T))) of each (token, head), -inf where nothing is
- * seen.  max_seq_len bounds the entries of seq_len; a longer one counts as max_seq_len.
- * max_q_len (not 0) bounds the tokens of one sequence: the first max_q_len see what they see
- * without the bound, those after them, and tokens that no sequence holds, see nothing.  Dim 64,
- * 96, 128 or 256; all rows 16-byte aligned and all strides multiples of 8 elements, but those
- * of dimensions of one, which are not read. */
+ * batch, followed by the seq_len[b] tokens of its own pages.  Query head j uses key head
+ * j / (q_heads / cache->heads).  With TG_FLAG_CAUSAL the i-th of the n queries of sequence b
+ * sees the first prefix_len + seq_len[b] - n + i + 1 keys, without it all; a query that sees
+ * none gives zeros.  What lies in the cache beyond what a query sees (NaN and infinities
+ * included) has no effect on it.  lse, where not NULL, receives log(sum(exp(scale * q k^T)))
+ * of each (token, head), -inf where nothing is seen.
+ *
+ * The prefix is fetched once for every 256 rows (tokens times the query heads of a key head)
+ * where dim is 64 or 128 and rows are more than 32, else once for every 16 or 32; those
+ * fetches meet in L2.  Products are summed and the softmax is taken in 32 bits.  The weights
+ * exp(...) are rounded to the values' type for their product with them: relative errors of
+ * half an ulp that average out over the keys, together with the output's own rounding about
+ * 1.4 times the error of that alone.
+ *
+ * max_seq_len bounds the entries of seq_len; a longer one counts as max_seq_len.  max_q_len
+ * (not 0) bounds the tokens of one sequence: the first max_q_len see what they see without
+ * the bound, those after them, and tokens that no sequence holds, see nothing.  Dim 64, 96,
+ * 128 or 256; all rows 16-byte aligned and all strides multiples of 8 elements, but those of
+ * dimensions of one, which are not read.  out may not share memory with q. */
 typedef struct tg_prefix_attention_args {
     const tg_paged_kv* cache;
     const tg_csr* pages;

@@ -627,7 +627,7 @@ size_t parts_bytes(int64_t rows, int dim) { return sum_bytes(rows, dim) + ((size
 // goes on to; the SMs that they leave, and their time after them, go to the own parts (own_bytes at
 // 6 TB/s, 12 us at least); and each part of a row is written and read once more.  As many CTAs for
 // each pair, or fewer than pairs and even shares.  It finds the best of a sweep of 64 sequences of
-// 540 keys behind 8192 (56 CTAs: 56 us; 32: 69, 128: 75), of 256 behind 32768 (128: 172; 64: 243,
+// 540 keys behind 8192 (56 CTAs: 56 us; 32: 69, 128: 75), of 256 of 180 keys behind 32768 (128: 172; 64: 243,
 // 144: 180) and of 48 of 5 tokens and 320 keys behind 5003 (96: 49; 64: 58, 128: 59).
 void share_prefix(AttnParams& p, int64_t rows, int dim, double own_bytes) {
     const int64_t units = (int64_t)p.prefix_tiles * p.kv_heads;

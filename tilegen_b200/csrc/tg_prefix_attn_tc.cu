@@ -18,8 +18,8 @@
 // 107 bytes a cycle; with P V (P from TMEM) and the tiles' arrival that is 2500 cycles for 128 keys
 // of two tiles, of 3200 that a step takes; the rest is the chain S, maximum, P, product of a tile
 // where the other tile does not cover it.  4608 rows of each of 8 key heads of 128 over 16384 keys:
-// 275 us, 1.12 PFLOP/s, 68 % of the library product's burst; tensor pipe 64 % active, special-function
-// unit 48 %, issue slots 48 %.
+// 270 us, 1.14 PFLOP/s, 69 % of the library product's burst; tensor pipe 63 % active, special-function
+// unit 64 %, issue slots 38 %.
 //
 // O is rescaled only where a row's maximum has grown by more than 2^8 since the value that P is
 // taken relative to: P stays below 2^8 (2^15 in float16, where the largest weight is at least 2^7, so

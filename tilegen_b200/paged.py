@@ -8,9 +8,11 @@ the given (default: current) stream, arguments checked here and in the library, 
 A decoding step of a batch behind a shared prefix::
 
     q = kv_append(cache, table, seq_len, k, v, rope=rope, q=q, position_base=prefix_len)
-    out = prefix_attention(q, cache, table, seq_len, prefix_pages=pages, prefix_len=prefix_len)
+    out = prefix_attention(q, cache, table, seq_len, prefix_pages=pages, prefix_len=prefix_len, max_seq_len=longest)
 
-and the prefix itself is written once, as a table of one row.
+and the prefix itself is written once, as a table of one row.  max_seq_len is a bound that the
+host knows (lengths stay on the GPU); without it a sequence is taken to be as long as all listed
+pages together, which plans the work worse.
 """
 
 from __future__ import annotations
@@ -391,14 +393,16 @@ def prefix_attention(q: torch.Tensor, cache: PagedKV, table: PageTable, seq_len:
                      stream: Optional[torch.cuda.Stream] = None):
     """softmax(scale * q k^T) v for the queries q [tokens, q_heads, dim] of a batch whose
     sequences share the first prefix_len keys (in prefix_pages), each followed by the seq_len[b]
-    keys of its own pages.  The prefix is read once for the whole batch.
+    keys of its own pages.  The prefix is fetched once for every 256 rows (tokens times query heads
+    of a key head) of a batch of more than 32, for heads of 64 and 128, else once for every 16 or 32.
 
     Queries are given as for kv_append: q_indptr, or one for each sequence.  With ``causal`` the
     last query of a sequence sees all its keys, the one before it one key less, and so on; a
     query that sees nothing gives zeros, and so does one that no sequence holds.  max_q_len and
     max_seq_len bound the tokens and the own length of a sequence (defaults: what the arrays' sizes
-    allow; tighter bounds plan better): tokens past the first max_q_len see nothing, a longer
-    sequence counts as max_seq_len.
+    allow; tighter ones plan better, by up to half of the time): tokens past the first max_q_len
+    see nothing, a longer sequence counts as max_seq_len.  Softmax and sums are 32-bit; the weights
+    are rounded to the values' type for their product with them.  out may not share memory with q.
     scale defaults to dim ** -0.5.  ``lse=True`` (or a float32 [tokens, q_heads] tensor) returns
     (out, log of the softmax's sum).  ``workspace`` (prefix_attention_workspace_bytes for one to
     keep) is allocated on the call's stream where it is not given; ``check`` checks the index arrays
