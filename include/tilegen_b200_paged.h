@@ -100,6 +100,66 @@ TG_API int tg_kv_append_f32(const tg_kv_append_args* a, tg_stream_t stream);
 TG_API int tg_kv_append_f16(const tg_kv_append_args* a, tg_stream_t stream);
 TG_API int tg_kv_append_bf16(const tg_kv_append_args* a, tg_stream_t stream);
 
+/* The norm of a head x of `dim` elements: x / sqrt(mean(x^2) + eps) * (offset + weight[i]), or
+ * without that factor where weight is NULL.  The mean and all sums are 32-bit. */
+typedef struct tg_head_norm {
+    const void* weight; /* dim values, or NULL */
+    int32_t weight_f32; /* the weight is float, else of the rows' type */
+    double eps;         /* >= 0 */
+    double offset;
+} tg_head_norm;
+
+/* q_out = rotation of the normed q at the tokens' positions, and the same for k, in one pass.  An
+ * output may be its input.  A norm NULL: that tensor is only rotated; rope NULL: nothing turns and
+ * positions are not read; a number of heads 0: that tensor is not there.  dim at most 256. */
+typedef struct tg_norm_rope_args {
+    int64_t tokens;
+    int32_t dim;
+    int32_t q_heads, k_heads;
+    tg_rows q, k, q_out, k_out;
+    const tg_head_norm* q_norm;
+    const tg_head_norm* k_norm;
+    const tg_rope* rope;
+    const int64_t* positions;
+    uint32_t flags; /* 0 */
+} tg_norm_rope_args;
+TG_API int tg_norm_rope_f32(const tg_norm_rope_args* a, tg_stream_t stream);
+TG_API int tg_norm_rope_f16(const tg_norm_rope_args* a, tg_stream_t stream);
+TG_API int tg_norm_rope_bf16(const tg_norm_rope_args* a, tg_stream_t stream);
+
+/* Its gradient: for the gradients dq_out and dk_out of the outputs, those of the inputs (dq, dk;
+ * each may be dq_out, dk_out or the input itself) and of the weights (of the weight's type, summed
+ * over all tokens and heads of the tensor in 32 bits and in a fixed order; NULL: not wanted). */
+typedef struct tg_norm_rope_grad_args {
+    int64_t tokens;
+    int32_t dim;
+    int32_t q_heads, k_heads;
+    tg_rows q, k, dq_out, dk_out, dq, dk;
+    const tg_head_norm* q_norm;
+    const tg_head_norm* k_norm;
+    void* dq_weight;
+    void* dk_weight;
+    const tg_rope* rope;
+    const int64_t* positions;
+    uint32_t flags; /* 0 */
+} tg_norm_rope_grad_args;
+/* Bytes of its workspace; it serves every call with heads no longer and as many tokens or fewer. */
+TG_API size_t tg_norm_rope_backward_workspace_bytes(const tg_norm_rope_grad_args* a);
+TG_API int tg_norm_rope_backward_f32(const tg_norm_rope_grad_args* a, void* workspace, size_t workspace_bytes,
+                                     tg_stream_t stream);
+TG_API int tg_norm_rope_backward_f16(const tg_norm_rope_grad_args* a, void* workspace, size_t workspace_bytes,
+                                     tg_stream_t stream);
+TG_API int tg_norm_rope_backward_bf16(const tg_norm_rope_grad_args* a, void* workspace, size_t workspace_bytes,
+                                      tg_stream_t stream);
+
+/* tg_kv_append_* with norms of q and k before the rotation (NULL: none).  dim at most 256. */
+TG_API int tg_kv_append_normed_f32(const tg_kv_append_args* a, const tg_head_norm* q_norm, const tg_head_norm* k_norm,
+                                   tg_stream_t stream);
+TG_API int tg_kv_append_normed_f16(const tg_kv_append_args* a, const tg_head_norm* q_norm, const tg_head_norm* k_norm,
+                                   tg_stream_t stream);
+TG_API int tg_kv_append_normed_bf16(const tg_kv_append_args* a, const tg_head_norm* q_norm, const tg_head_norm* k_norm,
+                                    tg_stream_t stream);
+
 /* out = softmax(scale * q k^T) v for the queries of a batch (tokens by q_indptr as above).
  * The keys of sequence b are the prefix_len tokens of the prefix pages, shared by the whole
  * batch, followed by the seq_len[b] tokens of its own pages.  Query head j uses key head

@@ -2,6 +2,7 @@
 #include <algorithm>
 
 #include "tg_prefix_attn.cuh"
+#include "tg_rope.cuh"
 
 namespace tg {
 
@@ -106,6 +107,28 @@ int paged_bounds_check(const tg_csr& t, int64_t page_size, const int64_t* seq_le
                          (h & 4) ? " indptr[rows]!=nnz" : "", (h & 8) ? " page out of range" : "",
                          (h & 16) ? " seq_len out of range" : "", (h & 32) ? " q_indptr" : "",
                          (h & 64) ? " prefix page out of range" : "", (h & 128) ? " more new tokens than seq_len" : "");
+    return TG_OK;
+}
+
+int check_append(const tg_kv_append_args* a, const char* op, cudaStream_t st, bool& done) {
+    done = false;
+    if (!a) return set_error(TG_EINVAL, "%s: null arguments", op);
+    int rc = check_cache(a->cache, op);
+    if (rc == TG_OK) rc = check_table(a->pages, a->cache, a->tokens, a->q_indptr, a->seq_len, op);
+    if (rc == TG_OK && a->rope) rc = check_rope(a->rope, a->cache->dim, op);
+    if (rc == TG_OK && a->rope) rc = check_rot(a->rope, op);
+    if (rc != TG_OK) return rc;
+    if (a->flags & ~TG_FLAG_BOUNDS_CHECK) return set_error(TG_EINVAL, "%s: unknown flags 0x%x", op, a->flags);
+    if (a->q && (!a->q_out || a->q_heads < 0)) return set_error(TG_EINVAL, "%s: q without q_out, or q_heads < 0", op);
+    if (a->tokens == 0) {
+        done = true;
+        return TG_OK;
+    }
+    if (!a->k.data || !a->v.data) return set_error(TG_EINVAL, "%s: null k/v", op);
+    if (a->q && a->q_heads > 0 && (!a->q->data || !a->q_out->data)) return set_error(TG_EINVAL, "%s: null q/q_out", op);
+    if (a->flags & TG_FLAG_BOUNDS_CHECK)
+        return paged_bounds_check(*a->pages, a->cache->page_size, a->seq_len, INT64_MAX, a->tokens, a->q_indptr, INT64_MAX,
+                                  nullptr, 0, true, op, st);
     return TG_OK;
 }
 

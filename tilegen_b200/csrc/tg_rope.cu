@@ -16,13 +16,13 @@
 //   output's type (for float32 outputs 3.5e-8 off on average, where a 64-bit sine gives 2.9e-8).
 #include <algorithm>
 
-#include "tg_paged.cuh"
+#include "tg_rope.cuh"
 
 namespace tg {
 namespace {
 
 template <typename T>
-struct RopeParams {
+struct RopeParams : NewTokens {
     // q, k, v rows: input and output with their token and head strides (k and v go to the
     // slot offset of the token instead of a token stride)
     const T *q, *k, *v;
@@ -33,45 +33,9 @@ struct RopeParams {
     int dim, rot;
     const double* freq;
     float scale, sign;
-    int64_t tokens;
     int tile;  // tokens of a CTA
-    const int64_t* positions;
-    // append only
-    int64_t position_base;
-    const int64_t *q_indptr, *seq_len, *indptr, *indices;
-    int64_t rows, pages, nnz, page_size;
     int lanes, chunks, blocks;  // threads along a row, items of a row, rounds of the threads over them
 };
-
-template <typename T, int VEC>
-struct alignas(sizeof(T) * VEC) Pack {
-    T v[VEC];
-    __device__ __forceinline__ void get(float (&f)[VEC]) const {
-        if constexpr (VEC > 1 && sizeof(T) == 2) {
-#pragma unroll
-            for (int i = 0; i < VEC; i += 2) {
-                const float2 x = unpack2<T>(reinterpret_cast<const uint32_t*>(v)[i / 2]);
-                f[i] = x.x, f[i + 1] = x.y;
-            }
-        } else {
-#pragma unroll
-            for (int i = 0; i < VEC; ++i) f[i] = to_f32(v[i]);
-        }
-    }
-    __device__ __forceinline__ void put(const float (&f)[VEC]) {
-        if constexpr (VEC > 1 && sizeof(T) == 2) {
-#pragma unroll
-            for (int i = 0; i < VEC; i += 2) reinterpret_cast<uint32_t*>(v)[i / 2] = pack2<T>(f[i], f[i + 1]);
-        } else {
-#pragma unroll
-            for (int i = 0; i < VEC; ++i) v[i] = from_f32<T>(f[i]);
-        }
-    }
-};
-
-constexpr int kRopeThreads = 256;
-constexpr int kRopeTile = 32;         // most tokens of a CTA
-constexpr int kRopeSmem = 32 * 1024;  // most bytes of cosines and sines of a CTA
 
 // VEC elements (a pack) are moved at once: 16 bytes where rows, strides and the parts of a row are
 // multiples of that, else single elements.  A thread's item is two packs of a row: the two halves
@@ -98,19 +62,7 @@ __global__ void __launch_bounds__(kRopeThreads, APPEND ? 6 : 5) rope_kernel(cons
     if (tid < tile) {
         const int64_t t = t0 + tid;
         if constexpr (APPEND) {
-            const int64_t b = sequence_of(p.q_indptr, p.rows, t);
-            int64_t first, n, page0, npages;
-            tokens_of(p.q_indptr, p.tokens, b, first, n);
-            pages_of(p.indptr, p.nnz, b, page0, npages);
-            const int64_t at = p.seq_len[b] - n + (t - first);
-            int64_t page = -1;
-            if (at >= 0 && t >= first && t < first + n) {
-                const int64_t j = at / p.page_size;
-                if (j < npages) page = p.indices[page0 + j];
-                if (page >= p.pages) page = -1;
-                s_slot[tid] = at - j * p.page_size;
-            }
-            s_page[tid] = page;
+            const int64_t at = slot_of_token(p, t, s_page[tid], s_slot[tid]);
             s_pos[tid] = (double)(p.positions ? p.positions[t] : p.position_base + at);
         } else {
             s_pos[tid] = (double)p.positions[t];
@@ -212,13 +164,8 @@ __global__ void __launch_bounds__(kRopeThreads, APPEND ? 6 : 5) rope_kernel(cons
 
     for (int i = tid; i < tile * pairs; i += blockDim.x) {
         const int k = i / pairs;
-        const double t = s_pos[k] * p.freq[i - k * pairs];
-        const double whole = rint(t * 0.15915494309189533577);  // turns
-        const double rest = fma(-whole, 2.4492935982947064e-16, fma(-whole, 6.283185307179586, t));  // 2 pi in two parts
-        float s, c;
-        sincospif((float)(rest * 0.31830988618379067154), &s, &c);
         const int pair = i - k * pairs;
-        s_turn[k * pairs + place(pair / kPairs, pair % kPairs)] = make_float2(c * p.scale, s * p.scale * p.sign);
+        s_turn[k * pairs + place(pair / kPairs, pair % kPairs)] = turn_of(s_pos[k], p.freq[pair], p.scale, p.sign);
     }
     __syncthreads();
 
@@ -287,12 +234,6 @@ int rope_run(RopeParams<T> p, int layout, cudaStream_t st, const char* what) {
     return check_launch(what);
 }
 
-constexpr int kMaxRot = 2 * (kRopeSmem / 8);  // one token's cosines and sines fit a CTA
-
-int check_rot(const tg_rope* r, const char* op) {
-    return r->rot_dim > kMaxRot ? set_error(TG_EUNSUPPORTED, "%s: rot_dim above %d", op, kMaxRot) : TG_OK;
-}
-
 template <typename T>
 int rope(const tg_rope* r, const tg_rows* x, const tg_rows* y, int64_t tokens, int32_t heads, int32_t dim,
          const int64_t* positions, uint32_t flags, tg_stream_t stream, const char* op) {
@@ -321,26 +262,12 @@ int rope(const tg_rope* r, const tg_rows* x, const tg_rows* y, int64_t tokens, i
 
 template <typename T>
 int append(const tg_kv_append_args* a, tg_stream_t stream, const char* op) {
-    if (!a) return set_error(TG_EINVAL, "%s: null arguments", op);
-    int rc = check_cache(a->cache, op);
-    if (rc == TG_OK) rc = check_table(a->pages, a->cache, a->tokens, a->q_indptr, a->seq_len, op);
-    if (rc == TG_OK && a->rope) rc = check_rope(a->rope, a->cache->dim, op);
-    if (rc == TG_OK && a->rope) rc = check_rot(a->rope, op);
-    if (rc != TG_OK) return rc;
-    if (a->flags & ~TG_FLAG_BOUNDS_CHECK) return set_error(TG_EINVAL, "%s: unknown flags 0x%x", op, a->flags);
-    if (a->q && (!a->q_out || a->q_heads < 0)) return set_error(TG_EINVAL, "%s: q without q_out, or q_heads < 0", op);
-    if (a->tokens == 0) return TG_OK;
-    if (!a->k.data || !a->v.data) return set_error(TG_EINVAL, "%s: null k/v", op);
-    const bool with_q = a->q && a->q_heads > 0;
-    if (with_q && (!a->q->data || !a->q_out->data)) return set_error(TG_EINVAL, "%s: null q/q_out", op);
-    const tg_paged_kv& c = *a->cache;
-    const tg_csr& t = *a->pages;
+    bool done;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    if (a->flags & TG_FLAG_BOUNDS_CHECK) {
-        rc = paged_bounds_check(t, c.page_size, a->seq_len, INT64_MAX, a->tokens, a->q_indptr, INT64_MAX, nullptr, 0,
-                                true, op, st);
-        if (rc != TG_OK) return rc;
-    }
+    const int rc = check_append(a, op, st, done);
+    if (rc != TG_OK || done) return rc;
+    const tg_paged_kv& c = *a->cache;
+    const bool with_q = a->q && a->q_heads > 0;
     RopeParams<T> p = {};
     p.k = static_cast<const T*>(a->k.data), p.ko = static_cast<T*>(c.k);
     p.v = static_cast<const T*>(a->v.data), p.vo = static_cast<T*>(c.v);
@@ -360,9 +287,7 @@ int append(const tg_kv_append_args* a, tg_stream_t stream, const char* op) {
         p.rot = a->rope->rot_dim, p.freq = a->rope->freq, p.scale = (float)a->rope->scale;
     }
     p.sign = 1.f;
-    p.tokens = a->tokens, p.positions = a->positions, p.position_base = a->position_base;
-    p.q_indptr = a->q_indptr, p.seq_len = a->seq_len, p.indptr = t.indptr, p.indices = t.indices;
-    p.rows = t.rows, p.pages = c.pages, p.nnz = t.nnz, p.page_size = c.page_size;
+    new_tokens(*a, p);
     return rope_run<T, true>(p, a->rope ? a->rope->layout : TG_ROPE_HALF, st, op);
 }
 

@@ -144,6 +144,55 @@ class TgKvAppendArgs(ctypes.Structure):
     ]
 
 
+class TgHeadNorm(ctypes.Structure):
+    _fields_ = [
+        ("weight", ctypes.c_void_p),
+        ("weight_f32", ctypes.c_int32),
+        ("eps", ctypes.c_double),
+        ("offset", ctypes.c_double),
+    ]
+
+
+class TgNormRopeArgs(ctypes.Structure):
+    _fields_ = [
+        ("tokens", ctypes.c_int64),
+        ("dim", ctypes.c_int32),
+        ("q_heads", ctypes.c_int32),
+        ("k_heads", ctypes.c_int32),
+        ("q", TgRows),
+        ("k", TgRows),
+        ("q_out", TgRows),
+        ("k_out", TgRows),
+        ("q_norm", ctypes.c_void_p),  # TgHeadNorm
+        ("k_norm", ctypes.c_void_p),  # TgHeadNorm
+        ("rope", ctypes.c_void_p),  # TgRope
+        ("positions", ctypes.c_void_p),
+        ("flags", ctypes.c_uint32),
+    ]
+
+
+class TgNormRopeGradArgs(ctypes.Structure):
+    _fields_ = [
+        ("tokens", ctypes.c_int64),
+        ("dim", ctypes.c_int32),
+        ("q_heads", ctypes.c_int32),
+        ("k_heads", ctypes.c_int32),
+        ("q", TgRows),
+        ("k", TgRows),
+        ("dq_out", TgRows),
+        ("dk_out", TgRows),
+        ("dq", TgRows),
+        ("dk", TgRows),
+        ("q_norm", ctypes.c_void_p),  # TgHeadNorm
+        ("k_norm", ctypes.c_void_p),  # TgHeadNorm
+        ("dq_weight", ctypes.c_void_p),
+        ("dk_weight", ctypes.c_void_p),
+        ("rope", ctypes.c_void_p),  # TgRope
+        ("positions", ctypes.c_void_p),
+        ("flags", ctypes.c_uint32),
+    ]
+
+
 class TgPrefixAttentionArgs(ctypes.Structure):
     _fields_ = [
         ("cache", ctypes.c_void_p),  # TgPagedKV
@@ -235,6 +284,8 @@ SIGNATURES = {
 _ROPE = [ctypes.POINTER(TgRope), ctypes.POINTER(TgRows), ctypes.POINTER(TgRows), _I64, ctypes.c_int32,
          ctypes.c_int32, _P, ctypes.c_uint32, _P]
 
+_TYPES = ("f32", "f16", "bf16")
+
 # every symbol declared in include/tilegen_b200_paged.h
 SIGNATURES_PAGED = {
     "tg_rope_f32": (ctypes.c_int, _ROPE),
@@ -243,6 +294,11 @@ SIGNATURES_PAGED = {
     "tg_kv_append_f32": (ctypes.c_int, [ctypes.POINTER(TgKvAppendArgs), _P]),
     "tg_kv_append_f16": (ctypes.c_int, [ctypes.POINTER(TgKvAppendArgs), _P]),
     "tg_kv_append_bf16": (ctypes.c_int, [ctypes.POINTER(TgKvAppendArgs), _P]),
+    **{"tg_norm_rope_" + t: (ctypes.c_int, [ctypes.POINTER(TgNormRopeArgs), _P]) for t in _TYPES},
+    "tg_norm_rope_backward_workspace_bytes": (_SZ, [ctypes.POINTER(TgNormRopeGradArgs)]),
+    **{"tg_norm_rope_backward_" + t: (ctypes.c_int, [ctypes.POINTER(TgNormRopeGradArgs), _P, _SZ, _P]) for t in _TYPES},
+    **{"tg_kv_append_normed_" + t: (ctypes.c_int, [ctypes.POINTER(TgKvAppendArgs), ctypes.POINTER(TgHeadNorm),
+                                                   ctypes.POINTER(TgHeadNorm), _P]) for t in _TYPES},
     "tg_prefix_attention_workspace_bytes": (_SZ, [ctypes.POINTER(TgPrefixAttentionArgs)]),
     "tg_prefix_attention_needed_bytes": (_SZ, [ctypes.POINTER(TgPrefixAttentionArgs)]),
     "tg_prefix_attention_f16": (ctypes.c_int, [ctypes.POINTER(TgPrefixAttentionArgs), _P, _SZ, _P]),

@@ -27,8 +27,9 @@ import torch
 from . import lib as _lib
 from .device import _dev
 
-__all__ = ["Rope", "rope_frequencies", "rope", "rope_backward", "PagedKV", "PageTable", "kv_append",
-           "prefix_attention", "prefix_attention_workspace_bytes"]
+__all__ = ["Rope", "rope_frequencies", "rope", "rope_backward", "HeadNorm", "norm_rope", "norm_rope_backward",
+           "norm_rope_backward_workspace_bytes", "PagedKV", "PageTable", "kv_append", "prefix_attention",
+           "prefix_attention_workspace_bytes"]
 
 _SUFFIX = {torch.float32: "f32", torch.float16: "f16", torch.bfloat16: "bf16"}
 _LAYOUT = {"half": _lib.TG_ROPE_HALF, "interleaved": _lib.TG_ROPE_INTERLEAVED}
@@ -113,6 +114,27 @@ class Rope:
 
 
 @dataclass
+class HeadNorm:
+    """The norm of a head x [dim]: x / sqrt(mean(x^2) + eps) * (offset + weight), or without that factor
+    where weight is None.  weight: [dim], float32 or the heads' type, on their GPU; offset is 1 for
+    models that keep the weights' distance from one."""
+
+    weight: Optional[torch.Tensor] = None
+    eps: float = 1e-6
+    offset: float = 0.0
+
+    def desc(self, dim: int, dtype: torch.dtype, index: int) -> _lib.TgHeadNorm:
+        w = self.weight
+        if w is None:
+            return _lib.TgHeadNorm(None, 0, self.eps, self.offset)
+        if w.shape != (dim,) or (w.dtype is not dtype and w.dtype is not torch.float32) or not w.is_contiguous() \
+                or w.get_device() != index:
+            raise ValueError("a norm's weight must be a contiguous %s or float32 vector of %d on cuda:%d (got %s %s on %s)"
+                             % (dtype, dim, index, tuple(w.shape), w.dtype, w.device))
+        return _lib.TgHeadNorm(w.data_ptr(), w.dtype is not dtype or dtype is torch.float32, self.eps, self.offset)
+
+
+@dataclass
 class PagedKV:
     """Keys and values in pages: [pages, page_size, heads, dim] each, any strides with the last
     one 1 (a cache stored head by head is passed transposed)."""
@@ -188,7 +210,7 @@ def _rows(t: torch.Tensor, name: str, shape: Tuple, dtype: torch.dtype, index: i
         raise ValueError("%s must be a %s tensor of shape %s on cuda:%d (got %s %s on %s)"
                          % (name, dtype, tuple(shape), index, t.dtype, tuple(t.shape), t.device))
     st = t.stride()
-    if st[2] != 1 and shape[2] > 1:
+    if st[2] != 1 and shape[2] > 1 and t.numel():
         raise ValueError("%s: the last stride must be 1 (got %d)" % (name, st[2]))
     return _lib.TgRows(t.data_ptr(), st[0], st[1])
 
@@ -282,13 +304,176 @@ def rope_backward(dout: torch.Tensor, r: Rope, positions: torch.Tensor, out: Opt
     return _turn(dout, r, positions, out, _lib.TG_FLAG_ROPE_INVERSE, stream)
 
 
+def _norm_shape(q: torch.Tensor, k: Optional[torch.Tensor]):
+    """(suffix, device, dim, q's shape, k's shape) of a pair of queries and keys."""
+    suffix = _SUFFIX.get(q.dtype)
+    if q.dim() != 3 or not q.is_cuda or suffix is None:
+        raise ValueError("q must be [tokens, heads, dim], float32, float16 or bfloat16, on a CUDA device (got %s %s on %s)"
+                         % (tuple(q.shape), q.dtype, q.device))
+    if k is not None and k.dim() != 3:
+        raise ValueError("k must be [tokens, heads, dim] (got %s)" % (tuple(k.shape),))
+    tokens, heads, dim = q.shape
+    return suffix, q.get_device(), dim, q.shape, (tokens, 0 if k is None else k.shape[1], dim)
+
+
+def _norm_args(args, held, q, k, q_norm, k_norm, rope, positions):
+    """Fills what the forward and the gradient have in common; what it points to goes into held."""
+    _, index, dim, qs, ks = _norm_shape(q, k)
+    dt = q.dtype
+    args.tokens, args.dim, args.q_heads, args.k_heads = qs[0], dim, qs[1], ks[1]
+    args.q = _rows(q, "q", qs, dt, index)
+    if k is not None:
+        args.k = _rows(k, "k", ks, dt, index)
+    elif k_norm is not None:
+        raise ValueError("k_norm without k")
+    for name, norm in (("q_norm", q_norm), ("k_norm", k_norm)):
+        if norm is not None:
+            d = norm.desc(dim, dt, index)
+            held.append(d)
+            setattr(args, name, ctypes.addressof(d))
+    if rope is not None:
+        if positions is None:
+            raise ValueError("a rotation needs positions")
+        d = rope.desc(index)
+        held.append(d)
+        args.rope = ctypes.addressof(d)
+        args.positions = _vector(positions, "positions", index, qs[0])
+    return args
+
+
+def _norm_call(q, k, q_norm, k_norm, rope, positions, q_out, k_out, stream):
+    held: list = []
+    a = _norm_args(_lib.TgNormRopeArgs(), held, q, k, q_norm, k_norm, rope, positions)
+    suffix, index, _, qs, ks = _norm_shape(q, k)
+    if k is None and k_out is not None:
+        raise ValueError("k_out without k")
+    sp = _stream(index, stream)
+    where = _elsewhere(index, stream)
+    if where is not None:
+        with where:
+            return _norm_launch(a, suffix, q, k, q_out, k_out, qs, ks, index, sp)
+    return _norm_launch(a, suffix, q, k, q_out, k_out, qs, ks, index, sp)
+
+
+def _norm_launch(a, suffix, q, k, q_out, k_out, qs, ks, index, sp):
+    if q_out is None:
+        q_out = _like(q)
+    a.q_out = _rows(q_out, "q_out", qs, q.dtype, index)
+    if k is not None:
+        if k_out is None:
+            k_out = _like(k)
+        a.k_out = _rows(k_out, "k_out", ks, q.dtype, index)
+    _lib.check(_call("tg_norm_rope_" + suffix)(a, sp), "tg_norm_rope")
+    return q_out, k_out
+
+
+class _NormTurn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, q_weight, k_weight, freq, positions, how):
+        q_norm, k_norm, layout, scale = how
+        ctx.save_for_backward(q, k, q_weight, k_weight, freq, positions)
+        ctx.how = how
+        rope = None if freq is None else Rope(freq, layout, scale)
+        return _norm_call(q, k, q_norm and HeadNorm(q_weight, *q_norm), k_norm and HeadNorm(k_weight, *k_norm), rope, positions,
+                          None, None, None)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dq_out, dk_out):
+        q, k, q_weight, k_weight, freq, positions = ctx.saved_tensors
+        q_norm, k_norm, layout, scale = ctx.how
+        rope = None if freq is None else Rope(freq, layout, scale)
+        dq, dk, dqw, dkw = norm_rope_backward(dq_out, dk_out, q, k, q_norm and HeadNorm(q_weight, *q_norm),
+                                              k_norm and HeadNorm(k_weight, *k_norm), rope, positions)
+        return dq, dk, dqw, dkw, None, None, None
+
+
+def norm_rope(q: torch.Tensor, k: Optional[torch.Tensor] = None, q_norm: Optional[HeadNorm] = None,
+              k_norm: Optional[HeadNorm] = None, rope: Optional[Rope] = None, positions: Optional[torch.Tensor] = None,
+              q_out: Optional[torch.Tensor] = None, k_out: Optional[torch.Tensor] = None,
+              stream: Optional[torch.cuda.Stream] = None) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
+    """(q, k) [tokens, heads, dim], each head normed and then rotated at positions [tokens] (int64), in
+    one pass over both.  Without a norm that tensor is only rotated, without a rope nothing turns; k
+    may be None.  dim is 256 at most.  q_out and k_out may be q and k.
+
+    Differentiable with respect to q, k and the norms' weights (once), unless an out is given."""
+    tracked = [t for t in (q, k, q_norm and q_norm.weight, k_norm and k_norm.weight) if t is not None and t.requires_grad]
+    if not tracked or q_out is not None or k_out is not None or not torch.is_grad_enabled():
+        return _norm_call(q, k, q_norm, k_norm, rope, positions, q_out, k_out, stream)
+    if stream is not None:
+        _stream(q.get_device(), stream)  # it is on q's device
+    how = tuple(n and (n.eps, n.offset) for n in (q_norm, k_norm)) + ((rope.layout, rope.scale) if rope else (None, None))
+    with torch.cuda.stream(stream):  # the gradient is taken on the stream of the call (None: no change)
+        return _NormTurn.apply(q, k, q_norm and q_norm.weight, k_norm and k_norm.weight, rope and rope.freq,
+                               positions if rope else None, how)
+
+
+def norm_rope_backward(dq_out: torch.Tensor, dk_out: Optional[torch.Tensor], q: torch.Tensor, k: Optional[torch.Tensor] = None,
+                       q_norm: Optional[HeadNorm] = None, k_norm: Optional[HeadNorm] = None, rope: Optional[Rope] = None,
+                       positions: Optional[torch.Tensor] = None, dq: Optional[torch.Tensor] = None,
+                       dk: Optional[torch.Tensor] = None, workspace: Optional[torch.Tensor] = None,
+                       stream: Optional[torch.cuda.Stream] = None):
+    """(dq, dk, gradient of q_norm's weight, of k_norm's weight) of norm_rope(q, k, ...) for the gradients
+    dq_out and dk_out of its outputs; None where there is no such tensor.  The weights' gradients have
+    the weights' type; their sums are 32-bit and in a fixed order.  dq may be dq_out or q, dk likewise.
+    ``workspace``: norm_rope_backward_workspace_bytes, allocated on the call's stream where not given."""
+    held: list = []
+    a = _norm_args(_lib.TgNormRopeGradArgs(), held, q, k, q_norm, k_norm, rope, positions)
+    suffix, index, _, qs, ks = _norm_shape(q, k)
+    if (k is None) != (dk_out is None) or (k is None and dk is not None):
+        raise ValueError("k and the gradients of k go together")
+    # the gradient of a sum is one number, expanded
+    dq_out, dk_out = (t.contiguous() if t is not None and t.dim() == 3 and t.shape[2] > 1 and t.stride(2) != 1 else t
+                      for t in (dq_out, dk_out))
+    a.dq_out = _rows(dq_out, "dq_out", qs, q.dtype, index)
+    if k is not None:
+        a.dk_out = _rows(dk_out, "dk_out", ks, q.dtype, index)
+    sp = _stream(index, stream)
+    where = _elsewhere(index, stream)
+    if where is not None:
+        with where:
+            return _norm_grad_launch(a, suffix, q, k, q_norm, k_norm, dq, dk, qs, ks, workspace, index, sp)
+    return _norm_grad_launch(a, suffix, q, k, q_norm, k_norm, dq, dk, qs, ks, workspace, index, sp)
+
+
+def _norm_grad_launch(a, suffix, q, k, q_norm, k_norm, dq, dk, qs, ks, workspace, index, sp):
+    if dq is None:
+        dq = _like(q)
+    a.dq = _rows(dq, "dq", qs, q.dtype, index)
+    if k is not None:
+        if dk is None:
+            dk = _like(k)
+        a.dk = _rows(dk, "dk", ks, q.dtype, index)
+    dqw = torch.empty_like(q_norm.weight) if q_norm is not None and q_norm.weight is not None else None
+    dkw = torch.empty_like(k_norm.weight) if k_norm is not None and k_norm.weight is not None else None
+    a.dq_weight = None if dqw is None else dqw.data_ptr()
+    a.dk_weight = None if dkw is None else dkw.data_ptr()
+    need = _call("tg_norm_rope_backward_workspace_bytes")(a)
+    ws = size = 0
+    if workspace is None and need:
+        workspace, size = torch.empty(need, dtype=torch.uint8, device=q.device), need
+        ws = workspace.data_ptr()
+    elif workspace is not None:
+        ws, size = _workspace(workspace, need, index)
+    _lib.check(_call("tg_norm_rope_backward_" + suffix)(a, ws, size, sp), "tg_norm_rope_backward")
+    return dq, dk, dqw, dkw
+
+
+def norm_rope_backward_workspace_bytes(tokens: int, dim: int) -> int:
+    """Bytes of a workspace to keep for norm_rope_backward: it serves every call with heads of at most dim
+    elements and at most as many tokens."""
+    return int(_call("tg_norm_rope_backward_workspace_bytes")(_lib.TgNormRopeGradArgs(tokens, dim)))
+
+
 def kv_append(cache: PagedKV, table: PageTable, seq_len: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
               rope: Optional[Rope] = None, q: Optional[torch.Tensor] = None, q_out: Optional[torch.Tensor] = None,
               q_indptr: Optional[torch.Tensor] = None, position_base: int = 0,
               positions: Optional[torch.Tensor] = None, check: bool = False,
-              stream: Optional[torch.cuda.Stream] = None) -> Optional[torch.Tensor]:
+              stream: Optional[torch.cuda.Stream] = None, q_norm: Optional[HeadNorm] = None,
+              k_norm: Optional[HeadNorm] = None) -> Optional[torch.Tensor]:
     """Writes the new tokens' k and v [tokens, heads, dim] into the cache, k rotated on the way,
-    and returns q rotated at the same positions (None without q).
+    and returns q rotated at the same positions (None without q).  With q_norm or k_norm the heads of
+    that tensor are normed before they are rotated (heads of 256 at most).
 
     Sequence b brings the tokens q_indptr[b]:q_indptr[b + 1] (without q_indptr: token b) and is
     seq_len[b] tokens long after them; its new token i is token a = seq_len[b] - n + i of its
@@ -319,24 +504,30 @@ def kv_append(cache: PagedKV, table: PageTable, seq_len: torch.Tensor, k: torch.
         if q.dim() != 3:
             raise ValueError("q must be [tokens, q_heads, dim] (got %s)" % (tuple(q.shape),))
         a.q_heads = q.shape[1]
-    elif q_out is not None:
-        raise ValueError("q_out without q")
+    elif q_out is not None or q_norm is not None:
+        raise ValueError("q_out or q_norm without q")
+    norms = None
+    if q_norm is not None or k_norm is not None:
+        norms = tuple(None if n is None else n.desc(kv.dim, dt, index) for n in (q_norm, k_norm))
     sp = _stream(index, stream)
     where = _elsewhere(index, stream)
     if where is not None:
         with where:
-            return _append_launch(a, q, q_out, (tokens, a.q_heads, kv.dim), dt, index, sp)
-    return _append_launch(a, q, q_out, (tokens, a.q_heads, kv.dim), dt, index, sp)
+            return _append_launch(a, norms, q, q_out, (tokens, a.q_heads, kv.dim), dt, index, sp)
+    return _append_launch(a, norms, q, q_out, (tokens, a.q_heads, kv.dim), dt, index, sp)
 
 
-def _append_launch(a, q, q_out, qshape, dt, index, sp) -> Optional[torch.Tensor]:
+def _append_launch(a, norms, q, q_out, qshape, dt, index, sp) -> Optional[torch.Tensor]:
     if q is not None:
         qr = _rows(q, "q", qshape, dt, index)
         if q_out is None:
             q_out = _like(q)
         qo = _rows(q_out, "q_out", qshape, dt, index)
         a.q, a.q_out = ctypes.addressof(qr), ctypes.addressof(qo)
-    _lib.check(_call("tg_kv_append_" + _SUFFIX[dt])(a, sp), "tg_kv_append")
+    if norms is None:
+        _lib.check(_call("tg_kv_append_" + _SUFFIX[dt])(a, sp), "tg_kv_append")
+    else:
+        _lib.check(_call("tg_kv_append_normed_" + _SUFFIX[dt])(a, *norms, sp), "tg_kv_append")
     return q_out
 
 
