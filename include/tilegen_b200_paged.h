@@ -211,6 +211,48 @@ TG_API int tg_prefix_attention_f16(const tg_prefix_attention_args* a, void* work
 TG_API int tg_prefix_attention_bf16(const tg_prefix_attention_args* a, void* workspace, size_t workspace_bytes,
                                     tg_stream_t stream);
 
+/* A 32-bit number for each cached key, strides in elements. */
+typedef struct tg_paged_mass {
+    float* data;
+    int64_t page_stride, slot_stride, head_stride;
+} tg_paged_mass;
+
+/* The attention weight that the keys of the sequences' own pages gather from the queries of a batch:
+ *   mass[key] = decay * mass[key] + sum of exp(scale * q k - lse)
+ * over the rows (new token, query head of the key's head) that see the key, with q, lse
+ * ([tokens, q_heads]), scale and TG_FLAG_CAUSAL as given to and returned by tg_prefix_attention_*:
+ * with a prefix, lse holds the prefix's share too, and the own keys get theirs.  Tokens and lengths
+ * as there; tokens past the first max_q_len of a sequence add nothing, nor does a row whose lse is
+ * -inf.  With TG_FLAG_CAUSAL the last n keys are those of the n new tokens: what their slots held
+ * before is not read.  Nor is anything where decay is 0.  Every key of a sequence is written, keys
+ * that no row sees with decay * mass; slots behind a sequence's length are left alone, and slots of
+ * pages that do not exist dropped.  No page may be listed twice.  Scores, exponentials and sums are
+ * 32-bit and the sums' order is fixed.  cache->v is not read.  Dim 64, 96, 128 or 256, q and k
+ * aligned as for the attention. */
+typedef struct tg_attention_mass_args {
+    const tg_paged_kv* cache;
+    const tg_csr* pages;
+    const int64_t* seq_len;
+    int64_t max_seq_len;
+    int64_t tokens;
+    const int64_t* q_indptr;
+    int64_t max_q_len;
+    int32_t q_heads;
+    tg_rows q;
+    const float* lse;
+    double scale; /* > 0 */
+    tg_paged_mass mass;
+    double decay; /* >= 0 */
+    uint32_t flags;
+} tg_attention_mass_args;
+/* Bytes of a workspace, enough for this call and any of the same head sizes with no larger max_q_len
+ * (0 for few rows; never more than 10 MB). */
+TG_API size_t tg_attention_mass_workspace_bytes(const tg_attention_mass_args* a);
+TG_API int tg_attention_mass_f16(const tg_attention_mass_args* a, void* workspace, size_t workspace_bytes,
+                                 tg_stream_t stream);
+TG_API int tg_attention_mass_bf16(const tg_attention_mass_args* a, void* workspace, size_t workspace_bytes,
+                                  tg_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -175,4 +175,21 @@ int cache_maps(const AttnParams& p, bool is_half, int dim, int box_rows, CUtenso
     return TG_OK;
 }
 
+int rows_map(const AttnParams& p, bool is_half, int dim, int box_heads, int box_tokens, CUtensorMap* q) {
+    *q = CUtensorMap{};
+    if (p.tokens == 0) return TG_OK;  // no token, no box
+    if (!encoder()) return set_error(TG_ECUDA, "cuTensorMapEncodeTiled is not available");
+    const auto bytes = [&](int64_t n, int64_t stride) { return (cuuint64_t)(n > 1 ? stride : dim) * 2; };
+    const cuuint64_t size[3] = {(cuuint64_t)dim, (cuuint64_t)p.q_heads, (cuuint64_t)p.tokens};
+    const cuuint64_t stride[2] = {bytes(p.q_heads, p.q_head), bytes(p.tokens, p.q_tok)};
+    const cuuint32_t box[3] = {64, (cuuint32_t)box_heads, (cuuint32_t)box_tokens}, step[3] = {1, 1, 1};
+    const CUresult r = encoder()(q, is_half ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3,
+                                 const_cast<void*>(p.q), size, stride, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                                 CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS)
+        return set_error(TG_ECUDA, "cuTensorMapEncodeTiled: CUDA error %d (queries, strides %lld %lld)", (int)r,
+                         (long long)p.q_head, (long long)p.q_tok);
+    return TG_OK;
+}
+
 }  // namespace tg

@@ -182,6 +182,10 @@ __device__ __forceinline__ void mbar_expect_tx(uint64_t* bar, uint32_t bytes) {
 // elements of one head, rows of 128 bytes swizzled by 128 bytes (tg_paged_host.cu).
 int cache_maps(const AttnParams& p, bool is_half, int dim, int box_rows, CUtensorMap* k, CUtensorMap* v);
 
+// Tensor map of the queries as [token][head][dim], boxes of 64 elements of box_heads heads of
+// box_tokens tokens, swizzled the same way.
+int rows_map(const AttnParams& p, bool is_half, int dim, int box_heads, int box_tokens, CUtensorMap* q);
+
 // tg_prefix_attn_tc.cu
 template <typename T>
 int attn_tc_run(const AttnParams& p, int dim, int ctas, bool pdl, cudaStream_t st);

@@ -214,6 +214,34 @@ class TgPrefixAttentionArgs(ctypes.Structure):
     ]
 
 
+class TgPagedMass(ctypes.Structure):
+    _fields_ = [
+        ("data", ctypes.c_void_p),
+        ("page_stride", ctypes.c_int64),
+        ("slot_stride", ctypes.c_int64),
+        ("head_stride", ctypes.c_int64),
+    ]
+
+
+class TgAttentionMassArgs(ctypes.Structure):
+    _fields_ = [
+        ("cache", ctypes.c_void_p),  # TgPagedKV
+        ("pages", ctypes.c_void_p),  # TgCsr
+        ("seq_len", ctypes.c_void_p),
+        ("max_seq_len", ctypes.c_int64),
+        ("tokens", ctypes.c_int64),
+        ("q_indptr", ctypes.c_void_p),
+        ("max_q_len", ctypes.c_int64),
+        ("q_heads", ctypes.c_int32),
+        ("q", TgRows),
+        ("lse", ctypes.c_void_p),
+        ("scale", ctypes.c_double),
+        ("mass", TgPagedMass),
+        ("decay", ctypes.c_double),
+        ("flags", ctypes.c_uint32),
+    ]
+
+
 _I64 = ctypes.c_int64
 _P = ctypes.c_void_p
 _F64 = ctypes.c_double
@@ -303,6 +331,9 @@ SIGNATURES_PAGED = {
     "tg_prefix_attention_needed_bytes": (_SZ, [ctypes.POINTER(TgPrefixAttentionArgs)]),
     "tg_prefix_attention_f16": (ctypes.c_int, [ctypes.POINTER(TgPrefixAttentionArgs), _P, _SZ, _P]),
     "tg_prefix_attention_bf16": (ctypes.c_int, [ctypes.POINTER(TgPrefixAttentionArgs), _P, _SZ, _P]),
+    "tg_attention_mass_workspace_bytes": (_SZ, [ctypes.POINTER(TgAttentionMassArgs)]),
+    "tg_attention_mass_f16": (ctypes.c_int, [ctypes.POINTER(TgAttentionMassArgs), _P, _SZ, _P]),
+    "tg_attention_mass_bf16": (ctypes.c_int, [ctypes.POINTER(TgAttentionMassArgs), _P, _SZ, _P]),
 }
 
 _lib: Optional[ctypes.CDLL] = None

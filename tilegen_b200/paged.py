@@ -29,7 +29,7 @@ from .device import _dev
 
 __all__ = ["Rope", "rope_frequencies", "rope", "rope_backward", "HeadNorm", "norm_rope", "norm_rope_backward",
            "norm_rope_backward_workspace_bytes", "PagedKV", "PageTable", "kv_append", "prefix_attention",
-           "prefix_attention_workspace_bytes"]
+           "prefix_attention_workspace_bytes", "empty_mass", "attention_mass", "attention_mass_workspace_bytes"]
 
 _SUFFIX = {torch.float32: "f32", torch.float16: "f16", torch.bfloat16: "bf16"}
 _LAYOUT = {"half": _lib.TG_ROPE_HALF, "interleaved": _lib.TG_ROPE_INTERLEAVED}
@@ -641,3 +641,82 @@ def _attention_launch(a, q, out, lse, workspace, index, sp):
         ws, size = _workspace(workspace, need, index)
     _lib.check(_call("tg_prefix_attention_" + _SUFFIX[q.dtype])(a, ws, size, sp), "tg_prefix_attention")
     return (out, lse) if isinstance(lse, torch.Tensor) else out
+
+
+def _mass_desc(mass: torch.Tensor, name: str, cache: PagedKV, index: int) -> _lib.TgPagedMass:
+    shape = cache.k.shape[:3]
+    if mass.shape != shape or mass.dtype is not torch.float32 or mass.get_device() != index:
+        raise ValueError("%s must be a float32 tensor of shape %s on cuda:%d (got %s %s on %s)"
+                         % (name, tuple(shape), index, mass.dtype, tuple(mass.shape), mass.device))
+    return _lib.TgPagedMass(mass.data_ptr(), *mass.stride())
+
+
+def empty_mass(cache: PagedKV) -> torch.Tensor:
+    """A mass for the keys of a cache, [pages, page_size, heads] zeros in the order that reads and writes
+    fastest (slots side by side)."""
+    pages, size, heads, _ = cache.k.shape
+    return torch.zeros(pages, heads, size, dtype=torch.float32, device=cache.k.device).transpose(1, 2)
+
+
+def _mass_args(mass, q, cache, table, seq_len, lse, q_indptr, max_q_len, max_seq_len, scale, causal, decay, check):
+    a, held = _attention_args(q, cache, table, seq_len, None, 0, q_indptr, max_q_len, max_seq_len, scale, causal, check)
+    index = cache.k.get_device()
+    if lse is not None and (lse.shape != q.shape[:2] or lse.dtype is not torch.float32 or lse.get_device() != index
+                            or not lse.is_contiguous()):
+        raise ValueError("lse must be a contiguous float32 tensor of shape %s on cuda:%d (got %s %s on %s)"
+                         % (tuple(q.shape[:2]), index, tuple(lse.shape), lse.dtype, lse.device))
+    m = _lib.TgAttentionMassArgs(a.cache, a.pages, a.seq_len, a.max_seq_len, a.tokens, a.q_indptr, a.max_q_len, a.q_heads, a.q,
+                                 None if lse is None else lse.data_ptr(), a.scale)
+    if mass is not None:
+        m.mass = _mass_desc(mass, "mass", cache, index)
+    m.decay, m.flags = decay, a.flags
+    return m, held
+
+
+def attention_mass(mass: torch.Tensor, q: torch.Tensor, cache: PagedKV, table: PageTable, seq_len: torch.Tensor,
+                   lse: torch.Tensor, q_indptr: Optional[torch.Tensor] = None, max_q_len: Optional[int] = None,
+                   max_seq_len: Optional[int] = None, scale: Optional[float] = None, causal: bool = True,
+                   decay: float = 1.0, workspace: Optional[torch.Tensor] = None, check: bool = False,
+                   stream: Optional[torch.cuda.Stream] = None) -> torch.Tensor:
+    """Adds to mass [pages, page_size, heads] (float32, any strides; empty_mass) the attention weight that
+    each key of the sequences' own pages gets from the queries q, summed over the tokens that see it and
+    the query heads of its key head: mass = decay * mass + sum of exp(scale * q k - lse).  Returns mass.
+
+    q, table, seq_len, q_indptr, the bounds, scale and causal are those of the prefix_attention call and
+    lse [tokens, q_heads] what it returned (with lse=True); behind a prefix the own keys get their share
+    of the whole softmax.  With ``causal`` the queries are the sequence's last tokens, whose keys start
+    from nothing: what their slots held is not read.  decay=0 forgets all that came before.  To weigh a
+    prompt by its last tokens, pass these as q, with seq_len of the whole prompt, and decay=0.
+
+    No page may be in the table twice.  The cache's values are not read.  float16 or bfloat16, heads of
+    64, 96, 128 or 256; scores and sums are 32-bit, in a fixed order.  ``workspace``:
+    attention_mass_workspace_bytes, allocated on the call's stream where it is not given.  A call for
+    serving: no gradient goes through it."""
+    m, _held = _mass_args(mass, q, cache, table, seq_len, lse, q_indptr, max_q_len, max_seq_len, scale, causal, decay, check)
+    index = q.get_device()
+    sp = _stream(index, stream)
+    where = _elsewhere(index, stream)
+    if where is not None:
+        with where:
+            return _mass_launch(m, mass, q, workspace, index, sp)
+    return _mass_launch(m, mass, q, workspace, index, sp)
+
+
+def _mass_launch(m, mass, q, workspace, index, sp):
+    need = _call("tg_attention_mass_workspace_bytes")(m)
+    ws = size = 0
+    if workspace is None and need:
+        workspace, size = torch.empty(need, dtype=torch.uint8, device=q.device), need
+        ws = workspace.data_ptr()
+    elif workspace is not None:
+        ws, size = _workspace(workspace, need, index)
+    _lib.check(_call("tg_attention_mass_" + _SUFFIX[q.dtype])(m, ws, size, sp), "tg_attention_mass")
+    return mass
+
+
+def attention_mass_workspace_bytes(q: torch.Tensor, cache: PagedKV, table: PageTable, seq_len: torch.Tensor,
+                                   q_indptr: Optional[torch.Tensor] = None, max_q_len: Optional[int] = None) -> int:
+    """Bytes of a workspace to keep for attention_mass: enough for this call and every one of the same
+    head sizes with no larger max_q_len (0 for few rows)."""
+    m, _held = _mass_args(None, q, cache, table, seq_len, None, q_indptr, max_q_len, None, None, True, 1.0, False)
+    return int(_call("tg_attention_mass_workspace_bytes")(m))
