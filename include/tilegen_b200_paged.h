@@ -253,6 +253,40 @@ TG_API int tg_attention_mass_f16(const tg_attention_mass_args* a, void* workspac
 TG_API int tg_attention_mass_bf16(const tg_attention_mass_args* a, void* workspace, size_t workspace_bytes,
                                   tg_stream_t stream);
 
+/* Cuts each sequence longer than `budget` to it, in place: for each key head by itself the first
+ * `first` places, the last `recent` ones and, of those between, the places with the largest mass stay
+ * (equal ones from the lowest place on; NaN counts as the largest, -0 as 0).  Where the budget is
+ * smaller, `recent` goes before `first`.  New places: the first ones as they were; then the chosen
+ * ones, of which those that lie within the places of their number stay and the others, in the order of
+ * their places, fill what is free there, from the lowest place on; then the recent ones in their
+ * order.  Keys, values and mass move together; mass_out (data NULL: mass itself) receives the mass of
+ * all kept keys and must not share memory with mass otherwise.  What lies behind the new length is
+ * undefined, nothing else is written.  Shorter sequences stay as they are.
+ *
+ * seq_len_out (it may be seq_len) receives the lengths, kept[sequence][head][kept_width], where not
+ * NULL, each new place's old one, -1 behind the new length; kept_width is at least the smaller of
+ * budget and max_seq_len.  A sequence longer than max_seq_len counts as that long.  No page may be
+ * listed twice.  Of pages that do not exist mass, keys and values read as zeros and writes are
+ * dropped. */
+typedef struct tg_kv_evict_args {
+    const tg_paged_kv* cache;
+    const tg_csr* pages;
+    const int64_t* seq_len;
+    int64_t max_seq_len;
+    int64_t budget, first, recent;
+    tg_paged_mass mass, mass_out;
+    int64_t* seq_len_out;
+    int32_t* kept;
+    int64_t kept_width;
+    uint32_t flags; /* 0 or TG_FLAG_BOUNDS_CHECK */
+} tg_kv_evict_args;
+/* Bytes of a workspace: enough for any call of the same budget and number of heads with no more
+ * sequences and listed pages and no larger max_seq_len. */
+TG_API size_t tg_kv_evict_workspace_bytes(const tg_kv_evict_args* a);
+TG_API int tg_kv_evict_f32(const tg_kv_evict_args* a, void* workspace, size_t workspace_bytes, tg_stream_t stream);
+TG_API int tg_kv_evict_f16(const tg_kv_evict_args* a, void* workspace, size_t workspace_bytes, tg_stream_t stream);
+TG_API int tg_kv_evict_bf16(const tg_kv_evict_args* a, void* workspace, size_t workspace_bytes, tg_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,528 @@
+// Eviction from a paged cache by the weight that keys have gathered (tg_kv_evict_*).
+//
+// A sequence longer than the budget is cut to it: its first places, its recent (last) ones and, for
+// each key head by itself, the heaviest of those between stay; ties go to the lowest place.  With
+// `heavy` = budget - first - recent the new places are
+//   [0, first)                     what they were,
+//   [first, first + heavy)         the chosen keys: those that lie here already stay, the others fill
+//                                  the holes, both in the order of their places,
+//   [budget - recent, budget)      the recent ones, moved down, in their order.
+// So about half of what a compaction in order would move is moved, or one key and the recent ones for
+// a sequence one over its budget; attention does not depend on the order of keys that carry their
+// positions.
+//
+// * select_kernel: a cluster of CTAs for each (sequence, key head).  Weights as ordered 32-bit
+//   integers lie in shared memory; three rounds of 11, 11 and 10 bits find the value of the
+//   heavy-th largest (histograms of all CTAs, added over the cluster), then ranks in the order of the
+//   places give the holes and the keys that fill them.
+// * move_kernel: holes are filled from places behind the budget by all CTAs side by side: such places are
+//   not written, so nothing waits.  Sources before the budget lie where recent keys go: these fills
+//   and the recent keys are one list, sorted so that a place is read before it is written, that the
+//   CTAs of one cluster go through together, reading a batch before it writes it.
+#include <cooperative_groups.h>
+
+#include <algorithm>
+
+#include "tg_paged.cuh"
+
+namespace tg {
+namespace {
+
+namespace cg = cooperative_groups;
+
+constexpr int kSelThreads = 512;
+constexpr int kSelWarps = kSelThreads / 32;
+constexpr int kBins = 2048;
+constexpr int kSelKeys = 40960;  // most weights of a CTA in shared memory; further ones are read again
+constexpr int kMoveThreads = 256;
+
+struct EvictParams {
+    tg_csr pages;
+    int64_t page_size;
+    const int64_t* seq_len;
+    int64_t *seq_len_out, n_pages;
+    int max_seq, budget, first, recent, heads, rows;
+    const float* mass;
+    float* mass_out;
+    int64_t m_page, m_slot, m_head, mo_page, mo_slot, mo_head;
+    int32_t* kept;  // [sequence][head][kept_width] or null
+    int kept_width;
+    char *k, *v;  // strides in bytes
+    int64_t k_page, k_slot, k_head, v_page, v_slot, v_head;
+    int row_bytes, moved;  // moved: mass_out is not mass
+    // workspace: of each (sequence, head) its counts, holes and the places of what fills them
+    int4* counts;  // fills, those of them from places before the new length, new length, places gone
+    int* holes;
+    int* fills;
+    int width;  // places of each
+    int parts;  // clusters of the move for each (sequence, head)
+};
+
+// A sequence as it is cut: its parts of a length.
+struct Cut {
+    int len, size, gone, first, recent, heavy;
+};
+__device__ __forceinline__ Cut cut_of(const EvictParams& p, int64_t b, int64_t& page0) {
+    int64_t npages;
+    pages_of(p.pages.indptr, p.pages.nnz, b, page0, npages);
+    Cut c;
+    const int64_t len = min(min(p.seq_len[b], npages * p.page_size), (int64_t)p.max_seq);
+    c.len = (int)max(len, (int64_t)0);
+    c.size = min(c.len, p.budget);
+    c.gone = c.len - c.size;
+    c.recent = min(p.recent, c.size);
+    c.first = min(p.first, c.size - c.recent);
+    c.heavy = c.size - c.recent - c.first;
+    return c;
+}
+
+struct Place {
+    int page, slot;  // page -1: not in the cache
+};
+__device__ __forceinline__ Place place_of(const EvictParams& p, int64_t page0, int at) {
+    const int j = at / (int)p.page_size;
+    const int64_t id = __ldg(p.pages.indices + page0 + j);
+    return {id >= 0 && id < p.n_pages ? (int)id : -1, at - j * (int)p.page_size};
+}
+__device__ __forceinline__ float mass_of(const EvictParams& p, int64_t page0, int at, int h) {
+    const Place x = place_of(p, page0, at);
+    return x.page < 0 ? 0.f : p.mass[x.page * p.m_page + x.slot * p.m_slot + h * p.m_head];
+}
+__device__ __forceinline__ void put_mass(const EvictParams& p, int64_t page0, int at, int h, float v) {
+    const Place x = place_of(p, page0, at);
+    if (x.page >= 0) p.mass_out[x.page * p.mo_page + x.slot * p.mo_slot + h * p.mo_head] = v;
+}
+// Weights in their order as integers; the two zeros are one, NaN is above all.
+__device__ __forceinline__ uint32_t ordered(float v) {
+    if (v != v) return 0xffffffffu;
+    const uint32_t u = __float_as_uint(v + 0.f);
+    return u & 0x80000000u ? ~u : u | 0x80000000u;
+}
+
+// Sum over the warps before mine, and over all, of v (the same in all lanes of a warp).
+struct Before {
+    int mine, all;
+};
+__device__ __forceinline__ Before warps_before(int v, int* s) {  // s: [kSelWarps]
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    __syncthreads();
+    if (lane == 0) s[warp] = v;
+    __syncthreads();
+    const int x = lane < kSelWarps ? s[lane] : 0;
+    return {(int)__reduce_add_sync(kFull, lane < warp ? x : 0), (int)__reduce_add_sync(kFull, x)};
+}
+// The same over the CTAs of a cluster: of what they wrote into *s.
+__device__ __forceinline__ Before ctas_before(cg::cluster_group& cl, int v, int* s) {
+    if (cl.num_blocks() == 1) return {0, v};
+    cl.sync();  // the last values have been read
+    if (threadIdx.x == 0) *s = v;
+    cl.sync();
+    Before r = {0, 0};
+    for (unsigned i = 0; i < cl.num_blocks(); ++i) {
+        const int x = *cl.map_shared_rank(s, i);
+        r.all += x;
+        if (i < cl.block_rank()) r.mine += x;
+    }
+    return r;
+}
+
+__global__ void __launch_bounds__(kSelThreads) select_kernel(const __grid_constant__ EvictParams p, const int held) {
+    extern __shared__ uint32_t s_keys[];  // [held]
+    __shared__ __align__(16) uint32_t s_hist[kBins];
+    __shared__ int s_warp[kSelWarps], s_cta, s_pick[2];
+    cg::cluster_group cl = cg::this_cluster();
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int ctas = cl.num_blocks(), rank = cl.block_rank();
+    pdl_trigger();
+    const int unit = blockIdx.x / ctas, h = unit % p.heads, b = unit / p.heads;
+    int64_t page0;
+    const Cut c = cut_of(p, b, page0);
+    const int new_end = c.first + c.heavy;  // of the new places of the chosen ones
+
+    // what stays where it is, and the ends of the lists
+    auto stays = [&](int at) {
+        if (p.moved) put_mass(p, page0, at, h, mass_of(p, page0, at, h));
+        if (p.kept) p.kept[((int64_t)b * p.heads + h) * p.kept_width + at] = at;
+    };
+    const int step = ctas * kSelThreads, me = rank * kSelThreads + tid;
+    if (p.kept)
+        for (int at = c.size + me; at < p.kept_width; at += step) p.kept[((int64_t)b * p.heads + h) * p.kept_width + at] = -1;
+    for (int at = me; at < (c.gone ? c.first : c.size); at += step) stays(at);
+    if (c.gone == 0 || c.heavy == 0) {  // the same for the whole cluster
+        if (me == 0) p.counts[unit] = make_int4(0, 0, c.size, c.gone);
+        return;
+    }
+
+    // my share of the candidates, a multiple of 32 for each warp
+    const int all = c.len - c.recent - c.first;
+    const int per_warp = ((all + ctas * kSelWarps - 1) / (ctas * kSelWarps) + 31) & ~31, per = per_warp * kSelWarps;
+    const int lo = min(rank * per, all), n = min(lo + per, all) - lo;  // candidates lo .. lo + n, from place c.first
+    const int base = c.first + lo;
+    for (int i = tid; i < min(n, held); i += kSelThreads) s_keys[i] = ordered(mass_of(p, page0, base + i, h));
+    auto key = [&](int i) { return i < held ? s_keys[i] : ordered(mass_of(p, page0, base + i, h)); };
+
+    // the value of the heavy-th largest, from its high bits on
+    uint32_t prefix = 0;
+    int need = c.heavy;  // how many of those that begin with the prefix are chosen
+    int shift = 32;
+#pragma unroll 1
+    for (int round = 0; round < 3; ++round) {
+        const int bits = round < 2 ? 11 : 10;
+        const uint32_t above = shift == 32 ? 0u : ~0u << shift;
+        shift -= bits;
+        for (int i = tid; i < kBins; i += kSelThreads) s_hist[i] = 0;
+        __syncthreads();
+        for (int i = tid; i < n; i += kSelThreads) {
+            const uint32_t k = key(i);
+            if ((k & above) == prefix) atomicAdd(&s_hist[k >> shift & ((1u << bits) - 1)], 1u);
+        }
+        cl.sync();
+        // each thread adds four bins of all CTAs; the scan goes from the highest bin down
+        const int bin0 = kBins - 4 - tid * 4;
+        uint32_t v[4] = {0, 0, 0, 0};
+        for (int r = 0; r < ctas; ++r) {
+            const uint4 x = *reinterpret_cast<const uint4*>(cl.map_shared_rank(s_hist, r) + bin0);
+            v[0] += x.x, v[1] += x.y, v[2] += x.z, v[3] += x.w;
+        }
+        const int mine = (int)(v[0] + v[1] + v[2] + v[3]);
+        int scan = mine;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int x = __shfl_up_sync(kFull, scan, o);
+            if (lane >= o) scan += x;
+        }
+        const Before w = warps_before(__shfl_sync(kFull, scan, 31), s_warp);
+        int higher = w.mine + scan - mine;  // keys in the bins above mine
+        if (higher < need && higher + mine >= need) {
+#pragma unroll
+            for (int i = 3; i >= 0; --i) {
+                if (higher < need && higher + (int)v[i] >= need) s_pick[0] = bin0 + i, s_pick[1] = need - higher;
+                higher += v[i];
+            }
+        }
+        cl.sync();  // the histograms have been read
+        prefix |= (uint32_t)s_pick[0] << shift;
+        need = s_pick[1];
+    }
+
+    // A warp's places are consecutive.  Equal ones are chosen from the lowest place on: how many lie
+    // before the warp's?
+    const int w0 = min(warp * per_warp, n), w1 = min(w0 + per_warp, n);
+    int equal = 0;
+    for (int i = w0; i < w1; i += 32) equal += __popc(__ballot_sync(kFull, i + lane < w1 && key(i + lane) == prefix));
+    Before wb = warps_before(equal, s_warp);
+    Before cb = ctas_before(cl, wb.all, &s_cta);
+    const int equal0 = cb.mine + wb.mine;
+    // walks the warp's places: what(hole, moved, place) with the masks of the 32
+    auto walk = [&](auto what) {
+        int eq = equal0;
+        for (int i = w0; i < w1; i += 32) {
+            const bool in = i + lane < w1;
+            const uint32_t k = in ? key(i + lane) : 0u;
+            const uint32_t same = __ballot_sync(kFull, in && k == prefix);
+            const bool chosen = in && (k > prefix || (k == prefix && eq + __popc(same & ((1u << lane) - 1)) < need));
+            eq += __popc(same);
+            const int at = base + i + lane;
+            const bool front = at < new_end;
+            what(__ballot_sync(kFull, in && front && !chosen), __ballot_sync(kFull, chosen && !front), at, chosen && front);
+        }
+    };
+    int holes = 0, moved = 0, early = 0;
+    walk([&](uint32_t hole, uint32_t move, int at, bool) {
+        holes += __popc(hole);
+        moved += __popc(move);
+        early += __popc(__ballot_sync(kFull, at < c.size) & move);
+    });
+    wb = warps_before(holes, s_warp);
+    cb = ctas_before(cl, wb.all, &s_cta);
+    int hole_at = cb.mine + wb.mine;
+    wb = warps_before(early, s_warp);
+    cb = ctas_before(cl, wb.all, &s_cta);
+    const int early_all = cb.all;
+    wb = warps_before(moved, s_warp);
+    cb = ctas_before(cl, wb.all, &s_cta);
+    int move_at = cb.mine + wb.mine;
+    if (me == 0) p.counts[unit] = make_int4(cb.all, early_all, c.size, c.gone);
+    int* const hole_list = p.holes + (int64_t)unit * p.width;
+    int* const fill_list = p.fills + (int64_t)unit * p.width;
+    walk([&](uint32_t hole, uint32_t move, int at, bool stay) {
+        const uint32_t below = (1u << lane) - 1;
+        if (hole >> lane & 1) hole_list[hole_at + __popc(hole & below)] = at;
+        if (move >> lane & 1) fill_list[move_at + __popc(move & below)] = at;
+        if (stay) stays(at);
+        hole_at += __popc(hole);
+        move_at += __popc(move);
+    });
+    cl.sync();  // no CTA leaves while its counts are read
+}
+
+// Rows of U bytes at a time.
+template <int U>
+struct Unit;
+template <>
+struct Unit<16> { using type = uint4; };
+template <>
+struct Unit<4> { using type = uint32_t; };
+template <>
+struct Unit<2> { using type = uint16_t; };
+
+template <int U>
+__global__ void __launch_bounds__(kMoveThreads) move_kernel(const __grid_constant__ EvictParams p) {
+    using W = typename Unit<U>::type;
+    constexpr int kAhead = 4;  // rows of a thread under way
+    cg::cluster_group cl = cg::this_cluster();
+    const int ctas = cl.num_blocks(), rank = cl.block_rank();
+    const int cluster = blockIdx.x / ctas, part = cluster % p.parts, unit = cluster / p.parts;
+    const int h = unit % p.heads, b = unit / p.heads;
+    const int words = p.row_bytes / U;
+    // lanes of a row: words of k, words of v, and one for the mass and the list of what was kept
+    const int tid = threadIdx.x, per_row = 2 * words + 1, lanes = min(per_row, kMoveThreads), group = tid / lanes,
+              groups = kMoveThreads / lanes, lane = tid - group * lanes;
+    pdl_wait();
+    const int4 n = p.counts[unit];
+    const int fills = n.x, early = n.y, size = n.z, gone = n.w;
+    if (part == 0 && h == 0 && rank == 0 && tid == 0) p.seq_len_out[b] = size;
+    if (gone == 0) return;
+    int64_t page0, npages;
+    pages_of(p.pages.indptr, p.pages.nnz, b, page0, npages);
+    const int recent = min(p.recent, size);
+    const int* const hole_list = p.holes + (int64_t)unit * p.width;
+    const int* const fill_list = p.fills + (int64_t)unit * p.width;
+
+    // Move i of the list: the early fills, the recent keys, then the other fills.
+    auto move = [&](int i, int& to, int& from) {
+        if (i < early || i >= early + recent) {
+            const int f = i < early ? i : i - recent;
+            to = hole_list[f], from = fill_list[f];
+        } else {
+            to = size - recent + i - early, from = to + gone;
+        }
+    };
+    struct Row {
+        W w;
+        char* out;
+        int mass_to;  // >= 0: the lane has the mass
+        float m;
+        int from;
+    };
+    auto load = [&](int i, int word, Row& r) {
+        int to, from;
+        move(i, to, from);
+        r.out = nullptr;
+        r.mass_to = -1;
+        if (word == 2 * words) {
+            r.mass_to = to, r.from = from;
+            r.m = mass_of(p, page0, from, h);
+            return;
+        }
+        const Place x = place_of(p, page0, from), y = place_of(p, page0, to);
+        const bool is_v = word >= words;
+        const int64_t off = (int64_t)(is_v ? word - words : word) * U;
+        memset(&r.w, 0, sizeof(W));
+        const char* in = is_v ? p.v + x.page * p.v_page + x.slot * p.v_slot + h * p.v_head
+                              : p.k + x.page * p.k_page + x.slot * p.k_slot + h * p.k_head;
+        if (x.page >= 0) r.w = *reinterpret_cast<const W*>(in + off);
+        if (y.page >= 0)
+            r.out = (is_v ? p.v + y.page * p.v_page + y.slot * p.v_slot + h * p.v_head
+                          : p.k + y.page * p.k_page + y.slot * p.k_slot + h * p.k_head) + off;
+    };
+    auto store = [&](const Row& r) {
+        if (r.out) *reinterpret_cast<W*>(r.out) = r.w;
+        if (r.mass_to >= 0) {
+            put_mass(p, page0, r.mass_to, h, r.m);
+            if (p.kept) p.kept[((int64_t)b * p.heads + h) * p.kept_width + r.mass_to] = r.from;
+        }
+    };
+
+    if (part == 0) {
+        // in order, a batch of the cluster read before it is written
+        const int list = early + recent, batch = ctas * groups * kAhead;
+        for (int w0 = 0; w0 < per_row; w0 += lanes) {
+            const int word = w0 + lane;
+            for (int i0 = 0; i0 < list; i0 += batch) {
+                Row r[kAhead];
+#pragma unroll
+                for (int k = 0; k < kAhead; ++k) {
+                    const int i = i0 + (k * ctas + rank) * groups + group;
+                    r[k].out = nullptr, r[k].mass_to = -1;
+                    if (group < groups && word < per_row && i < list) load(i, word, r[k]);
+                }
+                cl.sync();
+#pragma unroll
+                for (int k = 0; k < kAhead; ++k) store(r[k]);
+            }
+        }
+        return;
+    }
+    const int rest = fills - early, share = ((p.parts - 1) * ctas), mine = (part - 1) * ctas + rank;
+    const int begin = (int)((int64_t)rest * mine / share), end = (int)((int64_t)rest * (mine + 1) / share);
+    if (group >= groups) return;
+    for (int w0 = 0; w0 < per_row; w0 += lanes) {
+        const int word = w0 + lane;
+        if (word >= per_row) break;
+        for (int i0 = begin + group; i0 < end; i0 += groups * kAhead) {
+            Row r[kAhead];
+#pragma unroll
+            for (int k = 0; k < kAhead; ++k) {
+                r[k].out = nullptr, r[k].mass_to = -1;
+                if (i0 + k * groups < end) load(early + recent + i0 + k * groups, word, r[k]);
+            }
+#pragma unroll
+            for (int k = 0; k < kAhead; ++k) store(r[k]);
+        }
+    }
+}
+
+// ------------------------------------------------------------------ host
+struct Plan {
+    EvictParams p;
+    int unit;           // bytes moved at once
+    int select_ctas, move_ctas;
+    int held;
+    size_t bytes, counts_bytes;
+};
+
+int make_plan(const tg_kv_evict_args* a, int elem, Plan* plan, const char* op) {
+    if (!a) return set_error(TG_EINVAL, "%s: null arguments", op);
+    int rc = check_cache(a->cache, op);
+    if (rc == TG_OK && !a->pages) rc = set_error(TG_EINVAL, "%s: null page table", op);
+    if (rc != TG_OK) return rc;
+    const tg_paged_kv& c = *a->cache;
+    const tg_csr& t = *a->pages;
+    if (t.rows < 0 || t.rows > INT32_MAX || t.nnz < 0)
+        return set_error(TG_EINVAL, "%s: bad size (sequences=%lld pages=%lld)", op, (long long)t.rows, (long long)t.nnz);
+    if (t.cols != c.pages)
+        return set_error(TG_EINVAL, "%s: the page table has %lld columns and the cache %lld pages", op, (long long)t.cols,
+                         (long long)c.pages);
+    if (a->max_seq_len < 0 || a->budget < 0 || a->first < 0 || a->recent < 0)
+        return set_error(TG_EINVAL, "%s: negative max_seq_len, budget, first or recent", op);
+    if (a->flags & ~TG_FLAG_BOUNDS_CHECK) return set_error(TG_EINVAL, "%s: unknown flags 0x%x", op, a->flags);
+    if (a->kept && a->kept_width < 0) return set_error(TG_EINVAL, "%s: negative kept_width", op);
+    const int64_t slots = c.pages == 0 ? 0 : t.nnz > INT32_MAX / c.page_size ? INT32_MAX / 2 : t.nnz * c.page_size;
+    const int64_t max_seq = std::min({a->max_seq_len, slots, (int64_t)INT32_MAX / 2});
+    EvictParams& p = plan->p;
+    p = {};
+    p.pages = t, p.page_size = c.page_size, p.n_pages = c.pages;
+    p.seq_len = a->seq_len, p.seq_len_out = a->seq_len_out;
+    p.max_seq = (int)max_seq;
+    p.budget = (int)std::min<int64_t>(a->budget, INT32_MAX / 2);
+    p.first = (int)std::min<int64_t>(a->first, INT32_MAX / 2), p.recent = (int)std::min<int64_t>(a->recent, INT32_MAX / 2);
+    p.heads = c.heads, p.rows = (int)t.rows;
+    const int64_t units = t.rows * c.heads;
+    p.mass = a->mass.data, p.mass_out = a->mass_out.data ? a->mass_out.data : a->mass.data;
+    p.m_page = stride_of(c.pages, a->mass.page_stride), p.m_slot = stride_of(c.page_size, a->mass.slot_stride);
+    p.m_head = stride_of(c.heads, a->mass.head_stride);
+    const tg_paged_mass& mo = a->mass_out.data ? a->mass_out : a->mass;
+    p.mo_page = stride_of(c.pages, mo.page_stride), p.mo_slot = stride_of(c.page_size, mo.slot_stride);
+    p.mo_head = stride_of(c.heads, mo.head_stride);
+    p.moved = p.mass_out != p.mass;
+    p.kept = a->kept, p.kept_width = (int)std::min<int64_t>(a->kept_width, INT32_MAX / 2);
+    p.k = static_cast<char*>(c.k), p.v = static_cast<char*>(c.v);
+    p.k_page = stride_of(c.pages, c.k_page_stride) * elem, p.v_page = stride_of(c.pages, c.v_page_stride) * elem;
+    p.k_slot = stride_of(c.page_size, c.k_slot_stride) * elem, p.v_slot = stride_of(c.page_size, c.v_slot_stride) * elem;
+    p.k_head = stride_of(c.heads, c.k_head_stride) * elem, p.v_head = stride_of(c.heads, c.v_head_stride) * elem;
+    p.row_bytes = c.dim * elem;
+    const uint64_t all = reinterpret_cast<uint64_t>(p.k) | reinterpret_cast<uint64_t>(p.v) |
+                         (uint64_t)(p.k_page | p.k_slot | p.k_head | p.v_page | p.v_slot | p.v_head | p.row_bytes);
+    plan->unit = all % 16 == 0 ? 16 : all % 4 == 0 ? 4 : 2;
+    // most places of a sequence that fill a hole: as many as it loses, and as the chosen ones are
+    const int64_t gone = std::max<int64_t>(0, max_seq - p.budget);
+    p.width = (int)std::min<int64_t>(gone, p.budget);
+    // The selection: 8192 candidates a CTA, and more CTAs where few pairs leave SMs idle.
+    const int64_t most = gone > 0 ? max_seq : 0;
+    plan->select_ctas = 1;
+    while (plan->select_ctas < 8 && (most > 8192ll * plan->select_ctas ||
+                                     (most > 2048ll * plan->select_ctas && units * plan->select_ctas * 2 <= kSMs)))
+        plan->select_ctas *= 2;
+    plan->held = (int)std::min<int64_t>(kSelKeys, ceil_div(ceil_div(most, plan->select_ctas * kSelWarps), 32) * 32 * kSelWarps);
+    // The move: the list in order by a cluster of up to eight CTAs, 64 rows each at once; the other
+    // fills in parts of 64 rows and more, about eight CTAs an SM in all.
+    const int64_t in_order = std::min<int64_t>(p.recent, p.budget) * 2;
+    plan->move_ctas = 1;
+    while (plan->move_ctas < 8 && in_order > 64ll * plan->move_ctas) plan->move_ctas *= 2;
+    const int64_t want = std::min(ceil_div(p.width, 64 * plan->move_ctas),
+                                  std::max<int64_t>(1, kSMs * 8 / std::max<int64_t>(1, units * plan->move_ctas)));
+    p.parts = 1 + (p.width > 0 ? (int)std::max<int64_t>(1, want) : 0);
+    if (units * std::max(p.parts * plan->move_ctas, plan->select_ctas) > INT32_MAX)
+        return set_error(TG_EUNSUPPORTED, "%s: too many sequences for one launch", op);
+    plan->counts_bytes = ((size_t)units * sizeof(int4) + 255) / 256 * 256;
+    plan->bytes = plan->counts_bytes + (size_t)units * p.width * 2 * sizeof(int);
+    return TG_OK;
+}
+
+template <typename... P, typename... A>
+int launch_clusters(const char* what, void (*kernel)(P...), int64_t grid, int block, int cluster, size_t smem, bool pdl,
+                    cudaStream_t st, A... args) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)grid);
+    cfg.blockDim = dim3((unsigned)block);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute at[2];
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = (unsigned)cluster, at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+    at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = pdl ? 2 : 1;
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, static_cast<P>(args)...);
+    const int rc = check_launch(what);
+    return e != cudaSuccess ? check_cuda(e, what) : rc;
+}
+
+int evict(const tg_kv_evict_args* a, int elem, void* ws, size_t ws_bytes, tg_stream_t stream, const char* op) {
+    Plan plan;
+    int rc = make_plan(a, elem, &plan, op);
+    if (rc != TG_OK) return rc;
+    EvictParams& p = plan.p;
+    if (p.rows == 0) return TG_OK;
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    if (!a->seq_len || !a->seq_len_out || !a->pages->indptr) return set_error(TG_EINVAL, "%s: null indptr/seq_len/seq_len_out", op);
+    if (a->pages->nnz > 0 && !a->pages->indices) return set_error(TG_EINVAL, "%s: null page indices", op);
+    if (a->cache->pages > 0 && !p.mass) return set_error(TG_EINVAL, "%s: null mass", op);
+    if (a->kept && p.kept_width < std::min<int64_t>(p.budget, p.max_seq))
+        return set_error(TG_EINVAL, "%s: kept has %d places, not the %lld that may be kept", op, p.kept_width,
+                         (long long)std::min<int64_t>(p.budget, p.max_seq));
+    if (a->flags & TG_FLAG_BOUNDS_CHECK) {
+        rc = paged_bounds_check(*a->pages, p.page_size, a->seq_len, a->max_seq_len, p.rows, nullptr, 1, nullptr, 0, false, op, st);
+        if (rc != TG_OK) return rc;
+    }
+    if (ws_bytes < plan.bytes || (plan.bytes && !ws))
+        return set_error(TG_EINVAL, "%s: workspace of %zu bytes needed (got %zu)", op, plan.bytes, ws_bytes);
+    if (reinterpret_cast<uintptr_t>(ws) % 16) return set_error(TG_EINVAL, "%s: the workspace must be 16-byte aligned", op);
+    p.counts = static_cast<int4*>(ws);
+    p.holes = reinterpret_cast<int*>(static_cast<char*>(ws) + plan.counts_bytes);
+    p.fills = p.holes + (int64_t)p.rows * p.heads * p.width;
+    const int64_t units = (int64_t)p.rows * p.heads;
+    const size_t smem = (size_t)plan.held * sizeof(uint32_t);
+    static SmemOnce once;
+    rc = once.raise(reinterpret_cast<const void*>(select_kernel), kSelKeys * (int)sizeof(uint32_t));
+    if (rc != TG_OK) return rc;
+    rc = launch_clusters("select_kernel", select_kernel, units * plan.select_ctas, kSelThreads, plan.select_ctas, smem, false, st, p,
+                         plan.held);
+    if (rc != TG_OK) return rc;
+    auto kernel = plan.unit == 16 ? move_kernel<16> : plan.unit == 4 ? move_kernel<4> : move_kernel<2>;
+    return launch_clusters("move_kernel", kernel, units * p.parts * plan.move_ctas, kMoveThreads, plan.move_ctas, 0, true, st, p);
+}
+
+}  // namespace
+}  // namespace tg
+
+extern "C" {
+
+size_t tg_kv_evict_workspace_bytes(const tg_kv_evict_args* a) {
+    tg::Plan plan;
+    return tg::make_plan(a, 4, &plan, "tg_kv_evict") == TG_OK ? plan.bytes : 0;
+}
+
+int tg_kv_evict_f32(const tg_kv_evict_args* a, void* workspace, size_t workspace_bytes, tg_stream_t stream) {
+    return tg::evict(a, 4, workspace, workspace_bytes, stream, "tg_kv_evict_f32");
+}
+int tg_kv_evict_f16(const tg_kv_evict_args* a, void* workspace, size_t workspace_bytes, tg_stream_t stream) {
+    return tg::evict(a, 2, workspace, workspace_bytes, stream, "tg_kv_evict_f16");
+}
+int tg_kv_evict_bf16(const tg_kv_evict_args* a, void* workspace, size_t workspace_bytes, tg_stream_t stream) {
+    return tg::evict(a, 2, workspace, workspace_bytes, stream, "tg_kv_evict_bf16");
+}
+
+}  // extern "C"

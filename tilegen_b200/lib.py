@@ -242,6 +242,24 @@ class TgAttentionMassArgs(ctypes.Structure):
     ]
 
 
+class TgKvEvictArgs(ctypes.Structure):
+    _fields_ = [
+        ("cache", ctypes.c_void_p),  # TgPagedKV
+        ("pages", ctypes.c_void_p),  # TgCsr
+        ("seq_len", ctypes.c_void_p),
+        ("max_seq_len", ctypes.c_int64),
+        ("budget", ctypes.c_int64),
+        ("first", ctypes.c_int64),
+        ("recent", ctypes.c_int64),
+        ("mass", TgPagedMass),
+        ("mass_out", TgPagedMass),
+        ("seq_len_out", ctypes.c_void_p),
+        ("kept", ctypes.c_void_p),
+        ("kept_width", ctypes.c_int64),
+        ("flags", ctypes.c_uint32),
+    ]
+
+
 _I64 = ctypes.c_int64
 _P = ctypes.c_void_p
 _F64 = ctypes.c_double
@@ -334,6 +352,8 @@ SIGNATURES_PAGED = {
     "tg_attention_mass_workspace_bytes": (_SZ, [ctypes.POINTER(TgAttentionMassArgs)]),
     "tg_attention_mass_f16": (ctypes.c_int, [ctypes.POINTER(TgAttentionMassArgs), _P, _SZ, _P]),
     "tg_attention_mass_bf16": (ctypes.c_int, [ctypes.POINTER(TgAttentionMassArgs), _P, _SZ, _P]),
+    "tg_kv_evict_workspace_bytes": (_SZ, [ctypes.POINTER(TgKvEvictArgs)]),
+    **{"tg_kv_evict_" + t: (ctypes.c_int, [ctypes.POINTER(TgKvEvictArgs), _P, _SZ, _P]) for t in _TYPES},
 }
 
 _lib: Optional[ctypes.CDLL] = None

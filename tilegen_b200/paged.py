@@ -29,7 +29,8 @@ from .device import _dev
 
 __all__ = ["Rope", "rope_frequencies", "rope", "rope_backward", "HeadNorm", "norm_rope", "norm_rope_backward",
            "norm_rope_backward_workspace_bytes", "PagedKV", "PageTable", "kv_append", "prefix_attention",
-           "prefix_attention_workspace_bytes", "empty_mass", "attention_mass", "attention_mass_workspace_bytes"]
+           "prefix_attention_workspace_bytes", "empty_mass", "attention_mass", "attention_mass_workspace_bytes", "kv_evict",
+           "kv_evict_workspace_bytes"]
 
 _SUFFIX = {torch.float32: "f32", torch.float16: "f16", torch.bfloat16: "bf16"}
 _LAYOUT = {"half": _lib.TG_ROPE_HALF, "interleaved": _lib.TG_ROPE_INTERLEAVED}
@@ -720,3 +721,86 @@ def attention_mass_workspace_bytes(q: torch.Tensor, cache: PagedKV, table: PageT
     head sizes with no larger max_q_len (0 for few rows)."""
     m, _held = _mass_args(None, q, cache, table, seq_len, None, q_indptr, max_q_len, None, None, True, 1.0, False)
     return int(_call("tg_attention_mass_workspace_bytes")(m))
+
+
+def _evict_args(cache, table, seq_len, budget, first, recent, max_seq_len, check):
+    kv = cache.desc()
+    index = cache.k.get_device()
+    tb = table.desc(index, kv.pages)
+    slots = tb.nnz * kv.page_size
+    a = _lib.TgKvEvictArgs(ctypes.addressof(kv), ctypes.addressof(tb), _vector(seq_len, "seq_len", index, tb.rows),
+                           slots if max_seq_len is None else max_seq_len, budget, first, recent)
+    a.flags = _lib.TG_FLAG_BOUNDS_CHECK if check else 0
+    return a, (kv, tb), max(0, min(budget, slots, a.max_seq_len))
+
+
+def kv_evict(cache: PagedKV, table: PageTable, seq_len: torch.Tensor, mass: torch.Tensor, budget: int, first: int = 0,
+             recent: int = 0, max_seq_len: Optional[int] = None, mass_out: Optional[torch.Tensor] = None,
+             kept: Union[bool, torch.Tensor] = False, seq_len_out: Optional[torch.Tensor] = None,
+             workspace: Optional[torch.Tensor] = None, check: bool = False, stream: Optional[torch.cuda.Stream] = None):
+    """Cuts every sequence longer than budget to it, in place, and returns the new lengths (int64;
+    seq_len_out, which may be seq_len, or a new tensor).
+
+    For each key head by itself the first `first` keys, the last `recent` ones and, of those between,
+    the ones with the largest mass [pages, page_size, heads] stay: equal ones from the lowest place on,
+    NaN counts as the largest.  Where the budget is smaller than first + recent, recent goes first.  The
+    first keys stay in place; chosen ones that lie within the next budget - first - recent places stay,
+    the others fill the free places there, in order; the recent ones follow, in order.  So the order of
+    a sequence's keys changes between `first` and `recent`, which attention does not see: keys carry
+    their positions.  From then on new tokens' positions are not their places, and kv_append takes
+    ``positions``.  Moving the recent keys costs their bytes each time: a server lets sequences grow some
+    tokens over their budget and evicts every few steps.
+
+    Keys, values and mass move together; with mass_out (same shape, any strides) the mass of all kept
+    keys is written there and mass itself is not changed.  ``kept=True`` (or an int32 [sequences, heads,
+    width] tensor, width at least min(budget, max_seq_len)) returns (lengths, old place of each new one,
+    -1 behind the length).  Pages behind the new length may be given back; what they and the rest of the
+    last page hold is undefined.  No page may be in the table twice.  max_seq_len bounds the lengths (a
+    longer sequence counts as that long; default: what the listed pages hold).  ``workspace``:
+    kv_evict_workspace_bytes, allocated on the call's stream where it is not given.  No gradient goes
+    through it."""
+    a, _held, width = _evict_args(cache, table, seq_len, budget, first, recent, max_seq_len, check)
+    index = cache.k.get_device()
+    a.mass = _mass_desc(mass, "mass", cache, index)
+    if mass_out is not None and mass_out is not mass:
+        a.mass_out = _mass_desc(mass_out, "mass_out", cache, index)
+        if a.mass_out.data == a.mass.data and mass_out.stride() != mass.stride():
+            raise ValueError("mass_out must be mass or not share memory with it")
+    sp = _stream(index, stream)
+    where = _elsewhere(index, stream)
+    if where is not None:
+        with where:
+            return _evict_launch(a, seq_len, seq_len_out, kept, width, workspace, cache, index, sp)
+    return _evict_launch(a, seq_len, seq_len_out, kept, width, workspace, cache, index, sp)
+
+
+def _evict_launch(a, seq_len, seq_len_out, kept, width, workspace, cache, index, sp):
+    if seq_len_out is None:
+        seq_len_out = torch.empty_like(seq_len)
+    a.seq_len_out = _vector(seq_len_out, "seq_len_out", index, seq_len.shape[0])
+    shape = (seq_len.shape[0], cache.k.shape[2])
+    if kept is True:
+        kept = torch.empty(*shape, width, dtype=torch.int32, device=seq_len.device)
+    if isinstance(kept, torch.Tensor):
+        if kept.dim() != 3 or kept.shape[:2] != shape or kept.shape[2] < width or kept.dtype is not torch.int32 \
+                or kept.get_device() != index or not kept.is_contiguous():
+            raise ValueError("kept must be a contiguous int32 tensor [%d, %d, at least %d] on cuda:%d (got %s %s on %s)"
+                             % (*shape, width, index, tuple(kept.shape), kept.dtype, kept.device))
+        a.kept, a.kept_width = kept.data_ptr(), kept.shape[2]
+    need = _call("tg_kv_evict_workspace_bytes")(a)
+    ws = size = 0
+    if workspace is None and need:
+        workspace, size = torch.empty(need, dtype=torch.uint8, device=seq_len.device), need
+        ws = workspace.data_ptr()
+    elif workspace is not None:
+        ws, size = _workspace(workspace, need, index)
+    _lib.check(_call("tg_kv_evict_" + _SUFFIX[cache.k.dtype])(a, ws, size, sp), "tg_kv_evict")
+    return (seq_len_out, kept) if isinstance(kept, torch.Tensor) else seq_len_out
+
+
+def kv_evict_workspace_bytes(cache: PagedKV, table: PageTable, seq_len: torch.Tensor, budget: int,
+                             max_seq_len: Optional[int] = None) -> int:
+    """Bytes of a workspace to keep for kv_evict: enough for any call of the same budget on this cache with
+    no more sequences and listed pages and no larger max_seq_len."""
+    a, _held, _ = _evict_args(cache, table, seq_len, budget, 0, 0, max_seq_len, False)
+    return int(_call("tg_kv_evict_workspace_bytes")(a))
