@@ -64,13 +64,16 @@ __device__ __forceinline__ int64_t slot_of_token(const NewTokens& p, int64_t t, 
 }
 
 // scale * (cos, sign * sin) of position * freq.  The angle and its rest after whole turns (2 pi in two
-// parts, after Cody and Waite) are 64-bit.
+// parts, after Cody and Waite) are 64-bit.  QUICK: sine and cosine of the rest by the special-function
+// unit, 2^-21 off (absolute), a quarter of the instructions: for outputs of 16 bits.
+template <bool QUICK = false>
 __device__ __forceinline__ float2 turn_of(double position, double freq, float scale, float sign) {
     const double t = position * freq;
     const double whole = rint(t * 0.15915494309189533577);  // turns
     const double rest = fma(-whole, 2.4492935982947064e-16, fma(-whole, 6.283185307179586, t));  // 2 pi in two parts
     float s, c;
-    sincospif((float)(rest * 0.31830988618379067154), &s, &c);
+    if constexpr (QUICK) __sincosf((float)rest, &s, &c);
+    else sincospif((float)(rest * 0.31830988618379067154), &s, &c);
     return make_float2(c * scale, s * scale * sign);
 }
 
