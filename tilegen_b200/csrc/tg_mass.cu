@@ -2,23 +2,29 @@
 //   mass[key] = decay mass[key] + sum over the rows r that see it of exp(scale q_r k - lse_r),
 // the rows being the new tokens of the key's sequence times the query heads of its key head.
 //
-// A step is S^T = K Q^T of 128 keys and up to 256 rows: the keys lie along the lanes of TMEM, so a
-// thread has one key, its sum over the rows crosses no lanes, and a key that is NaN or lies behind the
-// sequence stays its own affair.  Two warpgroups take turns, so that one's exponentials run while the
-// tensor core works for the other.
+// A step is S^T = K Q^T of 128 keys and up to 128 rows (tcgen05): the keys lie along the lanes of TMEM,
+// so a thread has one key, its sum over the rows crosses no lanes, and a key that is NaN or lies behind
+// the sequence stays its own affair.  Two warpgroups make exponentials and sums, each from two buffers
+// of 128 rows, so that the tensor core works meanwhile.  Sums are 32-bit and in a fixed order: calls are
+// bit identical.
 //
-//   TMEM columns      [0,256) S^T of warpgroup 0    [256,512) of warpgroup 1
-//   warps 0-3, 4-7    exponentials and sums of every other step
-//   warp 8            fetches tiles of keys into a ring of shared memory by TMA, in boxes of as many
-//                     rows as divide both a page and a tile
+//   TMEM columns      [0,128) [128,256) S^T of warpgroup 0    [256,384) [384,512) of warpgroup 1
+//   warps 0-3, 4-7    exponentials and sums of the even and the odd tiles of keys
+//   warp 8            fetches tiles of keys by TMA, in boxes of as many rows as divide both a page and
+//                     a tile
 //   warp 9            issues the matrix instructions
 //   warp 10           fetches queries by TMA (a box of tokens times heads), and for each row its lse
 //                     and how many keys it sees
+//   warp 11           looks up the pages of the next unit's keys
 //
-// CTAs are persistent; a unit of work is (part of the row tiles, chunk of keys, sequence, key head).
-// A unit with one row tile (decoding; the last tokens of a prompt) writes its sums as they come, the
-// others keep them in shared memory, one place for each thread, until all row tiles are done.  Sums
-// are 32-bit, in a fixed order: calls are bit identical.
+// * Up to 256 rows of a key head (decoding; the last tokens of a prompt): bound by the keys' bytes.  The
+//   rows stay in shared memory, the keys pass through a ring (stream_kernel).
+// * More rows: bound by the exponentials, 16 a cycle and SM.  A chunk of 512 keys stays, the rows pass
+//   through a ring (rows_kernel), and a thread's sums stay in registers until all rows have passed.
+//
+// CTAs are persistent; a unit of work is (chunk of keys, part of the row tiles) of a (sequence, key
+// head).  Each CTA counts the units of all sequences at its begin and takes every gridDim.x-th, so that
+// ragged lengths and the causal mask leave no holes in the shares.
 #include <algorithm>
 #include <numeric>
 
@@ -28,11 +34,13 @@ namespace tg {
 namespace {
 
 constexpr int kTile = 128;      // keys of a step
-constexpr int kMostRows = 256;  // rows of a row tile: columns of an instruction
+constexpr int kHalfRows = 128;  // rows of a buffer in TMEM
+constexpr int kMostRows = 256;  // rows of a key head that stay in shared memory
 constexpr int kThreads = 384;
 constexpr uint32_t kCols = 512;
 constexpr int kStagesMax = 8;
 constexpr int kChunkMax = 8;  // most tiles of a chunk of keys
+constexpr int kSeqs = 512;    // sequences of a launch
 
 struct MassParams : AttnParams {
     const float* row_lse;
@@ -41,28 +49,35 @@ struct MassParams : AttnParams {
     float decay;
     // rows: tiles of tile_tokens tokens and tile_heads query heads, head_tiles of them side by side
     int tile_tokens, tile_heads, head_tiles, tile_rows;  // tile_rows: columns of the instructions, a multiple of 16
+    int stream;                                          // stream_kernel: one row tile
     int chunk, chunks, splits, split_tiles;              // tiles of keys of a chunk; row tiles of a part
-    int units, q_bufs, stages;
-    float* part;  // with splits > 1: [split][chunk][sequence][key head][key of the chunk]
+    int box, box_shift;                                  // keys of a box, their log2
+    int q_bufs, stages;
+    int first_seq, seqs;  // of this launch
+    float* part;          // with splits > 1: [split][chunk][sequence][key head][key of the chunk]
 };
 
 struct MassShared {
-    uint64_t q_full[2], q_empty[2], i_full[2], i_empty[2], full[kStagesMax], empty[kStagesMax], s_full[2], s_empty[2], drained;
+    uint64_t q_full[4], q_empty[4], i_full[2], i_empty[2], p_full[2], p_empty[2], full[kStagesMax], empty[kStagesMax], s_full[4],
+        s_empty[4], drained;
     uint32_t tmem;
     int fail;
-    int fewest[2], rows[2];          // keys that every row of the tile sees; rows
-    float lse2[2][kMostRows];        // lse * log2 e
-    int seen[2][kMostRows];          // keys that a row sees, 0 for what is no row
-    float acc[2][kChunkMax * kTile];  // [warpgroup][key of the chunk]
+    int fewest[2], rows[2];                            // keys that every row of the tile sees; rows
+    __align__(16) float lse2[2][kMostRows];            // -lse * log2 e
+    __align__(16) int seen[2][kMostRows];              // keys that a row sees, 0 for what is no row
+    int page[2][kChunkMax * kTile];                    // pages of a unit's boxes, -1: not in the cache
+    int64_t page0[kSeqs];
+    int first[kSeqs], n[kSeqs], len[kSeqs];
+    int before[kSeqs + 1];  // units of the sequences before
 };
-
 constexpr int kSmem = 226 * 1024;
 constexpr int kTiles = kSmem - ((int)sizeof(MassShared) + 1023) / 1024 * 1024;  // of them for queries and keys
+static_assert(kTiles >= 192 * 1024, "a chunk of keys and two row tiles");
 
 struct Unit {
     Sequence s;
-    int h, k0, keys, q0, q1, tiles;  // keys k0 .. k0 + keys, row tiles q0 .. q1, tiles of keys
-    int id;
+    int b, h, k0, keys, q0, q1, tiles;  // keys k0 .. k0 + keys, row tiles q0 .. q1, tiles of keys
+    int split, c;
 };
 
 __device__ __forceinline__ int row_tiles(const MassParams& p, const Sequence& s) {
@@ -74,46 +89,155 @@ __device__ __forceinline__ int steps_of(const MassParams& p, const Unit& u, int 
     const int seen = min(keys_seen(p, u.s, last, u.s.len, u.s.len) - u.k0, u.keys);
     return seen > 0 ? (seen + kTile - 1) / kTile : 0;
 }
+// With several parts of the row tiles: those that see keys from k0 on are part `first` to the last, none
+// where first is `all`.  (Parts have whole tokens: head_tiles is 1.)
+__device__ __forceinline__ int first_split(const MassParams& p, const Sequence& s, int k0, int& all) {
+    all = (row_tiles(p, s) + p.split_tiles - 1) / p.split_tiles;
+    if (!p.causal) return 0;
+    const int64_t behind = (int64_t)k0 - s.len + s.n;  // token i sees them where i >= behind
+    if (behind >= s.asked) return all;
+    return behind <= 0 ? 0 : (int)behind / (p.split_tiles * p.tile_tokens);
+}
+// Units of a sequence and one key head.
+__device__ __forceinline__ int units_of(const MassParams& p, const Sequence& s) {
+    const int step = p.chunk * kTile;
+    if (p.splits == 1) return s.n == 0 && p.decay == 1.f ? 0 : (s.len + step - 1) / step;  // (the old weights stay)
+    int units = 0;
+    for (int k0 = 0; k0 < s.len; k0 += step) {
+        int all;
+        const int first = first_split(p, s, k0, all);
+        units += all - first;
+    }
+    return units;
+}
+
+// Fills the table of the launch's sequences; by all threads.
+__device__ __forceinline__ void count_units(const MassParams& p, MassShared& sh) {
+    for (int i = threadIdx.x; i < kSeqs; i += kThreads) {
+        int units = 0;
+        if (i < p.seqs) {
+            const Sequence s = sequence(p, p.first_seq + i);
+            sh.page0[i] = s.page0, sh.first[i] = s.first, sh.n[i] = s.n, sh.len[i] = s.len;
+            units = units_of(p, s) * p.kv_heads;
+        }
+        sh.before[i + 1] = units;
+    }
+    __syncthreads();
+    if (threadIdx.x < 32) {
+        constexpr int kEach = kSeqs / 32;
+        int v[kEach], sum = 0;
+#pragma unroll
+        for (int i = 0; i < kEach; ++i) sum += v[i] = sh.before[threadIdx.x * kEach + i + 1];
+        int scan = sum;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int x = __shfl_up_sync(kFull, scan, o);
+            if ((int)threadIdx.x >= o) scan += x;
+        }
+        scan -= sum;
+        if (threadIdx.x == 0) sh.before[0] = 0;
+#pragma unroll
+        for (int i = 0; i < kEach; ++i) sh.before[threadIdx.x * kEach + i + 1] = scan += v[i];
+    }
+}
 
 // The units of a CTA, the same for all its warps.
 struct Units {
-    int at;
-    __device__ __forceinline__ Units() : at(blockIdx.x) {}
-    __device__ __forceinline__ bool next(const MassParams& p, Unit& u) {
-        for (; at < p.units; at += gridDim.x) {
-            int x = at;
-            u.id = at;
-            u.h = x % p.kv_heads, x /= p.kv_heads;
-            const int b = x % p.rows;
-            x /= p.rows;
-            const int c = x % p.chunks, split = x / p.chunks;
-            u.s = sequence(p, b);
-            u.k0 = c * p.chunk * kTile;
-            u.keys = min(u.s.len - u.k0, p.chunk * kTile);
-            if (u.keys <= 0) continue;
-            u.tiles = (u.keys + kTile - 1) / kTile;
-            const int all = row_tiles(p, u.s);
-            u.q0 = split * p.split_tiles;
-            u.q1 = min(u.q0 + p.split_tiles, all);
-            // nothing to add: the join does not ask for the part, or the old weight stays
-            if (p.splits > 1 ? u.q1 <= u.q0 || steps_of(p, u, u.q1 - 1) == 0 : u.s.n == 0 && p.decay == 1.f) continue;
-            at += gridDim.x;
-            return true;
+    int at, turn;  // turn: units so far
+    __device__ __forceinline__ Units() : at(blockIdx.x), turn(-1) {}
+    __device__ __forceinline__ bool next(const MassParams& p, const MassShared& sh, Unit& u) {
+        if (at >= sh.before[kSeqs]) return false;
+        ++turn;
+        // the sequence: the last one with no more units before it
+        const int lane = threadIdx.x & 31;
+        constexpr int kEach = kSeqs / 32;
+        const int coarse = 31 - __clz(__ballot_sync(kFull, sh.before[lane * kEach] <= at));
+        const uint32_t fine = __ballot_sync(kFull, lane < kEach && sh.before[coarse * kEach + (lane & (kEach - 1))] <= at);
+        const int i = coarse * kEach + 31 - __clz(fine);
+        int x = at - sh.before[i];
+        at += gridDim.x;
+        u.b = p.first_seq + i;
+        u.s.page0 = sh.page0[i], u.s.first = sh.first[i], u.s.n = sh.n[i], u.s.len = sh.len[i];
+        u.s.asked = min(u.s.n, p.max_q);
+        u.h = x % p.kv_heads;
+        x /= p.kv_heads;
+        const int step = p.chunk * kTile;
+        u.c = x, u.split = 0;
+        if (p.splits > 1) {
+            for (u.c = 0;; ++u.c) {
+                int all;
+                const int first = first_split(p, u.s, u.c * step, all);
+                if (x < all - first) {
+                    u.split = first + x;
+                    break;
+                }
+                x -= all - first;
+            }
         }
-        return false;
+        u.k0 = u.c * step;
+        u.keys = min(u.s.len - u.k0, step);
+        u.tiles = (u.keys + kTile - 1) / kTile;
+        u.q0 = u.split * p.split_tiles;
+        u.q1 = min(u.q0 + p.split_tiles, row_tiles(p, u.s));
+        return true;
     }
 };
 
-// Where a key's weight is kept; null where its page does not exist.
-__device__ __forceinline__ float* mass_at(const MassParams& p, const Unit& u, int key) {
-    int page, slot;
-    locate(p, p.indices + u.s.page0, key, page, slot);
-    return page < 0 ? nullptr : p.mass + page * p.m_page + slot * p.m_slot + u.h * p.m_head;
+// Where the sums of a unit start among the parts.
+__device__ __forceinline__ int64_t part_at(const MassParams& p, const Unit& u) {
+    return ((((int64_t)u.split * p.chunks + u.c) * p.rows + u.b) * p.kv_heads + u.h) * (p.chunk * kTile);
+}
+__device__ __forceinline__ int slot_of(const MassParams& p, int key) {
+    return p.page_shift >= 0 ? key & (p.page_size - 1) : key % p.page_size;
+}
+// Where key `at` of the unit keeps its weight, by the table of its pages; null where there is no such
+// page or key.
+__device__ __forceinline__ float* mass_at(const MassParams& p, const Unit& u, const int* pages, int at) {
+    if (at >= u.keys) return nullptr;
+    const int page = pages[at >> p.box_shift];
+    return page < 0 ? nullptr : p.mass + page * p.m_page + slot_of(p, u.k0 + at) * p.m_slot + u.h * p.m_head;
 }
 // Whether what a key has gathered is kept: not that of the call's own tokens, whose slots hold the
 // weights of whoever had them before, and not where decay is 0.
 __device__ __forceinline__ bool has_old(const MassParams& p, const Unit& u, int key) {
     return p.decay != 0.f && !(p.causal && key >= u.s.len - u.s.n);
+}
+__device__ __forceinline__ void put(const MassParams& p, const Unit& u, int key, float* to, float old, float sum) {
+    if (to) *to = has_old(p, u, key) ? fmaf(old, p.decay, sum) : sum;
+}
+
+// A key's sum over COLS rows of S^T: their -lse * log2 e and the keys that they see.  ALL: each sees the
+// key.
+template <int COLS, bool ALL>
+__device__ __forceinline__ float weigh(const uint32_t (&s)[COLS], const float* lse2, const int* seen, int key, float scale) {
+    const float4* l4 = reinterpret_cast<const float4*>(lse2);
+    if constexpr (ALL) {
+        uint64_t part[2] = {0, 0};
+        const uint64_t sc = pair(scale, scale);
+#pragma unroll
+        for (int e = 0; e < COLS; e += 4) {
+            const float4 l = l4[e / 4];
+            const float2 x = both(fma2(pair(__uint_as_float(s[e]), __uint_as_float(s[e + 1])), sc, pair(l.x, l.y)));
+            const float2 y = both(fma2(pair(__uint_as_float(s[e + 2]), __uint_as_float(s[e + 3])), sc, pair(l.z, l.w)));
+            part[0] = add2(part[0], pair(exp2_fast(x.x), exp2_fast(x.y)));
+            part[1] = add2(part[1], pair(exp2_fast(y.x), exp2_fast(y.y)));
+        }
+        const float2 v = both(add2(part[0], part[1]));
+        return v.x + v.y;
+    } else {
+        const int4* n4 = reinterpret_cast<const int4*>(seen);
+        float part = 0.f;
+#pragma unroll
+        for (int e = 0; e < COLS; e += 4) {
+            const float4 l = l4[e / 4];
+            const int4 n = n4[e / 4];
+            part += key < n.x ? exp2_fast(fmaf(__uint_as_float(s[e]), scale, l.x)) : 0.f;
+            part += key < n.y ? exp2_fast(fmaf(__uint_as_float(s[e + 1]), scale, l.y)) : 0.f;
+            part += key < n.z ? exp2_fast(fmaf(__uint_as_float(s[e + 2]), scale, l.z)) : 0.f;
+            part += key < n.w ? exp2_fast(fmaf(__uint_as_float(s[e + 3]), scale, l.w)) : 0.f;
+        }
+        return part;
+    }
 }
 
 __device__ __forceinline__ void load_box3(uint32_t dst, const CUtensorMap* map, int x, int y, int z, uint32_t bar) {
@@ -125,24 +249,25 @@ __device__ __forceinline__ void load_box3(uint32_t dst, const CUtensorMap* map, 
         : "memory");
 }
 
-// DIM: head size rounded up to 64 elements; KSTEPS: 16 elements each.
-template <typename T, int DIM, int KSTEPS>
-__global__ void __launch_bounds__(kThreads, 1) mass_kernel(const __grid_constant__ MassParams p, const int box,
-                                                           const __grid_constant__ CUtensorMap kmap,
-                                                           const __grid_constant__ CUtensorMap qmap) {
-    constexpr int kHalves = DIM / 64;
-    constexpr int kBlock = kTile * DIM * 2;
-    constexpr int kHalf = kTile * 128;
-    extern __shared__ __align__(1024) unsigned char smem[];
-    MassShared& sh = *reinterpret_cast<MassShared*>(smem + kTiles);
-    const int tid = threadIdx.x, warp = __shfl_sync(kFull, tid >> 5, 0), lane = tid & 31;
-    const int q_half = p.tile_rows * 128, q_block = q_half * kHalves;
-    const uint32_t sq = smem_addr(smem), ring = sq + p.q_bufs * q_block;
-    const uint32_t b_full = smem_addr(sh.full), b_empty = smem_addr(sh.empty), b_qf = smem_addr(sh.q_full),
-                   b_qe = smem_addr(sh.q_empty), b_if = smem_addr(sh.i_full), b_ie = smem_addr(sh.i_empty),
-                   b_sf = smem_addr(sh.s_full), b_se = smem_addr(sh.s_empty);
-    volatile int* fail = &sh.fail;
 
+// What the warps of a CTA share: addresses of its memory and barriers.
+struct Cta {
+    MassShared& sh;
+    uint32_t sq, ring, tmem, b_full, b_empty, b_qf, b_qe, b_if, b_ie, b_pf, b_pe, b_sf, b_se;
+    int q_half, q_block;  // bytes of 64 columns of a row tile, and of the whole tile
+    volatile int* fail;
+};
+
+template <int DIM>
+__device__ __forceinline__ Cta enter(const MassParams& p, unsigned char* smem, int warp, int lane) {
+    MassShared& sh = *reinterpret_cast<MassShared*>(smem + kTiles);
+    Cta c{sh};
+    c.q_half = p.tile_rows * 128, c.q_block = c.q_half * (DIM / 64);
+    c.sq = smem_addr(smem), c.ring = c.sq + p.q_bufs * c.q_block;
+    c.b_full = smem_addr(sh.full), c.b_empty = smem_addr(sh.empty), c.b_qf = smem_addr(sh.q_full), c.b_qe = smem_addr(sh.q_empty);
+    c.b_if = smem_addr(sh.i_full), c.b_ie = smem_addr(sh.i_empty), c.b_pf = smem_addr(sh.p_full), c.b_pe = smem_addr(sh.p_empty);
+    c.b_sf = smem_addr(sh.s_full), c.b_se = smem_addr(sh.s_empty);
+    c.fail = &sh.fail;
     if (warp == 9) {
         tmem_alloc(smem_addr(&sh.tmem), kCols);
         if (lane == 0) {
@@ -151,10 +276,14 @@ __global__ void __launch_bounds__(kThreads, 1) mass_kernel(const __grid_constant
                 mbar_init(&sh.empty[i], 1);
             }
             for (int i = 0; i < 2; ++i) {
-                mbar_init(&sh.q_full[i], 1);
-                mbar_init(&sh.q_empty[i], 1);
                 mbar_init(&sh.i_full[i], 1);
                 mbar_init(&sh.i_empty[i], 8);
+                mbar_init(&sh.p_full[i], 1);
+                mbar_init(&sh.p_empty[i], 9);
+            }
+            for (int i = 0; i < 4; ++i) {
+                mbar_init(&sh.q_full[i], 1);
+                mbar_init(&sh.q_empty[i], 1);
                 mbar_init(&sh.s_full[i], 1);
                 mbar_init(&sh.s_empty[i], 4);
             }
@@ -163,246 +292,395 @@ __global__ void __launch_bounds__(kThreads, 1) mass_kernel(const __grid_constant
             fence_mbar_init();
         }
     }
-    for (int i = tid; i < 2 * kChunkMax * kTile; i += kThreads) (&sh.acc[0][0])[i] = 0.f;
+    count_units(p, sh);
     fence_before();
     __syncthreads();
     fence_after();
-    const uint32_t tmem = sh.tmem;
+    c.tmem = sh.tmem;
+    return c;
+}
+__device__ __forceinline__ void leave(const Cta& c, int warp) {
+    __syncwarp();
+    __syncthreads();
+    if (warp == 9) {
+        fence_after();
+        tmem_free(c.tmem, kCols);
+    }
+}
+
+// S^T of a tile of keys and `rows` rows into a buffer, whose barrier completes with it.
+template <typename T, int KSTEPS>
+__device__ __forceinline__ void product(const Cta& c, uint32_t k, uint32_t q, int rows, int buf) {
+    constexpr uint32_t kType = std::is_same<T, __half>::value ? 0 : 1;
+    constexpr int kHalf = kTile * 128;
+    const uint32_t idesc = 1u << 4 | kType << 7 | kType << 10 | (kTile / 16) << 24 | (uint32_t)(rows / 8) << 17;
+#pragma unroll
+    for (int kk = 0; kk < KSTEPS; ++kk)
+        mma_ss(c.tmem + buf * kHalfRows, operand(k + (kk >> 2) * kHalf + (kk & 3) * 32, 16),
+               operand(q + (kk >> 2) * c.q_half + (kk & 3) * 32, 16), idesc, kk > 0);
+    commit(c.b_sf + buf * 8);
+}
+
+// Warp 11: the pages of each unit's boxes.
+__device__ __forceinline__ void find_pages(const MassParams& p, const Cta& c, int lane) {
+    Units units;
+    Unit u;
+    bool ok = true;
+    while (ok && units.next(p, c.sh, u)) {
+        const int buf = units.turn & 1;
+        ok = units.turn < 2 || wait_warp(c.b_pe + buf * 8, (units.turn / 2 - 1) & 1, c.fail);
+        if (!ok) break;
+        const int64_t* list = p.indices + u.s.page0;
+        for (int i = lane; i << p.box_shift < u.keys; i += 32) {
+            int page, slot;
+            locate(p, list, u.k0 + (i << p.box_shift), page, slot);
+            c.sh.page[buf][i] = page;
+        }
+        __syncwarp();
+        if (lane == 0) arrive(c.b_pf + buf * 8);
+    }
+}
+
+// A tile of keys from the unit's key `at` on into shared memory.  A box past the end is not fetched; a page
+// that does not exist is fetched from behind the last one, which reads as zeros.
+template <int DIM>
+__device__ __forceinline__ void fetch_keys(const MassParams& p, const Cta& c, const Unit& u, const int* pages, int at, uint32_t dst,
+                                           uint64_t* land, const CUtensorMap* map, int lane) {
+    const int boxes = (min(kTile, u.keys - at) + p.box - 1) >> p.box_shift;
+    if (lane == 0) mbar_arrive_expect_tx(land, boxes * p.box * DIM * 2);
+    __syncwarp();
+    for (int b = 0; b < boxes; b += 32) {
+        const int i = min(b + lane, boxes - 1), key = at + (i << p.box_shift);
+        int page = pages[key >> p.box_shift];
+        if (page < 0) page = p.pages;
+        const int slot = slot_of(p, u.k0 + key);
+        for (int j = 0; j < min(boxes - b, 32); ++j) {
+            const int pg = __shfl_sync(kFull, page, j), sl = __shfl_sync(kFull, slot, j);
+#pragma unroll
+            for (int half = 0; half < DIM / 64; ++half)
+                load_box(dst + half * (kTile * 128) + ((b + j) << p.box_shift) * 128, map, half * 64, sl, u.h, pg, smem_addr(land));
+        }
+    }
+}
+
+// Warp 10: row tile qi of the unit into buffer qb, and of its rows what the exponentials take.
+template <int DIM>
+__device__ __forceinline__ bool fetch_rows(const MassParams& p, const Cta& c, const Unit& u, int qi, int nq, const CUtensorMap* map, int lane) {
+    const int qb = nq % p.q_bufs, ib = nq & 1;
+    const int t0 = qi / p.head_tiles * p.tile_tokens, h0 = qi % p.head_tiles * p.tile_heads;
+    if (nq >= p.q_bufs && !wait_warp(c.b_qe + qb * 8, (nq / p.q_bufs - 1) & 1, c.fail)) return false;
+    if (lane == 0) mbar_arrive_expect_tx(&c.sh.q_full[qb], p.tile_tokens * p.tile_heads * DIM * 2);
+    __syncwarp();
+#pragma unroll
+    for (int half = 0; half < DIM / 64; ++half)
+        load_box3(c.sq + qb * c.q_block + half * c.q_half, map, half * 64, u.h * p.group + h0, u.s.first + t0, c.b_qf + qb * 8);
+    if (nq >= 2 && !wait_warp(c.b_ie + ib * 8, (nq / 2 - 1) & 1, c.fail)) return false;
+    const int rows = min(p.tile_tokens, u.s.asked - t0) * p.tile_heads;
+    int fewest = INT_MAX;
+    for (int r = lane; r < ((rows + 31) & ~31); r += 32) {
+        const int i = t0 + r / p.tile_heads, x = h0 + r % p.tile_heads;
+        int seen = 0;
+        float l = 0.f;
+        if (r < rows && x < p.group) {
+            l = __ldg(p.row_lse + (int64_t)(u.s.first + i) * p.q_heads + u.h * p.group + x) * -1.4426950408889634f;
+            if (l != INFINITY) seen = keys_seen(p, u.s, i, u.s.len, u.s.len);
+        }
+        c.sh.lse2[ib][r] = l;
+        c.sh.seen[ib][r] = seen;
+        if (r < rows) fewest = min(fewest, seen);
+    }
+    fewest = __reduce_min_sync(kFull, fewest);
+    if (lane == 0) {
+        c.sh.fewest[ib] = fewest;
+        c.sh.rows[ib] = rows;
+    }
+    __syncwarp();
+    if (lane == 0) arrive(c.b_if + ib * 8);
+    return true;
+}
+// Leaves no copy of rows under way.
+__device__ __forceinline__ void drain_rows(const MassParams& p, const Cta& c, int nq) {
+    __syncwarp();
+    if (*c.fail)
+        for (int i = max(0, nq - p.q_bufs); i <= nq; ++i) mbar_wait_brief(&c.sh.q_full[i % p.q_bufs], i / p.q_bufs & 1);
+}
+
+// A key's sum over the rows [row0, row0 + cols) of row tile ib, whose S^T is in TMEM at t.
+__device__ __forceinline__ float sum_rows(const MassParams& p, const Cta& c, uint32_t t, int ib, int row0, int cols, int key, bool all) {
+    const float* lse2 = &c.sh.lse2[ib][row0];
+    const int* seen = &c.sh.seen[ib][row0];
+    float sum = 0.f;
+    if (p.tile_rows <= 16) {
+        uint32_t s[16];
+        tmem_ld16(t, s);
+        wait_ld();
+        return weigh<16, false>(s, lse2, seen, key, p.scale_log2);
+    }
+    if (cols <= 0) return 0.f;
+    uint32_t s[2][32];  // the next columns are under way
+    tmem_ld32(t, s[0]);
+#pragma unroll
+    for (int x = 0; x < kHalfRows; x += 32) {
+        if (x >= cols) break;
+        wait_ld();
+        if (x + 32 < kHalfRows && x + 32 < cols) tmem_ld32(t + x + 32, s[(x / 32 + 1) & 1]);
+        sum += all && x + 32 <= cols ? weigh<32, true>(s[x / 32 & 1], lse2 + x, seen + x, key, p.scale_log2)
+                                     : weigh<32, false>(s[x / 32 & 1], lse2 + x, seen + x, key, p.scale_log2);
+    }
+    return sum;
+}
+
+// One row tile: DIM is the head size rounded up to 64 elements, KSTEPS its steps of 16.
+template <typename T, int DIM, int KSTEPS>
+__global__ void __launch_bounds__(kThreads, 1) stream_kernel(const __grid_constant__ MassParams p,
+                                                             const __grid_constant__ CUtensorMap kmap,
+                                                             const __grid_constant__ CUtensorMap qmap) {
+    constexpr int kBlock = kTile * DIM * 2;
+    extern __shared__ __align__(1024) unsigned char smem[];
+    const int tid = threadIdx.x, warp = __shfl_sync(kFull, tid >> 5, 0), lane = tid & 31;
+    const Cta c = enter<DIM>(p, smem, warp, lane);
+    const int halves = p.tile_rows > kHalfRows ? 2 : 1;
     Units units;
     Unit u;
     bool ok = true;
 
     if (warp == 9) {
-        constexpr uint32_t kType = std::is_same<T, __half>::value ? 0 : 1;
-        const uint32_t idesc = 1u << 4 | kType << 7 | kType << 10 | (kTile / 16) << 24 | (uint32_t)(p.tile_rows / 8) << 17;
-        int f = 0, nq = 0;  // fills of the ring (steps) and row tiles so far
-        while (ok && units.next(p, u)) {
+        int f = 0, nq = 0;  // tiles of keys and row tiles so far
+        while (ok && units.next(p, c.sh, u)) {
+            if (u.s.asked == 0) continue;
+            const int qb = nq % p.q_bufs;
+            ok = wait_warp(c.b_qf + qb * 8, nq / p.q_bufs & 1, c.fail);
+            for (int j = 0; ok && j < u.tiles; ++j, ++f) {
+                const int st = f % p.stages, w = f & 1;
+                ok = wait_warp(c.b_full + st * 8, f / p.stages & 1, c.fail);
+                for (int half = 0; ok && half < halves; ++half) {
+                    const int i = f / 2 * halves + half, buf = w * 2 + (i & 1);
+                    ok = i < 2 || wait_warp(c.b_se + buf * 8, (i / 2 - 1) & 1, c.fail);
+                    if (!ok) break;
+                    fence_after();
+                    product<T, KSTEPS>(c, c.ring + st * kBlock, c.sq + qb * c.q_block + half * kHalfRows * 128,
+                                       half ? p.tile_rows - kHalfRows : min(p.tile_rows, kHalfRows), buf);
+                }
+                if (!ok) break;
+                commit(c.b_empty + st * 8);
+            }
+            if (ok) commit(c.b_qe + qb * 8);
+            ++nq;
+        }
+        if (!ok) {  // leave no product under way
+            commit(smem_addr(&c.sh.drained));
+            mbar_wait(&c.sh.drained, 0);
+        }
+    } else if (warp == 8) {
+        int f = 0;
+        while (ok && units.next(p, c.sh, u)) {
+            const int buf = units.turn & 1;
+            ok = wait_warp(c.b_pf + buf * 8, units.turn / 2 & 1, c.fail);
+            for (int j = 0; ok && u.s.asked > 0 && j < u.tiles; ++j, ++f) {
+                const int st = f % p.stages;
+                if (f >= p.stages && !(ok = wait_warp(c.b_empty + st * 8, (f / p.stages - 1) & 1, c.fail))) break;
+                fetch_keys<DIM>(p, c, u, c.sh.page[buf], j * kTile, c.ring + st * kBlock, &c.sh.full[st], &kmap, lane);
+            }
+            __syncwarp();
+            if (ok && lane == 0) arrive(c.b_pe + buf * 8);
+        }
+        __syncwarp();
+        if (*c.fail)  // leave no copy under way
+            for (int i = max(0, f - p.stages); i < f + p.stages; ++i)
+                mbar_wait_brief(&c.sh.full[i % p.stages], i / p.stages & 1);
+    } else if (warp == 10) {
+        int nq = 0;
+        while (ok && units.next(p, c.sh, u)) {
+            if (u.s.asked == 0) continue;
+            ok = fetch_rows<DIM>(p, c, u, 0, nq, &qmap, lane);
+            if (ok) ++nq;
+        }
+        drain_rows(p, c, nq);
+    } else if (warp == 11) {
+        find_pages(p, c, lane);
+    } else {
+        const int my = warp >> 2, key_of = tid & (kTile - 1);
+        const uint32_t ts = c.tmem + my * 2 * kHalfRows + ((uint32_t)(warp & 3) << 21);
+        int f = 0, nq = 0;
+        while (units.next(p, c.sh, u)) {
+            const int pb = units.turn & 1, ib = nq & 1, f0 = f, tiles = u.s.asked > 0 ? u.tiles : 0;
+            ok = ok && wait_warp(c.b_pf + pb * 8, units.turn / 2 & 1, c.fail);
+            const int* pages = c.sh.page[pb];
+            auto old_of = [&](int at, float*& to, float& old) {
+                to = mass_at(p, u, pages, at), old = 0.f;
+                if (to && has_old(p, u, u.k0 + at)) old = *to;
+            };
+            float *to = nullptr, *to_next;
+            float old = 0.f, old_next;
+            if (tiles > 0) {
+                // the old weights of my next tile are under way
+                if (ok) old_of(((f & 1) != my) * kTile + key_of, to, old);
+                ok = ok && wait_warp(c.b_if + ib * 8, nq / 2 & 1, c.fail);
+                const int rows = c.sh.rows[ib], fewest = c.sh.fewest[ib];
+                for (f += (f & 1) != my; ok && f < f0 + tiles; f += 2) {
+                    const int at = (f - f0) * kTile + key_of, key = u.k0 + at;
+                    old_of(at + 2 * kTile, to_next, old_next);
+                    const bool all = u.k0 + min(at - key_of + kTile, u.keys) <= fewest;  // every row sees every key
+                    float sum = 0.f;
+                    for (int half = 0; ok && half < halves; ++half) {
+                        const int i = f / 2 * halves + half, buf = i & 1;
+                        ok = wait_warp(c.b_sf + (my * 2 + buf) * 8, i / 2 & 1, c.fail);
+                        if (!ok) break;
+                        fence_after();
+                        sum += sum_rows(p, c, ts + buf * kHalfRows, ib, half * kHalfRows, min(rows - half * kHalfRows, kHalfRows), key, all);
+                        fence_before();
+                        __syncwarp();
+                        if (lane == 0) arrive(c.b_se + (my * 2 + buf) * 8);
+                    }
+                    put(p, u, key, to, old, ok ? sum : NAN);  // loud: a wait that ran out leaves no number
+                    to = to_next, old = old_next;
+                }
+                f = f0 + tiles;
+                __syncwarp();
+                if (lane == 0) arrive(c.b_ie + ib * 8);
+                ++nq;
+            } else if (ok) {  // no row: the old weights decay
+                for (int at = tid; at < u.keys; at += 2 * kTile) {
+                    old_of(at, to, old);
+                    put(p, u, u.k0 + at, to, old, 0.f);
+                }
+            }
+            __syncwarp();
+            if (lane == 0) arrive(c.b_pe + pb * 8);
+        }
+    }
+    leave(c, warp);
+}
+
+// Many row tiles: a chunk of keys stays in shared memory while they pass.
+template <typename T, int DIM, int KSTEPS>
+__global__ void __launch_bounds__(kThreads, 1) rows_kernel(const __grid_constant__ MassParams p,
+                                                           const __grid_constant__ CUtensorMap kmap,
+                                                           const __grid_constant__ CUtensorMap qmap) {
+    constexpr int kBlock = kTile * DIM * 2;
+    constexpr int kMine = DIM > 128 ? 1 : 2;  // tiles of a chunk of a warpgroup
+    extern __shared__ __align__(1024) unsigned char smem[];
+    const int tid = threadIdx.x, warp = __shfl_sync(kFull, tid >> 5, 0), lane = tid & 31;
+    const Cta c = enter<DIM>(p, smem, warp, lane);
+    Units units;
+    Unit u;
+    bool ok = true;
+
+    if (warp == 9) {
+        int nq = 0, made[2] = {0, 0};  // row tiles; steps of each warpgroup
+        uint32_t used = 0;             // parity of the tiles of keys, by bit
+        while (ok && units.next(p, c.sh, u)) {
+            int here = 0;  // tiles of keys that have come
             for (int qi = u.q0; ok && qi < u.q1; ++qi) {
                 const int steps = steps_of(p, u, qi);
                 if (steps == 0) continue;
                 const int qb = nq % p.q_bufs;
-                ok = wait_warp(b_qf + qb * 8, nq / p.q_bufs & 1, fail);
-                for (int j = 0; ok && j < steps; ++j, ++f) {
-                    const int st = f % p.stages, w = f & 1;
-                    ok = wait_warp(b_full + st * 8, f / p.stages & 1, fail) &&
-                         (f < 2 || wait_warp(b_se + w * 8, (f / 2 - 1) & 1, fail));
+                ok = wait_warp(c.b_qf + qb * 8, nq / p.q_bufs & 1, c.fail);
+                for (int j = 0; ok && j < steps; ++j) {
+                    if (j >= here) {
+                        ok = wait_warp(c.b_full + j * 8, used >> j & 1, c.fail);
+                        used ^= 1u << j;
+                        here = j + 1;
+                    }
+                    const int w = j & 1, i = w ? made[1]++ : made[0]++, buf = w * 2 + (i & 1);
+                    ok = ok && (i < 2 || wait_warp(c.b_se + buf * 8, (i / 2 - 1) & 1, c.fail));
                     if (!ok) break;
                     fence_after();
-                    const uint32_t k = ring + st * kBlock, q = sq + qb * q_block;
-#pragma unroll
-                    for (int kk = 0; kk < KSTEPS; ++kk)
-                        mma_ss(tmem + w * kMostRows, operand(k + (kk >> 2) * kHalf + (kk & 3) * 32, 16),
-                               operand(q + (kk >> 2) * q_half + (kk & 3) * 32, 16), idesc, kk > 0);
-                    commit(b_sf + w * 8);
-                    commit(b_empty + st * 8);
+                    product<T, KSTEPS>(c, c.ring + j * kBlock, c.sq + qb * c.q_block, p.tile_rows, buf);
+                    if (qi == u.q1 - 1) commit(c.b_empty + j * 8);  // the last rows see the most keys
                 }
-                if (ok) commit(b_qe + qb * 8);
+                if (ok) commit(c.b_qe + qb * 8);
                 ++nq;
             }
         }
         if (!ok) {  // leave no product under way
-            commit(smem_addr(&sh.drained));
-            mbar_wait(&sh.drained, 0);
+            commit(smem_addr(&c.sh.drained));
+            mbar_wait(&c.sh.drained, 0);
         }
     } else if (warp == 8) {
-        // Lane l looks up the page of box l of a tile one tile ahead.  A box past the end is not
-        // fetched; a page that does not exist is fetched from behind the last one, which reads as zeros.
-        const int boxes = kTile / box;
-        int f = 0;
-        while (ok && units.next(p, u)) {
-            const int64_t* list = p.indices + u.s.page0;
-            const int end = u.k0 + u.keys;
-            for (int qi = u.q0; ok && qi < u.q1; ++qi) {
-                const int steps = steps_of(p, u, qi);
-                if (steps == 0) continue;
-                int page, slot;
-                auto find = [&](int at) {
-                    page = -1, slot = 0;
-                    if (at < end) {
-                        locate(p, list, at, page, slot);
-                        if (page < 0) page = p.pages;
-                    }
-                };
-                if (lane < boxes) find(u.k0 + lane * box);
-                for (int j = 0; j < steps; ++j, ++f) {
-                    const int st = f % p.stages, kt = u.k0 + j * kTile;
-                    const uint32_t dst = ring + st * kBlock, bar = b_full + st * 8;
-                    if (f >= p.stages && !(ok = wait_warp(b_empty + st * 8, (f / p.stages - 1) & 1, fail))) break;
-                    for (int b = 0; b < boxes; b += 32) {
-                        if (b > 0) find(kt + (b + lane) * box);
-                        const uint32_t held = __ballot_sync(kFull, lane < boxes - b && page >= 0);
-                        if (lane == 0) {
-                            const uint32_t bytes = __popc(held) * box * DIM * 2;
-                            if (b + 32 >= boxes) mbar_arrive_expect_tx(&sh.full[st], bytes);
-                            else mbar_expect_tx(&sh.full[st], bytes);
-                        }
-                        __syncwarp();
-                        for (int i = 0; i < min(boxes - b, 32); ++i) {
-                            const int pg = __shfl_sync(kFull, page, i), sl = __shfl_sync(kFull, slot, i);
-                            if (!(held >> i & 1)) continue;
-#pragma unroll
-                            for (int half = 0; half < kHalves; ++half)
-                                load_box(dst + half * kHalf + (b + i) * box * 128, &kmap, half * 64, sl, u.h, pg, bar);
-                        }
-                    }
-                    if (lane < boxes) find(kt + kTile + lane * box);
+        uint32_t began = 0, freed = 0;  // whether a place was filled before, and the parity of its emptying
+        uint32_t landed = 0;
+        while (ok && units.next(p, c.sh, u)) {
+            const int buf = units.turn & 1, tiles = u.q1 > u.q0 ? steps_of(p, u, u.q1 - 1) : 0;
+            ok = wait_warp(c.b_pf + buf * 8, units.turn / 2 & 1, c.fail);
+            for (int j = 0; ok && j < tiles; ++j) {
+                if (began >> j & 1) {
+                    ok = wait_warp(c.b_empty + j * 8, freed >> j & 1, c.fail);
+                    freed ^= 1u << j;
                 }
+                if (!ok) break;
+                began |= 1u << j;
+                landed ^= 1u << j;
+                fetch_keys<DIM>(p, c, u, c.sh.page[buf], j * kTile, c.ring + j * kBlock, &c.sh.full[j], &kmap, lane);
             }
+            __syncwarp();
+            if (ok && lane == 0) arrive(c.b_pe + buf * 8);
         }
         __syncwarp();
-        if (*fail)  // leave no copy under way
-            for (int i = max(0, f - p.stages); i < f + p.stages; ++i)
-                mbar_wait_brief(&sh.full[i % p.stages], i / p.stages & 1);
+        if (*c.fail)  // leave no copy under way
+            for (int j = 0; j < p.chunk; ++j)
+                if (began >> j & 1) mbar_wait_brief(&c.sh.full[j], (landed >> j & 1) ^ 1);
     } else if (warp == 10) {
         int nq = 0;
-        while (ok && units.next(p, u)) {
+        while (ok && units.next(p, c.sh, u))
             for (int qi = u.q0; ok && qi < u.q1; ++qi) {
                 if (steps_of(p, u, qi) == 0) continue;
-                const int qb = nq % p.q_bufs, ib = nq & 1;
-                const int t0 = qi / p.head_tiles * p.tile_tokens, h0 = qi % p.head_tiles * p.tile_heads;
-                ok = nq < p.q_bufs || wait_warp(b_qe + qb * 8, (nq / p.q_bufs - 1) & 1, fail);
-                if (!ok) break;
-                if (lane == 0) mbar_arrive_expect_tx(&sh.q_full[qb], p.tile_tokens * p.tile_heads * DIM * 2);
-                __syncwarp();
-#pragma unroll
-                for (int half = 0; half < kHalves; ++half)
-                    load_box3(sq + qb * q_block + half * q_half, &qmap, half * 64, u.h * p.group + h0, u.s.first + t0, b_qf + qb * 8);
-                ok = nq < 2 || wait_warp(b_ie + ib * 8, (nq / 2 - 1) & 1, fail);
-                if (!ok) break;
-                const int rows = min(p.tile_tokens, u.s.asked - t0) * p.tile_heads;
-                int fewest = INT_MAX;
-                for (int r = lane; r < ((rows + 31) & ~31); r += 32) {
-                    const int i = t0 + r / p.tile_heads, x = h0 + r % p.tile_heads;
-                    int seen = 0;
-                    float l = 0.f;
-                    if (r < rows && x < p.group) {
-                        l = __ldg(p.row_lse + (int64_t)(u.s.first + i) * p.q_heads + u.h * p.group + x) * 1.4426950408889634f;
-                        if (l != -INFINITY) seen = keys_seen(p, u.s, i, u.s.len, u.s.len);
-                    }
-                    sh.lse2[ib][r] = l;
-                    sh.seen[ib][r] = seen;
-                    if (r < rows) fewest = min(fewest, seen);
-                }
-                fewest = __reduce_min_sync(kFull, fewest);
-                if (lane == 0) {
-                    sh.fewest[ib] = fewest;
-                    sh.rows[ib] = rows;
-                }
-                __syncwarp();
-                if (lane == 0) arrive(b_if + ib * 8);
-                ++nq;
+                ok = fetch_rows<DIM>(p, c, u, qi, nq, &qmap, lane);
+                if (ok) ++nq;
             }
-        }
-        __syncwarp();
-        if (*fail)
-            for (int i = max(0, nq - 2); i <= nq; ++i) mbar_wait_brief(&sh.q_full[i % p.q_bufs], i / p.q_bufs & 1);
-    } else if (warp < 8) {
+        drain_rows(p, c, nq);
+    } else if (warp == 11) {
+        find_pages(p, c, lane);
+    } else {
         const int my = warp >> 2, key_of = tid & (kTile - 1);
-        const uint32_t ts = tmem + my * kMostRows + ((uint32_t)(warp & 3) << 21);
-        int f = 0, nq = 0;
-        while (units.next(p, u)) {
-            const bool direct = p.splits == 1 && u.q1 - u.q0 <= 1;
-            auto add = [&](int key, float* at, float old, float sum) {
-                if (at) *at = has_old(p, u, key) ? fmaf(old, p.decay, sum) : sum;
-            };
-            int done = 0;  // tiles of a direct unit that are written by their steps
+        const uint32_t ts = c.tmem + my * 2 * kHalfRows + ((uint32_t)(warp & 3) << 21);
+        int nq = 0, made = 0;
+        while (units.next(p, c.sh, u)) {
+            const int pb = units.turn & 1;
+            float acc[kMine];
+#pragma unroll
+            for (int m = 0; m < kMine; ++m) acc[m] = 0.f;
             for (int qi = u.q0; ok && qi < u.q1; ++qi) {
                 const int steps = steps_of(p, u, qi);
                 if (steps == 0) continue;
                 const int ib = nq & 1;
-                ok = wait_warp(b_if + ib * 8, nq / 2 & 1, fail);
-                const int rows = sh.rows[ib], fewest = sh.fewest[ib];
-                for (int j = 0; ok && j < steps; ++j, ++f) {
-                    if ((f & 1) != my) continue;
-                    const int at = j * kTile + key_of, key = u.k0 + at;
-                    float* to = nullptr;
-                    float old = 0.f;
-                    if (direct && at < u.keys) {
-                        to = mass_at(p, u, key);
-                        if (to && has_old(p, u, key)) old = *to;
-                    }
-                    ok = wait_warp(b_sf + my * 8, f / 2 & 1, fail);
+                ok = wait_warp(c.b_if + ib * 8, nq / 2 & 1, c.fail);
+                const int rows = c.sh.rows[ib], fewest = c.sh.fewest[ib];
+#pragma unroll
+                for (int m = 0; m < kMine; ++m) {
+                    const int j = 2 * m + my, buf = made & 1;
+                    if (!ok || j >= steps) continue;
+                    ok = wait_warp(c.b_sf + (my * 2 + buf) * 8, made / 2 & 1, c.fail);
+                    if (!ok) continue;
                     fence_after();
                     const bool all = u.k0 + min((j + 1) * kTile, u.keys) <= fewest;  // every row sees every key
-                    float sum = 0.f;
-                    if (ok) {
-#pragma unroll 1
-                        for (int c = 0; c < rows; c += 32) {
-                            uint32_t s[32];
-                            tmem_ld32(ts + c, s);
-                            wait_ld();
-                            const float4* l4 = reinterpret_cast<const float4*>(&sh.lse2[ib][c]);
-                            if (all && c + 32 <= rows) {
-                                uint64_t part[2] = {0, 0};
-                                const uint64_t sc = pair(p.scale_log2, p.scale_log2);
-#pragma unroll
-                                for (int e = 0; e < 32; e += 4) {
-                                    const float4 l = l4[e / 4];
-                                    const float2 x = both(fma2(pair(__uint_as_float(s[e]), __uint_as_float(s[e + 1])), sc, pair(-l.x, -l.y)));
-                                    const float2 y = both(fma2(pair(__uint_as_float(s[e + 2]), __uint_as_float(s[e + 3])), sc, pair(-l.z, -l.w)));
-                                    part[0] = add2(part[0], pair(exp2_fast(x.x), exp2_fast(x.y)));
-                                    part[1] = add2(part[1], pair(exp2_fast(y.x), exp2_fast(y.y)));
-                                }
-                                const float2 v = both(add2(part[0], part[1]));
-                                sum += v.x + v.y;
-                            } else {
-                                const int4* n4 = reinterpret_cast<const int4*>(&sh.seen[ib][c]);
-                                float part = 0.f;
-#pragma unroll
-                                for (int e = 0; e < 32; e += 4) {
-                                    const float4 l = l4[e / 4];
-                                    const int4 n = n4[e / 4];
-                                    part += key < n.x ? exp2_fast(fmaf(__uint_as_float(s[e]), p.scale_log2, -l.x)) : 0.f;
-                                    part += key < n.y ? exp2_fast(fmaf(__uint_as_float(s[e + 1]), p.scale_log2, -l.y)) : 0.f;
-                                    part += key < n.z ? exp2_fast(fmaf(__uint_as_float(s[e + 2]), p.scale_log2, -l.z)) : 0.f;
-                                    part += key < n.w ? exp2_fast(fmaf(__uint_as_float(s[e + 3]), p.scale_log2, -l.w)) : 0.f;
-                                }
-                                sum += part;
-                            }
-                        }
-                    } else {
-                        sum = NAN;  // loud: a wait that ran out leaves no number
-                    }
+                    acc[m] += sum_rows(p, c, ts + buf * kHalfRows, ib, 0, rows, u.k0 + j * kTile + key_of, all);
                     fence_before();
                     __syncwarp();
-                    if (lane == 0) arrive(b_se + my * 8);
-                    if (direct) add(key, to, old, sum);
-                    else sh.acc[my][at] += sum;
+                    if (lane == 0) arrive(c.b_se + (my * 2 + buf) * 8);
+                    ++made;
                 }
                 __syncwarp();
-                if (lane == 0) arrive(b_ie + ib * 8);
+                if (lane == 0) arrive(c.b_ie + ib * 8);
                 ++nq;
-                done = steps;
             }
-            if (direct) {  // keys that no row sees
-                for (int at = done * kTile + tid; at < u.keys; at += 2 * kTile) {
-                    float* to = mass_at(p, u, u.k0 + at);
-                    add(u.k0 + at, to, to && has_old(p, u, u.k0 + at) ? *to : 0.f, ok ? 0.f : NAN);
-                }
-                continue;
-            }
-            asm volatile("bar.sync 1, 256;" ::: "memory");
-            for (int at = tid; at < u.keys; at += 2 * kTile) {
-                float sum = sh.acc[0][at] + sh.acc[1][at];
-                if (!ok) sum = NAN;
+            ok = ok && wait_warp(c.b_pf + pb * 8, units.turn / 2 & 1, c.fail);
+#pragma unroll
+            for (int m = 0; m < kMine; ++m) {
+                const int at = (2 * m + my) * kTile + key_of, key = u.k0 + at;
+                if (!ok) acc[m] = NAN;  // loud: a wait that ran out leaves no number
                 if (p.splits > 1) {
-                    p.part[(int64_t)u.id * (p.chunk * kTile) + at] = sum;
-                } else {
-                    float* to = mass_at(p, u, u.k0 + at);
-                    add(u.k0 + at, to, to && has_old(p, u, u.k0 + at) ? *to : 0.f, sum);
+                    if (at < u.keys) p.part[part_at(p, u) + at] = acc[m];
+                } else if (ok) {
+                    float* const to = mass_at(p, u, c.sh.page[pb], at);
+                    put(p, u, key, to, to && has_old(p, u, key) ? *to : 0.f, acc[m]);
                 }
             }
-            // (keys behind the end were summed too)
-            for (int at = tid; at < u.tiles * kTile; at += 2 * kTile) sh.acc[0][at] = sh.acc[1][at] = 0.f;
-            asm volatile("bar.sync 1, 256;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) arrive(c.b_pe + pb * 8);
         }
     }
-    __syncwarp();
-    __syncthreads();
-    if (warp == 9) {
-        fence_after();
-        tmem_free(tmem, kCols);
-    }
+    leave(c, warp);
 }
 
 // mass of the keys of a (chunk, sequence, key head) from the parts of its row tiles, in their order.
@@ -411,27 +689,29 @@ __global__ void __launch_bounds__(256) mass_join_kernel(const __grid_constant__ 
     Unit u;
     int x = blockIdx.x;
     u.h = x % p.kv_heads, x /= p.kv_heads;
-    const int b = x % p.rows, c = x / p.rows;
-    u.s = sequence(p, b);
-    u.k0 = c * p.chunk * kTile;
+    u.b = x % p.rows, u.c = x / p.rows;
+    u.s = sequence(p, u.b);
+    u.k0 = u.c * p.chunk * kTile;
     u.keys = min(u.s.len - u.k0, p.chunk * kTile);
     if (u.keys <= 0 || (u.s.n == 0 && p.decay == 1.f)) return;
-    const int all = row_tiles(p, u.s), per = p.chunks * p.rows * p.kv_heads;
+    int all;
+    const int first = first_split(p, u.s, u.k0, all);
     for (int at = threadIdx.x; at < u.keys; at += blockDim.x) {
-        float* const to = mass_at(p, u, u.k0 + at);
-        if (!to) continue;
+        int page, slot;
+        locate(p, p.indices + u.s.page0, u.k0 + at, page, slot);
+        if (page < 0) continue;
+        float* const to = p.mass + page * p.m_page + slot * p.m_slot + u.h * p.m_head;
+        const bool kept = has_old(p, u, u.k0 + at);
+        const float old = kept ? *to : 0.f;
         float sum = 0.f;
-        for (int s = 0; s < p.splits; ++s) {
-            const int end = min((s + 1) * p.split_tiles, all);
-            if (s * p.split_tiles >= end) break;
-            if (steps_of(p, u, end - 1) == 0) continue;
-            sum += p.part[((int64_t)s * per + blockIdx.x) * (p.chunk * kTile) + at];
-        }
-        *to = has_old(p, u, u.k0 + at) ? fmaf(*to, p.decay, sum) : sum;
+        for (u.split = first; u.split < all; ++u.split) sum += p.part[part_at(p, u) + at];
+        *to = kept ? fmaf(old, p.decay, sum) : sum;
     }
 }
 
 // ------------------------------------------------------------------ host
+constexpr int64_t kManyUnits = kSMs * 32;  // with the causal mask about half of them have steps
+
 int make_plan(const tg_attention_mass_args* a, MassParams* out, const char* op) {
     if (!a) return set_error(TG_EINVAL, "%s: null arguments", op);
     int rc = check_cache(a->cache, op);
@@ -477,51 +757,62 @@ int make_plan(const tg_attention_mass_args* a, MassParams* out, const char* op) 
     p.m_page = stride_of(c.pages, a->mass.page_stride), p.m_slot = stride_of(c.page_size, a->mass.slot_stride);
     p.m_head = stride_of(c.heads, a->mass.head_stride);
 
-    // Row tiles: as many tokens as 256 rows hold (128 for heads of 256, whose tiles take twice the room),
-    // or where one token's heads are more than that, a part of its heads.
+    p.box = std::gcd(p.page_size, kTile);
+    while (1 << p.box_shift < p.box) ++p.box_shift;
+    // Row tiles: up to 256 rows of a key head (128 for heads of 256, whose tiles take twice the room) stay in
+    // shared memory; of more rows 128 (64) at a time pass.  A tile has whole tokens, or where one token's
+    // heads are more than that, a part of its heads.
     const int dim = (c.dim + 63) / 64 * 64, most = dim > 128 ? kMostRows / 2 : kMostRows;
-    p.tile_heads = std::min(p.group, most);
+    p.stream = max_q * p.group <= most;
+    const int rows = p.stream ? most : most / 2;
+    p.tile_heads = std::min(p.group, rows);
     p.head_tiles = (p.group + p.tile_heads - 1) / p.tile_heads;
-    p.tile_tokens = (int)std::max<int64_t>(1, std::min<int64_t>(max_q, most / p.tile_heads));
+    p.tile_tokens = (int)std::max<int64_t>(1, std::min<int64_t>(max_q, rows / p.tile_heads));
     p.tile_rows = (p.tile_tokens * p.tile_heads + 15) / 16 * 16;
     const int64_t q_tiles = std::max<int64_t>(1, ceil_div(max_q, p.tile_tokens)) * p.head_tiles, k_tiles = std::max<int64_t>(1, ceil_div(max_seq, kTile));
-    // Chunks of keys: one row tile is loaded for each, so as long as leaves eight units a CTA; several row
-    // tiles go over a chunk one after the other, its sums in shared memory.
+    const int q_block = p.tile_rows * dim * 2, k_block = kTile * dim * 2;
     const int64_t pairs = std::max<int64_t>(1, t.rows * c.heads);
-    p.chunk = (int)std::min<int64_t>(kChunkMax, q_tiles > 1 ? kChunkMax : std::max<int64_t>(1, pairs * k_tiles / (kSMs * 8)));
+    if (p.stream) {
+        // Chunks as long as leaves 16 units a CTA: each fetches its rows anew.
+        p.chunk = (int)std::min<int64_t>(kChunkMax, std::max<int64_t>(1, pairs * k_tiles / (kSMs * 16)));
+        p.q_bufs = 2 * q_block + 4 * k_block <= kTiles ? 2 : 1;
+        p.stages = std::min(kStagesMax, (kTiles - p.q_bufs * q_block) / k_block);
+    } else {
+        p.chunk = dim > 128 ? 2 : 4;
+        p.q_bufs = std::min(4, (kTiles - p.chunk * k_block) / q_block);
+    }
     p.chunks = (int)ceil_div(k_tiles, p.chunk);
-    // Where that makes few units the row tiles are shared out too, at least two to a part.
-    p.splits = (int)std::max<int64_t>(1, std::min(ceil_div(kSMs * 8, pairs * p.chunks), q_tiles / 2));
+    // Where that makes few units the row tiles are shared out too, at least four to a part.
+    p.splits = p.head_tiles > 1 ? 1 : (int)std::max<int64_t>(1, std::min(ceil_div(kManyUnits, pairs * p.chunks), q_tiles / 4));
     p.split_tiles = (int)ceil_div(q_tiles, p.splits);
     p.splits = (int)std::max<int64_t>(1, ceil_div(q_tiles, p.split_tiles));
     if (pairs * p.chunks * p.splits > INT32_MAX - kSMs) return set_error(TG_EUNSUPPORTED, "%s: too many sequences for one launch", op);
-    p.units = (int)(t.rows * c.heads * p.chunks * p.splits);
-    const int q_block = p.tile_rows * dim * 2, k_block = kTile * dim * 2;
-    p.q_bufs = 2 * q_block + 4 * k_block <= kTiles ? 2 : 1;
-    p.stages = std::min(kStagesMax, (kTiles - p.q_bufs * q_block) / k_block);
     return TG_OK;
 }
 
 size_t mass_bytes(const MassParams& p) {
-    return p.splits > 1 ? (size_t)p.units * p.chunk * kTile * sizeof(float) : 0;
+    return p.splits > 1 ? (size_t)p.splits * p.chunks * p.rows * p.kv_heads * p.chunk * kTile * sizeof(float) : 0;
 }
-// Of any smaller call: parts are made only until there are eight units an SM, rounded up by less than
-// that.
+// Of any smaller call: parts are made only until there are kManyUnits units, of one row of parts less.
 size_t mass_enough(const MassParams& p) {
-    const int64_t tiles = ceil_div(p.max_q, std::max(1, p.tile_tokens)) * p.head_tiles;
-    return tiles < 2 && p.head_tiles < 2 ? 0 : (size_t)(2 * kSMs * 8) * kChunkMax * kTile * sizeof(float);
+    return p.stream || p.head_tiles > 1 ? 0 : (size_t)(2 * kManyUnits) * p.chunk * kTile * sizeof(float);
 }
 
 template <typename T, int DIM, int KSTEPS>
 int mass_run(const MassParams& p, const CUtensorMap& kmap, const CUtensorMap& qmap, cudaStream_t st) {
-    auto kernel = mass_kernel<T, DIM, KSTEPS>;
-    static SmemOnce once;
-    int rc = once.raise(reinterpret_cast<const void*>(kernel), kSmem);
+    auto kernel = p.stream ? stream_kernel<T, DIM, KSTEPS> : rows_kernel<T, DIM, KSTEPS>;
+    static SmemOnce once[2];
+    int rc = once[p.stream].raise(reinterpret_cast<const void*>(kernel), kSmem);
     if (rc != TG_OK) return rc;
-    const int grid = std::min(p.units, kSMs);
-    kernel<<<(unsigned)grid, kThreads, kSmem, st>>>(p, std::gcd(p.page_size, kTile), kmap, qmap);
-    rc = check_launch("mass_kernel");
-    if (rc != TG_OK || p.splits == 1) return rc;
+    MassParams some = p;
+    for (some.first_seq = 0; some.first_seq < p.rows; some.first_seq += kSeqs) {
+        some.seqs = std::min(kSeqs, p.rows - some.first_seq);
+        const int grid = (int)std::min<int64_t>((int64_t)some.seqs * p.kv_heads * p.chunks * p.splits, kSMs);
+        kernel<<<(unsigned)grid, kThreads, kSmem, st>>>(some, kmap, qmap);
+        rc = check_launch("attention_mass kernel");
+        if (rc != TG_OK) return rc;
+    }
+    if (p.splits == 1) return TG_OK;
     return launch_pdl("mass_join_kernel", mass_join_kernel, dim3((unsigned)(p.rows * p.kv_heads * p.chunks)), 256, 0, st, p);
 }
 
@@ -552,7 +843,7 @@ int attention_mass(const tg_attention_mass_args* a, void* ws, size_t ws_bytes, t
     p.part = static_cast<float*>(ws);
     constexpr bool kIsHalf = std::is_same<T, __half>::value;
     CUtensorMap kmap, vmap, qmap;
-    rc = cache_maps(p, kIsHalf, c.dim, std::gcd(p.page_size, kTile), &kmap, &vmap);
+    rc = cache_maps(p, kIsHalf, c.dim, p.box, &kmap, &vmap);
     if (rc == TG_OK) rc = rows_map(p, kIsHalf, c.dim, p.tile_heads, p.tile_tokens, &qmap);
     if (rc != TG_OK) return rc;
     switch (c.dim) {
