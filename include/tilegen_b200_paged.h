@@ -245,9 +245,11 @@ typedef struct tg_attention_mass_args {
     double decay; /* >= 0 */
     uint32_t flags;
 } tg_attention_mass_args;
-/* Bytes of a workspace, enough for this call and any of the same head sizes with no larger max_q_len
- * (0 for few rows; never more than 64 MB). */
+/* Bytes of a workspace to keep, enough for this call and any of the same head sizes with no larger
+ * max_q_len (0 for few rows; never more than 80 MB). */
 TG_API size_t tg_attention_mass_workspace_bytes(const tg_attention_mass_args* a);
+/* What a call with these very arguments takes, at most the former. */
+TG_API size_t tg_attention_mass_needed_bytes(const tg_attention_mass_args* a);
 TG_API int tg_attention_mass_f16(const tg_attention_mass_args* a, void* workspace, size_t workspace_bytes,
                                  tg_stream_t stream);
 TG_API int tg_attention_mass_bf16(const tg_attention_mass_args* a, void* workspace, size_t workspace_bytes,

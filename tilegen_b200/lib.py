@@ -350,6 +350,7 @@ SIGNATURES_PAGED = {
     "tg_prefix_attention_f16": (ctypes.c_int, [ctypes.POINTER(TgPrefixAttentionArgs), _P, _SZ, _P]),
     "tg_prefix_attention_bf16": (ctypes.c_int, [ctypes.POINTER(TgPrefixAttentionArgs), _P, _SZ, _P]),
     "tg_attention_mass_workspace_bytes": (_SZ, [ctypes.POINTER(TgAttentionMassArgs)]),
+    "tg_attention_mass_needed_bytes": (_SZ, [ctypes.POINTER(TgAttentionMassArgs)]),
     "tg_attention_mass_f16": (ctypes.c_int, [ctypes.POINTER(TgAttentionMassArgs), _P, _SZ, _P]),
     "tg_attention_mass_bf16": (ctypes.c_int, [ctypes.POINTER(TgAttentionMassArgs), _P, _SZ, _P]),
     "tg_kv_evict_workspace_bytes": (_SZ, [ctypes.POINTER(TgKvEvictArgs)]),

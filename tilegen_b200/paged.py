@@ -704,7 +704,7 @@ def attention_mass(mass: torch.Tensor, q: torch.Tensor, cache: PagedKV, table: P
 
 
 def _mass_launch(m, mass, q, workspace, index, sp):
-    need = _call("tg_attention_mass_workspace_bytes")(m)
+    need = _call("tg_attention_mass_needed_bytes")(m)
     ws = size = 0
     if workspace is None and need:
         workspace, size = torch.empty(need, dtype=torch.uint8, device=q.device), need
