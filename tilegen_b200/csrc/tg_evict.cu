@@ -30,15 +30,16 @@ namespace {
 
 namespace cg = cooperative_groups;
 
-constexpr int kSelThreads = 512;
-constexpr int kSelWarps = kSelThreads / 32;
 constexpr int kBins = 2048;
 constexpr int kSelKeys = 40960;  // most weights of a CTA in shared memory; further ones are read again
 constexpr int kMoveThreads = 256;
+constexpr int kListed = 2048; // keys of one beginning that are listed
+constexpr int kMostCtas = 8;  // of a cluster
 
 struct EvictParams {
     tg_csr pages;
     int64_t page_size;
+    int page_shift;  // log2(page_size), -1 where it is no power of two
     const int64_t* seq_len;
     int64_t *seq_len_out, n_pages;
     int max_seq, budget, first, recent, heads, rows;
@@ -80,7 +81,7 @@ struct Place {
     int page, slot;  // page -1: not in the cache
 };
 __device__ __forceinline__ Place place_of(const EvictParams& p, int64_t page0, int at) {
-    const int j = at / (int)p.page_size;
+    const int j = p.page_shift >= 0 ? at >> p.page_shift : at / (int)p.page_size;
     const int64_t id = __ldg(p.pages.indices + page0 + j);
     return {id >= 0 && id < p.n_pages ? (int)id : -1, at - j * (int)p.page_size};
 }
@@ -99,40 +100,58 @@ __device__ __forceinline__ uint32_t ordered(float v) {
     return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
-// Sum over the warps before mine, and over all, of v (the same in all lanes of a warp).
+// Sums over the warps before mine, and over all, of three numbers (the same in all lanes of a warp).
 struct Before {
-    int mine, all;
+    int3 mine, all;
 };
-__device__ __forceinline__ Before warps_before(int v, int* s) {  // s: [kSelWarps]
+template <int WARPS>
+__device__ __forceinline__ Before warps_before(int3 v, int3* s) {  // s: [WARPS]
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     __syncthreads();
     if (lane == 0) s[warp] = v;
     __syncthreads();
-    const int x = lane < kSelWarps ? s[lane] : 0;
-    return {(int)__reduce_add_sync(kFull, lane < warp ? x : 0), (int)__reduce_add_sync(kFull, x)};
+    const int3 x = lane < WARPS ? s[lane] : make_int3(0, 0, 0);
+    const bool before = lane < warp;
+    Before r;
+    r.mine = make_int3(__reduce_add_sync(kFull, before ? x.x : 0), __reduce_add_sync(kFull, before ? x.y : 0),
+                       __reduce_add_sync(kFull, before ? x.z : 0));
+    r.all = make_int3(__reduce_add_sync(kFull, x.x), __reduce_add_sync(kFull, x.y), __reduce_add_sync(kFull, x.z));
+    return r;
 }
-// The same over the CTAs of a cluster: of what they wrote into *s.
-__device__ __forceinline__ Before ctas_before(cg::cluster_group& cl, int v, int* s) {
-    if (cl.num_blocks() == 1) return {0, v};
+// The same over the CTAs of a cluster (32 at most), of what they write into *s.
+__device__ __forceinline__ Before ctas_before(cg::cluster_group& cl, int3 v, int3* s) {
+    if (cl.num_blocks() == 1) return {make_int3(0, 0, 0), v};
     cl.sync();  // the last values have been read
     if (threadIdx.x == 0) *s = v;
     cl.sync();
-    Before r = {0, 0};
-    for (unsigned i = 0; i < cl.num_blocks(); ++i) {
-        const int x = *cl.map_shared_rank(s, i);
-        r.all += x;
-        if (i < cl.block_rank()) r.mine += x;
-    }
+    const unsigned lane = threadIdx.x & 31;
+    const int3 x = lane < cl.num_blocks() ? *cl.map_shared_rank(s, lane) : make_int3(0, 0, 0);
+    const bool before = lane < cl.block_rank();
+    Before r;
+    r.mine = make_int3(__reduce_add_sync(kFull, before ? x.x : 0), __reduce_add_sync(kFull, before ? x.y : 0),
+                       __reduce_add_sync(kFull, before ? x.z : 0));
+    r.all = make_int3(__reduce_add_sync(kFull, x.x), __reduce_add_sync(kFull, x.y), __reduce_add_sync(kFull, x.z));
     return r;
 }
 
-__global__ void __launch_bounds__(kSelThreads) select_kernel(const __grid_constant__ EvictParams p, const int held) {
-    extern __shared__ uint32_t s_keys[];  // [held]
+// THREADS: 256 where a CTA has up to 4096 candidates, whose time goes into scans of all warps, else 512 (with
+// 1024, of which an SM holds one CTA, sixteen clusters of eight did not fit at once: 80 us for two long
+// sequences).
+template <int THREADS>
+__global__ void __launch_bounds__(THREADS) select_kernel(const __grid_constant__ EvictParams p, const int held) {
+    constexpr int kWarps = THREADS / 32, kLoads = THREADS / 128;  // weights of a thread under way
+    extern __shared__ float s_mass[];  // [held]
     __shared__ __align__(16) uint32_t s_hist[kBins];
-    __shared__ int s_warp[kSelWarps], s_cta, s_pick[2];
+    __shared__ int3 s_warp[kWarps], s_cta;
+    __shared__ int s_pick[3], s_listed;
+    __shared__ uint32_t s_list[kListed];
     cg::cluster_group cl = cg::this_cluster();
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int ctas = cl.num_blocks(), rank = cl.block_rank();
+    auto sync = [&] {
+        if (ctas == 1) __syncthreads();
+        else cl.sync();
+    };
     pdl_trigger();
     const int unit = blockIdx.x / ctas, h = unit % p.heads, b = unit / p.heads;
     int64_t page0;
@@ -140,144 +159,202 @@ __global__ void __launch_bounds__(kSelThreads) select_kernel(const __grid_consta
     const int new_end = c.first + c.heavy;  // of the new places of the chosen ones
 
     // what stays where it is, and the ends of the lists
-    auto stays = [&](int at) {
-        if (p.moved) put_mass(p, page0, at, h, mass_of(p, page0, at, h));
-        if (p.kept) p.kept[((int64_t)b * p.heads + h) * p.kept_width + at] = at;
+    int32_t* const kept = p.kept ? p.kept + ((int64_t)b * p.heads + h) * p.kept_width : nullptr;
+    auto stays = [&](int at, float m) {
+        if (p.moved) put_mass(p, page0, at, h, m);
+        if (kept) kept[at] = at;
     };
-    const int step = ctas * kSelThreads, me = rank * kSelThreads + tid;
-    if (p.kept)
-        for (int at = c.size + me; at < p.kept_width; at += step) p.kept[((int64_t)b * p.heads + h) * p.kept_width + at] = -1;
-    for (int at = me; at < (c.gone ? c.first : c.size); at += step) stays(at);
+    const int step = ctas * THREADS, me = rank * THREADS + tid;
+    if (kept)
+        for (int at = c.size + me; at < p.kept_width; at += step) kept[at] = -1;
+    auto first_stay = [&] {
+        if (p.moved || kept)
+            for (int at = me; at < (c.gone ? c.first : c.size); at += step) stays(at, p.moved ? mass_of(p, page0, at, h) : 0.f);
+    };
     if (c.gone == 0 || c.heavy == 0) {  // the same for the whole cluster
+        first_stay();
         if (me == 0) p.counts[unit] = make_int4(0, 0, c.size, c.gone);
         return;
     }
 
     // my share of the candidates, a multiple of 32 for each warp
     const int all = c.len - c.recent - c.first;
-    const int per_warp = ((all + ctas * kSelWarps - 1) / (ctas * kSelWarps) + 31) & ~31, per = per_warp * kSelWarps;
+    const int per_warp = ((all + ctas * kWarps - 1) / (ctas * kWarps) + 31) & ~31, per = per_warp * kWarps;
     const int lo = min(rank * per, all), n = min(lo + per, all) - lo;  // candidates lo .. lo + n, from place c.first
     const int base = c.first + lo;
-    for (int i = tid; i < min(n, held); i += kSelThreads) s_keys[i] = ordered(mass_of(p, page0, base + i, h));
-    auto key = [&](int i) { return i < held ? s_keys[i] : ordered(mass_of(p, page0, base + i, h)); };
+    for (int i0 = tid; i0 < min(n, held); i0 += kLoads * THREADS) {  // several pages, then several weights under way
+        Place x[kLoads];
+        float m[kLoads];
+#pragma unroll
+        for (int k = 0; k < kLoads; ++k) {
+            x[k].page = -1;
+            if (i0 + k * THREADS < n) x[k] = place_of(p, page0, base + i0 + k * THREADS);
+        }
+#pragma unroll
+        for (int k = 0; k < kLoads; ++k)
+            m[k] = x[k].page < 0 ? 0.f : p.mass[x[k].page * p.m_page + x[k].slot * p.m_slot + h * p.m_head];
+#pragma unroll
+        for (int k = 0; k < kLoads; ++k)
+            if (i0 + k * THREADS < min(n, held)) s_mass[i0 + k * THREADS] = m[k];
+    }
+    auto mass = [&](int i) { return i < held ? s_mass[i] : mass_of(p, page0, base + i, h); };
 
-    // the value of the heavy-th largest, from its high bits on
+    // The value of the heavy-th largest, from its high bits on: 11 of them, then 8, 8 and 5 of the keys that
+    // begin alike, which the second round lists (where they are not too many).
     uint32_t prefix = 0;
-    int need = c.heavy;  // how many of those that begin with the prefix are chosen
-    int shift = 32;
-#pragma unroll 1
-    for (int round = 0; round < 3; ++round) {
-        const int bits = round < 2 ? 11 : 10;
-        const uint32_t above = shift == 32 ? 0u : ~0u << shift;
-        shift -= bits;
-        for (int i = tid; i < kBins; i += kSelThreads) s_hist[i] = 0;
-        __syncthreads();
-        for (int i = tid; i < n; i += kSelThreads) {
-            const uint32_t k = key(i);
-            if ((k & above) == prefix) atomicAdd(&s_hist[k >> shift & ((1u << bits) - 1)], 1u);
+    int need = c.heavy, alike = 0;  // how many of those that begin with the prefix are chosen, and are there
+    // the bin of the need-th key from above, over all CTAs; EACH bins a thread
+    auto pick = [&](int bins, int shift, auto each_) {
+        constexpr int EACH = decltype(each_)::value;
+        const int bin0 = bins - EACH - tid * EACH;
+        uint32_t v[EACH] = {};
+        if (bin0 >= 0) {
+            if (ctas == 1) {
+#pragma unroll
+                for (int i = 0; i < EACH; ++i) v[i] = s_hist[bin0 + i];
+            } else {
+#pragma unroll
+                for (int r = 0; r < kMostCtas; ++r) {
+                    if (r >= ctas) continue;
+                    const uint32_t* from = cl.map_shared_rank(s_hist, r) + bin0;
+#pragma unroll
+                    for (int i = 0; i < EACH; ++i) v[i] += from[i];
+                }
+            }
         }
-        cl.sync();
-        // each thread adds four bins of all CTAs; the scan goes from the highest bin down
-        const int bin0 = kBins - 4 - tid * 4;
-        uint32_t v[4] = {0, 0, 0, 0};
-        for (int r = 0; r < ctas; ++r) {
-            const uint4 x = *reinterpret_cast<const uint4*>(cl.map_shared_rank(s_hist, r) + bin0);
-            v[0] += x.x, v[1] += x.y, v[2] += x.z, v[3] += x.w;
-        }
-        const int mine = (int)(v[0] + v[1] + v[2] + v[3]);
+        int mine = 0;
+#pragma unroll
+        for (int i = 0; i < EACH; ++i) mine += (int)v[i];
         int scan = mine;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
             const int x = __shfl_up_sync(kFull, scan, o);
             if (lane >= o) scan += x;
         }
-        const Before w = warps_before(__shfl_sync(kFull, scan, 31), s_warp);
-        int higher = w.mine + scan - mine;  // keys in the bins above mine
+        if (lane == 31) s_warp[warp].x = scan;
+        __syncthreads();
+        const int below = __reduce_add_sync(kFull, lane < warp ? s_warp[lane].x : 0);
+        int higher = below + scan - mine;  // keys in the bins above mine
         if (higher < need && higher + mine >= need) {
 #pragma unroll
-            for (int i = 3; i >= 0; --i) {
-                if (higher < need && higher + (int)v[i] >= need) s_pick[0] = bin0 + i, s_pick[1] = need - higher;
+            for (int i = EACH - 1; i >= 0; --i) {
+                if (higher < need && higher + (int)v[i] >= need) s_pick[0] = bin0 + i, s_pick[1] = need - higher, s_pick[2] = v[i];
                 higher += v[i];
             }
         }
-        cl.sync();  // the histograms have been read
+        sync();  // the histograms have been read
         prefix |= (uint32_t)s_pick[0] << shift;
-        need = s_pick[1];
+        need = s_pick[1], alike = s_pick[2];
+    };
+#pragma unroll 1
+    for (int round = 0; round < 4; ++round) {
+        const int bits = round == 0 ? 11 : round < 3 ? 8 : 5, shift = round == 0 ? 21 : round == 1 ? 13 : round == 2 ? 5 : 0;
+        const uint32_t above = round == 0 ? 0u : ~0u << (shift + bits), mask = (1u << bits) - 1;
+        for (int i = tid; i < 1 << bits; i += THREADS) s_hist[i] = 0;
+        if (tid == 0 && round == 0) s_listed = 0;
+        __syncthreads();
+        const int listed = s_listed;
+        if (round > 1 && listed <= kListed) {
+            for (int i = tid; i < listed; i += THREADS)
+                if ((s_list[i] & above) == prefix) atomicAdd(&s_hist[s_list[i] >> shift & mask], 1u);
+        } else {
+            for (int i0 = 0; i0 < n; i0 += THREADS) {
+                const uint32_t k = i0 + tid < n ? ordered(mass(i0 + tid)) : 0u;
+                const bool same = i0 + tid < n && (k & above) == prefix;
+                if (same) atomicAdd(&s_hist[k >> shift & mask], 1u);
+                if (round == 1) {
+                    const uint32_t all_same = __ballot_sync(kFull, same);
+                    if (all_same) {
+                        int at = 0;
+                        if (lane == 0) at = atomicAdd(&s_listed, __popc(all_same));
+                        at = __shfl_sync(kFull, at, 0) + __popc(all_same & ((1u << lane) - 1));
+                        if (same && at < kListed) s_list[at] = k;
+                    }
+                }
+            }
+        }
+        sync();
+        if (round == 0) pick(1 << bits, shift, std::integral_constant<int, kBins / THREADS>());
+        else pick(1 << bits, shift, std::integral_constant<int, 1>());
     }
 
     // A warp's places are consecutive.  Equal ones are chosen from the lowest place on: how many lie
     // before the warp's?
     const int w0 = min(warp * per_warp, n), w1 = min(w0 + per_warp, n);
-    int equal = 0;
-    for (int i = w0; i < w1; i += 32) equal += __popc(__ballot_sync(kFull, i + lane < w1 && key(i + lane) == prefix));
-    Before wb = warps_before(equal, s_warp);
-    Before cb = ctas_before(cl, wb.all, &s_cta);
-    const int equal0 = cb.mine + wb.mine;
-    // walks the warp's places: what(hole, moved, place) with the masks of the 32
+    int equal0 = 0;
+    if (need < alike) {  // the same for the whole cluster
+        int equal = 0;
+        for (int i = w0; i < w1; i += 32) equal += __popc(__ballot_sync(kFull, i + lane < w1 && ordered(mass(i + lane)) == prefix));
+        const Before wb = warps_before<kWarps>(make_int3(equal, 0, 0), s_warp), cb = ctas_before(cl, wb.all, &s_cta);
+        equal0 = cb.mine.x + wb.mine.x;
+    }
+    // walks the warp's places: what(holes, moved, place, stays, weight) with the masks of the 32
+    const bool ties = need < alike;
     auto walk = [&](auto what) {
         int eq = equal0;
         for (int i = w0; i < w1; i += 32) {
             const bool in = i + lane < w1;
-            const uint32_t k = in ? key(i + lane) : 0u;
-            const uint32_t same = __ballot_sync(kFull, in && k == prefix);
-            const bool chosen = in && (k > prefix || (k == prefix && eq + __popc(same & ((1u << lane) - 1)) < need));
-            eq += __popc(same);
+            const float m = in ? mass(i + lane) : 0.f;
+            const uint32_t k = ordered(m);
+            bool chosen = in && k >= prefix;
+            if (ties) {
+                const uint32_t same = __ballot_sync(kFull, in && k == prefix);
+                chosen = in && (k > prefix || (k == prefix && eq + __popc(same & ((1u << lane) - 1)) < need));
+                eq += __popc(same);
+            }
             const int at = base + i + lane;
             const bool front = at < new_end;
-            what(__ballot_sync(kFull, in && front && !chosen), __ballot_sync(kFull, chosen && !front), at, chosen && front);
+            what(__ballot_sync(kFull, in && front && !chosen), __ballot_sync(kFull, chosen && !front), at, chosen && front, m);
         }
     };
-    int holes = 0, moved = 0, early = 0;
-    walk([&](uint32_t hole, uint32_t move, int at, bool) {
-        holes += __popc(hole);
-        moved += __popc(move);
-        early += __popc(__ballot_sync(kFull, at < c.size) & move);
+    int3 sums = make_int3(0, 0, 0);  // holes, those that fill them, those of them from places before the new length
+    walk([&](uint32_t hole, uint32_t move, int at, bool, float) {
+        sums.x += __popc(hole);
+        sums.y += __popc(move);
+        sums.z += __popc(__ballot_sync(kFull, at < c.size) & move);
     });
-    wb = warps_before(holes, s_warp);
-    cb = ctas_before(cl, wb.all, &s_cta);
-    int hole_at = cb.mine + wb.mine;
-    wb = warps_before(early, s_warp);
-    cb = ctas_before(cl, wb.all, &s_cta);
-    const int early_all = cb.all;
-    wb = warps_before(moved, s_warp);
-    cb = ctas_before(cl, wb.all, &s_cta);
-    int move_at = cb.mine + wb.mine;
-    if (me == 0) p.counts[unit] = make_int4(cb.all, early_all, c.size, c.gone);
+    const Before wb = warps_before<kWarps>(sums, s_warp), cb = ctas_before(cl, wb.all, &s_cta);
+    int hole_at = cb.mine.x + wb.mine.x, move_at = cb.mine.y + wb.mine.y;
+    if (me == 0) p.counts[unit] = make_int4(cb.all.y, cb.all.z, c.size, c.gone);
     int* const hole_list = p.holes + (int64_t)unit * p.width;
     int* const fill_list = p.fills + (int64_t)unit * p.width;
-    walk([&](uint32_t hole, uint32_t move, int at, bool stay) {
+    walk([&](uint32_t hole, uint32_t move, int at, bool stay, float m) {
         const uint32_t below = (1u << lane) - 1;
         if (hole >> lane & 1) hole_list[hole_at + __popc(hole & below)] = at;
         if (move >> lane & 1) fill_list[move_at + __popc(move & below)] = at;
-        if (stay) stays(at);
+        if (stay) stays(at, m);
         hole_at += __popc(hole);
         move_at += __popc(move);
     });
-    cl.sync();  // no CTA leaves while its counts are read
+    first_stay();
+    if (ctas > 1) cl.sync();  // no CTA leaves while its counts are read
 }
 
-// Rows of U bytes at a time.
+// Words of U bytes.
 template <int U>
-struct Unit;
+struct Word;
 template <>
-struct Unit<16> { using type = uint4; };
+struct Word<16> { using type = uint4; };
 template <>
-struct Unit<4> { using type = uint32_t; };
+struct Word<4> { using type = uint32_t; };
 template <>
-struct Unit<2> { using type = uint16_t; };
+struct Word<2> { using type = uint16_t; };
 
 template <int U>
-__global__ void __launch_bounds__(kMoveThreads) move_kernel(const __grid_constant__ EvictParams p) {
-    using W = typename Unit<U>::type;
-    constexpr int kAhead = 4;  // rows of a thread under way
+__global__ void __launch_bounds__(kMoveThreads, 4) move_kernel(const __grid_constant__ EvictParams p) {
+    using W = typename Word<U>::type;
+    constexpr int kAhead = 8;  // words of a thread under way
+    // of each staged move: bytes from the head's first element to its old and new rows of k and of v, -1:
+    // no such page
+    __shared__ int64_t s_k[2][kMoveThreads], s_v[2][kMoveThreads];
     cg::cluster_group cl = cg::this_cluster();
     const int ctas = cl.num_blocks(), rank = cl.block_rank();
     const int cluster = blockIdx.x / ctas, part = cluster % p.parts, unit = cluster / p.parts;
-    const int h = unit % p.heads, b = unit / p.heads;
-    const int words = p.row_bytes / U;
-    // lanes of a row: words of k, words of v, and one for the mass and the list of what was kept
-    const int tid = threadIdx.x, per_row = 2 * words + 1, lanes = min(per_row, kMoveThreads), group = tid / lanes,
-              groups = kMoveThreads / lanes, lane = tid - group * lanes;
+    const int h = unit % p.heads, b = unit / p.heads, tid = threadIdx.x;
+    const int words = p.row_bytes / U, lanes = min(2 * words, kMoveThreads), groups = kMoveThreads / lanes, group = tid / lanes,
+              lane = tid - group * lanes;
+    const int ahead = min(kAhead, kMoveThreads / groups), batch = groups * ahead;  // rows of a CTA under way
+    const int staged = kMoveThreads / batch * batch;
     pdl_wait();
     const int4 n = p.counts[unit];
     const int fills = n.x, early = n.y, size = n.z, gone = n.w;
@@ -288,87 +365,72 @@ __global__ void __launch_bounds__(kMoveThreads) move_kernel(const __grid_constan
     const int recent = min(p.recent, size);
     const int* const hole_list = p.holes + (int64_t)unit * p.width;
     const int* const fill_list = p.fills + (int64_t)unit * p.width;
+    int32_t* const kept = p.kept ? p.kept + ((int64_t)b * p.heads + h) * p.kept_width : nullptr;
+    char *const k0 = p.k + h * p.k_head, *const v0 = p.v + h * p.v_head;
 
-    // Move i of the list: the early fills, the recent keys, then the other fills.
-    auto move = [&](int i, int& to, int& from) {
-        if (i < early || i >= early + recent) {
-            const int f = i < early ? i : i - recent;
-            to = hole_list[f], from = fill_list[f];
-        } else {
-            to = size - recent + i - early, from = to + gone;
+    // The list: the early fills, the recent keys, then the other fills.  Part 0 goes through the first two
+    // in order, a batch of the cluster read before it is written, and through all where it is the only
+    // part; the others share the rest.
+    const bool in_order = part == 0;
+    const int all = recent + fills, ordered_end = p.parts == 1 ? all : early + recent;
+    const int rest = all - ordered_end, shares = max(1, (p.parts - 1) * ctas), share = (part - 1) * ctas + rank;
+    const int begin = in_order ? 0 : ordered_end + (int)((int64_t)rest * share / shares);
+    const int end = in_order ? ordered_end : ordered_end + (int)((int64_t)rest * (share + 1) / shares);
+    const int spread = in_order ? ctas : 1;  // CTAs that share a batch
+    for (int at = begin; at < end; at += staged * spread) {
+        // move `tid` of mine: its places, weight and number
+        const int s = tid / batch, i = at + (s * spread + (in_order ? rank : 0)) * batch + tid - s * batch;
+        const bool mine = tid < staged && i < end;
+        int to = 0, from = 0;
+        float m = 0.f;
+        __syncthreads();  // the places before have been used
+        if (mine) {
+            if (i < early || i >= early + recent) {
+                const int f = i < early ? i : i - recent;
+                to = hole_list[f], from = fill_list[f];
+            } else {
+                to = size - recent + i - early, from = to + gone;
+            }
+            const Place x = place_of(p, page0, from), y = place_of(p, page0, to);
+            s_k[0][tid] = x.page < 0 ? -1 : x.page * p.k_page + x.slot * p.k_slot;
+            s_v[0][tid] = x.page < 0 ? -1 : x.page * p.v_page + x.slot * p.v_slot;
+            s_k[1][tid] = y.page < 0 ? -1 : y.page * p.k_page + y.slot * p.k_slot;
+            s_v[1][tid] = y.page < 0 ? -1 : y.page * p.v_page + y.slot * p.v_slot;
+            m = x.page < 0 ? 0.f : p.mass[x.page * p.m_page + x.slot * p.m_slot + h * p.m_head];
         }
-    };
-    struct Row {
-        W w;
-        char* out;
-        int mass_to;  // >= 0: the lane has the mass
-        float m;
-        int from;
-    };
-    auto load = [&](int i, int word, Row& r) {
-        int to, from;
-        move(i, to, from);
-        r.out = nullptr;
-        r.mass_to = -1;
-        if (word == 2 * words) {
-            r.mass_to = to, r.from = from;
-            r.m = mass_of(p, page0, from, h);
-            return;
-        }
-        const Place x = place_of(p, page0, from), y = place_of(p, page0, to);
-        const bool is_v = word >= words;
-        const int64_t off = (int64_t)(is_v ? word - words : word) * U;
-        memset(&r.w, 0, sizeof(W));
-        const char* in = is_v ? p.v + x.page * p.v_page + x.slot * p.v_slot + h * p.v_head
-                              : p.k + x.page * p.k_page + x.slot * p.k_slot + h * p.k_head;
-        if (x.page >= 0) r.w = *reinterpret_cast<const W*>(in + off);
-        if (y.page >= 0)
-            r.out = (is_v ? p.v + y.page * p.v_page + y.slot * p.v_slot + h * p.v_head
-                          : p.k + y.page * p.k_page + y.slot * p.k_slot + h * p.k_head) + off;
-    };
-    auto store = [&](const Row& r) {
-        if (r.out) *reinterpret_cast<W*>(r.out) = r.w;
-        if (r.mass_to >= 0) {
-            put_mass(p, page0, r.mass_to, h, r.m);
-            if (p.kept) p.kept[((int64_t)b * p.heads + h) * p.kept_width + r.mass_to] = r.from;
-        }
-    };
-
-    if (part == 0) {
-        // in order, a batch of the cluster read before it is written
-        const int list = early + recent, batch = ctas * groups * kAhead;
-        for (int w0 = 0; w0 < per_row; w0 += lanes) {
+        __syncthreads();
+        bool first = true;
+        for (int w0 = 0; w0 < 2 * words; w0 += lanes) {
             const int word = w0 + lane;
-            for (int i0 = 0; i0 < list; i0 += batch) {
-                Row r[kAhead];
+            const bool is_v = word >= words, has = group < groups && word < 2 * words;
+            const int64_t* const where = is_v ? s_v[0] : s_k[0];
+            char* const rows = (is_v ? v0 : k0) + (int64_t)(is_v ? word - words : word) * U;
+            for (int r0 = 0; r0 < staged; r0 += batch) {
+                const int left = end - (at + (r0 / batch * spread + (in_order ? rank : 0)) * batch);  // of the list, from this batch on
+                if (in_order ? end <= at + r0 * spread : left <= 0) break;                            // the same for the cluster
+                W w[kAhead];
 #pragma unroll
                 for (int k = 0; k < kAhead; ++k) {
-                    const int i = i0 + (k * ctas + rank) * groups + group;
-                    r[k].out = nullptr, r[k].mass_to = -1;
-                    if (group < groups && word < per_row && i < list) load(i, word, r[k]);
+                    const int r = group + k * groups;
+                    memset(&w[k], 0, sizeof(W));
+                    if (k < ahead && has && r < left && where[r0 + r] >= 0) w[k] = *reinterpret_cast<const W*>(rows + where[r0 + r]);
                 }
-                cl.sync();
+                if (in_order) {
+                    if (ctas == 1) __syncthreads();
+                    else cl.sync();
+                }
+                if (first && mine) {
+                    put_mass(p, page0, to, h, m);
+                    if (kept) kept[to] = from;
+                }
+                first = false;
 #pragma unroll
-                for (int k = 0; k < kAhead; ++k) store(r[k]);
+                for (int k = 0; k < kAhead; ++k) {
+                    const int r = group + k * groups;
+                    if (k < ahead && has && r < left && where[kMoveThreads + r0 + r] >= 0)
+                        *reinterpret_cast<W*>(rows + where[kMoveThreads + r0 + r]) = w[k];
+                }
             }
-        }
-        return;
-    }
-    const int rest = fills - early, share = ((p.parts - 1) * ctas), mine = (part - 1) * ctas + rank;
-    const int begin = (int)((int64_t)rest * mine / share), end = (int)((int64_t)rest * (mine + 1) / share);
-    if (group >= groups) return;
-    for (int w0 = 0; w0 < per_row; w0 += lanes) {
-        const int word = w0 + lane;
-        if (word >= per_row) break;
-        for (int i0 = begin + group; i0 < end; i0 += groups * kAhead) {
-            Row r[kAhead];
-#pragma unroll
-            for (int k = 0; k < kAhead; ++k) {
-                r[k].out = nullptr, r[k].mass_to = -1;
-                if (i0 + k * groups < end) load(early + recent + i0 + k * groups, word, r[k]);
-            }
-#pragma unroll
-            for (int k = 0; k < kAhead; ++k) store(r[k]);
         }
     }
 }
@@ -377,7 +439,7 @@ __global__ void __launch_bounds__(kMoveThreads) move_kernel(const __grid_constan
 struct Plan {
     EvictParams p;
     int unit;           // bytes moved at once
-    int select_ctas, move_ctas;
+    int select_ctas, select_threads, move_ctas;
     int held;
     size_t bytes, counts_bytes;
 };
@@ -403,6 +465,9 @@ int make_plan(const tg_kv_evict_args* a, int elem, Plan* plan, const char* op) {
     EvictParams& p = plan->p;
     p = {};
     p.pages = t, p.page_size = c.page_size, p.n_pages = c.pages;
+    p.page_shift = -1;
+    for (int i = 0; i < 31; ++i)
+        if (c.page_size == (1ll << i)) p.page_shift = i;
     p.seq_len = a->seq_len, p.seq_len_out = a->seq_len_out;
     p.max_seq = (int)max_seq;
     p.budget = (int)std::min<int64_t>(a->budget, INT32_MAX / 2);
@@ -431,18 +496,21 @@ int make_plan(const tg_kv_evict_args* a, int elem, Plan* plan, const char* op) {
     // The selection: 8192 candidates a CTA, and more CTAs where few pairs leave SMs idle.
     const int64_t most = gone > 0 ? max_seq : 0;
     plan->select_ctas = 1;
-    while (plan->select_ctas < 8 && (most > 8192ll * plan->select_ctas ||
-                                     (most > 2048ll * plan->select_ctas && units * plan->select_ctas * 2 <= kSMs)))
+    while (plan->select_ctas < kMostCtas && (most > 8192ll * plan->select_ctas ||
+                                             (most > 2048ll * plan->select_ctas && units * plan->select_ctas * 2 <= kSMs)))
         plan->select_ctas *= 2;
-    plan->held = (int)std::min<int64_t>(kSelKeys, ceil_div(ceil_div(most, plan->select_ctas * kSelWarps), 32) * 32 * kSelWarps);
+    const int64_t each = ceil_div(most, plan->select_ctas);
+    plan->select_threads = each > 4096 ? 512 : 256;
+    plan->held = (int)std::min<int64_t>(kSelKeys, ceil_div(each, plan->select_threads) * plan->select_threads);
     // The move: the list in order by a cluster of up to eight CTAs, 64 rows each at once; the other
-    // fills in parts of 64 rows and more, about eight CTAs an SM in all.
+    // fills in parts of 64 rows and more, about eight CTAs an SM in all, or at the end of the list where
+    // they are few.
     const int64_t in_order = std::min<int64_t>(p.recent, p.budget) * 2;
     plan->move_ctas = 1;
-    while (plan->move_ctas < 8 && in_order > 64ll * plan->move_ctas) plan->move_ctas *= 2;
+    while (plan->move_ctas < kMostCtas && in_order > 128ll * plan->move_ctas) plan->move_ctas *= 2;
     const int64_t want = std::min(ceil_div(p.width, 64 * plan->move_ctas),
                                   std::max<int64_t>(1, kSMs * 8 / std::max<int64_t>(1, units * plan->move_ctas)));
-    p.parts = 1 + (p.width > 0 ? (int)std::max<int64_t>(1, want) : 0);
+    p.parts = 1 + (p.width > 32 ? (int)std::max<int64_t>(1, want) : 0);
     if (units * std::max(p.parts * plan->move_ctas, plan->select_ctas) > INT32_MAX)
         return set_error(TG_EUNSUPPORTED, "%s: too many sequences for one launch", op);
     plan->counts_bytes = ((size_t)units * sizeof(int4) + 255) / 256 * 256;
@@ -495,10 +563,11 @@ int evict(const tg_kv_evict_args* a, int elem, void* ws, size_t ws_bytes, tg_str
     p.fills = p.holes + (int64_t)p.rows * p.heads * p.width;
     const int64_t units = (int64_t)p.rows * p.heads;
     const size_t smem = (size_t)plan.held * sizeof(uint32_t);
-    static SmemOnce once;
-    rc = once.raise(reinterpret_cast<const void*>(select_kernel), kSelKeys * (int)sizeof(uint32_t));
+    auto select = plan.select_threads == 256 ? select_kernel<256> : select_kernel<512>;
+    static SmemOnce once[2];
+    rc = once[plan.select_threads == 256].raise(reinterpret_cast<const void*>(select), kSelKeys * (int)sizeof(uint32_t));
     if (rc != TG_OK) return rc;
-    rc = launch_clusters("select_kernel", select_kernel, units * plan.select_ctas, kSelThreads, plan.select_ctas, smem, false, st, p,
+    rc = launch_clusters("select_kernel", select, units * plan.select_ctas, plan.select_threads, plan.select_ctas, smem, false, st, p,
                          plan.held);
     if (rc != TG_OK) return rc;
     auto kernel = plan.unit == 16 ? move_kernel<16> : plan.unit == 4 ? move_kernel<4> : move_kernel<2>;
