@@ -80,8 +80,11 @@ __device__ __forceinline__ Cut cut_of(const EvictParams& p, int64_t b, int64_t& 
 struct Place {
     int page, slot;  // page -1: not in the cache
 };
+__device__ __forceinline__ int page_index(const EvictParams& p, int at) {
+    return p.page_shift >= 0 ? at >> p.page_shift : at / (int)p.page_size;
+}
 __device__ __forceinline__ Place place_of(const EvictParams& p, int64_t page0, int at) {
-    const int j = p.page_shift >= 0 ? at >> p.page_shift : at / (int)p.page_size;
+    const int j = page_index(p, at);
     const int64_t id = __ldg(p.pages.indices + page0 + j);
     return {id >= 0 && id < p.n_pages ? (int)id : -1, at - j * (int)p.page_size};
 }
@@ -139,11 +142,12 @@ __device__ __forceinline__ Before ctas_before(cg::cluster_group& cl, int3 v, int
 // sequences).
 template <int THREADS>
 __global__ void __launch_bounds__(THREADS) select_kernel(const __grid_constant__ EvictParams p, const int held) {
-    constexpr int kWarps = THREADS / 32, kLoads = THREADS / 128;  // weights of a thread under way
+    constexpr int kWarps = THREADS / 32, kLoads = 8;                  // weights of a thread under way
+    constexpr int kList = kListed / kWarps;  // places of a warp's list
     extern __shared__ float s_mass[];  // [held]
-    __shared__ __align__(16) uint32_t s_hist[kBins];
+    __shared__ uint32_t s_hist[kBins], s_total[kBins];  // s_total: of the cluster
     __shared__ int3 s_warp[kWarps], s_cta;
-    __shared__ int s_pick[3], s_listed;
+    __shared__ int s_pick[3], s_over;
     __shared__ uint32_t s_list[kListed];
     cg::cluster_group cl = cg::this_cluster();
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -182,20 +186,22 @@ __global__ void __launch_bounds__(THREADS) select_kernel(const __grid_constant__
     const int per_warp = ((all + ctas * kWarps - 1) / (ctas * kWarps) + 31) & ~31, per = per_warp * kWarps;
     const int lo = min(rank * per, all), n = min(lo + per, all) - lo;  // candidates lo .. lo + n, from place c.first
     const int base = c.first + lo;
-    for (int i0 = tid; i0 < min(n, held); i0 += kLoads * THREADS) {  // several pages, then several weights under way
-        Place x[kLoads];
+    // several pages, then several weights under way (of a place that is none, some)
+    for (int i0 = tid; i0 < min(n, held); i0 += kLoads * THREADS) {
+        int64_t id[kLoads];
         float m[kLoads];
+        bool there[kLoads];
+#pragma unroll
+        for (int k = 0; k < kLoads; ++k) id[k] = __ldg(p.pages.indices + page0 + page_index(p, base + min(i0 + k * THREADS, n - 1)));
 #pragma unroll
         for (int k = 0; k < kLoads; ++k) {
-            x[k].page = -1;
-            if (i0 + k * THREADS < n) x[k] = place_of(p, page0, base + i0 + k * THREADS);
+            const int at = base + min(i0 + k * THREADS, n - 1), slot = at - page_index(p, at) * (int)p.page_size;
+            there[k] = id[k] >= 0 && id[k] < p.n_pages;
+            m[k] = __ldg(p.mass + (there[k] ? id[k] : 0) * p.m_page + slot * p.m_slot + h * p.m_head);
         }
 #pragma unroll
         for (int k = 0; k < kLoads; ++k)
-            m[k] = x[k].page < 0 ? 0.f : p.mass[x[k].page * p.m_page + x[k].slot * p.m_slot + h * p.m_head];
-#pragma unroll
-        for (int k = 0; k < kLoads; ++k)
-            if (i0 + k * THREADS < min(n, held)) s_mass[i0 + k * THREADS] = m[k];
+            if (i0 + k * THREADS < min(n, held)) s_mass[i0 + k * THREADS] = there[k] ? m[k] : 0.f;
     }
     auto mass = [&](int i) { return i < held ? s_mass[i] : mass_of(p, page0, base + i, h); };
 
@@ -206,22 +212,30 @@ __global__ void __launch_bounds__(THREADS) select_kernel(const __grid_constant__
     // the bin of the need-th key from above, over all CTAs; EACH bins a thread
     auto pick = [&](int bins, int shift, auto each_) {
         constexpr int EACH = decltype(each_)::value;
+        const uint32_t* hist = s_hist;
+        if (ctas > 1) {
+            // each CTA adds a share of the bins of all, then everyone takes all shares: in steps of whole lines,
+            // as other CTAs' memory is read slowly otherwise
+            const int part = bins / ctas;
+            for (int i = tid; i < part; i += THREADS) {
+                uint32_t sum = 0;
+#pragma unroll
+                for (int r = 0; r < kMostCtas; ++r)
+                    if (r < ctas) sum += cl.map_shared_rank(s_hist, r)[rank * part + i];
+                s_total[rank * part + i] = sum;
+            }
+            cl.sync();
+#pragma unroll 4
+            for (int i = tid; i < bins; i += THREADS)
+                if (i / part != rank) s_total[i] = cl.map_shared_rank(s_total, i / part)[i];
+            __syncthreads();
+            hist = s_total;
+        }
         const int bin0 = bins - EACH - tid * EACH;
         uint32_t v[EACH] = {};
-        if (bin0 >= 0) {
-            if (ctas == 1) {
+        if (bin0 >= 0)
 #pragma unroll
-                for (int i = 0; i < EACH; ++i) v[i] = s_hist[bin0 + i];
-            } else {
-#pragma unroll
-                for (int r = 0; r < kMostCtas; ++r) {
-                    if (r >= ctas) continue;
-                    const uint32_t* from = cl.map_shared_rank(s_hist, r) + bin0;
-#pragma unroll
-                    for (int i = 0; i < EACH; ++i) v[i] += from[i];
-                }
-            }
-        }
+            for (int i = 0; i < EACH; ++i) v[i] = hist[bin0 + i];
         int mine = 0;
 #pragma unroll
         for (int i = 0; i < EACH; ++i) mine += (int)v[i];
@@ -246,32 +260,33 @@ __global__ void __launch_bounds__(THREADS) select_kernel(const __grid_constant__
         prefix |= (uint32_t)s_pick[0] << shift;
         need = s_pick[1], alike = s_pick[2];
     };
+    int listed = 0;  // by my warp
+    uint32_t* const list = s_list + warp * kList;
 #pragma unroll 1
     for (int round = 0; round < 4; ++round) {
         const int bits = round == 0 ? 11 : round < 3 ? 8 : 5, shift = round == 0 ? 21 : round == 1 ? 13 : round == 2 ? 5 : 0;
         const uint32_t above = round == 0 ? 0u : ~0u << (shift + bits), mask = (1u << bits) - 1;
         for (int i = tid; i < 1 << bits; i += THREADS) s_hist[i] = 0;
-        if (tid == 0 && round == 0) s_listed = 0;
+        if (tid == 0 && round == 0) s_over = 0;
         __syncthreads();
-        const int listed = s_listed;
-        if (round > 1 && listed <= kListed) {
-            for (int i = tid; i < listed; i += THREADS)
-                if ((s_list[i] & above) == prefix) atomicAdd(&s_hist[s_list[i] >> shift & mask], 1u);
+        if (round > 1 && !s_over) {
+            for (int i = lane; i < listed; i += 32)
+                if ((list[i] & above) == prefix) atomicAdd(&s_hist[list[i] >> shift & mask], 1u);
         } else {
+#pragma unroll 4
             for (int i0 = 0; i0 < n; i0 += THREADS) {
                 const uint32_t k = i0 + tid < n ? ordered(mass(i0 + tid)) : 0u;
                 const bool same = i0 + tid < n && (k & above) == prefix;
                 if (same) atomicAdd(&s_hist[k >> shift & mask], 1u);
                 if (round == 1) {
                     const uint32_t all_same = __ballot_sync(kFull, same);
-                    if (all_same) {
-                        int at = 0;
-                        if (lane == 0) at = atomicAdd(&s_listed, __popc(all_same));
-                        at = __shfl_sync(kFull, at, 0) + __popc(all_same & ((1u << lane) - 1));
-                        if (same && at < kListed) s_list[at] = k;
-                    }
+                    const int at = listed + __popc(all_same & ((1u << lane) - 1));
+                    if (same && at < kList) list[at] = k;
+                    listed += __popc(all_same);
                 }
             }
+            if (round == 1 && listed > kList) s_over = 1;
+            __syncwarp();
         }
         sync();
         if (round == 0) pick(1 << bits, shift, std::integral_constant<int, kBins / THREADS>());
@@ -288,43 +303,72 @@ __global__ void __launch_bounds__(THREADS) select_kernel(const __grid_constant__
         const Before wb = warps_before<kWarps>(make_int3(equal, 0, 0), s_warp), cb = ctas_before(cl, wb.all, &s_cta);
         equal0 = cb.mine.x + wb.mine.x;
     }
-    // walks the warp's places: what(holes, moved, place, stays, weight) with the masks of the 32
+    // Walks the warp's places, kStep times 32 at a time: what(places, chosen, weights).
     const bool ties = need < alike;
+    constexpr int kStep = 4;
     auto walk = [&](auto what) {
         int eq = equal0;
-        for (int i = w0; i < w1; i += 32) {
-            const bool in = i + lane < w1;
-            const float m = in ? mass(i + lane) : 0.f;
-            const uint32_t k = ordered(m);
-            bool chosen = in && k >= prefix;
-            if (ties) {
-                const uint32_t same = __ballot_sync(kFull, in && k == prefix);
-                chosen = in && (k > prefix || (k == prefix && eq + __popc(same & ((1u << lane) - 1)) < need));
-                eq += __popc(same);
+        for (int i = w0; i < w1; i += 32 * kStep) {
+            float m[kStep];
+            bool chosen[kStep];
+#pragma unroll
+            for (int k = 0; k < kStep; ++k) m[k] = i + k * 32 + lane < w1 ? mass(i + k * 32 + lane) : 0.f;
+#pragma unroll
+            for (int k = 0; k < kStep; ++k) {
+                const bool in = i + k * 32 + lane < w1;
+                const uint32_t x = ordered(m[k]);
+                chosen[k] = in && x >= prefix;
+                if (ties) {
+                    const uint32_t same = __ballot_sync(kFull, in && x == prefix);
+                    chosen[k] = in && (x > prefix || (x == prefix && eq + __popc(same & ((1u << lane) - 1)) < need));
+                    eq += __popc(same);
+                }
             }
-            const int at = base + i + lane;
-            const bool front = at < new_end;
-            what(__ballot_sync(kFull, in && front && !chosen), __ballot_sync(kFull, chosen && !front), at, chosen && front, m);
+            what(base + i + lane, chosen, m);
         }
     };
+    const int place_end = base + w1;
     int3 sums = make_int3(0, 0, 0);  // holes, those that fill them, those of them from places before the new length
-    walk([&](uint32_t hole, uint32_t move, int at, bool, float) {
-        sums.x += __popc(hole);
-        sums.y += __popc(move);
-        sums.z += __popc(__ballot_sync(kFull, at < c.size) & move);
+    walk([&](int at, const bool (&chosen)[kStep], const float (&)[kStep]) {
+#pragma unroll
+        for (int k = 0; k < kStep; ++k) {
+            const bool front = at + k * 32 < new_end;
+            sums.x += front && !chosen[k] && at + k * 32 < place_end;
+            sums.y += chosen[k] && !front;
+            sums.z += chosen[k] && !front && at + k * 32 < c.size;
+        }
     });
+    sums = make_int3(__reduce_add_sync(kFull, sums.x), __reduce_add_sync(kFull, sums.y), __reduce_add_sync(kFull, sums.z));
     const Before wb = warps_before<kWarps>(sums, s_warp), cb = ctas_before(cl, wb.all, &s_cta);
     int hole_at = cb.mine.x + wb.mine.x, move_at = cb.mine.y + wb.mine.y;
     if (me == 0) p.counts[unit] = make_int4(cb.all.y, cb.all.z, c.size, c.gone);
     int* const hole_list = p.holes + (int64_t)unit * p.width;
     int* const fill_list = p.fills + (int64_t)unit * p.width;
-    walk([&](uint32_t hole, uint32_t move, int at, bool stay, float m) {
+    walk([&](int at, const bool (&chosen)[kStep], const float (&m)[kStep]) {
         const uint32_t below = (1u << lane) - 1;
-        if (hole >> lane & 1) hole_list[hole_at + __popc(hole & below)] = at;
-        if (move >> lane & 1) fill_list[move_at + __popc(move & below)] = at;
-        if (stay) stays(at, m);
-        hole_at += __popc(hole);
-        move_at += __popc(move);
+        bool stay[kStep];
+#pragma unroll
+        for (int k = 0; k < kStep; ++k) {
+            const bool front = at + k * 32 < new_end, is_hole = front && !chosen[k] && at + k * 32 < place_end, moves = chosen[k] && !front;
+            const uint32_t hole = __ballot_sync(kFull, is_hole), move = __ballot_sync(kFull, moves);
+            if (is_hole) hole_list[hole_at + __popc(hole & below)] = at + k * 32;
+            if (moves) fill_list[move_at + __popc(move & below)] = at + k * 32;
+            hole_at += __popc(hole);
+            move_at += __popc(move);
+            stay[k] = chosen[k] && front;
+        }
+        if (!p.moved && !kept) return;
+        Place x[kStep];
+#pragma unroll
+        for (int k = 0; k < kStep; ++k) {
+            x[k].page = -1;
+            if (p.moved && stay[k]) x[k] = place_of(p, page0, at + k * 32);
+        }
+#pragma unroll
+        for (int k = 0; k < kStep; ++k) {
+            if (x[k].page >= 0) p.mass_out[x[k].page * p.mo_page + x[k].slot * p.mo_slot + h * p.mo_head] = m[k];
+            if (kept && stay[k]) kept[at + k * 32] = at + k * 32;
+        }
     });
     first_stay();
     if (ctas > 1) cl.sync();  // no CTA leaves while its counts are read
