@@ -305,65 +305,62 @@ def rope_backward(dout: torch.Tensor, r: Rope, positions: torch.Tensor, out: Opt
     return _turn(dout, r, positions, out, _lib.TG_FLAG_ROPE_INVERSE, stream)
 
 
-def _norm_shape(q: torch.Tensor, k: Optional[torch.Tensor]):
-    """(suffix, device, dim, q's shape, k's shape) of a pair of queries and keys."""
+_NO_ROWS = _lib.TgRows()
+
+
+def _norm_inputs(q, k, q_norm, k_norm, rope, positions):
+    """(suffix, device, q's rows, k's rows, k's shape, descriptors of the norms and the rope, positions)."""
     suffix = _SUFFIX.get(q.dtype)
     if q.dim() != 3 or not q.is_cuda or suffix is None:
         raise ValueError("q must be [tokens, heads, dim], float32, float16 or bfloat16, on a CUDA device (got %s %s on %s)"
                          % (tuple(q.shape), q.dtype, q.device))
-    if k is not None and k.dim() != 3:
-        raise ValueError("k must be [tokens, heads, dim] (got %s)" % (tuple(k.shape),))
-    tokens, heads, dim = q.shape
-    return suffix, q.get_device(), dim, q.shape, (tokens, 0 if k is None else k.shape[1], dim)
-
-
-def _norm_args(args, held, q, k, q_norm, k_norm, rope, positions):
-    """Fills what the forward and the gradient have in common; what it points to goes into held."""
-    _, index, dim, qs, ks = _norm_shape(q, k)
-    dt = q.dtype
-    args.tokens, args.dim, args.q_heads, args.k_heads = qs[0], dim, qs[1], ks[1]
-    args.q = _rows(q, "q", qs, dt, index)
+    index, dt, qs = q.get_device(), q.dtype, q.shape
+    qr, kr, ks = _rows(q, "q", qs, dt, index), _NO_ROWS, None
     if k is not None:
-        args.k = _rows(k, "k", ks, dt, index)
+        if k.dim() != 3:
+            raise ValueError("k must be [tokens, heads, dim] (got %s)" % (tuple(k.shape),))
+        ks = (qs[0], k.shape[1], qs[2])
+        kr = _rows(k, "k", ks, dt, index)
     elif k_norm is not None:
         raise ValueError("k_norm without k")
-    for name, norm in (("q_norm", q_norm), ("k_norm", k_norm)):
-        if norm is not None:
-            d = norm.desc(dim, dt, index)
-            held.append(d)
-            setattr(args, name, ctypes.addressof(d))
+    held = (None if q_norm is None else q_norm.desc(qs[2], dt, index), None if k_norm is None else k_norm.desc(qs[2], dt, index),
+            None if rope is None else rope.desc(index))
+    pos = None
     if rope is not None:
         if positions is None:
             raise ValueError("a rotation needs positions")
-        d = rope.desc(index)
-        held.append(d)
-        args.rope = ctypes.addressof(d)
-        args.positions = _vector(positions, "positions", index, qs[0])
-    return args
+        pos = _vector(positions, "positions", index, qs[0])
+    return suffix, index, qr, kr, ks, held, pos
+
+
+def _address(desc) -> Optional[int]:
+    return None if desc is None else ctypes.addressof(desc)
 
 
 def _norm_call(q, k, q_norm, k_norm, rope, positions, q_out, k_out, stream):
-    held: list = []
-    a = _norm_args(_lib.TgNormRopeArgs(), held, q, k, q_norm, k_norm, rope, positions)
-    suffix, index, _, qs, ks = _norm_shape(q, k)
+    inputs = _norm_inputs(q, k, q_norm, k_norm, rope, positions)
     if k is None and k_out is not None:
         raise ValueError("k_out without k")
-    sp = _stream(index, stream)
-    where = _elsewhere(index, stream)
+    sp = _stream(inputs[1], stream)
+    where = _elsewhere(inputs[1], stream)
     if where is not None:
         with where:
-            return _norm_launch(a, suffix, q, k, q_out, k_out, qs, ks, index, sp)
-    return _norm_launch(a, suffix, q, k, q_out, k_out, qs, ks, index, sp)
+            return _norm_launch(inputs, q, k, q_out, k_out, sp)
+    return _norm_launch(inputs, q, k, q_out, k_out, sp)
 
 
-def _norm_launch(a, suffix, q, k, q_out, k_out, qs, ks, index, sp):
+def _norm_launch(inputs, q, k, q_out, k_out, sp):
+    suffix, index, qr, kr, ks, held, pos = inputs
+    qs, ko = q.shape, _NO_ROWS
     if q_out is None:
         q_out = _like(q)
-    a.q_out = _rows(q_out, "q_out", qs, q.dtype, index)
+    qo = _rows(q_out, "q_out", qs, q.dtype, index)
     if k is not None:
         if k_out is None:
             k_out = _like(k)
-        a.k_out = _rows(k_out, "k_out", ks, q.dtype, index)
+        ko = _rows(k_out, "k_out", ks, q.dtype, index)
+    qn, kn, rd = held
+    a = _lib.TgNormRopeArgs(qs[0], qs[2], qs[1], ks[1] if ks else 0, qr, kr, qo, ko, _address(qn), _address(kn), _address(rd), pos)
     _lib.check(_call("tg_norm_rope_" + suffix)(a, sp), "tg_norm_rope")
     return q_out, k_out
 
@@ -398,8 +395,8 @@ def norm_rope(q: torch.Tensor, k: Optional[torch.Tensor] = None, q_norm: Optiona
     may be None.  dim is 256 at most.  q_out and k_out may be q and k.
 
     Differentiable with respect to q, k and the norms' weights (once), unless an out is given."""
-    tracked = [t for t in (q, k, q_norm and q_norm.weight, k_norm and k_norm.weight) if t is not None and t.requires_grad]
-    if not tracked or q_out is not None or k_out is not None or not torch.is_grad_enabled():
+    if q_out is not None or k_out is not None or not torch.is_grad_enabled() or not any(
+            t is not None and t.requires_grad for t in (q, k, q_norm and q_norm.weight, k_norm and k_norm.weight)):
         return _norm_call(q, k, q_norm, k_norm, rope, positions, q_out, k_out, stream)
     if stream is not None:
         _stream(q.get_device(), stream)  # it is on q's device
@@ -418,37 +415,41 @@ def norm_rope_backward(dq_out: torch.Tensor, dk_out: Optional[torch.Tensor], q: 
     dq_out and dk_out of its outputs; None where there is no such tensor.  The weights' gradients have
     the weights' type; their sums are 32-bit and in a fixed order.  dq may be dq_out or q, dk likewise.
     ``workspace``: norm_rope_backward_workspace_bytes, allocated on the call's stream where not given."""
-    held: list = []
-    a = _norm_args(_lib.TgNormRopeGradArgs(), held, q, k, q_norm, k_norm, rope, positions)
-    suffix, index, _, qs, ks = _norm_shape(q, k)
+    inputs = _norm_inputs(q, k, q_norm, k_norm, rope, positions)
     if (k is None) != (dk_out is None) or (k is None and dk is not None):
         raise ValueError("k and the gradients of k go together")
-    # the gradient of a sum is one number, expanded
-    dq_out, dk_out = (t.contiguous() if t is not None and t.dim() == 3 and t.shape[2] > 1 and t.stride(2) != 1 else t
-                      for t in (dq_out, dk_out))
-    a.dq_out = _rows(dq_out, "dq_out", qs, q.dtype, index)
-    if k is not None:
-        a.dk_out = _rows(dk_out, "dk_out", ks, q.dtype, index)
-    sp = _stream(index, stream)
-    where = _elsewhere(index, stream)
+    sp = _stream(inputs[1], stream)
+    where = _elsewhere(inputs[1], stream)
     if where is not None:
         with where:
-            return _norm_grad_launch(a, suffix, q, k, q_norm, k_norm, dq, dk, qs, ks, workspace, index, sp)
-    return _norm_grad_launch(a, suffix, q, k, q_norm, k_norm, dq, dk, qs, ks, workspace, index, sp)
+            return _norm_grad_launch(inputs, dq_out, dk_out, q, k, q_norm, k_norm, dq, dk, workspace, sp)
+    return _norm_grad_launch(inputs, dq_out, dk_out, q, k, q_norm, k_norm, dq, dk, workspace, sp)
 
 
-def _norm_grad_launch(a, suffix, q, k, q_norm, k_norm, dq, dk, qs, ks, workspace, index, sp):
+def _packed(t: torch.Tensor) -> torch.Tensor:
+    """The gradient of a sum is one number, expanded."""
+    return t.contiguous() if t.dim() == 3 and t.stride(2) != 1 and t.shape[2] > 1 else t
+
+
+def _norm_grad_launch(inputs, dq_out, dk_out, q, k, q_norm, k_norm, dq, dk, workspace, sp):
+    suffix, index, qr, kr, ks, held, pos = inputs
+    qs, dt, gk, ko = q.shape, q.dtype, _NO_ROWS, _NO_ROWS
+    dq_out = _packed(dq_out)
+    gq = _rows(dq_out, "dq_out", qs, dt, index)
     if dq is None:
         dq = _like(q)
-    a.dq = _rows(dq, "dq", qs, q.dtype, index)
+    qo = _rows(dq, "dq", qs, dt, index)
     if k is not None:
+        dk_out = _packed(dk_out)
+        gk = _rows(dk_out, "dk_out", ks, dt, index)
         if dk is None:
             dk = _like(k)
-        a.dk = _rows(dk, "dk", ks, q.dtype, index)
+        ko = _rows(dk, "dk", ks, dt, index)
     dqw = torch.empty_like(q_norm.weight) if q_norm is not None and q_norm.weight is not None else None
     dkw = torch.empty_like(k_norm.weight) if k_norm is not None and k_norm.weight is not None else None
-    a.dq_weight = None if dqw is None else dqw.data_ptr()
-    a.dk_weight = None if dkw is None else dkw.data_ptr()
+    qn, kn, rd = held
+    a = _lib.TgNormRopeGradArgs(qs[0], qs[2], qs[1], ks[1] if ks else 0, qr, kr, gq, gk, qo, ko, _address(qn), _address(kn),
+                                None if dqw is None else dqw.data_ptr(), None if dkw is None else dkw.data_ptr(), _address(rd), pos)
     need = _call("tg_norm_rope_backward_workspace_bytes")(a)
     ws = size = 0
     if workspace is None and need:
