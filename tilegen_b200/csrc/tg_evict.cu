@@ -600,7 +600,7 @@ int evict(const tg_kv_evict_args* a, int elem, void* ws, size_t ws_bytes, tg_str
         if (rc != TG_OK) return rc;
     }
     if (ws_bytes < plan.bytes || (plan.bytes && !ws))
-        return set_error(TG_EINVAL, "%s: workspace of %zu bytes needed (got %zu)", op, plan.bytes, ws_bytes);
+        return set_error(TG_ENOMEM, "%s: workspace of %zu bytes needed (got %zu)", op, plan.bytes, ws_bytes);
     if (reinterpret_cast<uintptr_t>(ws) % 16) return set_error(TG_EINVAL, "%s: the workspace must be 16-byte aligned", op);
     p.counts = static_cast<int4*>(ws);
     p.holes = reinterpret_cast<int*>(static_cast<char*>(ws) + plan.counts_bytes);

@@ -844,7 +844,7 @@ int attention_mass(const tg_attention_mass_args* a, void* ws, size_t ws_bytes, t
     if (at % 16 || strides % 8)
         return set_error(TG_EINVAL, "%s: rows must be 16-byte aligned (strides multiples of 8 elements)", op);
     const size_t need = mass_bytes(p);
-    if (ws_bytes < need || (need && !ws)) return set_error(TG_EINVAL, "%s: workspace of %zu bytes needed (got %zu)", op, need, ws_bytes);
+    if (ws_bytes < need || (need && !ws)) return set_error(TG_ENOMEM, "%s: workspace of %zu bytes needed (got %zu)", op, need, ws_bytes);
     if (reinterpret_cast<uintptr_t>(ws) % 16) return set_error(TG_EINVAL, "%s: the workspace must be 16-byte aligned", op);
     p.part = static_cast<float*>(ws);
     constexpr bool kIsHalf = std::is_same<T, __half>::value;

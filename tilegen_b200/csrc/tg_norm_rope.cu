@@ -877,8 +877,8 @@ int backward(const tg_norm_rope_grad_args* a, void* workspace, size_t workspace_
     if (a->tokens > 0 && a->q_heads + a->k_heads > 0) {
         const size_t need = gradient_bytes(a);
         if (!workspace || workspace_bytes < need)
-            return set_error(TG_EINVAL, "%s: workspace of %zu bytes needed (got %zu)", op, need, workspace_bytes);
-        if (reinterpret_cast<uintptr_t>(workspace) % 4) return set_error(TG_EINVAL, "%s: the workspace must be 4-byte aligned", op);
+            return set_error(TG_ENOMEM, "%s: workspace of %zu bytes needed (got %zu)", op, need, workspace_bytes);
+        if (reinterpret_cast<uintptr_t>(workspace) % 16) return set_error(TG_EINVAL, "%s: the workspace must be 16-byte aligned", op);
         p.part = static_cast<float*>(workspace);
         rc = run<T, kGradient>(p, a->rope ? a->rope->layout : TG_ROPE_HALF, ctas, st, op);
         if (rc != TG_OK) return rc;
