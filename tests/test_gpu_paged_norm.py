@@ -99,7 +99,7 @@ def check_gradient(dx, dw, dy, x, norm, r, pos):
 SHAPES = [  # tokens, heads, key heads, dim, rotating
     (1, 1, 1, 2, 2), (1, 32, 8, 128, 128), (5, 3, 1, 80, 40), (7, 5, 5, 96, 48), (33, 2, 1, 20, 12), (130, 8, 2, 64, 64),
     (3, 1, 1, 36, 0), (1201, 4, 1, 128, 32), (9, 40, 8, 256, 256), (64, 1, 1, 7, 4), (2000, 1, 0, 64, 64), (301, 0, 3, 72, 72),
-    (517, 6, 2, 250, 124), (40, 3, 3, 1, 0), (2500, 16, 4, 128, 128),
+    (517, 6, 2, 250, 124), (40, 3, 3, 1, 0), (300, 3, 1, 32, 32), (2500, 16, 4, 128, 128),
 ]
 
 

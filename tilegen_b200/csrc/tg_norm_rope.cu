@@ -683,15 +683,26 @@ Shape<T> shape_of(uint64_t all, int dim, int rot, bool half) {
     return s;
 }
 
+template <typename T>
+struct NormKernel {
+    void (*run)(NormParams<T>);
+    SmemOnce* once;
+};
+template <typename T, int VEC, bool HALF, int MODE, int LANES>
+NormKernel<T> norm_kernel_of() {
+    static SmemOnce once;
+    return {norm_rope_kernel<T, VEC, HALF, MODE, LANES>, &once};
+}
+// The kernel for packs of vec elements and, where every lane has an item that turns, rows of `lanes`.
 template <typename T, int WIDE, bool HALF, int MODE>
-auto norm_kernel(int vec, int lanes) {
-    if (vec == WIDE / 2) return norm_rope_kernel<T, WIDE / 2, HALF, MODE, 0>;
-    if (vec == 1) return norm_rope_kernel<T, 1, HALF, MODE, 0>;
+NormKernel<T> norm_kernel(int vec, int lanes) {
+    if (vec == WIDE / 2) return norm_kernel_of<T, WIDE / 2, HALF, MODE, 0>();
+    if (vec == 1) return norm_kernel_of<T, 1, HALF, MODE, 0>();
     constexpr int kOne = 64 / (2 * WIDE);  // lanes of heads of 64
-    return lanes == kOne       ? norm_rope_kernel<T, WIDE, HALF, MODE, kOne>
-           : lanes == 2 * kOne ? norm_rope_kernel<T, WIDE, HALF, MODE, 2 * kOne>
-           : lanes == 4 * kOne ? norm_rope_kernel<T, WIDE, HALF, MODE, 4 * kOne>
-                               : norm_rope_kernel<T, WIDE, HALF, MODE, 0>;
+    return lanes == kOne       ? norm_kernel_of<T, WIDE, HALF, MODE, kOne>()
+           : lanes == 2 * kOne ? norm_kernel_of<T, WIDE, HALF, MODE, 2 * kOne>()
+           : lanes == 4 * kOne ? norm_kernel_of<T, WIDE, HALF, MODE, 4 * kOne>()
+                               : norm_kernel_of<T, WIDE, HALF, MODE, 0>();
 }
 
 // Fits p to the rows and launches it.
@@ -739,12 +750,10 @@ int run(NormParams<T>& p, int layout, int& ctas, cudaStream_t st, const char* wh
     const bool full = s.vec == WIDE && p.rot == p.dim && s.chunks == s.lanes && p.dim == s.lanes * 2 * WIDE;
     auto kernel = half ? norm_kernel<T, WIDE, true, MODE>(s.vec, full ? s.lanes : 0) : norm_kernel<T, WIDE, false, MODE>(s.vec, full ? s.lanes : 0);
     if (smem > 40 * 1024) {  // (with what is declared, past 48 KB)
-        static SmemOnce once[2][6];
-        const int which = s.vec == WIDE ? (full ? 2 + (s.lanes >= 32 ? 3 : s.lanes / (64 / (2 * WIDE)) == 1 ? 0 : s.lanes / (64 / (2 * WIDE)) == 2 ? 1 : 2) : 0) : 1;
-        const int rc = once[half][which].raise(reinterpret_cast<const void*>(kernel), kNormSmem);
+        const int rc = kernel.once->raise(reinterpret_cast<const void*>(kernel.run), kNormSmem);
         if (rc != TG_OK) return rc;
     }
-    kernel<<<(unsigned)ctas, kRopeThreads, smem, st>>>(p);
+    kernel.run<<<(unsigned)ctas, kRopeThreads, smem, st>>>(p);
     return check_launch(what);
 }
 

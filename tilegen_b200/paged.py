@@ -650,7 +650,10 @@ def _mass_desc(mass: torch.Tensor, name: str, cache: PagedKV, index: int) -> _li
     if mass.shape != shape or mass.dtype is not torch.float32 or mass.get_device() != index:
         raise ValueError("%s must be a float32 tensor of shape %s on cuda:%d (got %s %s on %s)"
                          % (name, tuple(shape), index, mass.dtype, tuple(mass.shape), mass.device))
-    return _lib.TgPagedMass(mass.data_ptr(), *mass.stride())
+    strides = mass.stride()
+    if 0 in strides and any(st == 0 and n > 1 for st, n in zip(strides, shape)):
+        raise ValueError("%s must have a place of its own for every key (got strides %s)" % (name, strides))
+    return _lib.TgPagedMass(mass.data_ptr(), *strides)
 
 
 def empty_mass(cache: PagedKV) -> torch.Tensor:
