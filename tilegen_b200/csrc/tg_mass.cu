@@ -14,12 +14,15 @@
 //   warp 17        issues the matrix instructions
 //   warp 18        fetches queries by TMA (a box of tokens times heads), and for each row its lse and how
 //                  many keys it sees
-//   warp 19        looks up the pages of the next unit's keys
+//   warp 19        looks up the pages of the next unit's keys (and adds up the warpgroups' sums of a unit
+//                  with many rows)
 //
 // * Up to 256 rows of a key head (decoding; the last tokens of a prompt): bound by the keys' bytes.  The
 //   rows stay in shared memory, the keys pass through a ring (stream_kernel).
 // * More rows: bound by the exponentials, 16 a cycle and SM.  A chunk of 512 keys stays, the rows pass
-//   through a ring (rows_kernel), and a thread's sums stay in registers until all rows have passed.
+//   through a ring (rows_kernel), and a thread's sums stay in registers until all rows have passed.  The
+//   steps go round the warpgroups, so that under the causal mask, where rows see one to four of the
+//   chunk's tiles, none is idle.
 //
 // CTAs are persistent; a unit of work is (chunk of keys, part of the row tiles) of a (sequence, key
 // head).  Each CTA counts the units of all sequences at its begin and takes every gridDim.x-th, so that
@@ -40,7 +43,8 @@ constexpr int kThreads = kGroups * 128 + 128;
 constexpr int kKeysWarp = kGroups * 4, kMmaWarp = kKeysWarp + 1, kRowsWarp = kKeysWarp + 2, kPagesWarp = kKeysWarp + 3;
 constexpr uint32_t kCols = 512;
 constexpr int kStagesMax = 8;
-constexpr int kChunkMax = 8;  // most tiles of a chunk of keys
+constexpr int kChunkMax = 8;   // most tiles of a chunk of keys that passes
+constexpr int kRowsChunk = 4;  // and of one that stays
 constexpr int kSeqs = 512;    // sequences of a launch
 
 struct MassParams : AttnParams {
@@ -59,14 +63,14 @@ struct MassParams : AttnParams {
 };
 
 struct MassShared {
-    uint64_t q_full[4], q_empty[4], i_full[2], i_empty[2], p_full[2], p_empty[2], full[kStagesMax], empty[kStagesMax], s_full[4],
+    uint64_t q_full[4], q_empty[4], i_full[2], i_empty[2], p_full[2], p_empty[2], a_full, a_empty, full[kStagesMax], empty[kStagesMax], s_full[4],
         s_empty[4], drained;
     uint32_t tmem;
     int fail;
     int fewest[2], rows[2];                            // keys that every row of the tile sees; rows
     __align__(16) float lse2[2][kMostRows];            // -lse * log2 e
     __align__(16) int seen[2][kMostRows];              // keys that a row sees, 0 for what is no row
-    float acc[2][kTile];                               // sums on their way from one warpgroup to another
+    float acc[kGroups][kRowsChunk * kTile];            // rows_kernel: the sums of each warpgroup at a unit's end
     int page[2][kChunkMax * kTile];                    // pages of a unit's boxes, -1: not in the cache
     int64_t page0[kSeqs];
     int first[kSeqs], n[kSeqs], len[kSeqs];
@@ -261,7 +265,7 @@ struct Cta {
 };
 
 template <int DIM>
-__device__ __forceinline__ Cta enter(const MassParams& p, unsigned char* smem, int warp, int lane) {
+__device__ __forceinline__ Cta enter(const MassParams& p, unsigned char* smem, int page_readers, int warp, int lane) {
     MassShared& sh = *reinterpret_cast<MassShared*>(smem + kTiles);
     Cta c{sh};
     c.q_half = p.tile_rows * 128, c.q_block = c.q_half * (DIM / 64);
@@ -281,7 +285,7 @@ __device__ __forceinline__ Cta enter(const MassParams& p, unsigned char* smem, i
                 mbar_init(&sh.i_full[i], 1);
                 mbar_init(&sh.i_empty[i], kGroups * 4);
                 mbar_init(&sh.p_full[i], 1);
-                mbar_init(&sh.p_empty[i], kGroups * 4 + 1);
+                mbar_init(&sh.p_empty[i], page_readers);
             }
             for (int i = 0; i < 4; ++i) {
                 mbar_init(&sh.q_full[i], 1);
@@ -289,6 +293,8 @@ __device__ __forceinline__ Cta enter(const MassParams& p, unsigned char* smem, i
                 mbar_init(&sh.s_full[i], 1);
                 mbar_init(&sh.s_empty[i], 4);
             }
+            mbar_init(&sh.a_full, kGroups * 4);
+            mbar_init(&sh.a_empty, 1);
             mbar_init(&sh.drained, 1);
             sh.fail = 0;
             fence_mbar_init();
@@ -323,24 +329,19 @@ __device__ __forceinline__ void product(const Cta& c, uint32_t k, uint32_t q, in
     commit(c.b_sf + buf * 8);
 }
 
-// Warp 11: the pages of each unit's boxes.
-__device__ __forceinline__ void find_pages(const MassParams& p, const Cta& c, int lane) {
-    Units units;
-    Unit u;
-    bool ok = true;
-    while (ok && units.next(p, c.sh, u)) {
-        const int buf = units.turn & 1;
-        ok = units.turn < 2 || wait_warp(c.b_pe + buf * 8, (units.turn / 2 - 1) & 1, c.fail);
-        if (!ok) break;
-        const int64_t* list = p.indices + u.s.page0;
-        for (int i = lane; i << p.box_shift < u.keys; i += 32) {
-            int page, slot;
-            locate(p, list, u.k0 + (i << p.box_shift), page, slot);
-            c.sh.page[buf][i] = page;
-        }
-        __syncwarp();
-        if (lane == 0) arrive(c.b_pf + buf * 8);
+// Warp 19: the pages of a unit's boxes.
+__device__ __forceinline__ bool find_pages(const MassParams& p, const Cta& c, const Unit& u, int turn, int lane) {
+    const int buf = turn & 1;
+    if (turn >= 2 && !wait_warp(c.b_pe + buf * 8, (turn / 2 - 1) & 1, c.fail)) return false;
+    const int64_t* list = p.indices + u.s.page0;
+    for (int i = lane; i << p.box_shift < u.keys; i += 32) {
+        int page, slot;
+        locate(p, list, u.k0 + (i << p.box_shift), page, slot);
+        c.sh.page[buf][i] = page;
     }
+    __syncwarp();
+    if (lane == 0) arrive(c.b_pf + buf * 8);
+    return true;
 }
 
 // A tile of keys from the unit's key `at` on into shared memory.  A box past the end is not fetched; a page
@@ -411,6 +412,7 @@ __device__ __forceinline__ void drain_rows(const MassParams& p, const Cta& c, in
 __device__ __forceinline__ float sum_rows(const MassParams& p, const Cta& c, uint32_t t, int ib, int row0, int cols, int key, bool all) {
     const float* lse2 = &c.sh.lse2[ib][row0];
     const int* seen = &c.sh.seen[ib][row0];
+    const int lane = threadIdx.x & 31;
     float sum = 0.f;
     if (p.tile_rows <= 16) {
         uint32_t s[16];
@@ -424,8 +426,9 @@ __device__ __forceinline__ float sum_rows(const MassParams& p, const Cta& c, uin
         uint32_t s[32];
         tmem_ld32(t + x, s);
         wait_ld();
-        sum += all && x + 32 <= cols ? weigh<32, true>(s, lse2 + x, seen + x, key, p.scale_log2)
-                                     : weigh<32, false>(s, lse2 + x, seen + x, key, p.scale_log2);
+        if (all && x + 32 <= cols) sum += weigh<32, true>(s, lse2 + x, seen + x, key, p.scale_log2);
+        else if (__reduce_max_sync(kFull, seen[x + lane]) > key - lane)  // one of the 32 rows sees one of the warp's keys
+            sum += weigh<32, false>(s, lse2 + x, seen + x, key, p.scale_log2);
     }
     return sum;
 }
@@ -438,7 +441,7 @@ __global__ void __launch_bounds__(kThreads, 1) stream_kernel(const __grid_consta
     constexpr int kBlock = kTile * DIM * 2;
     extern __shared__ __align__(1024) unsigned char smem[];
     const int tid = threadIdx.x, warp = __shfl_sync(kFull, tid >> 5, 0), lane = tid & 31;
-    const Cta c = enter<DIM>(p, smem, warp, lane);
+    const Cta c = enter<DIM>(p, smem, kGroups * 4 + 1, warp, lane);
     const int halves = p.tile_rows > kHalfRows ? 2 : 1;
     Units units;
     Unit u;
@@ -497,7 +500,7 @@ __global__ void __launch_bounds__(kThreads, 1) stream_kernel(const __grid_consta
         }
         drain_rows(p, c, nq);
     } else if (warp == kPagesWarp) {
-        find_pages(p, c, lane);
+        while (ok && units.next(p, c.sh, u)) ok = find_pages(p, c, u, units.turn, lane);
     } else {
         const int my = warp >> 2, key_of = tid & (kTile - 1);
         const uint32_t ts = c.tmem + my * kHalfRows + ((uint32_t)(warp & 3) << 21);
@@ -558,12 +561,10 @@ __global__ void __launch_bounds__(kThreads, 1) rows_kernel(const __grid_constant
                                                            const __grid_constant__ CUtensorMap kmap,
                                                            const __grid_constant__ CUtensorMap qmap) {
     constexpr int kBlock = kTile * DIM * 2;
-    // Warpgroups have a tile of keys each; of heads of 256, where two tiles fill the memory, two
-    // warpgroups share one and take turns with the row tiles.
-    constexpr int kChunk = DIM > 128 ? 2 : 4, kShare = kGroups / kChunk;
+    constexpr int kChunk = DIM > 128 ? kRowsChunk / 2 : kRowsChunk;
     extern __shared__ __align__(1024) unsigned char smem[];
     const int tid = threadIdx.x, warp = __shfl_sync(kFull, tid >> 5, 0), lane = tid & 31;
-    const Cta c = enter<DIM>(p, smem, warp, lane);
+    const Cta c = enter<DIM>(p, smem, 2, warp, lane);
     Units units;
     Unit u;
     bool ok = true;
@@ -573,19 +574,19 @@ __global__ void __launch_bounds__(kThreads, 1) rows_kernel(const __grid_constant
         uint32_t used = 0;      // parity of the tiles of keys, by bit
         uint32_t began = 0, emptied = 0;  // buffers that were written, and the parity of their emptying
         while (ok && units.next(p, c.sh, u)) {
-            int here = 0;  // tiles of keys that have come
+            int here = 0, g = 0;  // tiles of keys that have come; steps of the unit
             for (int qi = u.q0; ok && qi < u.q1; ++qi) {
                 const int steps = steps_of(p, u, qi);
                 if (steps == 0) continue;
                 const int qb = nq % p.q_bufs;
                 ok = wait_warp(c.b_qf + qb * 8, nq / p.q_bufs & 1, c.fail);
-                for (int j = 0; ok && j < steps; ++j) {
+                for (int j = 0; ok && j < steps; ++j, ++g) {
                     if (j >= here) {
                         ok = wait_warp(c.b_full + j * 8, used >> j & 1, c.fail);
                         used ^= 1u << j;
                         here = j + 1;
                     }
-                    const int buf = nq % kShare * kChunk + j;
+                    const int buf = g % kGroups;
                     if (began >> buf & 1) {
                         ok = ok && wait_warp(c.b_se + buf * 8, emptied >> buf & 1, c.fail);
                         emptied ^= 1u << buf;
@@ -637,51 +638,71 @@ __global__ void __launch_bounds__(kThreads, 1) rows_kernel(const __grid_constant
             }
         drain_rows(p, c, nq);
     } else if (warp == kPagesWarp) {
-        find_pages(p, c, lane);
+        // the pages of a unit ahead, and the sums of one that has been made
+        Units made;
+        Unit v;
+        bool more = units.next(p, c.sh, u);
+        ok = !more || find_pages(p, c, u, units.turn, lane);
+        while (ok && made.next(p, c.sh, v)) {
+            more = more && units.next(p, c.sh, u);
+            ok = (!more || find_pages(p, c, u, units.turn, lane)) && wait_warp(smem_addr(&c.sh.a_full), made.turn & 1, c.fail);
+            if (!ok) break;
+            const int pb = made.turn & 1;
+            for (int at = lane; at < v.keys; at += 32) {
+                float sum = 0.f;
+#pragma unroll
+                for (int w = 0; w < kGroups; ++w) sum += c.sh.acc[w][at];
+                if (p.splits > 1) {
+                    p.part[part_at(p, v) + at] = sum;
+                } else {
+                    float* const to = mass_at(p, v, c.sh.page[pb], at);
+                    put(p, v, v.k0 + at, to, to && has_old(p, v, v.k0 + at) ? *to : 0.f, sum);
+                }
+            }
+            __syncwarp();
+            if (lane == 0) {
+                arrive(smem_addr(&c.sh.a_empty));
+                arrive(c.b_pe + pb * 8);
+            }
+        }
     } else {
-        const int my = warp >> 2, key_of = tid & (kTile - 1), j = my % kChunk, at = j * kTile + key_of;
+        const int my = warp >> 2, key_of = tid & (kTile - 1);
         const uint32_t ts = c.tmem + my * kHalfRows + ((uint32_t)(warp & 3) << 21);
         int nq = 0, made = 0;
         while (units.next(p, c.sh, u)) {
-            const int pb = units.turn & 1, key = u.k0 + at;
-            float acc = 0.f;
+            float acc[kChunk];
+#pragma unroll
+            for (int m = 0; m < kChunk; ++m) acc[m] = 0.f;
+            int g = 0;  // steps of the unit
             for (int qi = u.q0; ok && qi < u.q1; ++qi) {
                 const int steps = steps_of(p, u, qi);
                 if (steps == 0) continue;
                 const int ib = nq & 1;
                 ok = wait_warp(c.b_if + ib * 8, nq / 2 & 1, c.fail);
-                if (ok && j < steps && nq % kShare == my / kChunk) {
-                    const int rows = c.sh.rows[ib], fewest = c.sh.fewest[ib];
+                const int rows = c.sh.rows[ib], fewest = c.sh.fewest[ib];
+                for (int j = (my - g % kGroups + kGroups) % kGroups; ok && j < steps; j += kGroups) {
                     ok = wait_warp(c.b_sf + my * 8, made & 1, c.fail);
                     fence_after();
+                    const int at = j * kTile + key_of;
                     const bool all = u.k0 + min((j + 1) * kTile, u.keys) <= fewest;  // every row sees every key
-                    if (ok) acc += sum_rows(p, c, ts, ib, 0, rows, key, all);
+                    const float sum = ok ? sum_rows(p, c, ts, ib, 0, rows, u.k0 + at, all) : 0.f;
                     fence_before();
                     __syncwarp();
                     if (lane == 0) arrive(c.b_se + my * 8);
                     ++made;
+#pragma unroll
+                    for (int m = 0; m < kChunk; ++m) acc[m] += m == j ? sum : 0.f;
                 }
                 __syncwarp();
                 if (lane == 0) arrive(c.b_ie + ib * 8);
                 ++nq;
+                g += steps;
             }
-            ok = ok && wait_warp(c.b_pf + pb * 8, units.turn / 2 & 1, c.fail);
-            if (!ok) acc = NAN;  // loud: a wait that ran out leaves no number
-            if constexpr (kShare > 1) {
-                if (my >= kChunk) c.sh.acc[j][key_of] = acc;
-                asm volatile("bar.sync %0, 256;" ::"r"(1 + j) : "memory");
-                if (my < kChunk) acc += c.sh.acc[j][key_of];
-                asm volatile("bar.sync %0, 256;" ::"r"(1 + j) : "memory");
-            }
-            if (my >= kChunk) {
-            } else if (p.splits > 1) {
-                if (at < u.keys) p.part[part_at(p, u) + at] = acc;
-            } else if (ok) {
-                float* const to = mass_at(p, u, c.sh.page[pb], at);
-                put(p, u, key, to, to && has_old(p, u, key) ? *to : 0.f, acc);
-            }
+            ok = ok && (units.turn == 0 || wait_warp(smem_addr(&c.sh.a_empty), (units.turn - 1) & 1, c.fail));
+#pragma unroll
+            for (int m = 0; m < kChunk; ++m) c.sh.acc[my][m * kTile + key_of] = ok ? acc[m] : NAN;  // loud: a wait that ran out leaves no number
             __syncwarp();
-            if (lane == 0) arrive(c.b_pe + pb * 8);
+            if (lane == 0) arrive(smem_addr(&c.sh.a_full));
         }
     }
     leave(c, warp);
@@ -784,7 +805,7 @@ int make_plan(const tg_attention_mass_args* a, MassParams* out, const char* op) 
         p.q_bufs = 2 * q_block + 4 * k_block <= kTiles ? 2 : 1;
         p.stages = std::min(kStagesMax, (kTiles - p.q_bufs * q_block) / k_block);
     } else {
-        p.chunk = dim > 128 ? 2 : kGroups;
+        p.chunk = dim > 128 ? kRowsChunk / 2 : kRowsChunk;
         p.q_bufs = std::min(4, (kTiles - p.chunk * k_block) / q_block);
     }
     p.chunks = (int)ceil_div(k_tiles, p.chunk);
