@@ -54,6 +54,7 @@ struct MassParams : AttnParams {
     float decay;
     // rows: tiles of tile_tokens tokens and tile_heads query heads, head_tiles of them side by side
     int tile_tokens, tile_heads, head_tiles, tile_rows;  // tile_rows: columns of the instructions, a multiple of 16
+    int per_head;                                        // 2^16 / tile_heads, rounded up: divides numbers below 256
     int stream;                                          // stream_kernel: one row tile
     int chunk, chunks, splits, split_tiles;              // tiles of keys of a chunk; row tiles of a part
     int box, box_shift;                                  // keys of a box, their log2
@@ -366,11 +367,28 @@ __device__ __forceinline__ void fetch_keys(const MassParams& p, const Cta& c, co
     }
 }
 
-// Warp 10: row tile qi of the unit into buffer qb, and of its rows what the exponentials take.
+// Warp 18: row tile qi of the unit into its buffer, and of its rows what the exponentials take.  What is
+// read for them is under way while the buffers are waited for: the steps of a tile take less than that.
 template <int DIM>
 __device__ __forceinline__ bool fetch_rows(const MassParams& p, const Cta& c, const Unit& u, int qi, int nq, const CUtensorMap* map, int lane) {
+    constexpr int kEach = kMostRows / 32;
     const int qb = nq % p.q_bufs, ib = nq & 1;
-    const int t0 = qi / p.head_tiles * p.tile_tokens, h0 = qi % p.head_tiles * p.tile_heads;
+    const int tile = p.head_tiles == 1 ? qi : qi / p.head_tiles, t0 = tile * p.tile_tokens, h0 = (qi - tile * p.head_tiles) * p.tile_heads;
+    const int rows = min(p.tile_tokens, u.s.asked - t0) * p.tile_heads;
+    const float* lse = p.row_lse + (int64_t)(u.s.first + t0) * p.q_heads + u.h * p.group + h0;
+    float l[kEach];
+    int seen[kEach];
+#pragma unroll
+    for (int k = 0; k < kEach; ++k) {
+        const int r = lane + k * 32, i = r * p.per_head >> 16, x = r - i * p.tile_heads;  // token and head of the tile
+        const bool there = r < rows && h0 + x < p.group;
+        l[k] = 0.f;
+        seen[k] = 0;
+        if (there) {
+            l[k] = __ldg(lse + (int64_t)i * p.q_heads + x);
+            seen[k] = keys_seen(p, u.s, t0 + i, u.s.len, u.s.len);
+        }
+    }
     if (nq >= p.q_bufs && !wait_warp(c.b_qe + qb * 8, (nq / p.q_bufs - 1) & 1, c.fail)) return false;
     if (lane == 0) mbar_arrive_expect_tx(&c.sh.q_full[qb], p.tile_tokens * p.tile_heads * DIM * 2);
     __syncwarp();
@@ -378,19 +396,16 @@ __device__ __forceinline__ bool fetch_rows(const MassParams& p, const Cta& c, co
     for (int half = 0; half < DIM / 64; ++half)
         load_box3(c.sq + qb * c.q_block + half * c.q_half, map, half * 64, u.h * p.group + h0, u.s.first + t0, c.b_qf + qb * 8);
     if (nq >= 2 && !wait_warp(c.b_ie + ib * 8, (nq / 2 - 1) & 1, c.fail)) return false;
-    const int rows = min(p.tile_tokens, u.s.asked - t0) * p.tile_heads;
     int fewest = INT_MAX;
-    for (int r = lane; r < ((rows + 31) & ~31); r += 32) {
-        const int i = t0 + r / p.tile_heads, x = h0 + r % p.tile_heads;
-        int seen = 0;
-        float l = 0.f;
-        if (r < rows && x < p.group) {
-            l = __ldg(p.row_lse + (int64_t)(u.s.first + i) * p.q_heads + u.h * p.group + x) * -1.4426950408889634f;
-            if (l != INFINITY) seen = keys_seen(p, u.s, i, u.s.len, u.s.len);
-        }
-        c.sh.lse2[ib][r] = l;
-        c.sh.seen[ib][r] = seen;
-        if (r < rows) fewest = min(fewest, seen);
+#pragma unroll
+    for (int k = 0; k < kEach; ++k) {
+        const int r = lane + k * 32;
+        if (k * 32 >= rows) break;
+        l[k] *= -1.4426950408889634f;
+        if (l[k] == INFINITY) seen[k] = 0;
+        c.sh.lse2[ib][r] = l[k];
+        c.sh.seen[ib][r] = seen[k];
+        if (r < rows) fewest = min(fewest, seen[k]);
     }
     fewest = __reduce_min_sync(kFull, fewest);
     if (lane == 0) {
@@ -796,6 +811,7 @@ int make_plan(const tg_attention_mass_args* a, MassParams* out, const char* op) 
     p.head_tiles = (p.group + p.tile_heads - 1) / p.tile_heads;
     p.tile_tokens = (int)std::max<int64_t>(1, std::min<int64_t>(max_q, rows / p.tile_heads));
     p.tile_rows = (p.tile_tokens * p.tile_heads + 15) / 16 * 16;
+    p.per_head = (65536 + p.tile_heads - 1) / p.tile_heads;
     const int64_t q_tiles = std::max<int64_t>(1, ceil_div(max_q, p.tile_tokens)) * p.head_tiles, k_tiles = std::max<int64_t>(1, ceil_div(max_seq, kTile));
     const int q_block = p.tile_rows * dim * 2, k_block = kTile * dim * 2;
     const int64_t pairs = std::max<int64_t>(1, t.rows * c.heads);
