@@ -92,14 +92,17 @@ __device__ __forceinline__ int row_tiles(const MassParams& p, const Sequence& s)
 }
 // Tiles of the unit's keys that a row of row tile qi may see.
 __device__ __forceinline__ int steps_of(const MassParams& p, const Unit& u, int qi) {
-    const int last = min((qi / p.head_tiles + 1) * p.tile_tokens, u.s.asked) - 1;
-    const int seen = min(keys_seen(p, u.s, last, u.s.len, u.s.len) - u.k0, u.keys);
-    return seen > 0 ? (seen + kTile - 1) / kTile : 0;
+    if (!p.causal) return u.tiles;
+    const int last = min(((p.head_tiles == 1 ? qi : qi / p.head_tiles) + 1) * p.tile_tokens, u.s.asked) - 1;
+    const int64_t seen = (int64_t)u.s.len - u.s.n + last + 1 - u.k0;
+    return seen <= 0 ? 0 : ((int)min(seen, (int64_t)u.keys) + kTile - 1) / kTile;
 }
-// With several parts of the row tiles: those that see keys from k0 on are part `first` to the last, none
-// where first is `all`.  (Parts have whole tokens: head_tiles is 1.)
-__device__ __forceinline__ int first_split(const MassParams& p, const Sequence& s, int k0, int& all) {
-    all = (row_tiles(p, s) + p.split_tiles - 1) / p.split_tiles;
+// Parts of a sequence's row tiles, and the first of them that sees keys from k0 on (`all`: none does).
+// (Parts have whole tokens: head_tiles is 1.)
+__device__ __forceinline__ int splits_of(const MassParams& p, const Sequence& s) {
+    return (row_tiles(p, s) + p.split_tiles - 1) / p.split_tiles;
+}
+__device__ __forceinline__ int first_split(const MassParams& p, const Sequence& s, int k0, int all) {
     if (!p.causal) return 0;
     const int64_t behind = (int64_t)k0 - s.len + s.n;  // token i sees them where i >= behind
     if (behind >= s.asked) return all;
@@ -109,12 +112,9 @@ __device__ __forceinline__ int first_split(const MassParams& p, const Sequence& 
 __device__ __forceinline__ int units_of(const MassParams& p, const Sequence& s) {
     const int step = p.chunk * kTile;
     if (p.splits == 1) return s.n == 0 && p.decay == 1.f ? 0 : (s.len + step - 1) / step;  // (the old weights stay)
+    const int all = splits_of(p, s);
     int units = 0;
-    for (int k0 = 0; k0 < s.len; k0 += step) {
-        int all;
-        const int first = first_split(p, s, k0, all);
-        units += all - first;
-    }
+    for (int k0 = 0; k0 < s.len; k0 += step) units += all - first_split(p, s, k0, all);
     return units;
 }
 
@@ -171,8 +171,8 @@ struct Units {
         const int step = p.chunk * kTile;
         u.c = x, u.split = 0;
         if (p.splits > 1) {
+            const int all = splits_of(p, u.s);
             for (u.c = 0;; ++u.c) {
-                int all;
                 const int first = first_split(p, u.s, u.c * step, all);
                 if (x < all - first) {
                     u.split = first + x;
@@ -317,16 +317,49 @@ __device__ __forceinline__ void leave(const Cta& c, int warp) {
     }
 }
 
+// D (+)= A B of STEPS times 16 elements of one 64-column half, both operands in shared memory; `add`: D
+// holds something already.  One election and one pair of descriptors for all of them: the issuing warp
+// would otherwise take longer than the products (1070 cycles a step against 600).
+template <int STEPS>
+__device__ __forceinline__ void mma_half(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t add) {
+    static_assert(STEPS == 2 || STEPS == 4, "steps of a half");
+    if constexpr (STEPS == 4) {
+        asm volatile(
+            "{\n\t.reg .pred p, e, t;\n\t.reg .b64 a1, a2, a3, b1, b2, b3;\n\t"
+            "elect.sync _|e, 0xffffffff;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.eq.b32 t, 0, 0;\n\t"
+            "add.s64 a1, %1, 2;\n\tadd.s64 a2, %1, 4;\n\tadd.s64 a3, %1, 6;\n\t"
+            "add.s64 b1, %2, 2;\n\tadd.s64 b2, %2, 4;\n\tadd.s64 b3, %2, 6;\n\t"
+            "@e tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t"
+            "@e tcgen05.mma.cta_group::1.kind::f16 [%0], a1, b1, %3, t;\n\t"
+            "@e tcgen05.mma.cta_group::1.kind::f16 [%0], a2, b2, %3, t;\n\t"
+            "@e tcgen05.mma.cta_group::1.kind::f16 [%0], a3, b3, %3, t;\n\t}" ::"r"(d),
+            "l"(a), "l"(b), "r"(idesc), "r"(add)
+            : "memory");
+    } else {
+        asm volatile(
+            "{\n\t.reg .pred p, e, t;\n\t.reg .b64 a1, b1;\n\t"
+            "elect.sync _|e, 0xffffffff;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.eq.b32 t, 0, 0;\n\t"
+            "add.s64 a1, %1, 2;\n\tadd.s64 b1, %2, 2;\n\t"
+            "@e tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t"
+            "@e tcgen05.mma.cta_group::1.kind::f16 [%0], a1, b1, %3, t;\n\t}" ::"r"(d),
+            "l"(a), "l"(b), "r"(idesc), "r"(add)
+            : "memory");
+    }
+}
+
 // S^T of a tile of keys and `rows` rows into a buffer, whose barrier completes with it.
 template <typename T, int KSTEPS>
 __device__ __forceinline__ void product(const Cta& c, uint32_t k, uint32_t q, int rows, int buf) {
     constexpr uint32_t kType = std::is_same<T, __half>::value ? 0 : 1;
     constexpr int kHalf = kTile * 128;
     const uint32_t idesc = 1u << 4 | kType << 7 | kType << 10 | (kTile / 16) << 24 | (uint32_t)(rows / 8) << 17;
+    const uint64_t a = operand(k, 16), b = operand(q, 16);
+    const uint32_t d = c.tmem + buf * kHalfRows;
 #pragma unroll
-    for (int kk = 0; kk < KSTEPS; ++kk)
-        mma_ss(c.tmem + buf * kHalfRows, operand(k + (kk >> 2) * kHalf + (kk & 3) * 32, 16),
-               operand(q + (kk >> 2) * c.q_half + (kk & 3) * 32, 16), idesc, kk > 0);
+    for (int half = 0; half < KSTEPS / 4; ++half)
+        mma_half<4>(d, a + half * (kHalf / 16), b + half * (c.q_half / 16), idesc, half > 0);
+    if constexpr (KSTEPS % 4 != 0)
+        mma_half<KSTEPS % 4>(d, a + KSTEPS / 4 * (kHalf / 16), b + KSTEPS / 4 * (c.q_half / 16), idesc, 1);
     commit(c.b_sf + buf * 8);
 }
 
@@ -734,8 +767,7 @@ __global__ void __launch_bounds__(256) mass_join_kernel(const __grid_constant__ 
     u.k0 = u.c * p.chunk * kTile;
     u.keys = min(u.s.len - u.k0, p.chunk * kTile);
     if (u.keys <= 0 || (u.s.n == 0 && p.decay == 1.f)) return;
-    int all;
-    const int first = first_split(p, u.s, u.k0, all);
+    const int all = splits_of(p, u.s), first = first_split(p, u.s, u.k0, all);
     for (int at = threadIdx.x; at < u.keys; at += blockDim.x) {
         int page, slot;
         locate(p, p.indices + u.s.page0, u.k0 + at, page, slot);
