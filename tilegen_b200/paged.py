@@ -217,7 +217,7 @@ def _rows(t: torch.Tensor, name: str, shape: Tuple, dtype: torch.dtype, index: i
 
 
 def _like(t: torch.Tensor) -> torch.Tensor:
-    return torch.empty_like(t) if t.is_contiguous() else torch.empty(t.shape, dtype=t.dtype, device=t.device)
+    return torch.empty_like(t, memory_format=torch.contiguous_format)  # half the time of torch.empty with a shape
 
 
 def _stream(index: int, stream: Optional[torch.cuda.Stream]) -> int:
