@@ -167,10 +167,11 @@ def test_all_weights_alike_and_weights_that_are_no_numbers():
     c.check(400, 2, 30)
 
 
+@pytest.mark.parametrize("levels", [0, 3])
 @pytest.mark.parametrize("lens,budget,recent", [([130000], 20000, 64), ([350000, 9], 300000, 5000), ([70000, 60000], 6000, 3000)])
-def test_long_sequences(lens, budget, recent):
-    """Clusters of CTAs, weights that do not fit in shared memory, long lists."""
-    c = Cache(lens, 1, 8, 64, BF16, seed=5)
+def test_long_sequences(lens, budget, recent, levels):
+    """Clusters of CTAs, weights that do not fit in shared memory, long lists, thousands of equal weights."""
+    c = Cache(lens, 1, 8, 64, BF16, seed=5, levels=levels)
     k, v, mass = (x.clone() for x in c.tensors())
     got_len, kept = P.kv_evict(c.cache, c.table, c.seq_len, c.mass, budget, first=4, recent=recent, kept=True,
                                max_seq_len=max(lens))

@@ -94,6 +94,11 @@ MORE = [
     ([33, 1000], [40, 2100], 100, 6, 2, 64, 48),
     ([1] * 200, [200] * 200, 0, 8, 8, 64, 8),
     ([1, 1, 1], [1, 4000, 129], 0, 4, 2, 128, 6),  # 64 boxes a tile
+    ([1] * 700, list(range(700)), 30, 8, 2, 64, 16),  # more sequences than one launch takes
+    ([90] * 530, [90 + i % 70 for i in range(530)], 0, 4, 1, 64, 32),
+    ([300, 90, 1], [700, 90, 400], 0, 4, 2, 256, 16),  # many rows of heads of 256 and 96, shared out
+    ([600, 0, 31], [900, 300, 31], 50, 8, 2, 96, 24),
+    ([400, 700], [100, 650], 0, 8, 2, 128, 16),    # more queries than keys, many rows
 ]
 CASES = ATTEND + MORE
 
@@ -113,7 +118,7 @@ def test_mass(case, dtype):
     assert torch.equal(first.nan_to_num(-7.0), b.mass.nan_to_num(-7.0))  # the same twice
 
 
-@pytest.mark.parametrize("case", [4, 8, 10, 14, 16, 20, 22, 23])
+@pytest.mark.parametrize("case", [4, 8, 10, 14, 16, 20, 22, 23, 29, 30, 31])
 def test_without_a_mask(case):
     b = Weighed(*CASES[case], BF16, seed=case)
     lse = b.lse(causal=False, scale=0.3)
@@ -241,6 +246,21 @@ def test_offsets_beyond_32_bits():
     b.gather(lse)
     b.mass = far[moved]
     b.check(lse)
+
+
+def test_queries_of_one_number_for_all_tokens():
+    """Strides of zero, as an expanded tensor has them: taken or refused, never misread."""
+    b = Weighed([1, 1], [200, 90], 0, 8, 2, 64, 16, BF16, seed=3)
+    b.q = b.q[:1].expand(2, 8, 64)
+    lse = b.lse()
+    try:
+        b.gather(lse)
+    except lib.TgError as e:
+        assert e.status == lib.TG_ECUDA and torch.equal(b.mass.nan_to_num(-7.0), b.before.nan_to_num(-7.0))
+    else:
+        b.check(lse)
+    with pytest.raises(ValueError):  # one place for all heads
+        P.attention_mass(b.mass[..., :1].expand(b.mass.shape), b.q.contiguous(), b.cache, b.table, b.seq_len, lse)
 
 
 def test_graph_streams_and_workspace():

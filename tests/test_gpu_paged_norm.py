@@ -366,6 +366,43 @@ def test_graph_capture_and_streams():
     assert torch.equal(other[0], out[0])
 
 
+def test_one_row_for_all_tokens():
+    """Inputs with strides of zero, as an expanded tensor has them."""
+    g, q, k, (qn, kn), r, pos = problem((90, 5, 2, 128, 128), BF16, "half")
+    wide = q[:1, :1].expand(90, 5, 128)
+    check_forward(P.norm_rope(wide, k, qn, kn, r, pos)[0], wide.contiguous(), qn, r, pos)
+    one = q[:1, :1].clone().requires_grad_()
+    y, _ = P.norm_rope(one.expand(90, 5, 128), None, qn, None, r, pos)
+    dy = normal(g, 90, 5, 128, dtype=BF16)
+    (gx,) = torch.autograd.grad(y, one, dy)
+    each = P.norm_rope_backward(dy, None, wide, None, qn, None, r, pos)[0]
+    assert torch.equal(gx, each.sum((0, 1), keepdim=True))
+
+
+def test_a_training_step_in_a_captured_graph():
+    """Forward and gradient by autograd, captured with no eager graph of the same leaves alive."""
+    g, q, k, (qn, kn), r, pos = problem((40, 4, 2, 64, 64), BF16, "half")
+    dy, dz = normal(g, *q.shape, dtype=BF16), normal(g, *k.shape, dtype=BF16)
+    want = P.norm_rope_backward(dy, dz, q, k, qn, kn, r, pos)
+    st = torch.cuda.Stream()
+    st.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(st):
+        leaves = [t.clone().requires_grad_() for t in (q, k, qn.weight, kn.weight)]
+        norms = P.HeadNorm(leaves[2], qn.eps, qn.offset), P.HeadNorm(leaves[3], kn.eps, kn.offset)
+
+        def step():
+            return torch.autograd.grad(P.norm_rope(leaves[0], leaves[1], *norms, r, pos), leaves, (dy, dz))
+
+        step()
+    torch.cuda.current_stream().wait_stream(st)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=st):
+        grads = step()
+    graph.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(grads, want))
+
+
 def test_refusals():
     g, q, k, (qn, kn), r, pos = problem((4, 3, 1, 64, 64), BF16, "half")
     dy, dz = torch.empty_like(q), torch.empty_like(k)

@@ -15,10 +15,14 @@
 //   integers lie in shared memory; three rounds of 11, 11 and 10 bits find the value of the
 //   heavy-th largest (histograms of all CTAs, added over the cluster), then ranks in the order of the
 //   places give the holes and the keys that fill them.
+//   Bound: latency.  512 (sequence, head) pairs of 1000 keys 11 us, two sequences of 120000 (clusters of
+//   eight CTAs, 15000 keys each) 50 us: reading 8, histograms 12, their sums over the cluster 12, ranks
+//   and lists 15.
 // * move_kernel: holes are filled from places behind the budget by all CTAs side by side: such places are
 //   not written, so nothing waits.  Sources before the budget lie where recent keys go: these fills
 //   and the recent keys are one list, sorted so that a place is read before it is written, that the
-//   CTAs of one cluster go through together, reading a batch before it writes it.
+//   CTAs of one cluster go through together, reading a batch before it writes it.  Bound: HBM with
+//   rows of 256 bytes from pages in random order: 224 MB in 42 us, 5.3 TB/s.
 #include <cooperative_groups.h>
 
 #include <algorithm>

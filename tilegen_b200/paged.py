@@ -1,5 +1,6 @@
-"""Paged attention on torch tensors: rotary positions, appending to a paged key/value cache,
-and attention of a batch of sequences that share a prefix.
+"""Paged attention on torch tensors: rotary positions, norms of queries and keys with the rotation,
+appending to a paged key/value cache, attention of a batch of sequences that share a prefix, the
+attention weight that cached keys gather, and eviction of those that gathered least.
 
 Which pages hold a sequence's keys and values is a CSR pattern (:class:`PageTable`): row b
 lists the pages of sequence b.  The calls follow :mod:`tilegen_b200.device`: asynchronous on
