@@ -665,18 +665,34 @@ def empty_mass(cache: PagedKV) -> torch.Tensor:
 
 
 def _mass_args(mass, q, cache, table, seq_len, lse, q_indptr, max_q_len, max_seq_len, scale, causal, decay, check):
-    a, held = _attention_args(q, cache, table, seq_len, None, 0, q_indptr, max_q_len, max_seq_len, scale, causal, check)
-    index = cache.k.get_device()
-    if lse is not None and (lse.shape != q.shape[:2] or lse.dtype is not torch.float32 or lse.get_device() != index
+    """(arguments for the library, the descriptors that they point to); the checks of _attention_args."""
+    kv = cache.desc()
+    index, dt = cache.k.get_device(), cache.k.dtype
+    if dt is torch.float32:
+        raise ValueError("attention takes float16 or bfloat16 caches (got %s)" % dt)
+    tb = table.desc(index, kv.pages)
+    if q.dim() != 3:
+        raise ValueError("q must be [tokens, q_heads, dim] (got %s)" % (tuple(q.shape),))
+    tokens, heads, _ = q.shape
+    rows, starts = tb.rows, None
+    if q_indptr is not None:
+        starts = _vector(q_indptr, "q_indptr", index, rows + 1)
+        max_q_len = tokens if max_q_len is None else max_q_len
+    else:
+        if tokens != rows:
+            raise ValueError("%d tokens for %d sequences need a q_indptr" % (tokens, rows))
+        max_q_len = 1
+    if lse is not None and (lse.shape != (tokens, heads) or lse.dtype is not torch.float32 or lse.get_device() != index
                             or not lse.is_contiguous()):
         raise ValueError("lse must be a contiguous float32 tensor of shape %s on cuda:%d (got %s %s on %s)"
-                         % (tuple(q.shape[:2]), index, tuple(lse.shape), lse.dtype, lse.device))
-    m = _lib.TgAttentionMassArgs(a.cache, a.pages, a.seq_len, a.max_seq_len, a.tokens, a.q_indptr, a.max_q_len, a.q_heads, a.q,
-                                 None if lse is None else lse.data_ptr(), a.scale)
-    if mass is not None:
-        m.mass = _mass_desc(mass, "mass", cache, index)
-    m.decay, m.flags = decay, a.flags
-    return m, held
+                         % ((tokens, heads), index, tuple(lse.shape), lse.dtype, lse.device))
+    m = _lib.TgAttentionMassArgs(
+        ctypes.addressof(kv), ctypes.addressof(tb), _vector(seq_len, "seq_len", index, rows),
+        tb.nnz * kv.page_size if max_seq_len is None else max_seq_len, tokens, starts, max_q_len, heads,
+        _rows(q, "q", (tokens, heads, kv.dim), dt, index), None if lse is None else lse.data_ptr(),
+        kv.dim ** -0.5 if scale is None else scale, _lib.TgPagedMass() if mass is None else _mass_desc(mass, "mass", cache, index), decay,
+        (_lib.TG_FLAG_CAUSAL if causal else 0) | (_lib.TG_FLAG_BOUNDS_CHECK if check else 0))
+    return m, (kv, tb)
 
 
 def attention_mass(mass: torch.Tensor, q: torch.Tensor, cache: PagedKV, table: PageTable, seq_len: torch.Tensor,
