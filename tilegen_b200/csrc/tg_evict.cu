@@ -350,15 +350,24 @@ __global__ void __launch_bounds__(THREADS) select_kernel(const __grid_constant__
     int* const fill_list = p.fills + (int64_t)unit * p.width;
     walk([&](int at, const bool (&chosen)[kStep], const float (&m)[kStep]) {
         const uint32_t below = (1u << lane) - 1;
+        // most warps are on one side of the new places' end
+        if (at - lane + 32 * kStep > new_end) {
+#pragma unroll
+            for (int k = 0; k < kStep; ++k) {
+                const bool moves = chosen[k] && at + k * 32 >= new_end;
+                const uint32_t move = __ballot_sync(kFull, moves);
+                if (moves) fill_list[move_at + __popc(move & below)] = at + k * 32;
+                move_at += __popc(move);
+            }
+        }
+        if (at - lane >= new_end) return;
         bool stay[kStep];
 #pragma unroll
         for (int k = 0; k < kStep; ++k) {
-            const bool front = at + k * 32 < new_end, is_hole = front && !chosen[k] && at + k * 32 < place_end, moves = chosen[k] && !front;
-            const uint32_t hole = __ballot_sync(kFull, is_hole), move = __ballot_sync(kFull, moves);
+            const bool front = at + k * 32 < new_end, is_hole = front && !chosen[k] && at + k * 32 < place_end;
+            const uint32_t hole = __ballot_sync(kFull, is_hole);
             if (is_hole) hole_list[hole_at + __popc(hole & below)] = at + k * 32;
-            if (moves) fill_list[move_at + __popc(move & below)] = at + k * 32;
             hole_at += __popc(hole);
-            move_at += __popc(move);
             stay[k] = chosen[k] && front;
         }
         if (!p.moved && !kept) return;
