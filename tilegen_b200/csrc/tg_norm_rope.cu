@@ -114,13 +114,15 @@ __global__ void __launch_bounds__(kRopeThreads, MODE == kGradient ? 2 : 4)
     constexpr bool kApart = HALF || VEC == 1;       // a pair's elements are in different packs
     constexpr int kPairs = kApart ? VEC : VEC / 2;  // of a unit: an item (kApart) or a pack
     using P = Pack<T, VEC>;
-    constexpr bool kRing = VEC * sizeof(T) == 16;
+    constexpr int kPack = VEC * (int)sizeof(T);  // bytes
+    constexpr bool kRing = VEC > 1;
     constexpr int kDepth = kRingDepth, kRowPacks = NI * (MODE == kGradient ? 4 : 2);
     extern __shared__ __align__(16) unsigned char smem_bytes[];  // the ring; turns of [tile][pairs]; at the end the sums of the warps
     constexpr int s_ring = 0;
-    float* const s_turn = reinterpret_cast<float*>(smem_bytes + (kRing ? kDepth * kRowPacks * kRopeThreads * 16 : 0));
-    auto copy16 = [&](int to, const void* from) {
-        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_addr(smem_bytes) + to), "l"(from) : "memory");
+    float* const s_turn = reinterpret_cast<float*>(smem_bytes + (kRing ? kDepth * kRowPacks * kRopeThreads * kPack : 0));
+    auto copy = [&](int to, const void* from) {
+        if constexpr (kPack == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_addr(smem_bytes) + to), "l"(from) : "memory");
+        if constexpr (kPack == 8) asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(smem_addr(smem_bytes) + to), "l"(from) : "memory");
     };
     __shared__ __align__(16) float s_w[2][kNormDim];
     __shared__ double s_pos[kRopeTile];
@@ -365,17 +367,17 @@ __global__ void __launch_bounds__(kRopeThreads, MODE == kGradient ? 2 : 4)
         }
     };
     // Rows under way: in the thread's own places of a ring in shared memory (kRing), or in registers.
-    auto ring_at = [&](int n, int pack) { return s_ring + ((n % kDepth * kRowPacks + pack) * kRopeThreads + tid) * 16; };
+    auto ring_at = [&](int n, int pack) { return s_ring + ((n % kDepth * kRowPacks + pack) * kRopeThreads + tid) * kPack; };
     auto fetch = [&](const Walk& w, int n) {
         if (w.tt < tile) {
             const P *in = reinterpret_cast<const P*>(w.in), *g = reinterpret_cast<const P*>(w.grad);
 #pragma unroll
             for (int i = 0; i < NI; ++i) {
-                if ((kFixed || ia[i] >= 0)) copy16(ring_at(n, 2 * i), in + ia[i]);
-                if ((kFixed || ib[i] >= 0)) copy16(ring_at(n, 2 * i + 1), in + ib[i]);
+                if ((kFixed || ia[i] >= 0)) copy(ring_at(n, 2 * i), in + ia[i]);
+                if ((kFixed || ib[i] >= 0)) copy(ring_at(n, 2 * i + 1), in + ib[i]);
                 if constexpr (MODE == kGradient) {
-                    if ((kFixed || ia[i] >= 0)) copy16(ring_at(n, 2 * NI + 2 * i), g + ia[i]);
-                    if ((kFixed || ib[i] >= 0)) copy16(ring_at(n, 2 * NI + 2 * i + 1), g + ib[i]);
+                    if ((kFixed || ia[i] >= 0)) copy(ring_at(n, 2 * NI + 2 * i), g + ia[i]);
+                    if ((kFixed || ib[i] >= 0)) copy(ring_at(n, 2 * NI + 2 * i + 1), g + ib[i]);
                 }
             }
         }
@@ -747,7 +749,7 @@ int run(NormParams<T>& p, int layout, int& ctas, cudaStream_t st, const char* wh
     size_t smem = (size_t)p.tile * pairs * sizeof(float2);
     if (MODE == kGradient) smem = std::max(smem, (size_t)(kRopeThreads / 32) * p.dim * sizeof(float));
     constexpr int WIDE = 16 / (int)sizeof(T);
-    if (s.vec == WIDE) smem += (size_t)kRingDepth * packs * kRopeThreads * 16;
+    if (s.vec > 1) smem += (size_t)kRingDepth * packs * kRopeThreads * s.vec * sizeof(T);
     if (MODE == kGradient) {
         smem = (smem + 15) / 16 * 16;
         p.acc_at = (int)smem;
