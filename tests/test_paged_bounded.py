@@ -178,6 +178,7 @@ def evict(**kw):
     (dict(kept=4096, kept_width=-1), lib.TG_EINVAL, "kept_width"), (dict(cache=cache(k=None)), lib.TG_EINVAL, "null cache"),
     (dict(pages=table(cols=9)), lib.TG_EINVAL, "columns"), (dict(pages=table(indptr=None)), lib.TG_EINVAL, "indptr"),
     (dict(pages=table(indices=None)), lib.TG_EINVAL, "indices"), (dict(pages=table(nnz=-1)), lib.TG_EINVAL, "size"),
+    (dict(cache=cache(dim=1 << 30)), lib.TG_EUNSUPPORTED, "2^24"),
 ])
 def test_evict_refusals(kw, status, msg):
     refused(lib.load().tg_kv_evict_bf16(evict(**kw), 4096, 1 << 30, None), status, msg)

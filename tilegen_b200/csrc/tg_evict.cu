@@ -516,6 +516,7 @@ int make_plan(const tg_kv_evict_args* a, int elem, Plan* plan, const char* op) {
     if (a->max_seq_len < 0 || a->budget < 0 || a->first < 0 || a->recent < 0)
         return set_error(TG_EINVAL, "%s: negative max_seq_len, budget, first or recent", op);
     if (a->flags & ~TG_FLAG_BOUNDS_CHECK) return set_error(TG_EINVAL, "%s: unknown flags 0x%x", op, a->flags);
+    if (c.dim > 1 << 24) return set_error(TG_EUNSUPPORTED, "%s: heads of more than 2^24 elements (got %d)", op, c.dim);
     if (a->kept && a->kept_width < 0) return set_error(TG_EINVAL, "%s: negative kept_width", op);
     const int64_t slots = c.pages == 0 ? 0 : t.nnz > INT32_MAX / c.page_size ? INT32_MAX / 2 : t.nnz * c.page_size;
     const int64_t max_seq = std::min({a->max_seq_len, slots, (int64_t)INT32_MAX / 2});
