@@ -245,8 +245,8 @@ typedef struct tg_attention_mass_args {
     double decay; /* >= 0 */
     uint32_t flags;
 } tg_attention_mass_args;
-/* Bytes of a workspace to keep, enough for this call and any of the same head sizes with no larger
- * max_q_len (0 for few rows; never more than 80 MB). */
+/* Bytes of a workspace to keep, enough for any call of the same heads with no larger max_q_len, with or
+ * without q_indptr and however many tokens (0 for few rows; never more than 80 MB). */
 TG_API size_t tg_attention_mass_workspace_bytes(const tg_attention_mass_args* a);
 /* What a call with these very arguments takes, at most the former. */
 TG_API size_t tg_attention_mass_needed_bytes(const tg_attention_mass_args* a);

@@ -310,3 +310,19 @@ def test_refusals():
     with pytest.raises(lib.TgError) as e:
         P.attention_mass(P.empty_mass(cache), torch.zeros(1, 4, 80, dtype=BF16, device="cuda"), cache, wide.table, wide.seq_len, lse[:1])
     assert e.value.status == lib.TG_EUNSUPPORTED
+
+
+def test_a_workspace_kept_by_a_small_batch_serves_a_long_prompt():
+    """Asked for with one token, with and without a q_indptr; then parts of one long prompt are kept in it."""
+    small = Weighed([1], [9], 0, 32, 8, 128, 16, BF16, seed=1)
+    pos, _ = small.args()
+    n = P.attention_mass_workspace_bytes(*pos, max_q_len=2048)
+    starts = torch.tensor([0, 1], device="cuda")
+    assert n == P.attention_mass_workspace_bytes(*pos, q_indptr=starts, max_q_len=2048) > 0
+    assert P.attention_mass_workspace_bytes(*pos) == P.attention_mass_workspace_bytes(*pos, q_indptr=starts) == 0
+    ws = torch.full((n,), 255, dtype=torch.uint8, device="cuda")
+    b = Weighed([2048, 1], [2100, 50], 0, 32, 8, 128, 16, BF16, seed=2)
+    lse = b.lse()
+    b.gather(lse, 0.5, workspace=ws)
+    b.check(lse, 0.5)
+    small.gather(small.lse(), workspace=ws)

@@ -164,6 +164,29 @@ def test_a_mass_workspace_serves_every_smaller_call():
             assert L.tg_attention_mass_needed_bytes(a) <= kept <= 80 << 20
 
 
+def test_a_mass_workspace_does_not_depend_on_the_tokens():
+    """What is kept by a first small batch, or by a call without a q_indptr, serves all of the same max_q_len."""
+    L = lib.load()
+    rng = random.Random(4)
+    for _ in range(300):
+        kv, top = rng.choice([1, 2, 8]), rng.choice([1, 5, 300, 2048, 100000])
+        c = cache(pages=1 << 24, heads=kv, dim=rng.choice([64, 96, 128, 256]))
+        heads = kv * rng.choice([1, 4, 5, 300])
+
+        def args(rows, tokens, q, seq, ragged=True):
+            return mass(cache=c, pages=table(rows=rows, cols=1 << 24, nnz=rows * -(-seq // 16)), q_heads=heads, tokens=tokens,
+                        q_indptr=4096 if ragged else None, max_q_len=q, max_seq_len=seq)
+
+        ask = L.tg_attention_mass_workspace_bytes
+        kept = ask(args(1, 0, top, 16))
+        assert kept == ask(args(3, 3, top, 500, False)) == ask(args(1, rng.randint(1, top), top, 9000)) == ask(args(1, 1 << 20, top, 9000))
+        for _ in range(20):
+            rows, q, seq = rng.choice([1, 3, 64, 700]), rng.randint(1, top), rng.choice([1, 500, 9000, 200000])
+            assert L.tg_attention_mass_needed_bytes(args(rows, rows * q, q, seq)) <= kept <= 80 << 20
+    most = mass(q_indptr=4096, max_q_len=(1 << 63) - 1)
+    assert 0 < L.tg_attention_mass_workspace_bytes(most) <= 80 << 20
+
+
 # ------------------------------------------------------------------ eviction
 def evict(**kw):
     return filled(lib.TgKvEvictArgs, dict(cache=cache(), pages=table(), seq_len=4096, max_seq_len=96, budget=40, first=2, recent=5,

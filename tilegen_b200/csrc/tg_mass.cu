@@ -791,7 +791,8 @@ __global__ void __launch_bounds__(256) mass_join_kernel(const __grid_constant__ 
 // Whole prompts of 300 to 3500 tokens: 330 us with 64 an SM, 318 with 128.
 constexpr int64_t kManyUnits = kSMs * 128;
 
-int make_plan(const tg_attention_mass_args* a, MassParams* out, const char* op) {
+// kept: the plan of the most rows that max_q_len allows, whatever the call's tokens.
+int make_plan(const tg_attention_mass_args* a, MassParams* out, const char* op, bool kept = false) {
     if (!a) return set_error(TG_EINVAL, "%s: null arguments", op);
     int rc = check_cache(a->cache, op);
     if (rc == TG_OK && !a->pages) rc = set_error(TG_EINVAL, "%s: null page table", op);
@@ -813,7 +814,9 @@ int make_plan(const tg_attention_mass_args* a, MassParams* out, const char* op) 
     if (a->flags & ~(TG_FLAG_CAUSAL | TG_FLAG_BOUNDS_CHECK)) return set_error(TG_EINVAL, "%s: unknown flags 0x%x", op, a->flags);
     const int64_t slots = c.pages == 0 ? 0 : t.nnz > INT32_MAX / c.page_size ? INT32_MAX / 2 : t.nnz * c.page_size;
     const int64_t max_seq = std::min({a->max_seq_len, slots, (int64_t)INT32_MAX / 2});
-    const int64_t max_q = a->q_indptr ? std::min(a->max_q_len, a->tokens) : 1;
+    const int64_t max_q = kept ? std::min<int64_t>(std::max<int64_t>(a->max_q_len, 1), INT32_MAX)
+                          : a->q_indptr ? std::min(a->max_q_len, a->tokens)
+                                        : 1;
 
     MassParams& p = *out;
     p = {};
@@ -942,7 +945,7 @@ extern "C" {
 
 size_t tg_attention_mass_workspace_bytes(const tg_attention_mass_args* a) {
     tg::MassParams p;
-    return tg::make_plan(a, &p, "tg_attention_mass") == TG_OK ? tg::mass_enough(p) : 0;
+    return tg::make_plan(a, &p, "tg_attention_mass", true) == TG_OK ? tg::mass_enough(p) : 0;
 }
 
 size_t tg_attention_mass_needed_bytes(const tg_attention_mass_args* a) {

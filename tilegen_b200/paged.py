@@ -739,8 +739,11 @@ def _mass_launch(m, mass, q, workspace, index, sp):
 def attention_mass_workspace_bytes(q: torch.Tensor, cache: PagedKV, table: PageTable, seq_len: torch.Tensor,
                                    q_indptr: Optional[torch.Tensor] = None, max_q_len: Optional[int] = None) -> int:
     """Bytes of a workspace to keep for attention_mass: enough for this call and every one of the same
-    head sizes with no larger max_q_len (0 for few rows)."""
+    heads with no larger max_q_len, however many its tokens (0 for few rows).  max_q_len counts without a
+    q_indptr too, for calls with one that follow."""
     m, _held = _mass_args(None, q, cache, table, seq_len, None, q_indptr, max_q_len, None, None, True, 1.0, False)
+    if max_q_len is not None:
+        m.max_q_len = max_q_len
     return int(_call("tg_attention_mass_workspace_bytes")(m))
 
 
