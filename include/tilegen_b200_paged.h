@@ -228,7 +228,8 @@ typedef struct tg_paged_mass {
  * that no row sees with decay * mass; slots behind a sequence's length are left alone, and slots of
  * pages that do not exist dropped.  No page may be listed twice.  Scores, exponentials and sums are
  * 32-bit and the sums' order is fixed.  cache->v is not read.  Dim 64, 96, 128 or 256, q and k
- * aligned as for the attention. */
+ * aligned as for the attention.  A block of the kernel whose warps wait for one another longer than
+ * two seconds (environment: TG_MASS_WAIT_MS) leaves NaN in the mass of all its keys. */
 typedef struct tg_attention_mass_args {
     const tg_paged_kv* cache;
     const tg_csr* pages;

@@ -10,6 +10,9 @@ product and the last addition: 2^-22 of the result's terms.
 from __future__ import annotations
 
 import math
+import os
+import subprocess
+import sys
 
 import pytest
 import torch
@@ -326,3 +329,38 @@ def test_a_workspace_kept_by_a_small_batch_serves_a_long_prompt():
     b.gather(lse, 0.5, workspace=ws)
     b.check(lse, 0.5)
     small.gather(small.lse(), workspace=ws)
+
+
+GIVE_UP = [
+    ([1] * 5, [1, 50, 128, 300, 2000], 40, 8, 2, 128, 16),
+    ([32, 7], [3000, 90], 0, 8, 1, 64, 16),                  # two halves of rows
+    ([700, 1], [900, 130], 0, 8, 2, 128, 32),                # parts that are joined
+    ([90] * 530, [90 + i % 70 for i in range(530)], 0, 4, 1, 64, 32),  # more sequences than one launch takes
+    ([2, 1], [77, 200], 0, 300, 1, 256, 16),                 # several row tiles a token
+    ([300, 9], [700, 1900], 0, 16, 8, 96, 24),
+]
+
+
+def test_a_wait_that_runs_out_leaves_nan():
+    """Where a wait has run out (here: as if at once, in every CTA) no key keeps a number that may be wrong,
+    and nothing else is written."""
+    code = """
+import sys
+sys.path[:0] = %r
+from test_gpu_paged_mass import *
+for case, shape in enumerate(GIVE_UP):
+    for dtype in (BF16, F16):
+        b = Weighed(*shape, dtype, seed=case)
+        lse = b.lse()
+        for decay in (0.5, 0.0):
+            b.mass.copy_(b.before.nan_to_num(3.0))
+            b.gather(lse, decay, max_seq_len=max(b.lens))
+            want = b.before.nan_to_num(3.0)
+            for pages, length in zip(b.rows, b.lens):
+                at = torch.arange(length, device="cuda")
+                want[torch.tensor(pages, device="cuda")[at // b.page], at %% b.page] = math.nan
+            assert torch.equal(b.mass.nan_to_num(-7.0), want.nan_to_num(-7.0)), (case, dtype, decay)
+print("all", len(GIVE_UP))
+""" % [os.path.dirname(os.path.abspath(__file__)), os.path.dirname(os.path.dirname(os.path.abspath(__file__)))]
+    r = subprocess.run([sys.executable, "-c", code], env={**os.environ, "TG_MASS_WAIT_MS": "0"}, capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and "all %d" % len(GIVE_UP) in r.stdout, r.stdout + r.stderr

@@ -33,6 +33,7 @@
 // head).  Each CTA counts the units of all sequences at its begin and takes every gridDim.x-th, so that
 // ragged lengths and the causal mask leave no holes in the shares.
 #include <algorithm>
+#include <cstdlib>
 #include <numeric>
 
 #include "tg_tcgen05.cuh"
@@ -65,6 +66,7 @@ struct MassParams : AttnParams {
     int box, box_shift;                                  // keys of a box, their log2
     int q_bufs, stages;
     int first_seq, seqs;  // of this launch
+    uint64_t wait_ns;     // how long warps wait for one another; 0: a wait that is not over at once runs out
     float* part;          // with splits > 1: [split][chunk][sequence][key head][key of the chunk]
 };
 
@@ -302,7 +304,7 @@ __device__ __forceinline__ Cta enter(const MassParams& p, unsigned char* smem, i
             mbar_init(&sh.a_full, kGroups * 4);
             mbar_init(&sh.a_empty, 1);
             mbar_init(&sh.drained, 1);
-            sh.fail = 0;
+            sh.fail = p.wait_ns == 0;
             fence_mbar_init();
         }
     }
@@ -313,13 +315,31 @@ __device__ __forceinline__ Cta enter(const MassParams& p, unsigned char* smem, i
     c.tmem = sh.tmem;
     return c;
 }
-__device__ __forceinline__ void leave(const Cta& c, int warp) {
+// A warp whose wait has run out stops: it signals nothing and writes nothing more, so that no other takes a
+// buffer or a table of pages for what it is not.  The others stop at their next wait.  Then no number of
+// the CTA stands, and all keys of all its units get NaN, which the parts' join and a reader cannot miss.
+__device__ __noinline__ void spoil(const MassParams& p, const MassShared& sh) {
+    Units units;
+    Unit u;
+    while (units.next(p, sh, u))
+        for (int at = threadIdx.x; at < u.keys; at += kThreads) {
+            if (p.splits > 1) {
+                p.part[part_at(p, u) + at] = NAN;
+                continue;
+            }
+            int page, slot;
+            locate(p, p.indices + u.s.page0, u.k0 + at, page, slot);
+            if (page >= 0) p.mass[page * p.m_page + slot * p.m_slot + u.h * p.m_head] = NAN;
+        }
+}
+__device__ __forceinline__ void leave(const MassParams& p, const Cta& c, int warp) {
     __syncwarp();
     __syncthreads();
     if (warp == kMmaWarp) {
         fence_after();
         tmem_free(c.tmem, kCols);
     }
+    if (*c.fail) spoil(p, c.sh);
 }
 
 // D (+)= A B of STEPS times 16 elements of one 64-column half, both operands in shared memory; `add`: D
@@ -371,7 +391,7 @@ __device__ __forceinline__ void product(const Cta& c, uint32_t k, uint32_t q, in
 // Warp 19: the pages of a unit's boxes.
 __device__ __forceinline__ bool find_pages(const MassParams& p, const Cta& c, const Unit& u, int turn, int lane) {
     const int buf = turn & 1;
-    if (turn >= 2 && !wait_warp(c.b_pe + buf * 8, (turn / 2 - 1) & 1, c.fail)) return false;
+    if (turn >= 2 && !wait_warp(c.b_pe + buf * 8, (turn / 2 - 1) & 1, c.fail, p.wait_ns)) return false;
     const int64_t* list = p.indices + u.s.page0;
     for (int i = lane; i << p.box_shift < u.keys; i += 32) {
         int page, slot;
@@ -427,13 +447,13 @@ __device__ __forceinline__ bool fetch_rows(const MassParams& p, const Cta& c, co
             seen[k] = keys_seen(p, u.s, t0 + i, u.s.len, u.s.len);
         }
     }
-    if (nq >= p.q_bufs && !wait_warp(c.b_qe + qb * 8, (nq / p.q_bufs - 1) & 1, c.fail)) return false;
+    if (nq >= p.q_bufs && !wait_warp(c.b_qe + qb * 8, (nq / p.q_bufs - 1) & 1, c.fail, p.wait_ns)) return false;
     if (lane == 0) mbar_arrive_expect_tx(&c.sh.q_full[qb], p.tile_tokens * p.tile_heads * DIM * 2);
     __syncwarp();
 #pragma unroll
     for (int half = 0; half < DIM / 64; ++half)
         load_box3(c.sq + qb * c.q_block + half * c.q_half, map, half * 64, u.h * p.group + h0, u.s.first + t0, c.b_qf + qb * 8);
-    if (nq >= 2 && !wait_warp(c.b_ie + ib * 8, (nq / 2 - 1) & 1, c.fail)) return false;
+    if (nq >= 2 && !wait_warp(c.b_ie + ib * 8, (nq / 2 - 1) & 1, c.fail, p.wait_ns)) return false;
     int fewest = INT_MAX;
 #pragma unroll
     for (int k = 0; k < kEach; ++k) {
@@ -505,13 +525,13 @@ __global__ void __launch_bounds__(kThreads, 1) stream_kernel(const __grid_consta
         while (ok && units.next(p, c.sh, u)) {
             if (u.s.asked == 0) continue;
             const int qb = nq % p.q_bufs;
-            ok = wait_warp(c.b_qf + qb * 8, nq / p.q_bufs & 1, c.fail);
+            ok = wait_warp(c.b_qf + qb * 8, nq / p.q_bufs & 1, c.fail, p.wait_ns);
             for (int j = 0; ok && j < u.tiles; ++j, ++f) {
                 const int st = f % p.stages, buf = f % kGroups;
-                ok = wait_warp(c.b_full + st * 8, f / p.stages & 1, c.fail);
+                ok = wait_warp(c.b_full + st * 8, f / p.stages & 1, c.fail, p.wait_ns);
                 for (int half = 0; ok && half < halves; ++half) {
                     const int i = f / kGroups * halves + half;
-                    ok = i < 1 || wait_warp(c.b_se + buf * 8, (i - 1) & 1, c.fail);
+                    ok = i < 1 || wait_warp(c.b_se + buf * 8, (i - 1) & 1, c.fail, p.wait_ns);
                     if (!ok) break;
                     fence_after();
                     product<T, KSTEPS>(c, c.ring + st * kBlock, c.sq + qb * c.q_block + half * kHalfRows * 128,
@@ -523,7 +543,7 @@ __global__ void __launch_bounds__(kThreads, 1) stream_kernel(const __grid_consta
             if (ok) commit(c.b_qe + qb * 8);
             ++nq;
         }
-        if (!ok) {  // leave no product under way
+        if (!ok || *c.fail) {  // leave no product under way
             commit(smem_addr(&c.sh.drained));
             mbar_wait(&c.sh.drained, 0);
         }
@@ -531,10 +551,10 @@ __global__ void __launch_bounds__(kThreads, 1) stream_kernel(const __grid_consta
         int f = 0;
         while (ok && units.next(p, c.sh, u)) {
             const int buf = units.turn & 1;
-            ok = wait_warp(c.b_pf + buf * 8, units.turn / 2 & 1, c.fail);
+            ok = wait_warp(c.b_pf + buf * 8, units.turn / 2 & 1, c.fail, p.wait_ns);
             for (int j = 0; ok && u.s.asked > 0 && j < u.tiles; ++j, ++f) {
                 const int st = f % p.stages;
-                if (f >= p.stages && !(ok = wait_warp(c.b_empty + st * 8, (f / p.stages - 1) & 1, c.fail))) break;
+                if (f >= p.stages && !(ok = wait_warp(c.b_empty + st * 8, (f / p.stages - 1) & 1, c.fail, p.wait_ns))) break;
                 fetch_keys<DIM>(p, c, u, c.sh.page[buf], j * kTile, c.ring + st * kBlock, &c.sh.full[st], &kmap, lane);
             }
             __syncwarp();
@@ -558,9 +578,9 @@ __global__ void __launch_bounds__(kThreads, 1) stream_kernel(const __grid_consta
         const int my = warp >> 2, key_of = tid & (kTile - 1);
         const uint32_t ts = c.tmem + my * kHalfRows + ((uint32_t)(warp & 3) << 21);
         int f = 0, nq = 0;
-        while (units.next(p, c.sh, u)) {
+        while (ok && units.next(p, c.sh, u)) {
             const int pb = units.turn & 1, ib = nq & 1, f0 = f, tiles = u.s.asked > 0 ? u.tiles : 0;
-            ok = ok && wait_warp(c.b_pf + pb * 8, units.turn / 2 & 1, c.fail);
+            ok = wait_warp(c.b_pf + pb * 8, units.turn / 2 & 1, c.fail, p.wait_ns);
             const int* pages = c.sh.page[pb];
             auto old_of = [&](int at, float*& to, float& old) {
                 to = mass_at(p, u, pages, at), old = 0.f;
@@ -572,7 +592,7 @@ __global__ void __launch_bounds__(kThreads, 1) stream_kernel(const __grid_consta
                 // the old weights of my next tile are under way
                 const int skip = (my - f % kGroups + kGroups) % kGroups;
                 if (ok) old_of(skip * kTile + key_of, to, old);
-                ok = ok && wait_warp(c.b_if + ib * 8, nq / 2 & 1, c.fail);
+                ok = ok && wait_warp(c.b_if + ib * 8, nq / 2 & 1, c.fail, p.wait_ns);
                 const int rows = c.sh.rows[ib], fewest = c.sh.fewest[ib];
                 for (f += skip; ok && f < f0 + tiles; f += kGroups) {
                     const int at = (f - f0) * kTile + key_of, key = u.k0 + at;
@@ -580,7 +600,7 @@ __global__ void __launch_bounds__(kThreads, 1) stream_kernel(const __grid_consta
                     const bool all = u.k0 + min(at - key_of + kTile, u.keys) <= fewest;  // every row sees every key
                     float sum = 0.f;
                     for (int half = 0; ok && half < halves; ++half) {
-                        ok = wait_warp(c.b_sf + my * 8, (f / kGroups * halves + half) & 1, c.fail);
+                        ok = wait_warp(c.b_sf + my * 8, (f / kGroups * halves + half) & 1, c.fail, p.wait_ns);
                         if (!ok) break;
                         fence_after();
                         sum += sum_rows(p, c, ts, ib, half * kHalfRows, min(rows - half * kHalfRows, kHalfRows), key, all);
@@ -588,12 +608,13 @@ __global__ void __launch_bounds__(kThreads, 1) stream_kernel(const __grid_consta
                         __syncwarp();
                         if (lane == 0) arrive(c.b_se + my * 8);
                     }
-                    put(p, u, key, to, old, ok ? sum : NAN);  // loud: a wait that ran out leaves no number
+                    if (!ok) break;
+                    put(p, u, key, to, old, sum);
                     to = to_next, old = old_next;
                 }
                 f = f0 + tiles;
                 __syncwarp();
-                if (lane == 0) arrive(c.b_ie + ib * 8);
+                if (ok && lane == 0) arrive(c.b_ie + ib * 8);
                 ++nq;
             } else if (ok) {  // no row: the old weights decay
                 for (int at = tid; at < u.keys; at += kGroups * kTile) {
@@ -602,10 +623,10 @@ __global__ void __launch_bounds__(kThreads, 1) stream_kernel(const __grid_consta
                 }
             }
             __syncwarp();
-            if (lane == 0) arrive(c.b_pe + pb * 8);
+            if (ok && lane == 0) arrive(c.b_pe + pb * 8);
         }
     }
-    leave(c, warp);
+    leave(p, c, warp);
 }
 
 // Many row tiles: a chunk of keys stays in shared memory while they pass.
@@ -632,16 +653,16 @@ __global__ void __launch_bounds__(kThreads, 1) rows_kernel(const __grid_constant
                 const int steps = steps_of(p, u, qi);
                 if (steps == 0) continue;
                 const int qb = nq % p.q_bufs;
-                ok = wait_warp(c.b_qf + qb * 8, nq / p.q_bufs & 1, c.fail);
+                ok = wait_warp(c.b_qf + qb * 8, nq / p.q_bufs & 1, c.fail, p.wait_ns);
                 for (int j = 0; ok && j < steps; ++j, ++g) {
                     if (j >= here) {
-                        ok = wait_warp(c.b_full + j * 8, used >> j & 1, c.fail);
+                        ok = wait_warp(c.b_full + j * 8, used >> j & 1, c.fail, p.wait_ns);
                         used ^= 1u << j;
                         here = j + 1;
                     }
                     const int buf = g % kGroups;
                     if (began >> buf & 1) {
-                        ok = ok && wait_warp(c.b_se + buf * 8, emptied >> buf & 1, c.fail);
+                        ok = ok && wait_warp(c.b_se + buf * 8, emptied >> buf & 1, c.fail, p.wait_ns);
                         emptied ^= 1u << buf;
                     }
                     began |= 1u << buf;
@@ -654,7 +675,7 @@ __global__ void __launch_bounds__(kThreads, 1) rows_kernel(const __grid_constant
                 ++nq;
             }
         }
-        if (!ok) {  // leave no product under way
+        if (!ok || *c.fail) {  // leave no product under way
             commit(smem_addr(&c.sh.drained));
             mbar_wait(&c.sh.drained, 0);
         }
@@ -663,10 +684,10 @@ __global__ void __launch_bounds__(kThreads, 1) rows_kernel(const __grid_constant
         uint32_t landed = 0;
         while (ok && units.next(p, c.sh, u)) {
             const int buf = units.turn & 1, tiles = u.q1 > u.q0 ? steps_of(p, u, u.q1 - 1) : 0;
-            ok = wait_warp(c.b_pf + buf * 8, units.turn / 2 & 1, c.fail);
+            ok = wait_warp(c.b_pf + buf * 8, units.turn / 2 & 1, c.fail, p.wait_ns);
             for (int j = 0; ok && j < tiles; ++j) {
                 if (began >> j & 1) {
-                    ok = wait_warp(c.b_empty + j * 8, freed >> j & 1, c.fail);
+                    ok = wait_warp(c.b_empty + j * 8, freed >> j & 1, c.fail, p.wait_ns);
                     freed ^= 1u << j;
                 }
                 if (!ok) break;
@@ -698,7 +719,7 @@ __global__ void __launch_bounds__(kThreads, 1) rows_kernel(const __grid_constant
         ok = !more || find_pages(p, c, u, units.turn, lane);
         while (ok && made.next(p, c.sh, v)) {
             more = more && units.next(p, c.sh, u);
-            ok = (!more || find_pages(p, c, u, units.turn, lane)) && wait_warp(smem_addr(&c.sh.a_full), made.turn & 1, c.fail);
+            ok = (!more || find_pages(p, c, u, units.turn, lane)) && wait_warp(smem_addr(&c.sh.a_full), made.turn & 1, c.fail, p.wait_ns);
             if (!ok) break;
             const int pb = made.turn & 1;
             for (int at = lane; at < v.keys; at += 32) {
@@ -722,7 +743,7 @@ __global__ void __launch_bounds__(kThreads, 1) rows_kernel(const __grid_constant
         const int my = warp >> 2, key_of = tid & (kTile - 1);
         const uint32_t ts = c.tmem + my * kHalfRows + ((uint32_t)(warp & 3) << 21);
         int nq = 0, made = 0;
-        while (units.next(p, c.sh, u)) {
+        while (ok && units.next(p, c.sh, u)) {
             float acc[kChunk];
 #pragma unroll
             for (int m = 0; m < kChunk; ++m) acc[m] = 0.f;
@@ -731,14 +752,15 @@ __global__ void __launch_bounds__(kThreads, 1) rows_kernel(const __grid_constant
                 const int steps = steps_of(p, u, qi);
                 if (steps == 0) continue;
                 const int ib = nq & 1;
-                ok = wait_warp(c.b_if + ib * 8, nq / 2 & 1, c.fail);
+                ok = wait_warp(c.b_if + ib * 8, nq / 2 & 1, c.fail, p.wait_ns);
                 const int rows = c.sh.rows[ib], fewest = c.sh.fewest[ib];
                 for (int j = (my - g % kGroups + kGroups) % kGroups; ok && j < steps; j += kGroups) {
-                    ok = wait_warp(c.b_sf + my * 8, made & 1, c.fail);
+                    ok = wait_warp(c.b_sf + my * 8, made & 1, c.fail, p.wait_ns);
+                    if (!ok) break;
                     fence_after();
                     const int at = j * kTile + key_of;
                     const bool all = u.k0 + min((j + 1) * kTile, u.keys) <= fewest;  // every row sees every key
-                    const float sum = ok ? sum_rows(p, c, ts, ib, 0, rows, u.k0 + at, all) : 0.f;
+                    const float sum = sum_rows(p, c, ts, ib, 0, rows, u.k0 + at, all);
                     fence_before();
                     __syncwarp();
                     if (lane == 0) arrive(c.b_se + my * 8);
@@ -747,18 +769,19 @@ __global__ void __launch_bounds__(kThreads, 1) rows_kernel(const __grid_constant
                     for (int m = 0; m < kChunk; ++m) acc[m] += m == j ? sum : 0.f;
                 }
                 __syncwarp();
-                if (lane == 0) arrive(c.b_ie + ib * 8);
+                if (ok && lane == 0) arrive(c.b_ie + ib * 8);
                 ++nq;
                 g += steps;
             }
-            ok = ok && (units.turn == 0 || wait_warp(smem_addr(&c.sh.a_empty), (units.turn - 1) & 1, c.fail));
+            ok = ok && (units.turn == 0 || wait_warp(smem_addr(&c.sh.a_empty), (units.turn - 1) & 1, c.fail, p.wait_ns));
+            if (!ok) break;
 #pragma unroll
-            for (int m = 0; m < kChunk; ++m) c.sh.acc[my][m * kTile + key_of] = ok ? acc[m] : NAN;  // loud: a wait that ran out leaves no number
+            for (int m = 0; m < kChunk; ++m) c.sh.acc[my][m * kTile + key_of] = acc[m];
             __syncwarp();
             if (lane == 0) arrive(smem_addr(&c.sh.a_full));
         }
     }
-    leave(c, warp);
+    leave(p, c, warp);
 }
 
 // mass of the keys of a (chunk, sequence, key head) from the parts of its row tiles, in their order.
@@ -882,6 +905,18 @@ size_t mass_enough(const MassParams& p) {
     return p.stream || p.head_tiles > 1 ? 0 : (size_t)(2 * kManyUnits) * p.chunk * kTile * sizeof(float);
 }
 
+// Whole milliseconds from TG_MASS_WAIT_MS in the environment, a minute at most; else two seconds, where the
+// waits are microseconds.
+uint64_t wait_limit() {
+    static const uint64_t ns = [] {
+        const char* text = std::getenv("TG_MASS_WAIT_MS");
+        char* end = nullptr;
+        const long ms = text ? std::strtol(text, &end, 10) : 0;
+        return !text || end == text || *end || ms < 0 ? kWaitNs : (uint64_t)std::min(ms, 60000l) * 1000000;
+    }();
+    return ns;
+}
+
 template <typename T, int DIM, int KSTEPS>
 int mass_run(const MassParams& p, const CUtensorMap& kmap, const CUtensorMap& qmap, cudaStream_t st) {
     auto kernel = p.stream ? stream_kernel<T, DIM, KSTEPS> : rows_kernel<T, DIM, KSTEPS>;
@@ -925,6 +960,7 @@ int attention_mass(const tg_attention_mass_args* a, void* ws, size_t ws_bytes, t
     if (ws_bytes < need || (need && !ws)) return set_error(TG_ENOMEM, "%s: workspace of %zu bytes needed (got %zu)", op, need, ws_bytes);
     if (reinterpret_cast<uintptr_t>(ws) % 16) return set_error(TG_EINVAL, "%s: the workspace must be 16-byte aligned", op);
     p.part = static_cast<float*>(ws);
+    p.wait_ns = wait_limit();
     constexpr bool kIsHalf = std::is_same<T, __half>::value;
     CUtensorMap kmap, vmap, qmap;
     rc = cache_maps(p, kIsHalf, c.dim, p.box, &kmap, &vmap);

@@ -108,14 +108,16 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
     return r;
 }
 
-// Bounded wait; false once one has run out in this CTA (2 s; every wait here is microseconds).
-__device__ __forceinline__ bool wait(uint32_t bar, uint32_t parity, volatile int* fail) {
+constexpr uint64_t kWaitNs = 2000000000ull;
+
+// Bounded wait; false once one has run out in this CTA (two seconds, where the waits are microseconds).
+__device__ __forceinline__ bool wait(uint32_t bar, uint32_t parity, volatile int* fail, uint64_t limit = kWaitNs) {
     if (mbar_try(bar, parity)) return true;
     const uint64_t t0 = globaltimer_ns();
     for (;;) {
         if (mbar_try(bar, parity)) return true;
         if (*fail) return false;
-        if (globaltimer_ns() - t0 > 2000000000ull) {
+        if (globaltimer_ns() - t0 > limit) {
             *fail = 1;
             return false;
         }
@@ -123,8 +125,8 @@ __device__ __forceinline__ bool wait(uint32_t bar, uint32_t parity, volatile int
 }
 
 // The same answer for all lanes, which go on together (what follows is done by whole warps).
-__device__ __forceinline__ bool wait_warp(uint32_t bar, uint32_t parity, volatile int* fail) {
-    return __all_sync(kFull, wait(bar, parity, fail));
+__device__ __forceinline__ bool wait_warp(uint32_t bar, uint32_t parity, volatile int* fail, uint64_t limit = kWaitNs) {
+    return __all_sync(kFull, wait(bar, parity, fail, limit));
 }
 
 // As mbar_wait, for at most a millisecond: to let copies land before a kernel that gave up ends.
