@@ -364,3 +364,43 @@ print("all", len(GIVE_UP))
 """ % [os.path.dirname(os.path.abspath(__file__)), os.path.dirname(os.path.dirname(os.path.abspath(__file__)))]
     r = subprocess.run([sys.executable, "-c", code], env={**os.environ, "TG_MASS_WAIT_MS": "0"}, capture_output=True, text=True, timeout=300)
     assert r.returncode == 0 and "all %d" % len(GIVE_UP) in r.stdout, r.stdout + r.stderr
+
+
+def test_a_unit_may_take_longer_than_a_wait():
+    """1000 tokens of 256 heads a key head pass 512 keys, some milliseconds for a CTA's unit, of which it has
+    several: with a limit of one millisecond nothing runs out, as all waits but those for a whole unit are
+    microseconds.  The bound is that of the other cases, for 256000 rows."""
+    code = """
+import sys
+sys.path[:0] = %r
+from test_gpu_paged_mass import *
+n, kvh, group, dim, keys, page, batch = 1000, 8, 256, 64, 512, 32, 40
+g = gen(7)
+pages = batch * keys // page
+cache = P.PagedKV(normal(g, pages, page, kvh, dim, dtype=BF16), None)
+cache.v = cache.k
+table = P.PageTable.from_lists([list(range(b * keys // page, (b + 1) * keys // page)) for b in range(batch)])
+news = [0 if b %% 5 == 1 else n for b in range(batch)]
+starts = torch.tensor([0] + news, device="cuda").cumsum(0)
+one = normal(g, 1, kvh * group, dim, dtype=BF16)
+sc = torch.einsum("xhgd,bkhd->bhgk", one.double().view(1, kvh, group, dim), cache.k.double().view(batch, keys, kvh, dim)) * dim ** -0.5
+lse = sc.logsumexp(-1).float()  # [sequence, key head, head]
+rows = lse.flatten(1).repeat_interleave(torch.tensor(news, device="cuda"), 0).contiguous()
+mass = P.empty_mass(cache).fill_(2.0)
+lens = torch.full((batch,), keys, device="cuda")
+P.attention_mass(mass, one.expand(sum(news), kvh * group, dim), cache, table, lens, rows, q_indptr=starts, max_q_len=n,
+                 max_seq_len=keys, causal=False, decay=0.5)
+p = (sc - lse.double()[..., None]).exp()
+e = 2.0 ** -18 * (1 + torch.einsum("xhgd,bkhd->bhgk", one.double().abs().view(1, kvh, group, dim),
+                                   cache.k.double().abs().view(batch, keys, kvh, dim)) * dim ** -0.5)
+rel = 2 * e + 2.0 ** -22 * lse.double().abs()[..., None] + 2.0 ** -20 + (n * group / 4 + 64) * 2.0 ** -24
+count = torch.tensor(news, device="cuda", dtype=torch.float64)[:, None, None]
+gathered, tol = p.sum(2) * count, (p * rel).sum(2) * count
+got = mass.double().reshape(batch, keys, kvh).transpose(1, 2)
+err, tol = (got - gathered - 1.0).abs(), tol + 2.0 ** -22 * (gathered + 1.0)
+assert bool(got.isfinite().all()), int(got.isnan().sum())
+assert bool((err <= tol).all()), float((err / tol).max())
+print("all", batch)
+""" % [os.path.dirname(os.path.abspath(__file__)), os.path.dirname(os.path.dirname(os.path.abspath(__file__)))]
+    r = subprocess.run([sys.executable, "-c", code], env={**os.environ, "TG_MASS_WAIT_MS": "1"}, capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and "all 40" in r.stdout, r.stdout + r.stderr

@@ -75,6 +75,7 @@ struct MassShared {
         s_empty[4], drained;
     uint32_t tmem;
     int fail;
+    int passed;                                        // row tiles that have been fetched
     int fewest[2], rows[2];                            // keys that every row of the tile sees; rows
     __align__(16) float lse2[2][kMostRows];            // -lse * log2 e
     __align__(16) int seen[2][kMostRows];              // keys that a row sees, 0 for what is no row
@@ -272,6 +273,28 @@ struct Cta {
     volatile int* fail;
 };
 
+// As wait_warp, for what may take as long as all row tiles of a unit do, which are as many as a sequence has
+// tokens: the time starts anew with each of them.
+__device__ __forceinline__ bool wait_rows(const MassParams& p, const Cta& c, uint32_t bar, uint32_t parity) {
+    bool ok = mbar_try(bar, parity);
+    if (!ok) {
+        const volatile int* passed = &c.sh.passed;
+        uint64_t t0 = globaltimer_ns();
+        for (int last = *passed;;) {
+            if ((ok = mbar_try(bar, parity)) || *c.fail) break;
+            const uint64_t t = globaltimer_ns();
+            const int now = *passed;
+            if (now != last) {
+                last = now, t0 = t;
+            } else if (t - t0 > p.wait_ns) {
+                *c.fail = 1;
+                break;
+            }
+        }
+    }
+    return __all_sync(kFull, ok);
+}
+
 template <int DIM>
 __device__ __forceinline__ Cta enter(const MassParams& p, unsigned char* smem, int page_readers, int warp, int lane) {
     MassShared& sh = *reinterpret_cast<MassShared*>(smem + kTiles);
@@ -305,6 +328,7 @@ __device__ __forceinline__ Cta enter(const MassParams& p, unsigned char* smem, i
             mbar_init(&sh.a_empty, 1);
             mbar_init(&sh.drained, 1);
             sh.fail = p.wait_ns == 0;
+            sh.passed = 0;
             fence_mbar_init();
         }
     }
@@ -471,7 +495,10 @@ __device__ __forceinline__ bool fetch_rows(const MassParams& p, const Cta& c, co
         c.sh.rows[ib] = rows;
     }
     __syncwarp();
-    if (lane == 0) arrive(c.b_if + ib * 8);
+    if (lane == 0) {
+        *static_cast<volatile int*>(&c.sh.passed) = nq + 1;
+        arrive(c.b_if + ib * 8);
+    }
     return true;
 }
 // Leaves no copy of rows under way.
@@ -684,10 +711,10 @@ __global__ void __launch_bounds__(kThreads, 1) rows_kernel(const __grid_constant
         uint32_t landed = 0;
         while (ok && units.next(p, c.sh, u)) {
             const int buf = units.turn & 1, tiles = u.q1 > u.q0 ? steps_of(p, u, u.q1 - 1) : 0;
-            ok = wait_warp(c.b_pf + buf * 8, units.turn / 2 & 1, c.fail, p.wait_ns);
+            ok = wait_rows(p, c, c.b_pf + buf * 8, units.turn / 2 & 1);
             for (int j = 0; ok && j < tiles; ++j) {
                 if (began >> j & 1) {
-                    ok = wait_warp(c.b_empty + j * 8, freed >> j & 1, c.fail, p.wait_ns);
+                    ok = wait_rows(p, c, c.b_empty + j * 8, freed >> j & 1);
                     freed ^= 1u << j;
                 }
                 if (!ok) break;
@@ -719,7 +746,7 @@ __global__ void __launch_bounds__(kThreads, 1) rows_kernel(const __grid_constant
         ok = !more || find_pages(p, c, u, units.turn, lane);
         while (ok && made.next(p, c.sh, v)) {
             more = more && units.next(p, c.sh, u);
-            ok = (!more || find_pages(p, c, u, units.turn, lane)) && wait_warp(smem_addr(&c.sh.a_full), made.turn & 1, c.fail, p.wait_ns);
+            ok = (!more || find_pages(p, c, u, units.turn, lane)) && wait_rows(p, c, smem_addr(&c.sh.a_full), made.turn & 1);
             if (!ok) break;
             const int pb = made.turn & 1;
             for (int at = lane; at < v.keys; at += 32) {
