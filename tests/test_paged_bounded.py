@@ -8,6 +8,7 @@ import random
 
 import pytest
 import torch
+from torch.autograd import forward_ad
 
 from tilegen_b200 import lib
 from tilegen_b200 import paged as P
@@ -237,3 +238,23 @@ def test_cpu_tensors_are_refused():
         P.attention_mass(torch.zeros(4, 16, 2), x, kv, tb, none, torch.zeros(2, 3))
     with pytest.raises(ValueError, match="CUDA"):
         P.kv_evict(kv, tb, none, torch.zeros(4, 16, 2), 10)
+
+
+def test_forward_mode_tangents_are_refused():
+    """A dual tensor has an address like any other, and its tangent would be lost without a word."""
+    x, w, pos, r = torch.ones(2, 3, 64), torch.ones(64), torch.zeros(2, dtype=torch.int64), P.Rope(torch.ones(32, dtype=torch.float64))
+    n = P.HeadNorm(w)
+    with forward_ad.dual_level():
+        d, dn = forward_ad.make_dual(x, x.clone()), P.HeadNorm(forward_ad.make_dual(w, w.clone()))
+        for call in (lambda: P.rope(d, r, pos), lambda: P.rope_backward(d, r, pos), lambda: P.norm_rope(d, None, n),
+                     lambda: P.norm_rope(x, d, n), lambda: P.norm_rope(x, None, dn), lambda: P.norm_rope(x, x, n, dn),
+                     lambda: P.norm_rope_backward(d, None, x, None, n), lambda: P.norm_rope_backward(x, None, d, None, n),
+                     lambda: P.norm_rope_backward(x, d, x, x, n), lambda: P.norm_rope_backward(x, x, x, x, n, dn),
+                     lambda: P.rope(d.clone().requires_grad_(), r, pos)):
+            with pytest.raises(NotImplementedError, match="tangent"):
+                call()
+        for call in (lambda: P.rope(x, r, pos), lambda: P.norm_rope(x, x, n), lambda: P.rope(d, r, pos, out=x)):
+            with pytest.raises(ValueError, match="CUDA"):
+                call()
+    with pytest.raises(ValueError, match="CUDA"):  # the level has ended
+        P.rope(d, r, pos)

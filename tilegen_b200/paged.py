@@ -24,6 +24,7 @@ from dataclasses import dataclass
 from typing import List, Optional, Sequence, Tuple, Union
 
 import torch
+from torch.autograd import forward_ad
 
 from . import lib as _lib
 from .device import _dev
@@ -265,6 +266,13 @@ def _rope_launch(suffix, x, out, xr, rd, pos, flags, sp) -> torch.Tensor:
     return out
 
 
+def _no_tangent(name: str, *tensors: Optional[torch.Tensor]) -> None:
+    """Refuses tensors that carry a forward-mode tangent, which a call by address would drop.  (Asked for where a
+    level of dual tensors is open.)"""
+    if any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise NotImplementedError("%s has no forward-mode derivative: a dual tensor would lose its tangent" % name)
+
+
 class _Turn(torch.autograd.Function):
     """The rotation, or with TG_FLAG_ROPE_INVERSE its transpose: each is the other's gradient."""
 
@@ -283,6 +291,8 @@ class _Turn(torch.autograd.Function):
 
 
 def _turn(x, r, positions, out, flags, stream) -> torch.Tensor:
+    if out is None and forward_ad._current_level >= 0:
+        _no_tangent("rope", x)
     if out is None and x.requires_grad and torch.is_grad_enabled():
         if stream is not None:
             _stream(x.get_device(), stream)  # it is on x's device
@@ -295,7 +305,8 @@ def rope(x: torch.Tensor, r: Rope, positions: torch.Tensor, out: Optional[torch.
          stream: Optional[torch.cuda.Stream] = None) -> torch.Tensor:
     """x [tokens, heads, dim] rotated at positions [tokens] (int64); out may be x.
 
-    Differentiable with respect to x, unless the result is written to a given out."""
+    Differentiable with respect to x, unless the result is written to a given out; a dual tensor of
+    forward-mode differentiation is refused."""
     return _turn(x, r, positions, out, 0, stream)
 
 
@@ -395,7 +406,10 @@ def norm_rope(q: torch.Tensor, k: Optional[torch.Tensor] = None, q_norm: Optiona
     one pass over both.  Without a norm that tensor is only rotated, without a rope nothing turns; k
     may be None.  dim is 256 at most.  q_out and k_out may be q and k.
 
-    Differentiable with respect to q, k and the norms' weights (once), unless an out is given."""
+    Differentiable with respect to q, k and the norms' weights (once), unless an out is given; dual
+    tensors of forward-mode differentiation are refused."""
+    if q_out is None and k_out is None and forward_ad._current_level >= 0:
+        _no_tangent("norm_rope", q, k, q_norm and q_norm.weight, k_norm and k_norm.weight)
     if q_out is not None or k_out is not None or not torch.is_grad_enabled() or not any(
             t is not None and t.requires_grad for t in (q, k, q_norm and q_norm.weight, k_norm and k_norm.weight)):
         return _norm_call(q, k, q_norm, k_norm, rope, positions, q_out, k_out, stream)
@@ -416,6 +430,8 @@ def norm_rope_backward(dq_out: torch.Tensor, dk_out: Optional[torch.Tensor], q: 
     dq_out and dk_out of its outputs; None where there is no such tensor.  The weights' gradients have
     the weights' type; their sums are 32-bit and in a fixed order.  dq may be dq_out or q, dk likewise.
     ``workspace``: norm_rope_backward_workspace_bytes, allocated on the call's stream where not given."""
+    if forward_ad._current_level >= 0:
+        _no_tangent("norm_rope_backward", dq_out, dk_out, q, k, q_norm and q_norm.weight, k_norm and k_norm.weight)
     inputs = _norm_inputs(q, k, q_norm, k_norm, rope, positions)
     if (k is None) != (dk_out is None) or (k is None and dk is not None):
         raise ValueError("k and the gradients of k go together")
