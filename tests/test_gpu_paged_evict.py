@@ -305,3 +305,19 @@ def test_empty():
     assert got.shape == (0,) and kept.shape == (0, 2, 0)
     none = Cache([0, 0], 2, 64, 16, BF16)
     assert P.kv_evict(none.cache, none.table, none.seq_len, none.mass, 10).tolist() == [0, 0]
+
+
+def test_a_view_of_the_mass_is_the_mass():
+    """The stride of a dimension of one tells nothing: another view of the same weights is the mass itself."""
+    c = Cache([40, 9], 1, 64, 16, BF16, seed=5)
+    want = Cache([40, 9], 1, 64, 16, BF16, seed=5)
+    lens = P.kv_evict(want.cache, want.table, want.seq_len, want.mass, 20, first=2, recent=5)
+    view = torch.as_strided(c.mass, c.mass.shape, (16, 1, 3))
+    assert view.stride() != c.mass.stride() and view.data_ptr() == c.mass.data_ptr()
+    assert torch.equal(P.kv_evict(c.cache, c.table, c.seq_len, c.mass, 20, first=2, recent=5, mass_out=view), lens)
+    for x, y, pages, n in ((x, y, pages, int(n)) for x, y in zip(c.tensors(), want.tensors()) for pages, n in zip(c.rows, lens)):
+        at = torch.arange(n, device="cuda")
+        where = torch.tensor(pages, device="cuda")[at // 16], at % 16
+        assert torch.equal(x[where], y[where])
+    with pytest.raises(ValueError, match="share"):
+        P.kv_evict(c.cache, c.table, c.seq_len, c.mass, 20, mass_out=torch.as_strided(c.mass, c.mass.shape, (8, 1, 1)))

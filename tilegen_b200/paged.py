@@ -804,7 +804,8 @@ def kv_evict(cache: PagedKV, table: PageTable, seq_len: torch.Tensor, mass: torc
     a.mass = _mass_desc(mass, "mass", cache, index)
     if mass_out is not None and mass_out is not mass:
         a.mass_out = _mass_desc(mass_out, "mass_out", cache, index)
-        if a.mass_out.data == a.mass.data and mass_out.stride() != mass.stride():
+        if a.mass_out.data == a.mass.data and any(
+                n > 1 and x != y for n, x, y in zip(mass.shape, mass.stride(), mass_out.stride())):
             raise ValueError("mass_out must be mass or not share memory with it")
     sp = _stream(index, stream)
     where = _elsewhere(index, stream)
