@@ -404,3 +404,16 @@ print("all", batch)
 """ % [os.path.dirname(os.path.abspath(__file__)), os.path.dirname(os.path.dirname(os.path.abspath(__file__)))]
     r = subprocess.run([sys.executable, "-c", code], env={**os.environ, "TG_MASS_WAIT_MS": "1"}, capture_output=True, text=True, timeout=300)
     assert r.returncode == 0 and "all 40" in r.stdout, r.stdout + r.stderr
+
+
+@pytest.mark.parametrize("case", [0, 3])
+@pytest.mark.parametrize("how", ["tokens", "heads", "both", "overlapping"])
+def test_queries_of_any_strides(how, case):
+    """Expanded queries and rows that overlap are taken as they are, as the attention takes them."""
+    b = Weighed(*MORE[case], BF16, seed=6)
+    t, h, d = b.q.shape
+    b.q = {"tokens": lambda q: q[:1].expand(t, h, d), "heads": lambda q: q[:, :1].expand(t, h, d),
+           "both": lambda q: q[:1, :1].expand(t, h, d), "overlapping": lambda q: torch.as_strided(q, (t, h, d), (d, d, 1))}[how](b.q)
+    lse = b.lse()
+    b.gather(lse, 0.5)
+    b.check(lse, 0.5)

@@ -720,8 +720,8 @@ def attention_mass(mass: torch.Tensor, q: torch.Tensor, cache: PagedKV, table: P
     each key of the sequences' own pages gets from the queries q, summed over the tokens that see it and
     the query heads of its key head: mass = decay * mass + sum of exp(scale * q k - lse).  Returns mass.
 
-    q, table, seq_len, q_indptr, the bounds, scale and causal are those of the prefix_attention call and
-    lse [tokens, q_heads] what it returned (with lse=True); behind a prefix the own keys get their share
+    q (any strides, 0 too, as an expanded tensor has them), table, seq_len, q_indptr, the bounds, scale and
+    causal are those of the prefix_attention call and lse [tokens, q_heads] what it returned (with lse=True); behind a prefix the own keys get their share
     of the whole softmax.  With ``causal`` the queries are the sequence's last tokens, whose keys start
     from nothing: what their slots held is not read.  decay=0 forgets all that came before.  To weigh a
     prompt by its last tokens, pass these as q, with seq_len of the whole prompt, and decay=0.
