@@ -12,9 +12,10 @@
 // positions.
 //
 // * select_kernel: a cluster of CTAs for each (sequence, key head).  Weights as ordered 32-bit
-//   integers lie in shared memory; three rounds of 11, 11 and 10 bits find the value of the
-//   heavy-th largest (histograms of all CTAs, added over the cluster), then ranks in the order of the
-//   places give the holes and the keys that fill them.
+//   integers lie in shared memory; four rounds of 11, 8, 8 and 5 bits find the value of the heavy-th
+//   largest (histograms of all CTAs, added over the cluster), the last two over the keys that begin
+//   like it, which each warp lists in the second (over all keys again in a CTA where a warp's list
+//   overflows); then ranks in the order of the places give the holes and the keys that fill them.
 //   Bound: latency.  512 (sequence, head) pairs of 1000 keys 11 us, two sequences of 120000 (clusters of
 //   eight CTAs, 15000 keys each) 50 us: reading 8, histograms 12, their sums over the cluster 12, ranks
 //   and lists 15.

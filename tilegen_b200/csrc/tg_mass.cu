@@ -19,8 +19,9 @@
 //
 // * Up to 256 rows of a key head (decoding; the last tokens of a prompt): bound by the keys' bytes.  The
 //   rows stay in shared memory, the keys pass through a ring (stream_kernel).  64 sequences of 200 to 4000
-//   keys, one token each (284 MB): 56 us, 5.1 TB/s; windows of 32 tokens over 212 MB of keys 49 to 57 us,
-//   where the special-function units are 61 % busy too.
+//   keys, one token each (284 MB): 56 us, 5.1 TB/s; windows of 32 tokens over 212 MB of keys 48 to 57 us,
+//   where the special-function units are 61 % busy too: a warpgroup gives its buffer back only after
+//   its exponentials, so that neither unit has work all the time.
 // * More rows: bound by the exponentials, 16 a cycle and SM, and the hand-over of buffers between the tensor
 //   core and the warpgroups: whole prompts of 300 to 3500 tokens (191 GFLOP that count, 745 million
 //   exponentials) 304 us, special-function units 69 % and tensor pipe 35 % active; with exponentials

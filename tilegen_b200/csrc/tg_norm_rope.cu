@@ -10,8 +10,9 @@
 // * Bound: HBM, then issue slots.  A row is read once: a group of lanes holds it in registers, the sums
 //   over it are shuffles, and the cosines and sines of a few tokens lie in shared memory for all heads of
 //   q and k.  The gradient's two sums (x^2 and u x) are made in one round of shuffles.  16381 tokens of
-//   32 and 8 heads of 128 in bfloat16: forward (336 MB) 55 us, 6.0 TB/s, 78 % of issue slots; gradient
-//   (503 MB) 89 us, 5.6 TB/s; prompts into the cache (572 MB) 96 us, 6.0 TB/s (the measured copy: 6.5).
+//   32 and 8 heads of 128 in bfloat16, on several GPUs: forward (336 MB) 55 to 62 us, 5.4 to 6.1 TB/s,
+//   78 % of issue slots; gradient (503 MB) 89 to 91 us, 5.5 to 5.7 TB/s; prompts into the cache (572 MB)
+//   96 to 102 us, 5.6 to 6.0 TB/s (the measured copy: 6.5).
 // * Rows come by cp.async into a ring of the thread's own places, three deep: in registers the rows ahead
 //   cost the gradient its second CTA an SM (128 us without the ring) and the forward pass 11 of 66 us.
 // * Statistics, rotation and sums are 32-bit, the angle 64-bit; each output is rounded once.  Where that
