@@ -367,14 +367,14 @@ print("all", len(GIVE_UP))
 
 
 def test_a_unit_may_take_longer_than_a_wait():
-    """1000 tokens of 256 heads a key head pass 512 keys, some milliseconds for a CTA's unit, of which it has
-    several: with a limit of one millisecond nothing runs out, as all waits but those for a whole unit are
-    microseconds.  The bound is that of the other cases, for 256000 rows."""
+    """4000 tokens of 256 heads a key head pass 512 keys, 20 milliseconds for a CTA's unit, of which it has
+    several: with a limit of five milliseconds nothing runs out, as all waits but those for a whole unit are
+    microseconds.  The bound is that of the other cases, for 1024000 rows."""
     code = """
 import sys
 sys.path[:0] = %r
 from test_gpu_paged_mass import *
-n, kvh, group, dim, keys, page, batch = 1000, 8, 256, 64, 512, 32, 40
+n, kvh, group, dim, keys, page, batch = 4000, 8, 256, 64, 512, 32, 40
 g = gen(7)
 pages = batch * keys // page
 cache = P.PagedKV(normal(g, pages, page, kvh, dim, dtype=BF16), None)
@@ -402,7 +402,7 @@ assert bool(got.isfinite().all()), int(got.isnan().sum())
 assert bool((err <= tol).all()), float((err / tol).max())
 print("all", batch)
 """ % [os.path.dirname(os.path.abspath(__file__)), os.path.dirname(os.path.dirname(os.path.abspath(__file__)))]
-    r = subprocess.run([sys.executable, "-c", code], env={**os.environ, "TG_MASS_WAIT_MS": "1"}, capture_output=True, text=True, timeout=300)
+    r = subprocess.run([sys.executable, "-c", code], env={**os.environ, "TG_MASS_WAIT_MS": "5"}, capture_output=True, text=True, timeout=300)
     assert r.returncode == 0 and "all 40" in r.stdout, r.stdout + r.stderr
 
 
