@@ -67,7 +67,7 @@ struct MassParams : AttnParams {
     int box, box_shift;                                  // keys of a box, their log2
     int q_bufs, stages;
     int first_seq, seqs;  // of this launch
-    uint64_t wait_ns;     // how long warps wait for one another; 0: a wait that is not over at once runs out
+    uint64_t wait_ns;     // how long warps wait for one another; 0: as if a wait had run out in every CTA
     float* part;          // with splits > 1: [split][chunk][sequence][key head][key of the chunk]
 };
 
